@@ -282,6 +282,42 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
                                     int q_heads, int kv_heads, int head_dim, int page_size,
                                     float sm_scale, b200_stream_t stream);
 
+/* Attention of a batch whose requests share long prefixes (no counterpart in the reference, whose prefix cache hands out
+ * the slots but whose attention reads them once per request): the result of b200_attention_prefill, with the keys of a
+ * prefix read once for all of its requests.  Requests lie group by group: group g is requests [group_indptr[g],
+ * group_indptr[g + 1]), and positions [0, prefix_lens[g]) of every page-table row of the group name keys and values that
+ * are those of its first request's row, which is the one that is read.  prefix_lens may be longer than what lies before
+ * the query rows of some request; as much of it is shared as lies before all of them.  Requests of no group, and groups
+ * of one, share nothing.
+ * Request b owns query rows [qo_indptr[b], qo_indptr[b + 1]) of the `tokens` rows of q, the LAST positions of its
+ * seq_lens[b] keys, as for b200_attention_prefill (a decode step: one each; drafted tokens: a few each).  Rows of no
+ * request are left as they were; a row that sees no key becomes zeros.  out [tokens, q_heads * head_dim] contiguous.
+ * Everything per request and group is read on the device: a captured call follows what the arrays hold at its replay,
+ * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words, and so
+ * are query rows of overlapping requests (nothing is written then).
+ * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head.  workspace:
+ * b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
+ * run one after another. */
+typedef struct b200_shared_prefix_args {
+    void* out;
+    const void* q;
+    int64_t q_stride_token, q_stride_head;
+    const void *k_cache, *v_cache;
+    int64_t num_slots;
+    const int32_t* page_table;
+    int64_t page_table_stride;
+    const int32_t *table_idx, *seq_lens, *qo_indptr;
+    const int32_t *group_indptr, *prefix_lens;
+    int32_t tokens, batch, groups;
+    int32_t q_heads, kv_heads, head_dim, page_size;
+    float sm_scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} b200_shared_prefix_args;
+B200_API int64_t b200_attention_shared_prefix_workspace_bytes(int max_tokens, int max_batch, int q_heads, int kv_heads,
+                                                              int head_dim);
+B200_API int b200_attention_shared_prefix(const b200_shared_prefix_args* args, b200_stream_t stream);
+
 /* ---- sampler (include/sglang/engine/engine.h:36-55) ------------------------- */
 
 /* Sampler::sample, all-greedy branch (src/engine/engine.cc:294-298): argmax over
@@ -314,6 +350,34 @@ B200_API int b200_sample(int32_t* out, const void* logits, int rows, int vocab, 
 B200_API int b200_sample_from_probs(int32_t* out, const float* probs, int rows, int vocab,
                                     const int32_t* top_k, int top_k_value, const float* top_p,
                                     float top_p_value, const float* uniform, b200_stream_t stream);
+
+/* The distribution that b200_sample draws from, as numbers (no counterpart in the reference, which filters on the host):
+ * out[r, :] = softmax(logits[r, :] / temperatures[r]) over the top_k[r] largest (equal ones by index; below 1 or above vocab:
+ * all), of those over the entries whose cumulative probability, their own included, stays within top_p[r] (never without
+ * the largest; 1: all), zeros elsewhere.  A temperature of at most 1e-6 (or NaN) gives 1 at the first maximum.  top_k, top_p:
+ * device arrays or NULL.  bf16 logits [rows, vocab] of row stride ld, fp32 out [rows, vocab] contiguous.  A NaN counts as
+ * -inf; a row of nothing else becomes zeros.  Cuts are decided by 64-bit sums.  vocab up to 327680. */
+B200_API int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, int vocab,
+                                 const float* temperatures, const int32_t* top_k, const float* top_p,
+                                 b200_stream_t stream);
+
+/* Verification of drafted tokens (speculative sampling; no counterpart in the reference).  Request b of the batch has drafts
+ * draft_tokens[j], j in [draft_indptr[b], draft_indptr[b + 1]), each drawn from draft_probs[j, :] (NULL: they were certain,
+ * looked up for instance), and one row of target_probs more than drafts: rows draft_indptr[b] + b on, the first for what
+ * follows its context, the next for what follows its first draft, and so on.  Draft j is accepted if those before it are
+ * and accept_uniform[j] * draft_probs[j, token] < target_probs[row of j, token].  Behind the accepted drafts comes a token
+ * drawn with draw_uniform[b] by inverse CDF in index order: from max(target - draft, 0) at the first draft that was not
+ * accepted (from target where that is zero throughout), from the last row where all were.  Negative numbers and NaN among
+ * the probabilities count as 0; a row without a positive number gives token 0.  A drafted token outside [0, vocab) is not
+ * accepted and reported in the status words.
+ * tokens int32 [batch, max_drafts + 1]: the accepted drafts, the token behind them, then -1; accepted int32 [batch].  Of
+ * more than max_drafts drafts the first max_drafts are looked at.  All probabilities fp32, rows target_ld and draft_ld
+ * apart; uniform numbers fp32 in [0, 1).  total_drafts = draft_indptr[batch].  Decisions and sums in 64 bits, in a fixed
+ * order. */
+B200_API int b200_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_ld,
+                                const float* draft_probs, int64_t draft_ld, const int32_t* draft_tokens,
+                                const int32_t* draft_indptr, const float* accept_uniform, const float* draw_uniform,
+                                int batch, int total_drafts, int max_drafts, int vocab, b200_stream_t stream);
 
 /* ---- latent attention, table routing, fp32 residual (no counterparts in the reference) --------- */
 

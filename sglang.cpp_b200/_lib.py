@@ -92,6 +92,10 @@ PROTOTYPES: dict[str, tuple] = {
     "b200_argmax": (_I, [_P, _P, _I, _I, _L, _P]),
     "b200_sample": (_I, [_P, _P, _I, _I, _L, _P, _P, _P, _P, ctypes.c_uint64, _P, _P]),
     "b200_sample_from_probs": (_I, [_P, _P, _I, _I, _P, _I, _P, _F, _P, _P]),
+    "b200_sampling_probs": (_I, [_P, _P, _L, _I, _I, _P, _P, _P, _P]),
+    "b200_verify_drafts": (_I, [_P, _P, _P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "b200_attention_shared_prefix_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
+    "b200_attention_shared_prefix": (_I, [_P, _P]),
     "b200_comm_create": (_I, [_I, _I, _L, POINTER(c_void_p)]),
     "b200_comm_handle_bytes": (_I, []),
     "b200_comm_export": (_I, [_P, _P]),
@@ -221,6 +225,17 @@ class WindowAttentionArgs(ctypes.Structure):
         ("chunk", c_int32), ("sinks", _P), ("gate_per_head", c_int32), ("out_scale", c_float), ("out_stride", _L),
         ("head_mix", _P), ("value_rotary", c_int32), ("max_pos", c_int32), ("value_cos", _P), ("value_sin", _P),
         ("positions", _P), ("score_bound", c_float), ("mix_scratch", _P),
+    ]
+
+
+class SharedPrefixArgs(ctypes.Structure):
+    """b200_shared_prefix_args."""
+    _fields_ = [
+        ("out", _P), ("q", _P), ("q_stride_token", _L), ("q_stride_head", _L), ("k_cache", _P), ("v_cache", _P), ("num_slots", _L),
+        ("page_table", _P), ("page_table_stride", _L), ("table_idx", _P), ("seq_lens", _P), ("qo_indptr", _P),
+        ("group_indptr", _P), ("prefix_lens", _P), ("tokens", c_int32), ("batch", c_int32), ("groups", c_int32),
+        ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32), ("sm_scale", c_float),
+        ("workspace", _P), ("workspace_bytes", _L),
     ]
 
 

@@ -1,0 +1,191 @@
+// Which drafted tokens the target's probabilities accept, and the token that follows them (speculative sampling).
+//
+// A request with drafts x_1 .. x_n, drawn from q_1 .. q_n, has target rows p_0 .. p_n (p_i: what follows the first i drafts).
+// Draft i stands if those before it do and u_i q_i(x_i) < p_{i-1}(x_i), with u_i uniform in [0, 1): probability min(1, p / q).
+// The token behind the a accepted ones is drawn from max(p_a - q_{a+1}, 0), or from p_n where all stand; together that is a draw
+// from the target's own distribution.  The draw is the inverse of the summed probabilities in index order: the first index whose
+// running sum exceeds u * (sum of all).
+//
+// Everything is decided in fp64: a product of two fp32 numbers is exact there, and a sum of a row's is right to 1e-13 or so, so
+// that a border is missed by no more than that.  Sums are formed in a fixed order: equal calls, equal tokens.
+//
+// Bound by HBM: one row of p, and one of q where a draft was refused, 8 bytes per vocabulary entry and request, read once; the
+// other rows are looked at in one place each.  A cluster of CTAs shares a row: every warp sums a run of consecutive entries, the
+// CTAs exchange their sums, and the warp in whose run the target lies walks it once more (a few KB from L2).
+#include "common.cuh"
+#include "kernels.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+
+struct VerifyParams {
+    int32_t *tokens, *accepted;
+    const float *target, *draft;
+    int64_t target_ld, draft_ld;
+    const int32_t *draft_tokens, *draft_indptr;
+    const float *accept, *draw;
+    int batch, total, most, vocab, cluster;
+    int* status;
+};
+
+// What an entry counts for: nothing unless it is a positive number.
+__device__ __forceinline__ float entry(float p) { return p > 0.f ? fminf(p, 3.402823466e38f) : 0.f; }
+__device__ __forceinline__ float unit_interval(float u) { return u > 0.f ? fminf(u, 0.99999994f) : 0.f; }
+
+__global__ void __launch_bounds__(kThreads)
+verify_drafts_kernel(const VerifyParams p) {
+    __shared__ double s_sum[kWarps], s_cta[kMaxCluster];
+    __shared__ int s_accepted;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, b = static_cast<int>(blockIdx.x) / C;
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (waited for ahead of the first remote store)
+    pdl_launch_dependents();
+    pdl_wait_prior();
+
+    const int start = min(max(p.draft_indptr[b], 0), p.total);
+    const int n = min(min(max(p.draft_indptr[b + 1], start), p.total) - start, p.most);
+    const float* target = p.target + static_cast<int64_t>(start + b) * p.target_ld;   // the request's first row
+    // ---- the drafts, 32 at a time ----
+    if (warp == 0) {
+        int a = 0;
+        for (int base = 0; base < n; base += 32) {
+            const int j = base + lane;
+            bool refused = false;
+            if (j < n) {
+                const int x = p.draft_tokens[start + j];
+                const bool known = x >= 0 && x < p.vocab;
+                if (!known && rank == 0) atomicExch(&p.status[kStatusBadIndex], x + 1);
+                const double px = known ? entry(target[j * p.target_ld + x]) : 0.0;
+                const double qx = p.draft == nullptr ? 1.0 : known ? entry(p.draft[(start + j) * p.draft_ld + x]) : 0.0;
+                refused = !(unit_interval(p.accept[start + j]) * qx < px);
+            }
+            const uint32_t first = __ballot_sync(0xffffffffu, refused);
+            a = first != 0 ? base + __ffs(first) - 1 : min(base + 32, n);
+            if (first != 0) break;
+        }
+        if (lane == 0) s_accepted = a;
+    }
+    __syncthreads();
+    const int a = s_accepted;
+    if (rank == 0)
+        for (int j = threadIdx.x; j <= p.most; j += kThreads)
+            if (j != a) p.tokens[static_cast<int64_t>(b) * (p.most + 1) + j] = j < a ? p.draft_tokens[start + j] : -1;
+    if (rank == 0 && threadIdx.x == 0) p.accepted[b] = a;
+
+    // ---- the row to draw from: this warp's run of it ----
+    const float* prow = target + a * p.target_ld;
+    const bool refused = a < n;
+    const float* qrow = refused && p.draft != nullptr ? p.draft + (start + a) * p.draft_ld : nullptr;
+    const int without = refused && p.draft == nullptr ? p.draft_tokens[start + a] : -1;   // a draft that was certain
+    const int run = ((p.vocab + C * kWarps - 1) / (C * kWarps) + 127) / 128 * 128;
+    const int first = min((rank * kWarps + warp) * run, p.vocab), last = min(first + run, p.vocab);
+    bool rest = refused;   // p - q; or p, where no entry of p exceeds q
+    auto weight = [&](int i) -> double {
+        const float x = entry(__ldg(prow + i));
+        if (!rest) return x;
+        if (qrow == nullptr) return i == without ? static_cast<double>(fmaxf(x - 1.f, 0.f)) : static_cast<double>(x);
+        return fmax(static_cast<double>(x) - static_cast<double>(entry(__ldg(qrow + i))), 0.0);
+    };
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    double total = 0.0, before = 0.0, mine = 0.0;   // of the row, of the runs before this warp's, of this run
+    for (int pass = 0; pass < 2; ++pass) {
+        double sum = 0.0;
+#pragma unroll 8
+        for (int i = first + lane; i < last; i += 32) sum += weight(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        double cta = 0.0, ahead = 0.0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) ahead = cta;
+            cta += s_sum[w];
+        }
+        mine = sum;
+        if (C > 1) {
+            if (threadIdx.x < static_cast<unsigned>(C)) {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_cta[rank])), "r"(threadIdx.x));
+                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(cta) : "memory");
+            }
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        } else {
+            if (threadIdx.x == 0) s_cta[0] = cta;
+            __syncthreads();
+        }
+        total = 0.0;
+        for (int r = 0; r < C; ++r) {
+            if (r == rank) before = total + ahead;
+            total += s_cta[r];
+        }
+        if (total > 0.0 || !rest) break;   // (the same in every CTA of the cluster)
+        rest = false;
+        if (C > 1) {   // everyone has read the sums before the next ones arrive
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        } else {
+            __syncthreads();
+        }
+    }
+    int32_t* out = p.tokens + static_cast<int64_t>(b) * (p.most + 1) + a;
+    if (!(total > 0.0)) {
+        if (rank == 0 && threadIdx.x == 0) *out = 0;   // a row without a positive number
+        return;
+    }
+    const double goal = unit_interval(p.draw[b]) * total;
+    if (!(mine > 0.0) || goal < before || goal >= before + mine) return;
+    double ahead = before;
+    int pick = -1, positive = -1;
+    for (int base = first; base < last && pick < 0; base += 32) {
+        const int i = base + lane;
+        const double w = i < last ? weight(i) : 0.0;
+        double incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const uint32_t over = __ballot_sync(0xffffffffu, w > 0.0 && ahead + incl > goal);
+        const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
+        if (over != 0) pick = base + __ffs(over) - 1;
+        if (any != 0) positive = base + 31 - __clz(any);
+        ahead += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    // (the walk adds in another order than the sums: the last bits may put the goal behind the run's last entry)
+    if (lane == 0) *out = pick >= 0 ? pick : positive;
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" {
+
+int b200_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_ld, const float* draft_probs,
+                       int64_t draft_ld, const int32_t* draft_tokens, const int32_t* draft_indptr, const float* accept_uniform,
+                       const float* draw_uniform, int batch, int total_drafts, int max_drafts, int vocab, b200_stream_t stream) {
+    using namespace b200;
+    B200_CHECK_ARG(batch >= 0 && total_drafts >= 0 && max_drafts >= 0 && vocab > 0, "verify_drafts: bad shape");
+    B200_CHECK_ARG(batch <= (1 << 24) && vocab <= (1 << 30) && max_drafts <= (1 << 20), "verify_drafts: too large");
+    B200_CHECK_ARG(target_ld >= vocab && (draft_probs == nullptr || draft_ld >= vocab), "verify_drafts: row stride below vocab");
+    if (batch == 0) return B200_OK;
+    B200_CHECK_ARG(tokens && accepted && target_probs && draft_indptr && draw_uniform, "verify_drafts: NULL tensor");
+    B200_CHECK_ARG(total_drafts == 0 || (draft_tokens && accept_uniform), "verify_drafts: NULL tensor");
+    int err = B200_OK;
+    int* status = device_status_words(&err);
+    if (err != B200_OK) return err;
+    // CTAs per row: enough to fill the device, and no fewer than 4096 entries each.
+    int cluster = 1;
+    while (cluster < kMaxCluster && static_cast<int64_t>(batch) * cluster < 2 * sm_count() && vocab / (2 * cluster) >= 4096) cluster *= 2;
+    VerifyParams p = {tokens,       accepted,       target_probs, draft_probs, target_ld,    draft_ld, draft_tokens, draft_indptr,
+                      accept_uniform, draw_uniform, batch,        total_drafts, max_drafts, vocab,    cluster,      status};
+    B200_CHECK_CUDA(launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(batch) * cluster), dim3(kThreads), 0,
+                                  static_cast<cudaStream_t>(stream), dim3(cluster, 1, 1), p));
+    return B200_OK;
+}
+
+}  // extern "C"

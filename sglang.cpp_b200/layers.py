@@ -8,6 +8,7 @@ kernels.  Reference locations are given per item.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -30,6 +31,10 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 def _check(cond: bool, msg: str) -> None:
     if not cond:
         raise B200Error(1, msg)
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.size(0) > 1 else t.size(1)   # (a single row's says nothing)
 
 
 def _cuda_bf16(t: torch.Tensor, name: str) -> None:
@@ -316,6 +321,66 @@ class PagedAttention:
         return out
 
 
+class SharedPrefixAttention:
+    """Attention of a batch whose requests share long prefixes, the keys of a prefix read once for all of them (the reference's
+    prefix cache shares the slots, its attention reads them per request).  What ``PagedAttention.prefill`` returns, for a few
+    query rows per request: a decode step's, or those of drafted tokens.  One object's calls run one after another (they
+    share its workspace): use an object per stream, and per captured graph that may be replayed beside another."""
+
+    def __init__(self, kv_cache: MHAKVCache, num_qo_heads: int, num_kv_heads: int, head_dim: int, max_tokens: int,
+                 max_batch: int = 256):
+        self.kv_cache_ = kv_cache
+        self.num_qo_heads_ = num_qo_heads
+        self.num_kv_heads_ = num_kv_heads
+        self.head_dim_ = head_dim
+        self.max_tokens_ = max_tokens
+        self.max_batch_ = max_batch
+        self.sm_scale = 1.0 / math.sqrt(head_dim)
+        nbytes = _lib.load().b200_attention_shared_prefix_workspace_bytes(max_tokens, max_batch, num_qo_heads, num_kv_heads, head_dim)
+        _check(nbytes > 0, "unsupported head configuration or size for attention over a shared prefix")
+        _check(kv_cache.kv_heads_ == num_kv_heads and kv_cache.head_dim_ == head_dim, "KV cache layout mismatch")
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=kv_cache.kv_buffer_.device)
+
+    def forward(self, q: torch.Tensor, layer_id: int, page_table: torch.Tensor, table_idx: torch.Tensor, seq_lens: torch.Tensor,
+                qo_indptr: torch.Tensor, group_indptr: torch.Tensor, prefix_lens: torch.Tensor,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q [tokens, q_heads, head_dim]; request b owns rows [qo_indptr[b], qo_indptr[b + 1]), the last positions of its
+        seq_lens[b] keys.  Group g is requests [group_indptr[g], group_indptr[g + 1]), whose page-table rows agree in their first
+        prefix_lens[g] positions.  Rows that no request owns are not written."""
+        kc = self.kv_cache_
+        _cuda_bf16(q, "q")
+        _check(q.dim() == 3 and q.size(1) == self.num_qo_heads_ and q.size(2) == self.head_dim_, "q must be [tokens, q_heads, head_dim]")
+        _check(q.stride(2) == 1, "Last dimension must be contiguous")
+        index = {"page_table": page_table, "table_idx": table_idx, "seq_lens": seq_lens, "qo_indptr": qo_indptr,
+                 "group_indptr": group_indptr, "prefix_lens": prefix_lens}
+        for name, t in index.items():
+            _check(t.is_cuda and t.dtype == torch.int32, f"{name} must be a CUDA int32 tensor")
+            _check(t.device == q.device, f"{name} must be on the device of q")
+            _check(t.stride(-1) == 1 or t.size(-1) <= 1, f"{name} must be contiguous")
+        _check(q.device == kc.kv_buffer_.device == self.workspace.device, "q and the KV cache must be on one device")
+        batch, groups = table_idx.numel(), prefix_lens.numel()
+        _check(page_table.dim() == 2, "page_table must be rank 2")
+        _check(seq_lens.numel() == batch and qo_indptr.numel() == batch + 1, "seq_lens [batch], qo_indptr [batch + 1]")
+        _check(group_indptr.numel() == groups + 1, "group_indptr must be [groups + 1]")
+        _check(q.size(0) <= self.max_tokens_ and batch <= self.max_batch_, "more query rows or requests than the workspace is made for")
+        shape = (q.size(0), self.num_qo_heads_ * self.head_dim_)
+        if out is None:
+            out = torch.empty(shape, dtype=bf16, device=q.device)
+        _cuda_bf16(out, "out")
+        _check(tuple(out.shape) == shape and out.is_contiguous() and out.device == q.device, "out must be contiguous [tokens, q_heads * head_dim]")
+        args = _lib.SharedPrefixArgs(
+            out=out.data_ptr(), q=q.data_ptr(), q_stride_token=q.stride(0), q_stride_head=q.stride(1),
+            k_cache=kc.k_cache(layer_id).data_ptr(), v_cache=kc.v_cache(layer_id).data_ptr(), num_slots=kc.total_slots,
+            page_table=page_table.data_ptr(), page_table_stride=page_table.stride(0), table_idx=table_idx.data_ptr(),
+            seq_lens=seq_lens.data_ptr(), qo_indptr=qo_indptr.data_ptr(), group_indptr=group_indptr.data_ptr(),
+            prefix_lens=prefix_lens.data_ptr(), tokens=q.size(0), batch=batch, groups=groups, q_heads=self.num_qo_heads_,
+            kv_heads=self.num_kv_heads_, head_dim=self.head_dim_, page_size=kc.page_size_, sm_scale=self.sm_scale,
+            workspace=self.workspace.data_ptr(), workspace_bytes=self.workspace.numel())
+        with torch.cuda.device(q.device):
+            call("b200_attention_shared_prefix", ctypes.byref(args), _stream())
+        return out
+
+
 def qknorm_rope_store(qkv: torch.Tensor, q_norm: Optional[RMSNorm], k_norm: Optional[RMSNorm],
                       rotary: RotaryEmbedding, positions: torch.Tensor, out_loc: torch.Tensor,
                       kv_cache: MHAKVCache, layer_id: int, num_qo_heads: int, num_kv_heads: int,
@@ -438,6 +503,53 @@ def sample_from_probs(probs: torch.Tensor, uniform: torch.Tensor, top_k: Optiona
     call("b200_sample_from_probs", out.data_ptr(), probs.data_ptr(), probs.size(0), probs.size(1), _ptr(top_k),
          top_k_value, _ptr(top_p), top_p_value, uniform.data_ptr(), _stream())
     return out
+
+
+def sampling_probs(logits: torch.Tensor, temperatures: torch.Tensor, top_k: Optional[torch.Tensor] = None,
+                   top_p: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The distribution that ``sample`` draws from, with the same arguments: float32 [rows, vocab], zeros outside the kept set."""
+    _cuda_bf16(logits, "logits")
+    _check(logits.dim() == 2 and (logits.stride(1) == 1 or logits.size(1) == 1), "logits must be rank 2 with contiguous rows")
+    rows, vocab = logits.shape
+    for name, t, dtype in (("temperatures", temperatures, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32)):
+        if t is not None:
+            _check(t.device == logits.device and t.dtype == dtype and t.numel() == rows and t.is_contiguous(),
+                   f"{name} must be {dtype} [rows] on the device of logits")
+    out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+    with torch.cuda.device(logits.device):
+        call("b200_sampling_probs", out.data_ptr(), logits.data_ptr(), _row_stride(logits), rows, vocab,
+             temperatures.data_ptr(), _ptr(top_k), _ptr(top_p), _stream())
+    return out
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_indptr: torch.Tensor, accept_uniform: torch.Tensor,
+                  draw_uniform: torch.Tensor, max_drafts: int,
+                  draft_probs: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target's probabilities accept, and the token behind them (b200_verify_drafts).  target_probs
+    [drafts + batch, vocab]: request b's rows begin at draft_indptr[b] + b and are one more than its drafts; draft_probs [drafts,
+    vocab], or None where drafts were certain.  Returns int32 tokens [batch, max_drafts + 1] (accepted drafts, the token behind
+    them, -1) and int32 accepted [batch]."""
+    dev = target_probs.device
+    _check(target_probs.is_cuda and target_probs.dtype == torch.float32 and target_probs.dim() == 2
+           and (target_probs.stride(1) == 1 or target_probs.size(1) == 1), "target_probs must be CUDA float32 [rows, vocab] with contiguous rows")
+    vocab, batch, drafts = target_probs.size(1), draw_uniform.numel(), draft_tokens.numel()
+    for name, t, dtype in (("draft_tokens", draft_tokens, torch.int32), ("draft_indptr", draft_indptr, torch.int32),
+                           ("accept_uniform", accept_uniform, torch.float32), ("draw_uniform", draw_uniform, torch.float32)):
+        _check(t.device == dev and t.dtype == dtype and t.is_contiguous(), f"{name} must be contiguous {dtype} on the device of target_probs")
+    _check(max_drafts >= 0, "max_drafts must not be negative")
+    _check(draft_indptr.numel() == batch + 1, "draft_indptr must be [batch + 1]")
+    _check(target_probs.size(0) == drafts + batch, "target_probs must have one row per draft and one per request")
+    _check(accept_uniform.numel() == drafts, "accept_uniform must have one number per draft")
+    if draft_probs is not None:
+        _check(draft_probs.device == dev and draft_probs.dtype == torch.float32 and tuple(draft_probs.shape) == (drafts, vocab)
+               and (draft_probs.stride(1) == 1 or vocab == 1), "draft_probs must be float32 [drafts, vocab] with contiguous rows")
+    tokens = torch.empty(batch, max_drafts + 1, dtype=torch.int32, device=dev)
+    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        call("b200_verify_drafts", tokens.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(), _row_stride(target_probs),
+             _ptr(draft_probs), vocab if draft_probs is None else _row_stride(draft_probs), draft_tokens.data_ptr(),
+             draft_indptr.data_ptr(), accept_uniform.data_ptr(), draw_uniform.data_ptr(), batch, drafts, max_drafts, vocab, _stream())
+    return tokens, accepted
 
 
 def read_device_status() -> tuple[int, int]:
