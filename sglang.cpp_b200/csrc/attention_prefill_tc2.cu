@@ -595,8 +595,6 @@ int make_kv_tile_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, in
     return B200_OK;
 }
 
-namespace {
-
 // Whole rows of `keys` (a multiple of 8) neighbouring slots of 8 or more, the first of them a multiple of 8: groups of 8 keys, in each
 // both halves of the head dimension (coordinates: element of a half, key of a group, half, group, head).
 int make_kv_groups_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, int kv_heads, int keys) {
@@ -619,8 +617,6 @@ int make_kv_groups_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, 
     }
     return B200_OK;
 }
-
-}  // namespace
 
 int launch_attention_prefill_tc2(void* out, const void* q, int64_t q_st, int64_t q_sh, const void* k_cache,
                                  const void* v_cache, int64_t num_slots, const int32_t* page_table,

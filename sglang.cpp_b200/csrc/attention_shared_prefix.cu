@@ -30,6 +30,7 @@ constexpr int kSlotTab = 1024;
 constexpr int RT = 16;                               // query rows of a tile
 constexpr int kMinStagesPerCta = 2;
 constexpr int kMergeWarps = 4;
+constexpr int kTcRows = 32;
 constexpr int kNoLimit = 0x3fffffff;
 constexpr int kMaxUnits = 2 * kSharedMaxBatch;
 
@@ -112,7 +113,9 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
     }
-    pdl_wait_prior();
+    // Behind the tensor-core kernel nothing here waits for what it writes, and what came before it is complete: it has waited.  The
+    // wait is made up for at the end, since the kernel that joins the parts waits for this one alone.
+    if (!p.after_tc) pdl_wait_prior();
     pdl_launch_dependents();
 
     // ---- units, tiles and stages ----
@@ -144,7 +147,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     {
         auto size_of = [&](int u) {
             const Unit x = unit_of(u);
-            const int stages = (max(x.hi - x.start, 0) + SK - 1) / SK, tiles = stages > 0 ? (x.ntok * G + RT - 1) / RT : 0;
+            const int stages = (max(x.hi - x.start, 0) + SK - 1) / SK, tiles = stages > 0 && (u >= p.groups || x.ntok * G <= p.tc_rows) ? (x.ntok * G + RT - 1) / RT : 0;
             return make_int2(tiles * stages, tiles);
         };
         const int each = (U + kThreads - 1) / kThreads;
@@ -201,7 +204,10 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             if (!fits) atomicExch(&p.status[kStatusBadIndex], p.tokens + 1);
         }
     }
-    if (!fits) return;
+    if (!fits) {
+        if (p.after_tc) pdl_wait_prior();
+        return;
+    }
     const int g_begin = min(static_cast<int>(blockIdx.x) * per, total);
     const int g_end = min(total, g_begin + per);
 
@@ -266,6 +272,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                 }
             }
         }
+        if (p.after_tc) pdl_wait_prior();
         return;
     }
 
@@ -395,6 +402,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             if (t == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mx[rr], sum);
         }
     }
+    if (p.after_tc) pdl_wait_prior();
 }
 
 // Parts of a row: `count` of them, the first at `first`, `step` rows apart.
@@ -413,14 +421,22 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const int per = p.plan.per[0];
-    if (head >= p.q_heads || per <= 0) return;
+    const int tc_per = p.after_tc ? p.plan.per[1] : 0;
+    if (head >= p.q_heads || per <= 0 || (p.after_tc && tc_per <= 0)) return;
     const int h = head / p.group, KG = kConsumerWarps / p.kv_heads;
     const int row0 = shared_row(p, b), row1 = shared_row(p, b + 1);
     const int grp = p.plan.group_of[b];
     const int own_first = p.plan.stage[p.groups + b], own_stages = p.plan.stage[p.groups + b + 1] - own_first;
     const int own_tile = p.plan.tile[p.groups + b], own_tiles = p.plan.tile[p.groups + b + 1] - own_tile;
     int pre_first = 0, pre_stages = 0, pre_tile = 0, pre_tiles = 0, pre_row = 0;
+    int tc_first = 0, tc_unit = 0, tc_units = 0, tc_tiles = 0;
     if (grp >= 0) {
+        if (p.after_tc) {
+            tc_first = p.plan.tc_first[grp];
+            tc_unit = p.plan.tc_unit[grp];
+            tc_units = p.plan.tc_unit[grp + 1] - tc_unit;
+            tc_tiles = tc_units > 0 ? (p.plan.tc_first[grp + 1] - tc_first) / tc_units : 0;
+        }
         pre_first = p.plan.stage[grp];
         pre_stages = p.plan.stage[grp + 1] - pre_first;
         pre_tile = p.plan.tile[grp];
@@ -438,8 +454,15 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     };
     for (int tok = row0 + static_cast<int>(blockIdx.z); tok < row1; tok += static_cast<int>(gridDim.z)) {
         const int hh = head - h * p.group;
-        const Parts pre = parts_of(pre_first, pre_stages, pre_tile, pre_tiles, (tok - pre_row) * p.group + hh);
+        Parts pre = parts_of(pre_first, pre_stages, pre_tile, pre_tiles, (tok - pre_row) * p.group + hh);
         const Parts own = parts_of(own_first, own_stages, own_tile, own_tiles, (tok - row0) * p.group + hh);
+        const int r = (tok - pre_row) * p.group + hh, block = r / 256;
+        if (tc_units > 0 && r >= 0 && block < tc_units / p.kv_heads) {
+            const int unit = h * (tc_units / p.kv_heads) + block, from = tc_first + unit * tc_tiles, c0 = from / tc_per;
+            pre.count = (from + tc_tiles - 1) / tc_per - c0 + 1;
+            pre.first = p.tc_base + static_cast<int64_t>(tc_unit + unit + c0) * 256 + (r & 255);
+            pre.step = 256;
+        }
         const int n = pre.count + own.count;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float M = -INFINITY, L = 0.f;
@@ -478,16 +501,20 @@ int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
 // Where the pieces of the workspace begin, in bytes.
 struct SharedLayout {
-    int64_t slots, plan, ml, o, bytes;
+    int64_t slots, tc_slots, rows, plan, ml, o, bytes;   // rows: of the rows kernel's parts, ahead of the tensor-core kernel's
 };
 SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads) {
     const int64_t rows = tokens * (q_heads / kv_heads), kg = kConsumerWarps / kv_heads;
     SharedLayout x;
     // tiles: at most one more than full ones per unit, and every row is in two units
     x.slots = sm_count() + 2 * (rows / RT) + batch + groups;
-    const int64_t part_rows = x.slots * kg * kv_heads * RT;
+    x.rows = x.slots * kg * kv_heads * RT;
+    // units of the tensor-core kernel: the same of groups that have more than kTcRows rows
+    const int64_t tc_groups = groups < rows / (kTcRows + 1) ? groups : rows / (kTcRows + 1);
+    x.tc_slots = rows > kTcRows ? sm_count() + kv_heads * (rows / 256 + tc_groups) : 0;
+    const int64_t part_rows = x.rows + x.tc_slots * 256;
     x.plan = 0;
-    x.ml = round256((4 + 2 * (groups + batch + 1) + groups + batch) * 4);
+    x.ml = round256((4 + 2 * (groups + batch + 1) + groups + batch + 2 * (groups + 1)) * 4);
     x.o = x.ml + round256(part_rows * 8);
     x.bytes = x.o + part_rows * kD * 4;
     return x;
@@ -495,8 +522,8 @@ SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_
 
 // Launches of a call after its first may begin before the one ahead of them has ended.
 struct FollowOn {
-    bool was = pdl_launches_enabled();
-    FollowOn() { set_pdl_launches(true); }
+    const bool was = pdl_launches_enabled();
+    explicit FollowOn(bool on) { set_pdl_launches(was || on); }
     ~FollowOn() { set_pdl_launches(was); }
 };
 
@@ -529,6 +556,7 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     B200_CHECK_ARG(a->num_slots > 0 && a->num_slots <= 0x7fffffff, "attention_shared_prefix: num_slots must be in [1, 2^31)");
     B200_CHECK_ARG(a->page_table_stride > 0 && a->page_table_stride <= (1 << 29),
                    "attention_shared_prefix: page_table_stride must be in [1, 2^29]");
+    B200_CHECK_ARG(a->sm_scale > 0.f && a->sm_scale <= 1e30f, "attention_shared_prefix: sm_scale must be a positive number");
     B200_CHECK_ARG(static_cast<int64_t>(a->tokens) * a->q_heads <= (1 << 28), "attention_shared_prefix: too many query rows");
     if (a->batch == 0 || a->tokens == 0) return B200_OK;
     B200_CHECK_ARG(a->out && a->q && a->k_cache && a->v_cache && a->page_table && a->table_idx && a->seq_lens && a->qo_indptr &&
@@ -579,6 +607,15 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.ws_ml = reinterpret_cast<float*>(ws + x.ml);
     p.ws_o = reinterpret_cast<float*>(ws + x.o);
     p.max_slots = static_cast<int>(x.slots);
+    p.plan.tc_first = p.plan.group_of + a->batch;
+    p.plan.tc_unit = p.plan.tc_first + a->groups + 1;
+    // Whole rows of queries are copied 16 bytes at a time there.
+    const bool aligned = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0;
+    p.tc_rows = aligned ? kTcRows : 0x7fffffff;
+    p.tc_slots = static_cast<int>(x.tc_slots);
+    p.tc_base = x.rows;
+    // (a group has more rows than that only if all have)
+    p.after_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > p.tc_rows;
     CUtensorMap tk, tv;
     err = make_kv_tmap(&tk, a->k_cache, a->num_slots, a->kv_heads, a->page_size);
     if (err != B200_OK) return err;
@@ -586,10 +623,15 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     if (err != B200_OK) return err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int grid = sm_count();
+    if (p.after_tc) {
+        err = launch_shared_prefix_tc(p, a->k_cache, a->v_cache, a->page_size, s);
+        if (err != B200_OK) return err;
+    }
+    FollowOn follow(p.after_tc);
     const int smem = kStages * kStageBytes + 1024;
     B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(grid), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, p));
-    FollowOn follow;
+    FollowOn merge(true);
     const int turns = div_ceil(a->tokens, a->batch) < 64 ? div_ceil(a->tokens, a->batch) : 64;
     B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(div_ceil(a->q_heads, kMergeWarps), a->batch, turns),
                                   dim3(kMergeWarps * 32), 0, s, dim3(1, 1, 1), p));

@@ -1,0 +1,609 @@
+// The prefixes of attention over a shared prefix on the tcgen05 tensor cores: groups with more query rows than a warp's tile or two
+// (attention_shared_prefix.cu has the formulas, the other parts and the kernel that joins them).
+//
+// All query rows of a group that read one KV head are one matrix, [tokens * heads per KV head, 128], in blocks of 256 rows; no
+// row of a prefix is masked.  A unit is (group, KV head, block); the K/V tiles of 128 keys of all units form one sequence that is
+// cut into equal contiguous runs, one per CTA, on the device.  Per tile
+//     S = Q K^T     128 x 128 x 128 into TMEM; a thread per row takes its 128 scores to registers
+//     P = 2^(S - m) bf16 into TMEM, the A operand of      O += P V      128 x 128 x 128, accumulated in TMEM
+// with the reference m moved (and O rescaled) only when the true maximum is 2^8 ahead of it.  Two chains of S, softmax and P V take
+// turns on the tensor core, so that one chain's softmax runs under the other's products:
+//     a block of more than 128 rows: a chain per 128 rows, both on the same tiles;
+//     a block of up to 128 rows:     both on the same rows, one on the even, one on the odd tiles of the run, their sums joined at
+//                                    its end (in TMEM both have a row in the same lane).
+// Roles: warp 0 copies K tiles, warp 2 V tiles, one thread of warp 1 issues S, one of warp 3 issues P V, warps 4-7 and 8-11 are the
+// chains' softmax.  Every role walks the same items; the rings and the chains go on across them, so the next item's tiles are under
+// way while one is finished.  Barriers are tested by parity: whoever tests one knows that the phase before it is over (the rings
+// are filled and emptied in order, and a chain's barriers alternate between its two sides).
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "shared_prefix.cuh"
+#include "tcgen05.cuh"
+#include "tensormap.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kTile = 128;                  // keys per K/V tile, rows per chain
+constexpr int kThreads = 384;
+// The first warpgroup leaves its registers to the others; 384 x 168 are launched.
+constexpr int kIssueRegs = 72, kSoftmaxRegs = 216;
+static_assert(128 * (kIssueRegs + 2 * kSoftmaxRegs) <= kThreads * 168, "");
+constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16
+constexpr uint32_t kKVOff = 4 * kAtomBytes; // behind 2 tiles of queries of 2 atoms each
+constexpr uint32_t kSlotBytes = 2 * kAtomBytes;
+constexpr int kKSlots = 2, kVSlots = 2, kSlots = kKSlots + kVSlots;   // a ring of tiles each
+constexpr uint32_t kSmemBytes = kKVOff + kSlots * kSlotBytes;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns: S (128, both chains in turn), P (64 each), O (128 each)
+constexpr float kLazyLog2 = 8.0f;
+constexpr int kMinTilesPerCta = 2;
+
+// How K and V tiles are copied ([0] K, [1] V), into 16 groups of 8 keys, each both halves of the head dimension.
+struct SharedKvMaps {
+    CUtensorMap rows[2];   // half rows of min(page, 8) keys: any slot
+    CUtensorMap page[2];   // whole rows of min(page, 128) keys from a slot that 8 divides
+    CUtensorMap tile[2];   // whole rows of 128 keys: tiles whose pages are consecutive slots
+    int whole_pages, whole_tiles;   // are the latter two there?
+    int kpc;                        // keys of a page in a tile
+};
+
+struct Item {
+    int h, rows;          // KV head, query rows of the block
+    int row0;             // its first row among the group's
+    int tok0;             // first token of the group
+    int keys, t0, t1;     // of the prefix; tiles [t0, t1)
+    int table, slot;
+};
+
+__device__ __forceinline__ uint64_t as_pair(float2 x) { return *reinterpret_cast<uint64_t*>(&x); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__global__ void __launch_bounds__(kThreads, 1)
+shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedPrefixParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full[kSlots];    // slots of K tiles, then of V tiles
+    __shared__ __align__(8) uint64_t empty[kSlots];
+    __shared__ __align__(8) uint64_t q_full;          // an item's queries are in shared memory (8 warp arrivals)
+    __shared__ __align__(8) uint64_t s_full[2];       // per chain: S is in TMEM
+    __shared__ __align__(8) uint64_t s_free[2];       // ... and has been read from there (4 warp arrivals)
+    __shared__ __align__(8) uint64_t p_full[2];       // per chain: P is in TMEM (4 warp arrivals)
+    __shared__ __align__(8) uint64_t pv_done[2];      // per chain: O += P V has completed
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
+    __shared__ int s_first[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];   // tiles and units of the groups before
+    __shared__ int2 s_warp[kThreads / 32];
+    __shared__ float2 s_ml[kTile];                    // second chain's statistics, where both have the same rows
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int G = p.group, Hkv = p.kv_heads;
+    if (threadIdx.x == 0) {
+        for (int kv = 0; kv < 2; ++kv) {
+            if (maps.whole_pages) tma_prefetch_desc(&maps.page[kv]);
+            if (maps.whole_tiles) tma_prefetch_desc(&maps.tile[kv]);
+        }
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(&q_full), 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_free[i]), 4);
+            mbar_init(smem_u32(&p_full[i]), 4);
+            mbar_init(smem_u32(&pv_done[i]), 1);
+        }
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    __syncwarp();
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_base_slot), 512);
+        tmem_relinquish();
+    }
+
+    // ---- units and tiles ----
+    shared_prefixes(p, s_bound, s_prefix);
+    {
+        auto size_of = [&](int g) {   // (tiles, units)
+            const int rows = max(shared_row(p, s_bound[g + 1]) - shared_row(p, s_bound[g]), 0) * G;
+            if (rows <= p.tc_rows || s_prefix[g] == 0) return make_int2(0, 0);
+            const int units = Hkv * ((rows + 2 * kTile - 1) / (2 * kTile));
+            return make_int2(units * ((s_prefix[g] + kTile - 1) / kTile), units);
+        };
+        const int each = (p.groups + kThreads - 1) / kThreads;
+        const int g0 = min(static_cast<int>(threadIdx.x) * each, p.groups), g1 = min(g0 + each, p.groups);
+        int2 mine = make_int2(0, 0);
+        for (int g = g0; g < g1; ++g) {
+            const int2 n = size_of(g);
+            mine.x += n.x;
+            mine.y += n.y;
+        }
+        int2 incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, incl.x, o), b = __shfl_up_sync(0xffffffffu, incl.y, o);
+            if (lane >= o) {
+                incl.x += a;
+                incl.y += b;
+            }
+        }
+        if (lane == 31) s_warp[warp] = incl;
+        __syncthreads();
+        int2 at = make_int2(incl.x - mine.x, incl.y - mine.y);
+        for (int w = 0; w < warp; ++w) {
+            at.x += s_warp[w].x;
+            at.y += s_warp[w].y;
+        }
+        for (int g = g0; g < g1; ++g) {
+            s_first[g] = at.x;
+            s_unit[g] = at.y;
+            const int2 n = size_of(g);
+            at.x += n.x;
+            at.y += n.y;
+        }
+        if (threadIdx.x == kThreads - 1) {
+            s_first[p.groups] = at.x;
+            s_unit[p.groups] = at.y;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+    const int total = s_first[p.groups];
+    const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinTilesPerCta);
+    // (as in the rows kernel: index arrays whose requests or groups overlap ask for more room than there is)
+    const bool fits = static_cast<int>(gridDim.x) + s_unit[p.groups] <= p.tc_slots;
+    if (blockIdx.x == 0) {
+        for (int g = threadIdx.x; g <= p.groups; g += kThreads) {
+            p.plan.tc_first[g] = s_first[g];
+            p.plan.tc_unit[g] = s_unit[g];
+        }
+        if (threadIdx.x == 0) {
+            p.plan.per[1] = fits ? per : 0;
+            if (!fits) atomicExch(&p.status[kStatusBadIndex], p.tokens + 1);
+        }
+    }
+    const int g_begin = fits ? min(static_cast<int>(blockIdx.x) * per, total) : 0;
+    const int g_end = fits ? min(total, g_begin + per) : 0;
+    const int ntiles = g_end - g_begin;   // of all items
+
+    // The item that starts at tile gpos < g_end of the sequence.
+    auto locate = [&](int gpos) {
+        int lo = 0, hi = p.groups;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_first[mid] <= gpos) lo = mid; else hi = mid;
+        }
+        Item it;
+        it.keys = s_prefix[lo];
+        const int tiles = (it.keys + kTile - 1) / kTile, off = gpos - s_first[lo], unit = off / tiles;
+        const int blocks = (s_unit[lo + 1] - s_unit[lo]) / Hkv;
+        it.h = unit / blocks;
+        it.row0 = (unit - it.h * blocks) * 2 * kTile;
+        it.tok0 = shared_row(p, s_bound[lo]);
+        it.rows = min((shared_row(p, s_bound[lo + 1]) - it.tok0) * G - it.row0, 2 * kTile);
+        it.t0 = off - unit * tiles;
+        it.t1 = min(tiles, it.t0 + g_end - gpos);
+        it.table = p.table_idx[min(s_bound[lo], p.batch - 1)];
+        it.slot = s_unit[lo] + unit + static_cast<int>(blockIdx.x);
+        return it;
+    };
+
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 0 || warp == 2) {
+        // ================= producers: K tiles, V tiles =================
+        const int kv = warp >> 1, kpc = maps.kpc;
+        const uint32_t ring = kv == 0 ? 0 : kKSlots, ring_end = kv == 0 ? kKSlots : kSlots;
+        uint32_t slot = ring, phase = 1;   // (the first waits are for slots that nobody has used)
+        bool failed = false;
+        for (int gpos = g_begin; gpos < g_end && !failed;) {
+            const Item it = locate(gpos);
+            gpos += it.t1 - it.t0;
+            const int32_t* pt_row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride;
+            auto copies_of = [&](int kt) { return (min(kTile, it.keys - kt * kTile) + kpc - 1) / kpc; };
+            int next[4];
+            auto fetch_slots = [&](int kt) {   // a tile ahead: the table's trip to L2 would stand between a slot's release and its copy
+                const int n = copies_of(kt);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int copy = i * 32 + lane;
+                    next[i] = copy < n ? pt_row[kt * kTile + copy * kpc] : 0;
+                }
+            };
+            fetch_slots(it.t0);
+            for (int kt = it.t0; kt < it.t1; ++kt) {
+                // A tile whose pages are consecutive slots is one copy; so is a page, unless it is smaller than a group of 8 or starts
+                // inside one.
+                const int n = copies_of(kt);
+                bool whole = it.keys - kt * kTile >= kTile && maps.whole_tiles, groups = maps.whole_pages;
+                int sl[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sl[i] = next[i];
+                    if (sl[i] < 0 || static_cast<int64_t>(sl[i]) + kpc > p.num_slots) {
+                        atomicExch(&p.status[kStatusBadIndex], sl[i] + 1);
+                        sl[i] = 0;
+                    }
+                    if ((sl[i] & 7) != 0) groups = false;
+                }
+                const int first = __shfl_sync(0xffffffffu, sl[0], 0);
+                if ((first & 7) != 0) whole = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int copy = i * 32 + lane;
+                    if (copy < n && sl[i] != first + copy * kpc) whole = false;
+                }
+                whole = __all_sync(0xffffffffu, whole);
+                groups = __all_sync(0xffffffffu, groups);
+                if (kt + 1 < it.t1) fetch_slots(kt + 1);
+                if (!__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(&empty[slot]), phase, p.status, 331))) {
+                    failed = true;
+                    break;
+                }
+                const uint32_t bar = smem_u32(&full[slot]), base = smem_base + kKVOff + slot * kSlotBytes;
+                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n * kpc) * kD * 2u);
+                __syncwarp();
+                if (whole) {
+                    if (lane == 0) tma_load_5d(base, &maps.tile[kv], 0, 0, 0, first >> 3, it.h, bar);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int copy = i * 32 + lane;
+                        if (copy >= n) continue;
+                        if (groups) {
+                            tma_load_5d(base + copy * kpc * (kD * 2), &maps.page[kv], 0, 0, 0, sl[i] >> 3, it.h, bar);
+                            continue;
+                        }
+                        for (int key = copy * kpc; key < (copy + 1) * kpc; key += 8) {
+                            const uint32_t dst = base + (key >> 3) * 2048 + (key & 7) * 128;
+                            const int from = sl[i] + key - copy * kpc;
+                            tma_load_3d(dst, &maps.rows[kv], 0, it.h, from, bar);
+                            tma_load_3d(dst + 1024, &maps.rows[kv], 64, it.h, from, bar);
+                        }
+                    }
+                }
+                if (++slot == ring_end) {
+                    slot = ring;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ================= issuer of S = Q K^T =================
+        if (elect_one()) {
+            const uint32_t idesc = idesc_bf16_128x128(false);
+            const uint64_t q_desc = kmajor_sw128_desc(smem_base);
+            const uint64_t k_desc = grouped_keys_desc(smem_base + kKVOff, 0);
+            uint32_t slot = 0, phase = 0, items = 0;
+            uint32_t uses[2] = {0, 0};   // of each chain so far
+            int last = -1, tile = 0;     // the chain of the last scores; tiles so far
+            bool failed = false;
+            auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+                if (!failed && !mbar_wait_mostly_ready(bar, parity, p.status, site)) failed = true;
+            };
+            auto scores = [&](int chain, uint64_t a, uint64_t k) {
+                // both chains use the same columns: the last scores have to have been read
+                if (last >= 0) wait(smem_u32(&s_free[last]), (uses[last] - 1) & 1u, 338);
+                if (failed) return;
+                tc_fence_after();
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    tc_mma_bf16(tmem_base + kColS, a + (((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4),
+                                k + (((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), idesc, ks > 0 ? 1u : 0u);
+                tc_commit(smem_u32(&s_full[chain]));
+                last = chain;
+                ++uses[chain];
+            };
+            for (int gpos = g_begin; gpos < g_end && !failed; ++items) {
+                const Item it = locate(gpos);
+                gpos += it.t1 - it.t0;
+                const bool two = it.rows > kTile;
+                wait(smem_u32(&q_full), items & 1u, 339);
+                for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
+                    const uint64_t k = k_desc + slot * (kSlotBytes >> 4);
+                    wait(smem_u32(&full[slot]), phase, 332);
+                    if (two) {
+                        scores(0, q_desc, k);
+                        scores(1, q_desc + (2 * kAtomBytes >> 4), k);
+                    } else if (((kt - it.t0) & 1) == 0) {
+                        scores(0, q_desc, k);
+                    } else {
+                        scores(1, q_desc, k);
+                    }
+                    if (failed) break;
+                    // (a slot that is not filled again is not handed back: the arrival could be under way when the block ends)
+                    if (tile + kKSlots < ntiles) tc_commit(smem_u32(&empty[slot]));
+                    if (++slot == kKSlots) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp == 3) {
+        // ================= issuer of O += P V =================
+        if (elect_one()) {
+            const uint32_t idesc = idesc_bf16_128x128(true);
+            const uint64_t v_desc = grouped_keys_desc(smem_base + kKVOff, 1024);
+            uint32_t slot = kKSlots, phase = 0;
+            uint32_t uses[2] = {0, 0};
+            int tile = 0;
+            bool failed = false;
+            auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+                if (!failed && !mbar_wait_mostly_ready(bar, parity, p.status, site)) failed = true;
+            };
+            auto add = [&](int chain, uint64_t v, bool first) {
+                wait(smem_u32(&p_full[chain]), uses[chain] & 1u, 333);
+                if (failed) return;
+                tc_fence_after();
+                const uint32_t prob = tmem_base + kColP + static_cast<uint32_t>(chain) * 64u;
+                const uint32_t d = tmem_base + kColO + static_cast<uint32_t>(chain) * 128u;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)   // keys ks*16 .. +15: eight packed columns
+                    tc_mma_bf16_ts(d, prob + static_cast<uint32_t>(ks * 8), v + (ks * 4096 >> 4), idesc, !first || ks > 0 ? 1u : 0u);
+                tc_commit(smem_u32(&pv_done[chain]));
+                ++uses[chain];
+            };
+            for (int gpos = g_begin; gpos < g_end && !failed;) {
+                const Item it = locate(gpos);
+                gpos += it.t1 - it.t0;
+                const bool two = it.rows > kTile;
+                for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
+                    const uint64_t v = v_desc + slot * (kSlotBytes >> 4);
+                    wait(smem_u32(&full[slot]), phase, 336);
+                    if (two) {
+                        add(0, v, kt == it.t0);
+                        add(1, v, kt == it.t0);
+                    } else if (((kt - it.t0) & 1) == 0) {
+                        add(0, v, kt == it.t0);
+                    } else {
+                        add(1, v, kt == it.t0 + 1);
+                    }
+                    if (failed) break;
+                    if (tile + kVSlots < ntiles) tc_commit(smem_u32(&empty[slot]));
+                    if (++slot == kSlots) {
+                        slot = kKSlots;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else {
+        // ================= softmax, and the rows' results =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int chain = (warp >> 2) - 1;
+        const int qtr = warp & 3;                 // TMEM lane quarter this warp may read
+        const int r = qtr * 32 + lane;            // row = TMEM lane
+        const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(qtr * 32) << 16);
+        const uint32_t s_addr = lane_addr + kColS;
+        const uint32_t p_addr = lane_addr + kColP + static_cast<uint32_t>(chain) * 64u;
+        const uint32_t o_addr = lane_addr + kColO + static_cast<uint32_t>(chain) * 128u;
+        const float sc = p.scale_log2;
+        uint32_t uses = 0;
+        int tiles_before = 0;
+        bool failed = false;
+        for (int gpos = g_begin; gpos < g_end;) {
+            const Item it = locate(gpos);
+            gpos += it.t1 - it.t0;
+            const bool two = it.rows > kTile;
+            // ---- queries into shared memory, swizzled K-major; rows behind the block's last are zero.  Half a warp per row. ----
+            {
+                const int sw = warp - 4;
+                const int mine = two ? 16 : 8;   // pairs of rows of this warp
+                const int at0 = two ? sw * 32 : sw * 16;
+                uint4 v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int row = at0 + i * 2 + (lane >> 4);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (i < mine && row < it.rows) {
+                        const int fl = it.row0 + row, tok = fl / G, head = it.h * G + fl - tok * G;
+                        v[i] = reinterpret_cast<const uint4*>(p.q + (it.tok0 + tok) * p.q_st + head * p.q_sh)[lane & 15];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (i >= mine) continue;
+                    const int row = at0 + i * 2 + (lane >> 4);
+                    const uint32_t a = swz128(smem_base + ((row >> 7) * 2 + (lane >> 3 & 1)) * kAtomBytes + (row & 127) * 128, lane & 7);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
+                                 : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&q_full));
+            }
+            float m_ref = -INFINITY, l_run = 0.f;
+            const int step = two ? 1 : 2;
+            bool any = false;   // has this chain had a tile of the item?
+            for (int kt = it.t0 + (two ? 0 : chain); kt < it.t1; kt += step, ++uses) {
+                if (!failed && !mbar_wait_mostly_ready(smem_u32(&s_full[chain]), uses & 1u, p.status, 334)) failed = true;
+                tc_fence_after();
+                const int valid = it.keys - kt * kTile;   // keys of the tile that belong to the prefix
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_free[chain]));
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (valid < kTile) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (c * 32 + i >= valid) s[c][i] = 0xff800000u;   // -inf
+                            m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(s[c][i]));
+                        }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                }
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                // this chain's product before has read P and has added to O
+                if (any && !failed && !mbar_wait_mostly_ready(smem_u32(&pv_done[chain]), (uses - 1) & 1u, p.status, 337)) failed = true;
+                tc_fence_after();
+                float alpha = 1.f;
+                if (mx != -INFINITY && (m_ref == -INFINITY || (mx - m_ref) * sc > kLazyLog2)) {
+                    if (m_ref != -INFINITY) alpha = ex2((m_ref - mx) * sc);
+                    m_ref = mx;
+                }
+                if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                    l_run *= alpha;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t ov[16];
+                        tmem_ld_32x32b_x16(o_addr + c * 16, ov);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                        tmem_st_32x32b_x16(o_addr + c * 16, ov);
+                    }
+                }
+                const float mb = m_ref == -INFINITY ? INFINITY : m_ref * sc;
+                float2 sum = make_float2(0.f, 0.f);
+                const float2 sc2 = make_float2(sc, sc), mb2 = make_float2(-mb, -mb);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 e = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, mb2);
+                        const float2 pr = make_float2(ex2(e.x), ex2(e.y));
+                        sum = add2(sum, pr);
+                        packed[i >> 1] = pack_bf16(pr.x, pr.y);
+                    }
+                    tmem_st_32x32b_x16(p_addr + c * 16, packed);
+                }
+                if (valid < kTile) {
+                    // Values behind the prefix (of the page, or what the slot held before) must be numbers: their weights are 0.
+                    const int j = tiles_before + kt - it.t0;
+                    const uint32_t slot = kKSlots + static_cast<uint32_t>(j % kVSlots);
+                    if (!failed && !mbar_wait_mostly_ready(smem_u32(&full[slot]), static_cast<uint32_t>(j / kVSlots) & 1u, p.status, 340))
+                        failed = true;
+                    const uint32_t base = smem_base + kKVOff + slot * kSlotBytes;
+                    for (int i = r; i < (kTile - valid) * 16; i += kTile) {
+                        const int key = valid + (i >> 4), at = i & 15;
+                        const uint32_t a = base + (key >> 3) * 2048 + (at >> 3) * 1024 + (key & 7) * 128 + (at & 7) * 16;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
+                    }
+                    fence_proxy_async_smem();
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[chain]));
+                l_run += sum.x + sum.y;
+                any = true;
+            }
+            tiles_before += it.t1 - it.t0;
+            if (any && !failed && !mbar_wait_mostly_ready(smem_u32(&pv_done[chain]), (uses - 1) & 1u, p.status, 335)) failed = true;
+            __syncwarp();
+            tc_fence_after();
+            // ---- the rows' sums and statistics (maximum in the exponent's units) ----
+            float m = m_ref == -INFINITY ? -INFINITY : m_ref * sc, l = l_run, mine = 1.f, other = 0.f;
+            bool join = false;
+            if (!two) {
+                if (chain == 1) s_ml[r] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
+                tc_fence_before();
+                softmax_bar();   // the second chain's sums are complete and its statistics are there
+                tc_fence_after();
+                join = chain == 0 && it.t1 - it.t0 > 1;
+                if (join) {
+                    const float2 b = s_ml[r];
+                    const float top = fmaxf(m, b.x), ref = top == -INFINITY ? 0.f : top;
+                    mine = ex2(m - ref);
+                    other = ex2(b.x - ref);
+                    l = l * mine + b.y * other;
+                    m = top;
+                }
+            }
+            if (two || chain == 0) {
+                const int row = (two ? chain * kTile : 0) + r;
+                const bool store = row < it.rows;
+                const int64_t at = p.tc_base + static_cast<int64_t>(it.slot) * (2 * kTile) + row;
+                float* dst = p.ws_o + at * kD;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t a[16], b[16];
+                    tmem_ld_32x32b_x16(o_addr + c * 16, a);
+                    if (join) tmem_ld_32x32b_x16(o_addr + 128 + c * 16, b);
+                    tmem_ld_wait();
+                    if (join) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            a[i] = __float_as_uint(__uint_as_float(a[i]) * mine + __uint_as_float(b[i]) * other);
+                    }
+                    if (store) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8)   // a sector per store
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * 16 + i), "r"(a[i]), "r"(a[i + 1]),
+                                         "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+                                         : "memory");
+                    }
+                }
+                if (store) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m, failed ? 0.f : l);
+            }
+            tc_fence_before();
+            softmax_bar();   // the item's queries and sums have been read
+            tc_fence_after();
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+}  // namespace
+
+int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream) {
+    SharedKvMaps maps = {};
+    maps.kpc = page_size < kTile ? page_size : kTile;
+    maps.whole_pages = maps.kpc >= 8 && p.num_slots >= 8 ? 1 : 0;
+    maps.whole_tiles = maps.kpc < kTile && p.num_slots >= kTile ? 1 : 0;
+    for (int kv = 0; kv < 2; ++kv) {
+        const void* cache = kv == 0 ? k_cache : v_cache;
+        int err = make_kv_tile_tmap(&maps.rows[kv], cache, p.num_slots, p.kv_heads, maps.kpc < 8 ? maps.kpc : 8);
+        if (err == B200_OK && maps.whole_pages) err = make_kv_groups_tmap(&maps.page[kv], cache, p.num_slots, p.kv_heads, maps.kpc);
+        if (err == B200_OK && maps.whole_tiles) err = make_kv_groups_tmap(&maps.tile[kv], cache, p.num_slots, p.kv_heads, kTile);
+        if (err != B200_OK) return err;
+    }
+    const int smem = kSmemBytes + 1024;
+    B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    B200_CHECK_CUDA(launch_kernel(shared_prefix_tc_kernel, dim3(sm_count()), dim3(kThreads), smem, stream, dim3(1, 1, 1), maps, p));
+    return B200_OK;
+}
+
+}  // namespace b200

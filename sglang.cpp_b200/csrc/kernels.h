@@ -359,6 +359,8 @@ struct AttentionWindow {
 
 // A pool [slots, kv heads, 128] in boxes of 64 elements of one head of kpc slots (attention_prefill_tc2.cu).
 int make_kv_tile_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, int kv_heads, int kpc);
+// Whole rows of one head of `keys` neighbouring slots, in groups of 8 (the first slot a multiple of 8).
+int make_kv_groups_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, int kv_heads, int keys);
 int64_t decode_workspace_bytes(int max_batch, int q_heads, int kv_heads);
 int make_kv_tmap(CUtensorMap* out, const void* cache, int64_t num_slots, int kv_heads, int page_size);
 int launch_attention_decode(void* out, const void* q, int64_t q_st, int64_t q_sh,

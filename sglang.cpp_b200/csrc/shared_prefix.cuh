@@ -10,11 +10,12 @@ constexpr int kSharedMaxBatch = 1024;
 // What a call leaves in the workspace for the kernel that joins the parts.  Units are the groups' prefixes (0 .. groups), then
 // the requests' own keys; `stage` and `tile` count the stages and row tiles of the units before.
 struct SharedPlan {
-    int* per;        // [0] stages per CTA of the rows kernel
+    int* per;        // stages per CTA of the rows kernel, tiles per CTA of the tensor-core kernel
     int* stage;      // [groups + batch + 1]
     int* tile;       // [groups + batch + 1]
     int* prefix;     // [groups] keys that are read once for the group
     int* group_of;   // [batch], -1: none
+    int *tc_first, *tc_unit;   // [groups + 1] tiles and units of the groups before, in the tensor-core kernel
 };
 
 struct SharedPrefixParams {
@@ -31,6 +32,10 @@ struct SharedPrefixParams {
     float scale_log2;
     float *ws_ml, *ws_o;            // rows kernel: [max_slots, key groups, kv_heads, row tile] (maximum, sum), and x 128
     int max_slots;
+    int tc_rows;                    // groups of more rows (tokens x group) than this: their prefixes by the tensor-core kernel
+    int tc_slots;
+    int64_t tc_base;                // its partial rows in ws_ml and ws_o: [tc_slots, 256] from here
+    bool after_tc;                  // the rows kernel follows the tensor-core kernel
     SharedPlan plan;
     int* status;
 };
@@ -70,5 +75,7 @@ __device__ __forceinline__ void shared_prefixes(const SharedPrefixParams& p, int
     __syncthreads();
 }
 #endif
+
+int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream);
 
 }  // namespace b200

@@ -25,7 +25,8 @@ def _attention(pkg, **change):
     (dict(q_stride_head=129), "strides"), (dict(num_slots=0), "num_slots"), (dict(num_slots=1 << 31), "num_slots"),
     (dict(page_table_stride=0), "page_table_stride"), (dict(tokens=1 << 27), "too many"), (dict(out=None), "NULL"), (dict(q=None), "NULL"),
     (dict(group_indptr=None), "NULL"), (dict(prefix_lens=None), "NULL"), (dict(workspace=None), "NULL"), (dict(qo_indptr=None), "NULL"),
-    (dict(out=260), "aligned"), (dict(q=258), "aligned"),
+    (dict(sm_scale=0.0), "sm_scale"), (dict(sm_scale=-1.0), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"),
+    (dict(sm_scale=float("inf")), "sm_scale"), (dict(out=260), "aligned"), (dict(q=258), "aligned"),
 ])
 def test_attention_refusals(pkg, change, text):
     rc, said = _attention(pkg, **change)
