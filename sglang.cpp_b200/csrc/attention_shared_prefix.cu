@@ -429,11 +429,13 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     const int own_first = p.plan.stage[p.groups + b], own_stages = p.plan.stage[p.groups + b + 1] - own_first;
     const int own_tile = p.plan.tile[p.groups + b], own_tiles = p.plan.tile[p.groups + b + 1] - own_tile;
     int pre_first = 0, pre_stages = 0, pre_tile = 0, pre_tiles = 0, pre_row = 0;
-    int tc_first = 0, tc_unit = 0, tc_units = 0, tc_tiles = 0;
+    int tc_first = 0, tc_unit = 0, tc_units = 0, tc_tiles = 0, tc_cta = 0;
+    const bool chunked = p.after_tc && p.plan.per[2] != 0;
     if (grp >= 0) {
         if (p.after_tc) {
             tc_first = p.plan.tc_first[grp];
             tc_unit = p.plan.tc_unit[grp];
+            tc_cta = p.plan.tc_cta[grp];
             tc_units = p.plan.tc_unit[grp + 1] - tc_unit;
             tc_tiles = tc_units > 0 ? (p.plan.tc_first[grp + 1] - tc_first) / tc_units : 0;
         }
@@ -456,11 +458,14 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
         const int hh = head - h * p.group;
         Parts pre = parts_of(pre_first, pre_stages, pre_tile, pre_tiles, (tok - pre_row) * p.group + hh);
         const Parts own = parts_of(own_first, own_stages, own_tile, own_tiles, (tok - row0) * p.group + hh);
-        const int r = (tok - pre_row) * p.group + hh, block = r / 256;
-        if (tc_units > 0 && r >= 0 && block < tc_units / p.kv_heads) {
-            const int unit = h * (tc_units / p.kv_heads) + block, from = tc_first + unit * tc_tiles, c0 = from / tc_per;
-            pre.count = (from + tc_tiles - 1) / tc_per - c0 + 1;
-            pre.first = p.tc_base + static_cast<int64_t>(tc_unit + unit + c0) * 256 + (r & 255);
+        const int t = tok - pre_row, half = 128 / p.group, block = t / (2 * half);   // tokens of a chain
+        if (tc_units > 0 && t >= 0 && block < tc_units / p.kv_heads) {
+            const int unit = h * (tc_units / p.kv_heads) + block, from = tc_first + unit * tc_tiles;
+            const int in_block = t - block * 2 * half, chain = in_block >= half ? 1 : 0;
+            const int chunks = (tc_tiles + tc_per - 1) / tc_per;
+            const int c0 = chunked ? tc_cta + unit * chunks : from / tc_per;
+            pre.count = chunked ? chunks : (from + tc_tiles - 1) / tc_per - c0 + 1;
+            pre.first = p.tc_base + static_cast<int64_t>(tc_unit + unit + c0) * 256 + chain * 128 + (in_block - chain * half) * p.group + hh;
             pre.step = 256;
         }
         const int n = pre.count + own.count;
@@ -511,10 +516,10 @@ SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_
     x.rows = x.slots * kg * kv_heads * RT;
     // units of the tensor-core kernel: the same of groups that have more than kTcRows rows
     const int64_t tc_groups = groups < rows / (kTcRows + 1) ? groups : rows / (kTcRows + 1);
-    x.tc_slots = rows > kTcRows ? sm_count() + kv_heads * (rows / 256 + tc_groups) : 0;
+    x.tc_slots = rows > kTcRows ? sm_count() + kv_heads * (tokens / (2 * (128 / (q_heads / kv_heads))) + tc_groups) : 0;
     const int64_t part_rows = x.rows + x.tc_slots * 256;
     x.plan = 0;
-    x.ml = round256((4 + 2 * (groups + batch + 1) + groups + batch + 2 * (groups + 1)) * 4);
+    x.ml = round256((4 + 2 * (groups + batch + 1) + groups + batch + 3 * (groups + 1)) * 4);
     x.o = x.ml + round256(part_rows * 8);
     x.bytes = x.o + part_rows * kD * 4;
     return x;
@@ -609,8 +614,10 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.max_slots = static_cast<int>(x.slots);
     p.plan.tc_first = p.plan.group_of + a->batch;
     p.plan.tc_unit = p.plan.tc_first + a->groups + 1;
-    // Whole rows of queries are copied 16 bytes at a time there.
-    const bool aligned = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0;
+    p.plan.tc_cta = p.plan.tc_unit + a->groups + 1;
+    // Queries are copied by tensor maps there.
+    const bool aligned = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0 &&
+                         a->q_stride_token > 0 && a->q_stride_head > 0;
     p.tc_rows = aligned ? kTcRows : 0x7fffffff;
     p.tc_slots = static_cast<int>(x.tc_slots);
     p.tc_base = x.rows;

@@ -1,14 +1,16 @@
 // The prefixes of attention over a shared prefix on the tcgen05 tensor cores: groups with more query rows than a warp's tile or two
 // (attention_shared_prefix.cu has the formulas, the other parts and the kernel that joins them).
 //
-// All query rows of a group that read one KV head are one matrix, [tokens * heads per KV head, 128], in blocks of 256 rows; no
-// row of a prefix is masked.  A unit is (group, KV head, block); the K/V tiles of 128 keys of all units form one sequence that is
-// cut into equal contiguous runs, one per CTA, on the device.  Per tile
+// All query rows of a group that read one KV head are one matrix, [tokens * heads per KV head, 128], in blocks of up to 256 rows; no
+// row of a prefix is masked.  A unit is (group, KV head, block).  A unit's K/V tiles of 128 keys are cut into equal chunks, a CTA
+// each, with chunks as short as the number of CTAs allows; where there are more units than CTAs, the tiles of all units form one
+// sequence that is cut into equal contiguous runs.  (Runs throughout: one CTA in ten or so crosses from unit to unit, which costs it
+// 5 to 14 us of queries, first scores, last products and results, and all others wait for it.)  Per tile
 //     S = Q K^T     128 x 128 x 128 into TMEM; a thread per row takes its 128 scores to registers
 //     P = 2^(S - m) bf16 into TMEM, the A operand of      O += P V      128 x 128 x 128, accumulated in TMEM
 // with the reference m moved (and O rescaled) only when the true maximum is 2^8 ahead of it.  Two chains of S, softmax and P V take
 // turns on the tensor core, so that one chain's softmax runs under the other's products:
-//     a block of more than 128 rows: a chain per 128 rows, both on the same tiles;
+//     a block of more rows than a chain's 128: a chain per half, both on the same tiles;
 //     a block of up to 128 rows:     both on the same rows, one on the even, one on the odd tiles of the run, their sums joined at
 //                                    its end (in TMEM both have a row in the same lane).
 // Roles: warp 0 copies K tiles, warp 2 V tiles, one thread of warp 1 issues S, one of warp 3 issues P V, warps 4-7 and 8-11 are the
@@ -43,6 +45,7 @@ constexpr int kMinTilesPerCta = 2;
 
 // How K and V tiles are copied ([0] K, [1] V), into 16 groups of 8 keys, each both halves of the head dimension.
 struct SharedKvMaps {
+    CUtensorMap q;         // half rows of a chain's tokens, all heads of a KV head
     CUtensorMap rows[2];   // half rows of min(page, 8) keys: any slot
     CUtensorMap page[2];   // whole rows of min(page, 128) keys from a slot that 8 divides
     CUtensorMap tile[2];   // whole rows of 128 keys: tiles whose pages are consecutive slots
@@ -51,9 +54,8 @@ struct SharedKvMaps {
 };
 
 struct Item {
-    int h, rows;          // KV head, query rows of the block
-    int row0;             // its first row among the group's
-    int tok0;             // first token of the group
+    int h;                // KV head
+    int tok0, ntok;       // query tokens of the block
     int keys, t0, t1;     // of the prefix; tiles [t0, t1)
     int table, slot;
 };
@@ -86,7 +88,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full[kSlots];    // slots of K tiles, then of V tiles
     __shared__ __align__(8) uint64_t empty[kSlots];
-    __shared__ __align__(8) uint64_t q_full;          // an item's queries are in shared memory (8 warp arrivals)
+    __shared__ __align__(8) uint64_t q_full, q_empty; // an item's queries are in shared memory, have been multiplied
     __shared__ __align__(8) uint64_t s_full[2];       // per chain: S is in TMEM
     __shared__ __align__(8) uint64_t s_free[2];       // ... and has been read from there (4 warp arrivals)
     __shared__ __align__(8) uint64_t p_full[2];       // per chain: P is in TMEM (4 warp arrivals)
@@ -94,13 +96,16 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
     __shared__ int s_first[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];   // tiles and units of the groups before
-    __shared__ int2 s_warp[kThreads / 32];
+    __shared__ int2 s_warp[kThreads / 32], s_run;
+    __shared__ int s_chunks[kThreads / 32];
     __shared__ float2 s_ml[kTile];                    // second chain's statistics, where both have the same rows
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int G = p.group, Hkv = p.kv_heads;
+    const int QB = kTile / G;   // query tokens of a chain
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&maps.q);
         for (int kv = 0; kv < 2; ++kv) {
             if (maps.whole_pages) tma_prefetch_desc(&maps.page[kv]);
             if (maps.whole_tiles) tma_prefetch_desc(&maps.tile[kv]);
@@ -109,7 +114,8 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
-        mbar_init(smem_u32(&q_full), 8);
+        mbar_init(smem_u32(&q_full), 1);
+        mbar_init(smem_u32(&q_empty), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&s_full[i]), 1);
             mbar_init(smem_u32(&s_free[i]), 4);
@@ -131,9 +137,9 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     shared_prefixes(p, s_bound, s_prefix);
     {
         auto size_of = [&](int g) {   // (tiles, units)
-            const int rows = max(shared_row(p, s_bound[g + 1]) - shared_row(p, s_bound[g]), 0) * G;
-            if (rows <= p.tc_rows || s_prefix[g] == 0) return make_int2(0, 0);
-            const int units = Hkv * ((rows + 2 * kTile - 1) / (2 * kTile));
+            const int ntok = max(shared_row(p, s_bound[g + 1]) - shared_row(p, s_bound[g]), 0);
+            if (ntok * G <= p.tc_rows || s_prefix[g] == 0) return make_int2(0, 0);
+            const int units = Hkv * ((ntok + 2 * QB - 1) / (2 * QB));
             return make_int2(units * ((s_prefix[g] + kTile - 1) / kTile), units);
         };
         const int each = (p.groups + kThreads - 1) / kThreads;
@@ -176,10 +182,60 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_slot;
-    const int total = s_first[p.groups];
-    const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinTilesPerCta);
+    const int total = s_first[p.groups], units = s_unit[p.groups], ctas = static_cast<int>(gridDim.x);
     // (as in the rows kernel: index arrays whose requests or groups overlap ask for more room than there is)
-    const bool fits = static_cast<int>(gridDim.x) + s_unit[p.groups] <= p.tc_slots;
+    const bool fits = ctas + units <= p.tc_slots;
+    // Tiles per chunk: of a dozen candidates, from an equal share for every CTA to one that surely needs no more CTAs than there are,
+    // the smallest that does not (0: more units than half of the CTAs, equal runs).
+    int per = max((total + ctas - 1) / ctas, kMinTilesPerCta);
+    const bool chunked = units > 0 && 2 * units <= ctas;
+    if (chunked) {
+        const int sure = max((total + ctas - units - 1) / (ctas - units), per);
+        const int steps = kThreads / 32 - 1;
+        const int candidate = per + static_cast<int>(static_cast<int64_t>(sure - per) * warp / steps);
+        int n = 0;
+        for (int g = lane; g < p.groups; g += 32) {
+            const int mine = s_unit[g + 1] - s_unit[g];
+            if (mine > 0) n += mine * (((s_prefix[g] + kTile - 1) / kTile + candidate - 1) / candidate);
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) s_chunks[warp] = n;
+        __syncthreads();
+        int w = 0;
+        while (w < steps && s_chunks[w] > ctas) ++w;
+        per += static_cast<int>(static_cast<int64_t>(sure - per) * w / steps);
+    }
+    // This CTA's tiles, and for the kernel that joins the parts: the CTA of each group's first chunk.
+    if (warp == 0) {
+        int2 run = make_int2(0, 0);
+        int before = 0;
+        for (int base = 0; chunked && base < p.groups; base += 32) {
+            const int g = base + lane;
+            const int mine = g < p.groups ? s_unit[g + 1] - s_unit[g] : 0;
+            const int tiles = mine > 0 ? (s_prefix[g] + kTile - 1) / kTile : 0, chunks = (tiles + per - 1) / per;
+            int incl = mine * chunks;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            const int at = static_cast<int>(blockIdx.x) - (before + incl - mine * chunks);
+            if (mine > 0 && at >= 0 && at < mine * chunks) {
+                const int unit = at / chunks, from = (at - unit * chunks) * per;
+                run.x = s_first[g] + unit * tiles + from;
+                run.y = s_first[g] + unit * tiles + min(from + per, tiles);
+            }
+            if (blockIdx.x == 0 && g < p.groups) p.plan.tc_cta[g] = before + incl - mine * chunks;
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        run.x = __reduce_max_sync(0xffffffffu, run.x);   // (one lane has found it, or none)
+        run.y = __reduce_max_sync(0xffffffffu, run.y);
+        if (!chunked) {
+            run.x = min(static_cast<int>(blockIdx.x) * per, total);
+            run.y = min(total, run.x + per);
+        }
+        if (lane == 0) s_run = fits ? run : make_int2(0, 0);
+    }
     if (blockIdx.x == 0) {
         for (int g = threadIdx.x; g <= p.groups; g += kThreads) {
             p.plan.tc_first[g] = s_first[g];
@@ -187,11 +243,12 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         }
         if (threadIdx.x == 0) {
             p.plan.per[1] = fits ? per : 0;
+            p.plan.per[2] = chunked ? 1 : 0;
             if (!fits) atomicExch(&p.status[kStatusBadIndex], p.tokens + 1);
         }
     }
-    const int g_begin = fits ? min(static_cast<int>(blockIdx.x) * per, total) : 0;
-    const int g_end = fits ? min(total, g_begin + per) : 0;
+    __syncthreads();
+    const int g_begin = s_run.x, g_end = s_run.y;
     const int ntiles = g_end - g_begin;   // of all items
 
     // The item that starts at tile gpos < g_end of the sequence.
@@ -206,9 +263,8 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         const int tiles = (it.keys + kTile - 1) / kTile, off = gpos - s_first[lo], unit = off / tiles;
         const int blocks = (s_unit[lo + 1] - s_unit[lo]) / Hkv;
         it.h = unit / blocks;
-        it.row0 = (unit - it.h * blocks) * 2 * kTile;
-        it.tok0 = shared_row(p, s_bound[lo]);
-        it.rows = min((shared_row(p, s_bound[lo + 1]) - it.tok0) * G - it.row0, 2 * kTile);
+        it.tok0 = shared_row(p, s_bound[lo]) + (unit - it.h * blocks) * 2 * QB;
+        it.ntok = min(shared_row(p, s_bound[lo + 1]) - it.tok0, 2 * QB);
         it.t0 = off - unit * tiles;
         it.t1 = min(tiles, it.t0 + g_end - gpos);
         it.table = p.table_idx[min(s_bound[lo], p.batch - 1)];
@@ -221,6 +277,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         // ================= producers: K tiles, V tiles =================
         const int kv = warp >> 1, kpc = maps.kpc;
         const uint32_t ring = kv == 0 ? 0 : kKSlots, ring_end = kv == 0 ? kKSlots : kSlots;
+        uint32_t items = 0;
         uint32_t slot = ring, phase = 1;   // (the first waits are for slots that nobody has used)
         bool failed = false;
         for (int gpos = g_begin; gpos < g_end && !failed;) {
@@ -238,6 +295,19 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 }
             };
             fetch_slots(it.t0);
+            if (kv == 0) {   // the queries: rows (token, head) of each chain, in two halves
+                if (items > 0 && !__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(&q_empty), (items - 1) & 1u, p.status, 341))) {
+                    failed = true;
+                    break;
+                }
+                const int chains = it.ntok > QB ? 2 : 1;
+                const uint32_t bar = smem_u32(&q_full);
+                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(chains * QB * G) * kD * 2u);
+                __syncwarp();
+                if (lane < 2 * chains)
+                    tma_load_3d(smem_base + lane * kAtomBytes, &maps.q, (lane & 1) * 64, it.h * G, it.tok0 + (lane >> 1) * QB, bar);
+                ++items;
+            }
             for (int kt = it.t0; kt < it.t1; ++kt) {
                 // A tile whose pages are consecutive slots is one copy; so is a page, unless it is smaller than a group of 8 or starts
                 // inside one.
@@ -324,7 +394,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             for (int gpos = g_begin; gpos < g_end && !failed; ++items) {
                 const Item it = locate(gpos);
                 gpos += it.t1 - it.t0;
-                const bool two = it.rows > kTile;
+                const bool two = it.ntok > QB;
                 wait(smem_u32(&q_full), items & 1u, 339);
                 for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
                     const uint64_t k = k_desc + slot * (kSlotBytes >> 4);
@@ -345,6 +415,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                         phase ^= 1;
                     }
                 }
+                if (!failed && gpos < g_end) tc_commit(smem_u32(&q_empty));
             }
         }
     } else if (warp == 3) {
@@ -374,7 +445,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             for (int gpos = g_begin; gpos < g_end && !failed;) {
                 const Item it = locate(gpos);
                 gpos += it.t1 - it.t0;
-                const bool two = it.rows > kTile;
+                const bool two = it.ntok > QB;
                 for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
                     const uint64_t v = v_desc + slot * (kSlotBytes >> 4);
                     wait(smem_u32(&full[slot]), phase, 336);
@@ -411,40 +482,18 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         bool failed = false;
         for (int gpos = g_begin; gpos < g_end;) {
             const Item it = locate(gpos);
+            const int gpos0 = gpos;
             gpos += it.t1 - it.t0;
-            const bool two = it.rows > kTile;
-            // ---- queries into shared memory, swizzled K-major; rows behind the block's last are zero.  Half a warp per row. ----
-            {
-                const int sw = warp - 4;
-                const int mine = two ? 16 : 8;   // pairs of rows of this warp
-                const int at0 = two ? sw * 32 : sw * 16;
-                uint4 v[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int row = at0 + i * 2 + (lane >> 4);
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (i < mine && row < it.rows) {
-                        const int fl = it.row0 + row, tok = fl / G, head = it.h * G + fl - tok * G;
-                        v[i] = reinterpret_cast<const uint4*>(p.q + (it.tok0 + tok) * p.q_st + head * p.q_sh)[lane & 15];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (i >= mine) continue;
-                    const int row = at0 + i * 2 + (lane >> 4);
-                    const uint32_t a = swz128(smem_base + ((row >> 7) * 2 + (lane >> 3 & 1)) * kAtomBytes + (row & 127) * 128, lane & 7);
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
-                                 : "memory");
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&q_full));
-            }
+            const bool two = it.ntok > QB;
             float m_ref = -INFINITY, l_run = 0.f;
             const int step = two ? 1 : 2;
             bool any = false;   // has this chain had a tile of the item?
-            for (int kt = it.t0 + (two ? 0 : chain); kt < it.t1; kt += step, ++uses) {
-                if (!failed && !mbar_wait_mostly_ready(smem_u32(&s_full[chain]), uses & 1u, p.status, 334)) failed = true;
+            const int kt0 = it.t0 + (two ? 0 : chain);
+            // (The first round of all is made on whatever TMEM holds and undone, while the first copies are under way: it brings the
+            // loop's instructions, which the first tile waited 4 us for otherwise.)
+            for (int kt = gpos0 == g_begin ? kt0 - step : kt0; kt < it.t1; kt += step) {
+                const bool real = kt >= kt0;
+                if (real && !failed && !mbar_wait_mostly_ready(smem_u32(&s_full[chain]), uses & 1u, p.status, 334)) failed = true;
                 tc_fence_after();
                 const int valid = it.keys - kt * kTile;   // keys of the tile that belong to the prefix
                 uint32_t s[4][32];
@@ -453,7 +502,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&s_free[chain]));
+                if (real && lane == 0) mbar_arrive(smem_u32(&s_free[chain]));
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 if (valid < kTile) {
 #pragma unroll
@@ -506,7 +555,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                     }
                     tmem_st_32x32b_x16(p_addr + c * 16, packed);
                 }
-                if (valid < kTile) {
+                if (real && valid < kTile) {
                     // Values behind the prefix (of the page, or what the slot held before) must be numbers: their weights are 0.
                     const int j = tiles_before + kt - it.t0;
                     const uint32_t slot = kKSlots + static_cast<uint32_t>(j % kVSlots);
@@ -523,9 +572,15 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
+                if (!real) {
+                    m_ref = -INFINITY;
+                    l_run = 0.f;
+                    continue;
+                }
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[chain]));
                 l_run += sum.x + sum.y;
                 any = true;
+                ++uses;
             }
             tiles_before += it.t1 - it.t0;
             if (any && !failed && !mbar_wait_mostly_ready(smem_u32(&pv_done[chain]), (uses - 1) & 1u, p.status, 335)) failed = true;
@@ -550,11 +605,11 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 }
             }
             if (two || chain == 0) {
-                const int row = (two ? chain * kTile : 0) + r;
-                const bool store = row < it.rows;
-                const int64_t at = p.tc_base + static_cast<int64_t>(it.slot) * (2 * kTile) + row;
+                const int tok = r / G + (two ? chain * QB : 0);
+                const bool store = r < QB * G && tok < it.ntok;
+                const int64_t at = p.tc_base + static_cast<int64_t>(it.slot) * (2 * kTile) + (two ? chain * kTile : 0) + r;
                 float* dst = p.ws_o + at * kD;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 8; ++c) {
                     uint32_t a[16], b[16];
                     tmem_ld_32x32b_x16(o_addr + c * 16, a);
@@ -588,14 +643,41 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
 
 }  // namespace
 
+namespace {
+
+// Half rows (64 elements) of the queries [tokens][heads][128]: a KV head's heads of as many tokens as a chain has.
+int make_query_tmap(CUtensorMap* out, const SharedPrefixParams& p) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) {
+        set_last_error("cuTensorMapEncodeTiled is not available from this driver");
+        return B200_ERR_CUDA;
+    }
+    const cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(p.q_heads), static_cast<cuuint64_t>(p.tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.q_sh) * 2, static_cast<cuuint64_t>(p.q_st) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(kTile / p.group)};
+    const cuuint32_t es[3] = {1, 1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(p.q), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled (queries) failed with CUresult %d", static_cast<int>(r));
+        return B200_ERR_CUDA;
+    }
+    return B200_OK;
+}
+
+}  // namespace
+
 int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream) {
     SharedKvMaps maps = {};
+    int err = make_query_tmap(&maps.q, p);
+    if (err != B200_OK) return err;
     maps.kpc = page_size < kTile ? page_size : kTile;
     maps.whole_pages = maps.kpc >= 8 && p.num_slots >= 8 ? 1 : 0;
     maps.whole_tiles = maps.kpc < kTile && p.num_slots >= kTile ? 1 : 0;
     for (int kv = 0; kv < 2; ++kv) {
         const void* cache = kv == 0 ? k_cache : v_cache;
-        int err = make_kv_tile_tmap(&maps.rows[kv], cache, p.num_slots, p.kv_heads, maps.kpc < 8 ? maps.kpc : 8);
+        err = make_kv_tile_tmap(&maps.rows[kv], cache, p.num_slots, p.kv_heads, maps.kpc < 8 ? maps.kpc : 8);
         if (err == B200_OK && maps.whole_pages) err = make_kv_groups_tmap(&maps.page[kv], cache, p.num_slots, p.kv_heads, maps.kpc);
         if (err == B200_OK && maps.whole_tiles) err = make_kv_groups_tmap(&maps.tile[kv], cache, p.num_slots, p.kv_heads, kTile);
         if (err != B200_OK) return err;

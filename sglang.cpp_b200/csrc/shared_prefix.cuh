@@ -10,12 +10,13 @@ constexpr int kSharedMaxBatch = 1024;
 // What a call leaves in the workspace for the kernel that joins the parts.  Units are the groups' prefixes (0 .. groups), then
 // the requests' own keys; `stage` and `tile` count the stages and row tiles of the units before.
 struct SharedPlan {
-    int* per;        // stages per CTA of the rows kernel, tiles per CTA of the tensor-core kernel
+    int* per;        // stages per CTA of the rows kernel; tiles per CTA of the tensor-core kernel, and whether in chunks
     int* stage;      // [groups + batch + 1]
     int* tile;       // [groups + batch + 1]
     int* prefix;     // [groups] keys that are read once for the group
     int* group_of;   // [batch], -1: none
     int *tc_first, *tc_unit;   // [groups + 1] tiles and units of the groups before, in the tensor-core kernel
+    int* tc_cta;     // [groups] the CTA of a group's first chunk there
 };
 
 struct SharedPrefixParams {
