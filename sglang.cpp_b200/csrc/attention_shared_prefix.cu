@@ -6,11 +6,10 @@
 // and the parts of a row join exactly: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  Everything up to the output is fp32 but
 // the probabilities, which are rounded to bf16 as the other attention kernels here do (their products run on the tensor cores).
 //
-// Rows kernel (bound by HBM): a unit is a group's prefix or what a request has of its own; its rows are (token, head of the KV
-// head's group) pairs, in tiles of 16.  The stages of all tiles of all units form one sequence that is cut into equal
-// contiguous runs, one per CTA, from the lengths on the device: no host plan, so a captured call follows new lengths.  A stage is
-// 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages; eight warps each own 16 keys of one KV head in it
-// and multiply with mma.sync.
+// Rows kernel (bound by HBM): an item is a run of stages of a group's prefix or of what a request has of its own, for a tile of 16 of
+// its rows, (token, head of the KV head's group) pairs; the stages of all tiles of all units are dealt to the CTAs in contiguous runs
+// (shared_prefix_plan.cu).  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages, a warp for each
+// half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with mma.sync.
 #include "common.cuh"
 #include "kernels.h"
 #include "shared_prefix.cuh"
@@ -21,32 +20,15 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kConsumerWarps = 8;
-constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr int kProducerWarps = 4;                    // K lo, K hi, V lo, V hi
+constexpr int kThreads = (kConsumerWarps + kProducerWarps) * 32;
 constexpr int kStageRows = 128;
 constexpr uint32_t kHalfBytes = kStageRows * 128;    // 64 of the 128 elements of every row
-constexpr uint32_t kStageBytes = 4 * kHalfBytes;     // K lo, K hi, V lo, V hi
+constexpr uint32_t kStageBytes = 4 * kHalfBytes;
 constexpr int kStages = 3;
-constexpr int kSlotTab = 1024;
-constexpr int RT = 16;                               // query rows of a tile
-constexpr int kMinStagesPerCta = 2;
+constexpr int RT = kSharedRowTile;
 constexpr int kMergeWarps = 4;
 constexpr int kTcRows = 32;
-constexpr int kNoLimit = 0x3fffffff;
-constexpr int kMaxUnits = 2 * kSharedMaxBatch;
-
-struct Unit {
-    int tok0, ntok;    // query tokens
-    int lo, hi;        // keys [lo, hi) ...
-    int start;         // ... read from here: the beginning of lo's copy
-    int limit0;        // token i sees keys up to limit0 + i
-    int table;         // page-table row
-};
-
-struct Item {
-    Unit unit;
-    int tile, s_begin, s_end, slot;
-    bool reread;       // other tiles of rows read the same keys
-};
 
 // Values of keys behind limit0 that hold an infinity or NaN: weight times value for the rows that see the key, then zeros in
 // the key's place.  Weights x and sums o as the products' registers hold them.
@@ -96,183 +78,87 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages];
     __shared__ __align__(8) uint64_t empty_bar[kStages];
-    __shared__ int s_stage[kMaxUnits + 1], s_tile[kMaxUnits + 1];
-    __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
-    __shared__ int s_slot_tab[kSlotTab];
-    __shared__ int2 s_warp[kThreads / 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int Hkv = p.kv_heads, G = p.group, SK = p.stage_keys;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&full_bar[s]), kProducerWarps);
             mbar_init(smem_u32(&empty_bar[s]), kConsumerWarps);
         }
         fence_mbar_init();
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
     }
-    // Behind the tensor-core kernel nothing here waits for what it writes, and what came before it is complete: it has waited.  The
-    // wait is made up for at the end, since the kernel that joins the parts waits for this one alone.
-    if (!p.after_tc) pdl_wait_prior();
-    pdl_launch_dependents();
-
-    // ---- units, tiles and stages ----
-    shared_prefixes(p, s_bound, s_prefix);
-    auto unit_of = [&](int u) {
-        Unit x;
-        int b = u - p.groups;
-        if (b < 0) {
-            b = min(s_bound[u], p.batch - 1);
-            x.tok0 = shared_row(p, s_bound[u]);
-            x.ntok = max(shared_row(p, s_bound[u + 1]) - x.tok0, 0);
-            x.lo = 0;
-            x.hi = s_prefix[u];
-            x.limit0 = kNoLimit;
-        } else {
-            const int g = shared_group_of(s_bound, p.groups, b);
-            const int len = shared_len(p, b);
-            x.tok0 = shared_row(p, b);
-            x.ntok = max(shared_row(p, b + 1) - x.tok0, 0);
-            x.lo = g >= 0 ? s_prefix[g] : 0;
-            x.hi = len;
-            x.limit0 = len - x.ntok;
-        }
-        x.table = p.table_idx[b];
-        x.start = x.lo & ~(p.kpc - 1);
-        return x;
-    };
-    const int U = p.groups + p.batch;
-    {
-        auto size_of = [&](int u) {
-            const Unit x = unit_of(u);
-            const int stages = (max(x.hi - x.start, 0) + SK - 1) / SK, tiles = stages > 0 && (u >= p.groups || x.ntok * G <= p.tc_rows) ? (x.ntok * G + RT - 1) / RT : 0;
-            return make_int2(tiles * stages, tiles);
-        };
-        const int each = (U + kThreads - 1) / kThreads;
-        const int u0 = min(static_cast<int>(threadIdx.x) * each, U), u1 = min(u0 + each, U);
-        int2 mine = make_int2(0, 0);
-        for (int u = u0; u < u1; ++u) {
-            const int2 n = size_of(u);
-            mine.x += n.x;
-            mine.y += n.y;
-        }
-        int2 incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, incl.x, o), b = __shfl_up_sync(0xffffffffu, incl.y, o);
-            if (lane >= o) {
-                incl.x += a;
-                incl.y += b;
-            }
-        }
-        if (lane == 31) s_warp[warp] = incl;
-        __syncthreads();
-        int2 at = make_int2(incl.x - mine.x, incl.y - mine.y);
-        for (int w = 0; w < warp; ++w) {
-            at.x += s_warp[w].x;
-            at.y += s_warp[w].y;
-        }
-        for (int u = u0; u < u1; ++u) {
-            s_stage[u] = at.x;
-            s_tile[u] = at.y;
-            const int2 n = size_of(u);
-            at.x += n.x;
-            at.y += n.y;
-        }
-        if (threadIdx.x == kThreads - 1) {
-            s_stage[U] = at.x;
-            s_tile[U] = at.y;
-        }
-    }
     __syncthreads();
-    const int total = s_stage[U];
-    const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinStagesPerCta);
-    // Partial results lie at tile + CTA.  The host has made room for `tokens` rows; an index array whose requests overlap asks for
-    // more, and is reported instead.
-    const bool fits = static_cast<int>(gridDim.x) + s_tile[U] <= p.max_slots;
-    if (blockIdx.x == 0) {
-        for (int u = threadIdx.x; u <= U; u += kThreads) {
-            p.plan.stage[u] = s_stage[u];
-            p.plan.tile[u] = s_tile[u];
-        }
-        for (int g = threadIdx.x; g < p.groups; g += kThreads) p.plan.prefix[g] = s_prefix[g];
-        for (int b = threadIdx.x; b < p.batch; b += kThreads) p.plan.group_of[b] = shared_group_of(s_bound, p.groups, b);
-        if (threadIdx.x == 0) {
-            p.plan.per[0] = fits ? per : 0;
-            if (!fits) atomicExch(&p.status[kStatusBadIndex], p.tokens + 1);
-        }
-    }
-    if (!fits) {
-        if (p.after_tc) pdl_wait_prior();
-        return;
-    }
-    const int g_begin = min(static_cast<int>(blockIdx.x) * per, total);
-    const int g_end = min(total, g_begin + per);
-
-    // The item that starts at stage gpos < g_end of the sequence.
-    auto locate = [&](int gpos) {
-        int lo = 0, hi = U;   // the last unit that does not begin behind gpos (units without stages are skipped)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_stage[mid] <= gpos) lo = mid; else hi = mid;
-        }
-        Item it;
-        it.unit = unit_of(lo);
-        const int off = gpos - s_stage[lo], tiles = s_tile[lo + 1] - s_tile[lo];
-        const int stages = (s_stage[lo + 1] - s_stage[lo]) / tiles;
-        it.tile = off / stages;
-        it.s_begin = off - it.tile * stages;
-        it.s_end = min(stages, it.s_begin + (g_end - gpos));
-        it.slot = s_tile[lo] + it.tile + static_cast<int>(blockIdx.x);
-        it.reread = tiles > 1;
+    // Behind the tensor-core kernel nothing here waits for what that writes, and the plan is complete: it has waited for it.  The wait
+    // is made up for at the end, since the kernel that joins the parts waits for this one alone.
+    if (!p.with_tc) pdl_wait_prior();
+    pdl_launch_dependents();
+    const int2 items = p.plan.rows_of[blockIdx.x];
+    auto get_item = [&](int i) {
+        const int4* src = reinterpret_cast<const int4*>(p.plan.rows + i);
+        const int4 a = src[0], b = src[1], c = src[2];
+        RowsItem it;
+        it.tok0 = a.x, it.ntok = a.y, it.lo = a.z, it.hi = a.w, it.start = b.x, it.limit0 = b.y, it.table = b.z, it.tile = b.w;
+        it.s_begin = c.x, it.s_end = c.y, it.reread = c.z;
         return it;
     };
     uint32_t it_count = 0;
     bool failed = false;
 
-    if (warp == kConsumerWarps) {
-        // ================= producer =================
+    if (warp >= kConsumerWarps) {
+        // ================= producers =================
+        const int which = warp - kConsumerWarps;
         const uint32_t copy_bytes = static_cast<uint32_t>(p.kpc) * Hkv * 128u;
         const uint64_t once = l2_policy_evict_first();
-        for (int gpos = g_begin; gpos < g_end && !failed;) {
-            const Item it = locate(gpos);
-            gpos += it.s_end - it.s_begin;
-            const int32_t* row = p.page_table + static_cast<int64_t>(it.unit.table) * p.pt_stride;
-            const int first_key = it.unit.start + it.s_begin * SK;
-            const int copies = (min(it.unit.hi, it.unit.start + it.s_end * SK) - first_key + p.kpc - 1) / p.kpc;
-            __syncwarp();
-            for (int c = lane; c < min(copies, kSlotTab); c += 32) s_slot_tab[c] = row[first_key + c * p.kpc];
-            __syncwarp();
+        const void* map = which < 2 ? &tmap_k : &tmap_v;
+        for (int i = items.x; i < items.y && !failed; ++i) {
+            const RowsItem it = get_item(i);
+            const int32_t* row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride;
+            auto copies_of = [&](int st) { return (min(SK, it.hi - it.start - st * SK) + p.kpc - 1) / p.kpc; };
+            int next[4];   // this lane's slots of a stage's copies, fetched a stage ahead
+            auto fetch_slots = [&](int st) {
+                const int n = copies_of(st);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int copy = c * 32 + lane;
+                    next[c] = copy < n ? row[it.start + st * SK + copy * p.kpc] : 0;
+                }
+            };
+            fetch_slots(it.s_begin);
             for (int st = it.s_begin; st < it.s_end; ++st, ++it_count) {
+                const int n = copies_of(st);
+                int sl[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    sl[c] = next[c];
+                    if (sl[c] < 0 || static_cast<int64_t>(sl[c]) + p.kpc > p.num_slots) {
+                        atomicExch(&p.status[kStatusBadIndex], sl[c] + 1);
+                        sl[c] = 0;
+                    }
+                }
+                if (st + 1 < it.s_end) fetch_slots(st + 1);
                 const uint32_t slot = it_count % kStages;
                 if (!mbar_wait_warp(smem_u32(&empty_bar[slot]), ((it_count / kStages) & 1u) ^ 1u, p.status, 221)) {
                     failed = true;
                     break;
                 }
-                const int k0 = it.unit.start + st * SK;
-                const int n = (min(SK, it.unit.hi - k0) + p.kpc - 1) / p.kpc;
                 const uint32_t bar = smem_u32(&full_bar[slot]);
-                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * 4u * copy_bytes);
+                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * copy_bytes);
                 __syncwarp();
-                const uint32_t base = smem_base + slot * kStageBytes;
-                for (int ci = lane; ci < n * 4; ci += 32) {
-                    const int copy = ci >> 2, which = ci & 3;
-                    const int tab = (k0 - first_key) / p.kpc + copy;
-                    int64_t sl = tab < kSlotTab ? s_slot_tab[tab] : row[k0 + copy * p.kpc];
-                    if (sl < 0 || sl + p.kpc > p.num_slots) {
-                        atomicExch(&p.status[kStatusBadIndex], static_cast<int>(sl) + 1);
-                        sl = 0;
-                    }
-                    const uint32_t dst = base + which * kHalfBytes + copy * copy_bytes;
-                    const void* map = which < 2 ? &tmap_k : &tmap_v;
-                    if (it.reread) tma_load_3d(dst, map, (which & 1) * 64, static_cast<int>(sl), 0, bar);
-                    else tma_load_3d_hint(dst, map, (which & 1) * 64, static_cast<int>(sl), 0, bar, once);
+                const uint32_t base = smem_base + slot * kStageBytes + which * kHalfBytes;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int copy = c * 32 + lane;
+                    if (copy >= n) continue;
+                    if (it.reread) tma_load_3d(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar);
+                    else tma_load_3d_hint(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar, once);
                 }
             }
         }
-        if (p.after_tc) pdl_wait_prior();
+        if (p.with_tc) pdl_wait_prior();
         return;
     }
 
@@ -286,18 +172,16 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         return static_cast<uint32_t>((js & ~(p.kpc - 1)) * Hkv + h * p.kpc + (js & (p.kpc - 1)));
     };
     auto value_addr = [&](uint32_t base, int j, int c16) { return swz128(base + (2 + (c16 >> 3)) * kHalfBytes + tile_row(j) * 128u, c16 & 7); };
-    for (int gpos = g_begin; gpos < g_end;) {
-        const Item it = locate(gpos);
-        gpos += it.s_end - it.s_begin;
-        const Unit& un = it.unit;
-        const int rows = un.ntok * G - it.tile * RT;   // of this tile, at least one
+    for (int item = items.x; item < items.y; ++item) {
+        const RowsItem un = get_item(item);
+        const int rows = un.ntok * G - un.tile * RT;   // of this tile, at least one
         // Query fragments and the last key that a row sees.
         uint32_t qa[8][4];
         int limit[2];
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             const bool there = rr * 8 + g < rows;
-            const int r = it.tile * RT + rr * 8 + g, tok = there ? r / G : 0;
+            const int r = un.tile * RT + rr * 8 + g, tok = there ? r / G : 0;
             limit[rr] = there ? min(un.limit0 + tok, un.hi - 1) : -1;
             const __nv_bfloat16* q = p.q + (un.tok0 + tok) * p.q_st + (h * G + (there ? r - tok * G : 0)) * p.q_sh;
 #pragma unroll
@@ -309,7 +193,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[16][4];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        for (int st = it.s_begin; st < it.s_end; ++st, ++it_count) {
+        for (int st = un.s_begin; st < un.s_end; ++st, ++it_count) {
             const uint32_t slot = it_count % kStages;
             if (!failed && !mbar_wait_warp(smem_u32(&full_bar[slot]), (it_count / kStages) & 1u, p.status, 222)) failed = true;
             const int key0 = un.start + st * SK + kg * 16;
@@ -388,7 +272,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             mbar_release_stage(smem_u32(&empty_bar[slot]), lane);
         }
         // ---- the part's statistics and sums ----
-        const int64_t part = (static_cast<int64_t>(it.slot) * KG + kg) * Hkv + h;
+        const int64_t part = (static_cast<int64_t>(item) * KG + kg) * Hkv + h;
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             float sum = l[rr];
@@ -402,7 +286,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             if (t == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mx[rr], sum);
         }
     }
-    if (p.after_tc) pdl_wait_prior();
+    if (p.with_tc) pdl_wait_prior();
 }
 
 // Parts of a row: `count` of them, the first at `first`, `step` rows apart.
@@ -412,7 +296,7 @@ struct Parts {
 };
 
 // Joins the parts of every row.  One warp per (token, head), tokens of a request in turn; rows that no request owns stay as they
-// were.  Bound by the trips to L2: lengths, statistics, sums.
+// were.  Bound by the trips to L2: where the parts are, then their statistics and the first of their sums.
 __global__ void __launch_bounds__(kMergeWarps * 32)
 shared_prefix_merge_kernel(const SharedPrefixParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -420,78 +304,67 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     const int b = static_cast<int>(blockIdx.y);
     pdl_launch_dependents();
     pdl_wait_prior();
-    const int per = p.plan.per[0];
-    const int tc_per = p.after_tc ? p.plan.per[1] : 0;
-    if (head >= p.q_heads || per <= 0 || (p.after_tc && tc_per <= 0)) return;
-    const int h = head / p.group, KG = kConsumerWarps / p.kv_heads;
-    const int row0 = shared_row(p, b), row1 = shared_row(p, b + 1);
-    const int grp = p.plan.group_of[b];
-    const int own_first = p.plan.stage[p.groups + b], own_stages = p.plan.stage[p.groups + b + 1] - own_first;
-    const int own_tile = p.plan.tile[p.groups + b], own_tiles = p.plan.tile[p.groups + b + 1] - own_tile;
-    int pre_first = 0, pre_stages = 0, pre_tile = 0, pre_tiles = 0, pre_row = 0;
-    int tc_first = 0, tc_unit = 0, tc_units = 0, tc_tiles = 0, tc_cta = 0;
-    const bool chunked = p.after_tc && p.plan.per[2] != 0;
-    if (grp >= 0) {
-        if (p.after_tc) {
-            tc_first = p.plan.tc_first[grp];
-            tc_unit = p.plan.tc_unit[grp];
-            tc_cta = p.plan.tc_cta[grp];
-            tc_units = p.plan.tc_unit[grp + 1] - tc_unit;
-            tc_tiles = tc_units > 0 ? (p.plan.tc_first[grp + 1] - tc_first) / tc_units : 0;
-        }
-        pre_first = p.plan.stage[grp];
-        pre_stages = p.plan.stage[grp + 1] - pre_first;
-        pre_tile = p.plan.tile[grp];
-        pre_tiles = p.plan.tile[grp + 1] - pre_tile;
-        pre_row = shared_row(p, shared_bound(p, grp));
-    }
-    auto parts_of = [&](int first, int stages, int tile, int tiles, int r) {
+    const JoinItem j = p.plan.join[b];
+    const PlanHead plan = *p.plan.head;
+    if (head >= p.q_heads || !plan.fits) return;
+    const int h = head / p.group, hh = head - h * p.group, KG = kConsumerWarps / p.kv_heads;
+    // the CTA of the rows kernel that has a stage of the sequence
+    const int64_t early_end = static_cast<int64_t>(plan.early) * plan.early_stages;
+    auto cta_of = [&](int stage) {
+        return stage < early_end ? stage / plan.early_stages : plan.early + static_cast<int>((stage - early_end) / plan.late_stages);
+    };
+    auto parts_of = [&](int tile, int tiles, int first, int stages, int r) {
         Parts x = {0, static_cast<int64_t>(p.kv_heads) * RT, 0};
         const int mine = r / RT;
         if (r < 0 || mine >= tiles) return x;
-        const int n = stages / tiles, from = first + mine * n, c0 = from / per;
-        x.count = ((from + n - 1) / per - c0 + 1) * KG;
+        const int from = first + mine * stages, c0 = cta_of(from);
+        x.count = (cta_of(from + stages - 1) - c0 + 1) * KG;
         x.first = (static_cast<int64_t>(tile + mine + c0) * KG * p.kv_heads + h) * RT + r % RT;
         return x;
     };
-    for (int tok = row0 + static_cast<int>(blockIdx.z); tok < row1; tok += static_cast<int>(gridDim.z)) {
-        const int hh = head - h * p.group;
-        Parts pre = parts_of(pre_first, pre_stages, pre_tile, pre_tiles, (tok - pre_row) * p.group + hh);
-        const Parts own = parts_of(own_first, own_stages, own_tile, own_tiles, (tok - row0) * p.group + hh);
-        const int t = tok - pre_row, half = 128 / p.group, block = t / (2 * half);   // tokens of a chain
-        if (tc_units > 0 && t >= 0 && block < tc_units / p.kv_heads) {
-            const int unit = h * (tc_units / p.kv_heads) + block, from = tc_first + unit * tc_tiles;
-            const int in_block = t - block * 2 * half, chain = in_block >= half ? 1 : 0;
-            const int chunks = (tc_tiles + tc_per - 1) / tc_per;
-            const int c0 = chunked ? tc_cta + unit * chunks : from / tc_per;
-            pre.count = chunked ? chunks : (from + tc_tiles - 1) / tc_per - c0 + 1;
-            pre.first = p.tc_base + static_cast<int64_t>(tc_unit + unit + c0) * 256 + chain * 128 + (in_block - chain * half) * p.group + hh;
-            pre.step = 256;
+    for (int tok = j.row0 + static_cast<int>(blockIdx.z); tok < j.row1; tok += static_cast<int>(gridDim.z)) {
+        const Parts own = parts_of(j.own_tile, j.own_tiles, j.own_first, j.own_stages, (tok - j.row0) * p.group + hh);
+        const int t = tok - j.pre_row0;
+        Parts pre = parts_of(j.pre_tile, j.pre_tiles, j.pre_first, j.pre_stages, t * p.group + hh);
+        const int half = kSharedTcTile / p.group, block = t / (2 * half);   // tokens of a chain
+        if (t >= 0 && block < j.tc_blocks) {
+            const int unit = h * j.tc_blocks + block, in_block = t - block * 2 * half, chain = in_block >= half ? 1 : 0;
+            const int from = j.tc_first + unit * j.tc_tiles, chunks = (j.tc_tiles + plan.tc_per - 1) / plan.tc_per;
+            const int c0 = plan.tc_chunked ? j.tc_cta + unit * chunks : from / plan.tc_per;
+            pre.count = plan.tc_chunked ? chunks : (from + j.tc_tiles - 1) / plan.tc_per - c0 + 1;
+            pre.first = p.tc_base + static_cast<int64_t>(j.tc_unit + unit + c0) * (2 * kSharedTcTile) + chain * kSharedTcTile +
+                        (in_block - chain * half) * p.group + hh;
+            pre.step = 2 * kSharedTcTile;
         }
         const int n = pre.count + own.count;
+        auto at = [&](int i) { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; };
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float M = -INFINITY, L = 0.f;
+        constexpr int kAhead = 8;   // sums that are requested together with the statistics
         for (int base = 0; base < n; base += 32) {
-            const int i = base + lane;
-            int64_t at = 0;
+            const int m = min(32, n - base);
             float2 ml = make_float2(-INFINITY, 0.f);
-            if (i < n) {
-                at = i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step;
-                ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at);
-            }
+            if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at(base + lane));
+            float4 x[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
             const float Mn = fmaxf(M, warp_max(ml.x));
             const float ref = Mn == -INFINITY ? 0.f : Mn;
             const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
             M = Mn;
             L = L * shrink + warp_sum(w * ml.y);
             acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
-            const int m = min(32, n - base);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                if (i < m) acc.x += x[i].x * wi, acc.y += x[i].y * wi, acc.z += x[i].z * wi, acc.w += x[i].w * wi;
+            }
 #pragma unroll 4
-            for (int j = 0; j < m; ++j) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
-                const int64_t aj = __shfl_sync(0xffffffffu, at, j);
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(p.ws_o + aj * kD) + lane);
-                acc.x += x.x * wj, acc.y += x.y * wj, acc.z += x.z * wj, acc.w += x.w * wj;
+            for (int i = kAhead; i < m; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane);
+                acc.x += y.x * wi, acc.y += y.y * wi, acc.z += y.z * wi, acc.w += y.w * wi;
             }
         }
         const float inv = L > 0.f ? 1.f / L : 0.f;   // a row that sees no key: zeros
@@ -504,22 +377,26 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
 
 int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-// Where the pieces of the workspace begin, in bytes.
+// Where the pieces of the workspace begin, in bytes; partial rows ahead of the tensor-core kernel's.
 struct SharedLayout {
-    int64_t slots, tc_slots, rows, plan, ml, o, bytes;   // rows: of the rows kernel's parts, ahead of the tensor-core kernel's
+    int64_t slots, tc_slots, rows, rows_of, tc_of, rows_items, tc_items, join, ml, o, bytes;
 };
 SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads) {
-    const int64_t rows = tokens * (q_heads / kv_heads), kg = kConsumerWarps / kv_heads;
+    const int64_t group = q_heads / kv_heads, rows = tokens * group, kg = kConsumerWarps / kv_heads, ctas = sm_count();
     SharedLayout x;
     // tiles: at most one more than full ones per unit, and every row is in two units
-    x.slots = sm_count() + 2 * (rows / RT) + batch + groups;
+    x.slots = ctas + 2 * (rows / RT) + batch + groups;
     x.rows = x.slots * kg * kv_heads * RT;
     // units of the tensor-core kernel: the same of groups that have more than kTcRows rows
     const int64_t tc_groups = groups < rows / (kTcRows + 1) ? groups : rows / (kTcRows + 1);
-    x.tc_slots = rows > kTcRows ? sm_count() + kv_heads * (tokens / (2 * (128 / (q_heads / kv_heads))) + tc_groups) : 0;
-    const int64_t part_rows = x.rows + x.tc_slots * 256;
-    x.plan = 0;
-    x.ml = round256((4 + 2 * (groups + batch + 1) + groups + batch + 3 * (groups + 1)) * 4);
+    x.tc_slots = rows > kTcRows && groups > 0 ? ctas + kv_heads * (tokens / (2 * (kSharedTcTile / group)) + tc_groups) : 0;
+    const int64_t part_rows = x.rows + x.tc_slots * (2 * kSharedTcTile);
+    x.rows_of = round256(sizeof(PlanHead));
+    x.tc_of = x.rows_of + round256(ctas * sizeof(int2));
+    x.rows_items = x.tc_of + round256(ctas * sizeof(int2));
+    x.tc_items = x.rows_items + round256(x.slots * sizeof(RowsItem));
+    x.join = x.tc_items + round256(x.tc_slots * sizeof(TcItem));
+    x.ml = x.join + round256(batch * sizeof(JoinItem));
     x.o = x.ml + round256(part_rows * 8);
     x.bytes = x.o + part_rows * kD * 4;
     return x;
@@ -528,7 +405,7 @@ SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_
 // Launches of a call after its first may begin before the one ahead of them has ended.
 struct FollowOn {
     const bool was = pdl_launches_enabled();
-    explicit FollowOn(bool on) { set_pdl_launches(was || on); }
+    FollowOn() { set_pdl_launches(true); }
     ~FollowOn() { set_pdl_launches(was); }
 };
 
@@ -603,42 +480,40 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
         return B200_ERR_INVALID_ARGUMENT;
     }
     uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a->workspace) + 255) & ~uintptr_t(255));
-    int* ints = reinterpret_cast<int*>(ws + x.plan);
-    p.plan.per = ints;
-    p.plan.stage = ints + 4;
-    p.plan.tile = p.plan.stage + a->groups + a->batch + 1;
-    p.plan.prefix = p.plan.tile + a->groups + a->batch + 1;
-    p.plan.group_of = p.plan.prefix + a->groups;
+    p.plan.head = reinterpret_cast<PlanHead*>(ws);
+    p.plan.rows_of = reinterpret_cast<int2*>(ws + x.rows_of);
+    p.plan.tc_of = reinterpret_cast<int2*>(ws + x.tc_of);
+    p.plan.rows = reinterpret_cast<RowsItem*>(ws + x.rows_items);
+    p.plan.tc = reinterpret_cast<TcItem*>(ws + x.tc_items);
+    p.plan.join = reinterpret_cast<JoinItem*>(ws + x.join);
     p.ws_ml = reinterpret_cast<float*>(ws + x.ml);
     p.ws_o = reinterpret_cast<float*>(ws + x.o);
+    p.tc_base = x.rows;
     p.max_slots = static_cast<int>(x.slots);
-    p.plan.tc_first = p.plan.group_of + a->batch;
-    p.plan.tc_unit = p.plan.tc_first + a->groups + 1;
-    p.plan.tc_cta = p.plan.tc_unit + a->groups + 1;
+    p.tc_slots = static_cast<int>(x.tc_slots);
     // Queries are copied by tensor maps there.
     const bool aligned = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0 &&
                          a->q_stride_token > 0 && a->q_stride_head > 0;
     p.tc_rows = aligned ? kTcRows : 0x7fffffff;
-    p.tc_slots = static_cast<int>(x.tc_slots);
-    p.tc_base = x.rows;
     // (a group has more rows than that only if all have)
-    p.after_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > p.tc_rows;
+    p.with_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > p.tc_rows;
+    p.ctas = sm_count();
     CUtensorMap tk, tv;
     err = make_kv_tmap(&tk, a->k_cache, a->num_slots, a->kv_heads, a->page_size);
     if (err != B200_OK) return err;
     err = make_kv_tmap(&tv, a->v_cache, a->num_slots, a->kv_heads, a->page_size);
     if (err != B200_OK) return err;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int grid = sm_count();
-    if (p.after_tc) {
+    err = launch_shared_prefix_plan(p, s);
+    if (err != B200_OK) return err;
+    FollowOn follow;
+    if (p.with_tc) {
         err = launch_shared_prefix_tc(p, a->k_cache, a->v_cache, a->page_size, s);
         if (err != B200_OK) return err;
     }
-    FollowOn follow(p.after_tc);
     const int smem = kStages * kStageBytes + 1024;
     B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(grid), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, p));
-    FollowOn merge(true);
+    B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(p.ctas), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, p));
     const int turns = div_ceil(a->tokens, a->batch) < 64 ? div_ceil(a->tokens, a->batch) : 64;
     B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(div_ceil(a->q_heads, kMergeWarps), a->batch, turns),
                                   dim3(kMergeWarps * 32), 0, s, dim3(1, 1, 1), p));

@@ -3,9 +3,9 @@
 //
 // All query rows of a group that read one KV head are one matrix, [tokens * heads per KV head, 128], in blocks of up to 256 rows; no
 // row of a prefix is masked.  A unit is (group, KV head, block).  A unit's K/V tiles of 128 keys are cut into equal chunks, a CTA
-// each, with chunks as short as the number of CTAs allows; where there are more units than CTAs, the tiles of all units form one
-// sequence that is cut into equal contiguous runs.  (Runs throughout: one CTA in ten or so crosses from unit to unit, which costs it
-// 5 to 14 us of queries, first scores, last products and results, and all others wait for it.)  Per tile
+// each; where there are too many units for that, the tiles of all units form one sequence that is cut into equal contiguous runs
+// (shared_prefix_plan.cu).  Runs cross from unit to unit, which costs 5 to 14 us of queries, first scores, last products and
+// results.  Per tile
 //     S = Q K^T     128 x 128 x 128 into TMEM; a thread per row takes its 128 scores to registers
 //     P = 2^(S - m) bf16 into TMEM, the A operand of      O += P V      128 x 128 x 128, accumulated in TMEM
 // with the reference m moved (and O rescaled) only when the true maximum is 2^8 ahead of it.  Two chains of S, softmax and P V take
@@ -37,11 +37,10 @@ static_assert(128 * (kIssueRegs + 2 * kSoftmaxRegs) <= kThreads * 168, "");
 constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16
 constexpr uint32_t kKVOff = 4 * kAtomBytes; // behind 2 tiles of queries of 2 atoms each
 constexpr uint32_t kSlotBytes = 2 * kAtomBytes;
-constexpr int kKSlots = 2, kVSlots = 2, kSlots = kKSlots + kVSlots;   // a ring of tiles each
+constexpr int kKSlots = 2, kVSlots = 3, kSlots = kKSlots + kVSlots;   // a ring of tiles each
 constexpr uint32_t kSmemBytes = kKVOff + kSlots * kSlotBytes;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns: S (128, both chains in turn), P (64 each), O (128 each)
 constexpr float kLazyLog2 = 8.0f;
-constexpr int kMinTilesPerCta = 2;
 
 // How K and V tiles are copied ([0] K, [1] V), into 16 groups of 8 keys, each both halves of the head dimension.
 struct SharedKvMaps {
@@ -51,13 +50,6 @@ struct SharedKvMaps {
     CUtensorMap tile[2];   // whole rows of 128 keys: tiles whose pages are consecutive slots
     int whole_pages, whole_tiles;   // are the latter two there?
     int kpc;                        // keys of a page in a tile
-};
-
-struct Item {
-    int h;                // KV head
-    int tok0, ntok;       // query tokens of the block
-    int keys, t0, t1;     // of the prefix; tiles [t0, t1)
-    int table, slot;
 };
 
 __device__ __forceinline__ uint64_t as_pair(float2 x) { return *reinterpret_cast<uint64_t*>(&x); }
@@ -94,15 +86,11 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     __shared__ __align__(8) uint64_t p_full[2];       // per chain: P is in TMEM (4 warp arrivals)
     __shared__ __align__(8) uint64_t pv_done[2];      // per chain: O += P V has completed
     __shared__ uint32_t tmem_base_slot;
-    __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
-    __shared__ int s_first[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];   // tiles and units of the groups before
-    __shared__ int2 s_warp[kThreads / 32], s_run;
-    __shared__ int s_chunks[kThreads / 32];
     __shared__ float2 s_ml[kTile];                    // second chain's statistics, where both have the same rows
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const int G = p.group, Hkv = p.kv_heads;
+    const int G = p.group;
     const int QB = kTile / G;   // query tokens of a chain
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&maps.q);
@@ -125,164 +113,41 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         fence_mbar_init();
         fence_proxy_async_smem();
     }
-    __syncwarp();
-    pdl_wait_prior();
-    pdl_launch_dependents();
     if (warp == 1) {
         tmem_alloc(smem_u32(&tmem_base_slot), 512);
         tmem_relinquish();
-    }
-
-    // ---- units and tiles ----
-    shared_prefixes(p, s_bound, s_prefix);
-    {
-        auto size_of = [&](int g) {   // (tiles, units)
-            const int ntok = max(shared_row(p, s_bound[g + 1]) - shared_row(p, s_bound[g]), 0);
-            if (ntok * G <= p.tc_rows || s_prefix[g] == 0) return make_int2(0, 0);
-            const int units = Hkv * ((ntok + 2 * QB - 1) / (2 * QB));
-            return make_int2(units * ((s_prefix[g] + kTile - 1) / kTile), units);
-        };
-        const int each = (p.groups + kThreads - 1) / kThreads;
-        const int g0 = min(static_cast<int>(threadIdx.x) * each, p.groups), g1 = min(g0 + each, p.groups);
-        int2 mine = make_int2(0, 0);
-        for (int g = g0; g < g1; ++g) {
-            const int2 n = size_of(g);
-            mine.x += n.x;
-            mine.y += n.y;
-        }
-        int2 incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, incl.x, o), b = __shfl_up_sync(0xffffffffu, incl.y, o);
-            if (lane >= o) {
-                incl.x += a;
-                incl.y += b;
-            }
-        }
-        if (lane == 31) s_warp[warp] = incl;
-        __syncthreads();
-        int2 at = make_int2(incl.x - mine.x, incl.y - mine.y);
-        for (int w = 0; w < warp; ++w) {
-            at.x += s_warp[w].x;
-            at.y += s_warp[w].y;
-        }
-        for (int g = g0; g < g1; ++g) {
-            s_first[g] = at.x;
-            s_unit[g] = at.y;
-            const int2 n = size_of(g);
-            at.x += n.x;
-            at.y += n.y;
-        }
-        if (threadIdx.x == kThreads - 1) {
-            s_first[p.groups] = at.x;
-            s_unit[p.groups] = at.y;
-        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_slot;
-    const int total = s_first[p.groups], units = s_unit[p.groups], ctas = static_cast<int>(gridDim.x);
-    // (as in the rows kernel: index arrays whose requests or groups overlap ask for more room than there is)
-    const bool fits = ctas + units <= p.tc_slots;
-    // Tiles per chunk: of a dozen candidates, from an equal share for every CTA to one that surely needs no more CTAs than there are,
-    // the smallest that does not (0: more units than half of the CTAs, equal runs).
-    int per = max((total + ctas - 1) / ctas, kMinTilesPerCta);
-    const bool chunked = units > 0 && 2 * units <= ctas;
-    if (chunked) {
-        const int sure = max((total + ctas - units - 1) / (ctas - units), per);
-        const int steps = kThreads / 32 - 1;
-        const int candidate = per + static_cast<int>(static_cast<int64_t>(sure - per) * warp / steps);
-        int n = 0;
-        for (int g = lane; g < p.groups; g += 32) {
-            const int mine = s_unit[g + 1] - s_unit[g];
-            if (mine > 0) n += mine * (((s_prefix[g] + kTile - 1) / kTile + candidate - 1) / candidate);
-        }
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0) s_chunks[warp] = n;
-        __syncthreads();
-        int w = 0;
-        while (w < steps && s_chunks[w] > ctas) ++w;
-        per += static_cast<int>(static_cast<int64_t>(sure - per) * w / steps);
-    }
-    // This CTA's tiles, and for the kernel that joins the parts: the CTA of each group's first chunk.
-    if (warp == 0) {
-        int2 run = make_int2(0, 0);
-        int before = 0;
-        for (int base = 0; chunked && base < p.groups; base += 32) {
-            const int g = base + lane;
-            const int mine = g < p.groups ? s_unit[g + 1] - s_unit[g] : 0;
-            const int tiles = mine > 0 ? (s_prefix[g] + kTile - 1) / kTile : 0, chunks = (tiles + per - 1) / per;
-            int incl = mine * chunks;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
-            }
-            const int at = static_cast<int>(blockIdx.x) - (before + incl - mine * chunks);
-            if (mine > 0 && at >= 0 && at < mine * chunks) {
-                const int unit = at / chunks, from = (at - unit * chunks) * per;
-                run.x = s_first[g] + unit * tiles + from;
-                run.y = s_first[g] + unit * tiles + min(from + per, tiles);
-            }
-            if (blockIdx.x == 0 && g < p.groups) p.plan.tc_cta[g] = before + incl - mine * chunks;
-            before += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        run.x = __reduce_max_sync(0xffffffffu, run.x);   // (one lane has found it, or none)
-        run.y = __reduce_max_sync(0xffffffffu, run.y);
-        if (!chunked) {
-            run.x = min(static_cast<int>(blockIdx.x) * per, total);
-            run.y = min(total, run.x + per);
-        }
-        if (lane == 0) s_run = fits ? run : make_int2(0, 0);
-    }
-    if (blockIdx.x == 0) {
-        for (int g = threadIdx.x; g <= p.groups; g += kThreads) {
-            p.plan.tc_first[g] = s_first[g];
-            p.plan.tc_unit[g] = s_unit[g];
-        }
-        if (threadIdx.x == 0) {
-            p.plan.per[1] = fits ? per : 0;
-            p.plan.per[2] = chunked ? 1 : 0;
-            if (!fits) atomicExch(&p.status[kStatusBadIndex], p.tokens + 1);
-        }
-    }
-    __syncthreads();
-    const int g_begin = s_run.x, g_end = s_run.y;
-    const int ntiles = g_end - g_begin;   // of all items
 
-    // The item that starts at tile gpos < g_end of the sequence.
-    auto locate = [&](int gpos) {
-        int lo = 0, hi = p.groups;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_first[mid] <= gpos) lo = mid; else hi = mid;
-        }
-        Item it;
-        it.keys = s_prefix[lo];
-        const int tiles = (it.keys + kTile - 1) / kTile, off = gpos - s_first[lo], unit = off / tiles;
-        const int blocks = (s_unit[lo + 1] - s_unit[lo]) / Hkv;
-        it.h = unit / blocks;
-        it.tok0 = shared_row(p, s_bound[lo]) + (unit - it.h * blocks) * 2 * QB;
-        it.ntok = min(shared_row(p, s_bound[lo + 1]) - it.tok0, 2 * QB);
-        it.t0 = off - unit * tiles;
-        it.t1 = min(tiles, it.t0 + g_end - gpos);
-        it.table = p.table_idx[min(s_bound[lo], p.batch - 1)];
-        it.slot = s_unit[lo] + unit + static_cast<int>(blockIdx.x);
+    // This CTA's items, known once the plan is there (every role asks by itself: the softmax warps have something to do before).
+    int2 items;
+    int ntiles = 0;   // of all of them
+    auto get_items = [&]() {
+        pdl_wait_prior();
+        pdl_launch_dependents();
+        items = p.plan.tc_of[blockIdx.x];
+    };
+    auto get_item = [&](int i) {
+        const int4* src = reinterpret_cast<const int4*>(p.plan.tc + i);
+        const int4 a = src[0], b = src[1];
+        TcItem it;
+        it.h = a.x, it.tok0 = a.y, it.ntok = a.z, it.keys = a.w, it.t0 = b.x, it.t1 = b.y, it.table = b.z;
         return it;
     };
 
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 0 || warp == 2) {
         // ================= producers: K tiles, V tiles =================
+        get_items();
         const int kv = warp >> 1, kpc = maps.kpc;
         const uint32_t ring = kv == 0 ? 0 : kKSlots, ring_end = kv == 0 ? kKSlots : kSlots;
-        uint32_t items = 0;
         uint32_t slot = ring, phase = 1;   // (the first waits are for slots that nobody has used)
         bool failed = false;
-        for (int gpos = g_begin; gpos < g_end && !failed;) {
-            const Item it = locate(gpos);
-            gpos += it.t1 - it.t0;
+        for (int i = items.x; i < items.y && !failed; ++i) {
+            const TcItem it = get_item(i);
             const int32_t* pt_row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride;
             auto copies_of = [&](int kt) { return (min(kTile, it.keys - kt * kTile) + kpc - 1) / kpc; };
             int next[4];
@@ -296,7 +161,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             };
             fetch_slots(it.t0);
             if (kv == 0) {   // the queries: rows (token, head) of each chain, in two halves
-                if (items > 0 && !__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(&q_empty), (items - 1) & 1u, p.status, 341))) {
+                if (i > items.x && !__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(&q_empty), (i - items.x - 1) & 1, p.status, 341))) {
                     failed = true;
                     break;
                 }
@@ -306,7 +171,6 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 __syncwarp();
                 if (lane < 2 * chains)
                     tma_load_3d(smem_base + lane * kAtomBytes, &maps.q, (lane & 1) * 64, it.h * G, it.tok0 + (lane >> 1) * QB, bar);
-                ++items;
             }
             for (int kt = it.t0; kt < it.t1; ++kt) {
                 // A tile whose pages are consecutive slots is one copy; so is a page, unless it is smaller than a group of 8 or starts
@@ -371,7 +235,12 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             const uint32_t idesc = idesc_bf16_128x128(false);
             const uint64_t q_desc = kmajor_sw128_desc(smem_base);
             const uint64_t k_desc = grouped_keys_desc(smem_base + kKVOff, 0);
-            uint32_t slot = 0, phase = 0, items = 0;
+            get_items();
+            for (int i = items.x; i < items.y; ++i) {
+                const TcItem it = get_item(i);
+                ntiles += it.t1 - it.t0;
+            }
+            uint32_t slot = 0, phase = 0;
             uint32_t uses[2] = {0, 0};   // of each chain so far
             int last = -1, tile = 0;     // the chain of the last scores; tiles so far
             bool failed = false;
@@ -391,11 +260,10 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 last = chain;
                 ++uses[chain];
             };
-            for (int gpos = g_begin; gpos < g_end && !failed; ++items) {
-                const Item it = locate(gpos);
-                gpos += it.t1 - it.t0;
+            for (int i = items.x; i < items.y && !failed; ++i) {
+                const TcItem it = get_item(i);
                 const bool two = it.ntok > QB;
-                wait(smem_u32(&q_full), items & 1u, 339);
+                wait(smem_u32(&q_full), static_cast<uint32_t>(i - items.x) & 1u, 339);
                 for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
                     const uint64_t k = k_desc + slot * (kSlotBytes >> 4);
                     wait(smem_u32(&full[slot]), phase, 332);
@@ -415,7 +283,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                         phase ^= 1;
                     }
                 }
-                if (!failed && gpos < g_end) tc_commit(smem_u32(&q_empty));
+                if (!failed && i + 1 < items.y) tc_commit(smem_u32(&q_empty));
             }
         }
     } else if (warp == 3) {
@@ -423,6 +291,11 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         if (elect_one()) {
             const uint32_t idesc = idesc_bf16_128x128(true);
             const uint64_t v_desc = grouped_keys_desc(smem_base + kKVOff, 1024);
+            get_items();
+            for (int i = items.x; i < items.y; ++i) {
+                const TcItem it = get_item(i);
+                ntiles += it.t1 - it.t0;
+            }
             uint32_t slot = kKSlots, phase = 0;
             uint32_t uses[2] = {0, 0};
             int tile = 0;
@@ -442,9 +315,8 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 tc_commit(smem_u32(&pv_done[chain]));
                 ++uses[chain];
             };
-            for (int gpos = g_begin; gpos < g_end && !failed;) {
-                const Item it = locate(gpos);
-                gpos += it.t1 - it.t0;
+            for (int i = items.x; i < items.y && !failed; ++i) {
+                const TcItem it = get_item(i);
                 const bool two = it.ntok > QB;
                 for (int kt = it.t0; kt < it.t1 && !failed; ++kt, ++tile) {
                     const uint64_t v = v_desc + slot * (kSlotBytes >> 4);
@@ -480,19 +352,18 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         uint32_t uses = 0;
         int tiles_before = 0;
         bool failed = false;
-        for (int gpos = g_begin; gpos < g_end;) {
-            const Item it = locate(gpos);
-            const int gpos0 = gpos;
-            gpos += it.t1 - it.t0;
-            const bool two = it.ntok > QB;
+        // The first round of all is made on whatever TMEM holds and undone, while the plan and the first copies are under way: it brings
+        // the loop's instructions, which the first tile waited 4 us for otherwise.
+        TcItem it = {};
+        it.t0 = it.t1 = 0;
+        items = make_int2(0, 1);
+        for (int i = -1; i < items.y; ++i) {
+            if (i >= 0) it = get_item(i);
+            const bool real = i >= 0, two = it.ntok > QB;
             float m_ref = -INFINITY, l_run = 0.f;
             const int step = two ? 1 : 2;
             bool any = false;   // has this chain had a tile of the item?
-            const int kt0 = it.t0 + (two ? 0 : chain);
-            // (The first round of all is made on whatever TMEM holds and undone, while the first copies are under way: it brings the
-            // loop's instructions, which the first tile waited 4 us for otherwise.)
-            for (int kt = gpos0 == g_begin ? kt0 - step : kt0; kt < it.t1; kt += step) {
-                const bool real = kt >= kt0;
+            for (int kt = real ? it.t0 + (two ? 0 : chain) : -1; kt < it.t1; kt += step) {
                 if (real && !failed && !mbar_wait_mostly_ready(smem_u32(&s_full[chain]), uses & 1u, p.status, 334)) failed = true;
                 tc_fence_after();
                 const int valid = it.keys - kt * kTile;   // keys of the tile that belong to the prefix
@@ -572,15 +443,16 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (!real) {
-                    m_ref = -INFINITY;
-                    l_run = 0.f;
-                    continue;
-                }
+                if (!real) break;
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[chain]));
                 l_run += sum.x + sum.y;
                 any = true;
                 ++uses;
+            }
+            if (!real) {
+                get_items();
+                i = items.x - 1;
+                continue;
             }
             tiles_before += it.t1 - it.t0;
             if (any && !failed && !mbar_wait_mostly_ready(smem_u32(&pv_done[chain]), (uses - 1) & 1u, p.status, 335)) failed = true;
@@ -607,7 +479,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             if (two || chain == 0) {
                 const int tok = r / G + (two ? chain * QB : 0);
                 const bool store = r < QB * G && tok < it.ntok;
-                const int64_t at = p.tc_base + static_cast<int64_t>(it.slot) * (2 * kTile) + (two ? chain * kTile : 0) + r;
+                const int64_t at = p.tc_base + static_cast<int64_t>(i) * (2 * kTile) + (two ? chain * kTile : 0) + r;
                 float* dst = p.ws_o + at * kD;
 #pragma unroll 1
                 for (int c = 0; c < 8; ++c) {
@@ -617,14 +489,14 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                     tmem_ld_wait();
                     if (join) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            a[i] = __float_as_uint(__uint_as_float(a[i]) * mine + __uint_as_float(b[i]) * other);
+                        for (int j = 0; j < 16; ++j)
+                            a[j] = __float_as_uint(__uint_as_float(a[j]) * mine + __uint_as_float(b[j]) * other);
                     }
                     if (store) {
 #pragma unroll
-                        for (int i = 0; i < 16; i += 8)   // a sector per store
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * 16 + i), "r"(a[i]), "r"(a[i + 1]),
-                                         "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+                        for (int j = 0; j < 16; j += 8)   // a sector per store
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * 16 + j), "r"(a[j]), "r"(a[j + 1]),
+                                         "r"(a[j + 2]), "r"(a[j + 3]), "r"(a[j + 4]), "r"(a[j + 5]), "r"(a[j + 6]), "r"(a[j + 7])
                                          : "memory");
                     }
                 }
@@ -684,7 +556,7 @@ int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, co
     }
     const int smem = kSmemBytes + 1024;
     B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_tc_kernel, dim3(sm_count()), dim3(kThreads), smem, stream, dim3(1, 1, 1), maps, p));
+    B200_CHECK_CUDA(launch_kernel(shared_prefix_tc_kernel, dim3(p.ctas), dim3(kThreads), smem, stream, dim3(1, 1, 1), maps, p));
     return B200_OK;
 }
 

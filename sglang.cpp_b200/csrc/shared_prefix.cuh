@@ -1,4 +1,7 @@
-// Attention over a shared prefix: what its kernels have in common (parameters, and how the work is laid out on the device).
+// Attention over a shared prefix: what its kernels have in common.
+//
+// Four launches: a plan (one CTA) that cuts the work into items; the tensor-core kernel over the prefixes of groups with many query
+// rows; the rows kernel over everything else; and the kernel that joins a row's parts.
 #pragma once
 
 #include "common.cuh"
@@ -6,17 +9,59 @@
 namespace b200 {
 
 constexpr int kSharedMaxBatch = 1024;
+constexpr int kSharedRowTile = 16;     // query rows of a tile of the rows kernel
+constexpr int kSharedTcTile = 128;     // keys of a tile of the tensor-core kernel, and query rows of one of its chains
 
-// What a call leaves in the workspace for the kernel that joins the parts.  Units are the groups' prefixes (0 .. groups), then
-// the requests' own keys; `stage` and `tile` count the stages and row tiles of the units before.
+// Units are the groups' prefixes (0 .. groups) and the requests' own keys (groups .. groups + batch).
+
+// What a CTA of the rows kernel does in one go: stages [s_begin, s_end) of a unit's keys for a tile of its rows.
+struct __align__(16) RowsItem {
+    int tok0, ntok;    // query tokens of the unit
+    int lo, hi;        // its keys [lo, hi) ...
+    int start;         // ... read from here: where lo's page copy begins
+    int limit0;        // token i sees keys up to limit0 + i
+    int table;         // page-table row
+    int tile;          // row tile
+    int s_begin, s_end;
+    int reread;        // other row tiles read the same keys
+    int pad;
+};
+
+// ... and of the tensor-core kernel: tiles [t0, t1) of a prefix for a block of rows.
+struct __align__(16) TcItem {
+    int h;             // KV head
+    int tok0, ntok;    // query tokens of the block
+    int keys;          // of the prefix
+    int t0, t1;
+    int table;
+    int pad;
+};
+
+// Where the parts of a request's rows are.  A row tile's stages (a unit's key tiles) are spread over neighbouring CTAs, and parts lie
+// at tile + CTA (unit + CTA).
+struct __align__(16) JoinItem {
+    int row0, row1;                      // query rows
+    int own_tile, own_tiles, own_first, own_stages;   // tiles before, tiles, stages before, stages per tile
+    int pre_row0;                        // first query row of the group
+    int pre_tile, pre_tiles, pre_first, pre_stages;   // the group's prefix in the rows kernel, or ...
+    int tc_unit, tc_blocks, tc_first, tc_tiles, tc_cta;   // ... in the tensor-core kernel: units before, blocks per KV head, tiles before,
+                                                          // tiles per unit, first CTA
+};
+
+struct __align__(16) PlanHead {
+    int fits;                     // 0: index arrays ask for more room than the host has counted; nothing is written
+    int early, early_stages, late_stages;   // rows kernel: stages of each of the first `early` CTAs, and of each of the others
+    int tc_per, tc_chunked;       // tensor-core kernel: tiles per CTA, in chunks of one unit or in runs
+    int pad[2];
+};
+
 struct SharedPlan {
-    int* per;        // stages per CTA of the rows kernel; tiles per CTA of the tensor-core kernel, and whether in chunks
-    int* stage;      // [groups + batch + 1]
-    int* tile;       // [groups + batch + 1]
-    int* prefix;     // [groups] keys that are read once for the group
-    int* group_of;   // [batch], -1: none
-    int *tc_first, *tc_unit;   // [groups + 1] tiles and units of the groups before, in the tensor-core kernel
-    int* tc_cta;     // [groups] the CTA of a group's first chunk there
+    PlanHead* head;
+    int2* rows_of;       // [CTAs] items of a CTA of the rows kernel
+    int2* tc_of;         // [CTAs] ... of the tensor-core kernel
+    RowsItem* rows;      // [max_slots], item = slot of its partial results
+    TcItem* tc;          // [tc_slots]
+    JoinItem* join;      // [batch]
 };
 
 struct SharedPrefixParams {
@@ -31,52 +76,17 @@ struct SharedPrefixParams {
     int stage_keys, kpc;            // rows kernel: keys per stage and per copy
     int64_t num_slots;
     float scale_log2;
-    float *ws_ml, *ws_o;            // rows kernel: [max_slots, key groups, kv_heads, row tile] (maximum, sum), and x 128
-    int max_slots;
-    int tc_rows;                    // groups of more rows (tokens x group) than this: their prefixes by the tensor-core kernel
-    int tc_slots;
-    int64_t tc_base;                // its partial rows in ws_ml and ws_o: [tc_slots, 256] from here
-    bool after_tc;                  // the rows kernel follows the tensor-core kernel
+    float *ws_ml, *ws_o;            // partial rows, (maximum, sum) and x 128: the rows kernel's [max_slots, key groups, kv_heads, row tile],
+    int64_t tc_base;                // from here on the tensor-core kernel's [tc_slots, 2 chains, 128]
+    int max_slots, tc_slots;
+    int tc_rows;                    // groups of more query rows (tokens x group) than this: their prefixes by the tensor-core kernel
+    int with_tc;                    // is that kernel launched at all?
+    int ctas;                       // of either kernel
     SharedPlan plan;
     int* status;
 };
 
-#ifdef __CUDACC__
-// Query rows of the requests before b; bounds hold whatever the array says.
-__device__ __forceinline__ int shared_row(const SharedPrefixParams& p, int b) { return min(max(p.qo_indptr[b], 0), p.tokens); }
-__device__ __forceinline__ int shared_len(const SharedPrefixParams& p, int b) {
-    return static_cast<int>(min(static_cast<int64_t>(max(p.seq_lens[b], 0)), p.pt_stride));
-}
-__device__ __forceinline__ int shared_bound(const SharedPrefixParams& p, int g) { return min(max(p.group_indptr[g], 0), p.batch); }
-
-// The group that request b belongs to, -1 for none (s_bound: shared_bound of 0 .. groups).
-__device__ __forceinline__ int shared_group_of(const int* s_bound, int groups, int b) {
-    if (groups == 0 || b < s_bound[0] || b >= s_bound[groups]) return -1;
-    int lo = 0, hi = groups;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_bound[mid] <= b) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-// The keys that are read once for a group: those that its caller names, as far as they lie before every query row of its requests;
-// none for a request that shares with nobody.  All threads of a block; ends with a barrier.
-__device__ __forceinline__ void shared_prefixes(const SharedPrefixParams& p, int* s_bound, int* s_prefix) {
-    const int nt = static_cast<int>(blockDim.x);
-    for (int g = threadIdx.x; g <= p.groups; g += nt) s_bound[g] = p.groups > 0 ? shared_bound(p, g) : 0;
-    for (int g = threadIdx.x; g < p.groups; g += nt)
-        s_prefix[g] = shared_bound(p, g + 1) - shared_bound(p, g) > 1 ? max(p.prefix_lens[g], 0) : 0;
-    __syncthreads();
-    for (int b = threadIdx.x; b < p.batch; b += nt) {
-        const int rows = shared_row(p, b + 1) - shared_row(p, b);
-        const int g = shared_group_of(s_bound, p.groups, b);
-        if (g >= 0 && rows > 0) atomicMin(&s_prefix[g], max(shared_len(p, b) - rows, 0));
-    }
-    __syncthreads();
-}
-#endif
-
+int launch_shared_prefix_plan(const SharedPrefixParams& p, cudaStream_t stream);
 int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream);
 
 }  // namespace b200
