@@ -293,10 +293,11 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
  * seq_lens[b] keys, as for b200_attention_prefill (a decode step: one each; drafted tokens: a few each).  Rows of no
  * request are left as they were; a row that sees no key becomes zeros.  out [tokens, q_heads * head_dim] contiguous.
  * Everything per request and group is read on the device: a captured call follows what the arrays hold at its replay,
- * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words, and so
- * are query rows of overlapping requests (nothing is written then).
- * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head.  workspace:
- * b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
+ * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words.  A
+ * qo_indptr or group_indptr that decreases or leaves [0, tokens] or [0, batch] is reported as tokens + 1, and nothing is
+ * written.
+ * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head; q 16-byte aligned, its strides multiples of
+ * 8 elements.  workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
  * run one after another. */
 typedef struct b200_shared_prefix_args {
     void* out;

@@ -7,8 +7,8 @@
 // the probabilities, which are rounded to bf16 as the other attention kernels here do (their products run on the tensor cores).
 //
 // Rows kernel (bound by HBM): an item is a run of stages of a group's prefix or of what a request has of its own, for a tile of 16 of
-// its rows, (token, head of the KV head's group) pairs; the stages of all tiles of all units are dealt to the CTAs in contiguous runs
-// (shared_prefix_plan.cu).  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages, a warp for each
+// its rows, (token, head of the KV head's group) pairs.  Items are cut by shared_prefix_plan.cu; a CTA takes the next one that nobody
+// has taken (which CTA does an item changes no result), two ahead of the one it works on.  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages, a warp for each
 // half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with mma.sync.
 #include "common.cuh"
 #include "kernels.h"
@@ -26,7 +26,9 @@ constexpr int kStageRows = 128;
 constexpr uint32_t kHalfBytes = kStageRows * 128;    // 64 of the 128 elements of every row
 constexpr uint32_t kStageBytes = 4 * kHalfBytes;
 constexpr int kStages = 3;
-constexpr int RT = kSharedRowTile;
+constexpr uint32_t kItems = 4;                       // places for items that have been taken
+constexpr uint32_t kQueryBytes = 2 * kHalfBytes;     // 16 rows of each of 8 heads
+constexpr int RT = 16;                               // rows of a tile's products; as many whole tokens as fit are used
 constexpr int kMergeWarps = 4;
 constexpr int kTcRows = 32;
 
@@ -74,36 +76,61 @@ __device__ __forceinline__ void add_odd_values(uint32_t base, int key0, int vali
 
 __global__ void __launch_bounds__(kThreads, 1)
 shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                          const SharedPrefixParams p) {
+                          const __grid_constant__ CUtensorMap tmap_q, const SharedPrefixParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages];
     __shared__ __align__(8) uint64_t empty_bar[kStages];
+    __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems], query_full, query_empty;
+    __shared__ RowsItem s_item[kItems];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t query_base = smem_base + kStages * kStageBytes;
     const int Hkv = p.kv_heads, G = p.group, SK = p.stage_keys;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&full_bar[s]), kProducerWarps);
             mbar_init(smem_u32(&empty_bar[s]), kConsumerWarps);
         }
+        mbar_init(smem_u32(&query_full), 1);
+        mbar_init(smem_u32(&query_empty), kConsumerWarps);
+        for (uint32_t i = 0; i < kItems; ++i) {
+            mbar_init(smem_u32(&item_full[i]), 1);
+            mbar_init(smem_u32(&item_empty[i]), kConsumerWarps + kProducerWarps);
+        }
         fence_mbar_init();
         tma_prefetch_desc(&tmap_k);
         tma_prefetch_desc(&tmap_v);
+        tma_prefetch_desc(&tmap_q);
     }
     __syncthreads();
     // Behind the tensor-core kernel nothing here waits for what that writes, and the plan is complete: it has waited for it.  The wait
     // is made up for at the end, since the kernel that joins the parts waits for this one alone.
     if (!p.with_tc) pdl_wait_prior();
     pdl_launch_dependents();
-    const int2 items = p.plan.rows_of[blockIdx.x];
-    auto get_item = [&](int i) {
-        const int4* src = reinterpret_cast<const int4*>(p.plan.rows + i);
-        const int4 a = src[0], b = src[1], c = src[2];
+    // Item number `turn` of this CTA, for the whole warp; a slot of -1 ends it.
+    auto get_item = [&](uint32_t turn) {
         RowsItem it;
-        it.tok0 = a.x, it.ntok = a.y, it.lo = a.z, it.hi = a.w, it.start = b.x, it.limit0 = b.y, it.table = b.z, it.tile = b.w;
-        it.s_begin = c.x, it.s_end = c.y, it.reread = c.z;
+        it.slot = -1;
+        const uint32_t at = turn % kItems;
+        if (!mbar_wait_warp(smem_u32(&item_full[at]), turn / kItems & 1u, p.status, 223)) return it;
+        it = s_item[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&item_empty[at]));
         return it;
+    };
+    // By one lane of the first producer warp: items are handed on one or two ahead of the one whose copies are made (long and short
+    // ones: an item's description, its pages' slots and its first copies are three trips to memory, which short ones do not cover).
+    const int count = p.plan.head->rows_items;
+    const uint32_t lead = static_cast<uint32_t>(p.plan.head->rows_lead);
+    auto hand_on = [&](uint32_t turn, int taken) {
+        const uint32_t at = turn % kItems;
+        RowsItem it;
+        it.slot = -1;
+        if (taken < count) it = p.plan.rows[taken];
+        if (!mbar_wait_bounded(smem_u32(&item_empty[at]), (turn / kItems & 1u) ^ 1u, p.status, 224)) return;
+        s_item[at] = it;
+        mbar_arrive(smem_u32(&item_full[at]));
     };
     uint32_t it_count = 0;
     bool failed = false;
@@ -114,22 +141,43 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         const uint32_t copy_bytes = static_cast<uint32_t>(p.kpc) * Hkv * 128u;
         const uint64_t once = l2_policy_evict_first();
         const void* map = which < 2 ? &tmap_k : &tmap_v;
-        for (int i = items.x; i < items.y && !failed; ++i) {
-            const RowsItem it = get_item(i);
-            const int32_t* row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride;
-            auto copies_of = [&](int st) { return (min(SK, it.hi - it.start - st * SK) + p.kpc - 1) / p.kpc; };
-            int next[4];   // this lane's slots of a stage's copies, fetched a stage ahead
-            auto fetch_slots = [&](int st) {
-                const int n = copies_of(st);
+        const bool leads = which == 0 && lane == 0;
+        if (leads) {
+            const int taken = atomicAdd(&p.plan.head->next, static_cast<int>(lead));
+            for (uint32_t i = 0; i < lead; ++i) hand_on(i, taken + static_cast<int>(i));
+        }
+        __syncwarp();
+        auto copies_of = [&](const RowsItem& it, int st) { return (min(SK, it.hi - it.start - st * SK) + p.kpc - 1) / p.kpc; };
+        int next[4];   // this lane's slots of a stage's copies, fetched a stage ahead
+        auto fetch_slots = [&](const RowsItem& it, int st) {
+            const int32_t* row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride + it.start + st * SK;
+            const int n = copies_of(it, st);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int copy = c * 32 + lane;
-                    next[c] = copy < n ? row[it.start + st * SK + copy * p.kpc] : 0;
+            for (int c = 0; c < 4; ++c) {
+                const int copy = c * 32 + lane;
+                next[c] = copy < n ? row[copy * p.kpc] : 0;
+            }
+        };
+        RowsItem it = get_item(0);
+        if (it.slot >= 0) fetch_slots(it, it.s_begin);
+        for (uint32_t turn = 0; it.slot >= 0 && !failed; ++turn) {
+            int taken = 0;
+            if (leads) taken = atomicAdd(&p.plan.head->next, 1);
+            __syncwarp();
+            if (which == 3) {   // the queries, when the consumers have taken the last item's to registers
+                if (!mbar_wait_warp(smem_u32(&query_empty), (turn & 1u) ^ 1u, p.status, 226)) break;
+                const uint32_t half = static_cast<uint32_t>(p.row_tokens * p.q_heads) * 128u, bar = smem_u32(&query_full);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, 2 * half);
+                    for (int i = 0; i < 2; ++i)
+                        tma_load_3d(query_base + i * (half + 1023u & ~1023u), &tmap_q, i * 64, 0, it.tok0 + it.tile * p.row_tokens, bar);
                 }
-            };
-            fetch_slots(it.s_begin);
+                __syncwarp();
+            }
+            RowsItem after;
+            after.slot = -1;
             for (int st = it.s_begin; st < it.s_end; ++st, ++it_count) {
-                const int n = copies_of(st);
+                const int n = copies_of(it, st);
                 int sl[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -139,7 +187,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                         sl[c] = 0;
                     }
                 }
-                if (st + 1 < it.s_end) fetch_slots(st + 1);
+                if (st + 1 < it.s_end) fetch_slots(it, st + 1);
                 const uint32_t slot = it_count % kStages;
                 if (!mbar_wait_warp(smem_u32(&empty_bar[slot]), ((it_count / kStages) & 1u) ^ 1u, p.status, 221)) {
                     failed = true;
@@ -156,7 +204,14 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                     if (it.reread) tma_load_3d(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar);
                     else tma_load_3d_hint(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar, once);
                 }
+                if (st == it.s_begin) {
+                    if (leads) hand_on(turn + lead, taken);
+                    __syncwarp();
+                    after = get_item(turn + 1);
+                }
+                if (st + 1 == it.s_end && after.slot >= 0) fetch_slots(after, after.s_begin);
             }
+            it = after;
         }
         if (p.with_tc) pdl_wait_prior();
         return;
@@ -172,24 +227,32 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         return static_cast<uint32_t>((js & ~(p.kpc - 1)) * Hkv + h * p.kpc + (js & (p.kpc - 1)));
     };
     auto value_addr = [&](uint32_t base, int j, int c16) { return swz128(base + (2 + (c16 >> 3)) * kHalfBytes + tile_row(j) * 128u, c16 & 7); };
-    for (int item = items.x; item < items.y; ++item) {
-        const RowsItem un = get_item(item);
-        const int rows = un.ntok * G - un.tile * RT;   // of this tile, at least one
-        // Query fragments and the last key that a row sees.
+    const int QT = p.row_tokens;   // query tokens of a row tile
+    // Shared-memory row of a tile's row r: queries lie as [token][head].
+    auto query_row = [&](int r) -> uint32_t {
+        const int tok = min(r / G, QT - 1);
+        return static_cast<uint32_t>(tok * p.q_heads + h * G + min(r - tok * G, G - 1));
+    };
+    const uint32_t query_addr = query_base + query_row((mi & 1) * 8 + r8) * 128u;
+    const uint32_t query_half = static_cast<uint32_t>(QT * p.q_heads + 7 & ~7) * 128u;
+    const int row_tok[2] = {g / G, (g + 8) / G};   // of this lane's two rows
+    for (uint32_t turn = 0;; ++turn) {
+        const RowsItem un = get_item(turn);
+        if (un.slot < 0) break;
+        const int rows = min(un.ntok - un.tile * QT, QT) * G;   // of this tile, at least one
+        // Query fragments, and the last key that each of this lane's two rows sees.
         uint32_t qa[8][4];
         int limit[2];
+        if (!failed && !mbar_wait_warp(smem_u32(&query_full), turn & 1u, p.status, 225)) failed = true;
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-            const bool there = rr * 8 + g < rows;
-            const int r = un.tile * RT + rr * 8 + g, tok = there ? r / G : 0;
-            limit[rr] = there ? min(un.limit0 + tok, un.hi - 1) : -1;
-            const __nv_bfloat16* q = p.q + (un.tok0 + tok) * p.q_st + (h * G + (there ? r - tok * G : 0)) * p.q_sh;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                qa[ks][rr] = there ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 2 * t) : 0u;
-                qa[ks][2 + rr] = there ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 2 * t + 8) : 0u;
-            }
+        for (int ks = 0; ks < 8; ++ks) {
+            const int c16 = ks * 2 + (mi >> 1);
+            ldmatrix_x4(swz128(query_addr + (c16 >> 3) * query_half, c16 & 7), qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
         }
+        mbar_release_stage(smem_u32(&query_empty), lane);
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr)
+            limit[rr] = rr * 8 + g < rows ? min(un.limit0 + un.tile * QT + row_tok[rr], un.hi - 1) : -1;
         float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[16][4];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -272,7 +335,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             mbar_release_stage(smem_u32(&empty_bar[slot]), lane);
         }
         // ---- the part's statistics and sums ----
-        const int64_t part = (static_cast<int64_t>(item) * KG + kg) * Hkv + h;
+        const int64_t part = (static_cast<int64_t>(un.slot) * KG + kg) * Hkv + h;
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             float sum = l[rr];
@@ -295,108 +358,99 @@ struct Parts {
     int count;
 };
 
-// Joins the parts of every row.  One warp per (token, head), tokens of a request in turn; rows that no request owns stay as they
-// were.  Bound by the trips to L2: where the parts are, then their statistics and the first of their sums.
+// Joins the parts of every row, a warp per (token, head); rows that no request owns stay as they were.  Bound by the trips to L2:
+// where the parts are, then their statistics and the first of their sums.
 __global__ void __launch_bounds__(kMergeWarps * 32)
 shared_prefix_merge_kernel(const SharedPrefixParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = static_cast<int>(blockIdx.x) * kMergeWarps + warp;
-    const int b = static_cast<int>(blockIdx.y);
+    const int head = static_cast<int>(blockIdx.y) * kMergeWarps + warp;
+    const int tok = static_cast<int>(blockIdx.x);
     pdl_launch_dependents();
     pdl_wait_prior();
-    const JoinItem j = p.plan.join[b];
+    const JoinItem j = p.plan.join[tok];
     const PlanHead plan = *p.plan.head;
-    if (head >= p.q_heads || !plan.fits) return;
+    if (head >= p.q_heads || !j.owned) return;
     const int h = head / p.group, hh = head - h * p.group, KG = kConsumerWarps / p.kv_heads;
-    // the CTA of the rows kernel that has a stage of the sequence
-    const int64_t early_end = static_cast<int64_t>(plan.early) * plan.early_stages;
-    auto cta_of = [&](int stage) {
-        return stage < early_end ? stage / plan.early_stages : plan.early + static_cast<int>((stage - early_end) / plan.late_stages);
+    auto parts_of = [&](int first, int pieces, int t) {   // of token t of the unit
+        const int tile = t / p.row_tokens, r = (t - tile * p.row_tokens) * p.group + hh;
+        return Parts{(static_cast<int64_t>(first + tile * pieces) * KG * p.kv_heads + h) * RT + r, static_cast<int64_t>(p.kv_heads) * RT,
+                     pieces * KG};
     };
-    auto parts_of = [&](int tile, int tiles, int first, int stages, int r) {
-        Parts x = {0, static_cast<int64_t>(p.kv_heads) * RT, 0};
-        const int mine = r / RT;
-        if (r < 0 || mine >= tiles) return x;
-        const int from = first + mine * stages, c0 = cta_of(from);
-        x.count = (cta_of(from + stages - 1) - c0 + 1) * KG;
-        x.first = (static_cast<int64_t>(tile + mine + c0) * KG * p.kv_heads + h) * RT + r % RT;
-        return x;
-    };
-    for (int tok = j.row0 + static_cast<int>(blockIdx.z); tok < j.row1; tok += static_cast<int>(gridDim.z)) {
-        const Parts own = parts_of(j.own_tile, j.own_tiles, j.own_first, j.own_stages, (tok - j.row0) * p.group + hh);
-        const int t = tok - j.pre_row0;
-        Parts pre = parts_of(j.pre_tile, j.pre_tiles, j.pre_first, j.pre_stages, t * p.group + hh);
-        const int half = kSharedTcTile / p.group, block = t / (2 * half);   // tokens of a chain
-        if (t >= 0 && block < j.tc_blocks) {
-            const int unit = h * j.tc_blocks + block, in_block = t - block * 2 * half, chain = in_block >= half ? 1 : 0;
-            const int from = j.tc_first + unit * j.tc_tiles, chunks = (j.tc_tiles + plan.tc_per - 1) / plan.tc_per;
-            const int c0 = plan.tc_chunked ? j.tc_cta + unit * chunks : from / plan.tc_per;
-            pre.count = plan.tc_chunked ? chunks : (from + j.tc_tiles - 1) / plan.tc_per - c0 + 1;
-            pre.first = p.tc_base + static_cast<int64_t>(j.tc_unit + unit + c0) * (2 * kSharedTcTile) + chain * kSharedTcTile +
-                        (in_block - chain * half) * p.group + hh;
-            pre.step = 2 * kSharedTcTile;
-        }
-        const int n = pre.count + own.count;
-        auto at = [&](int i) { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; };
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float M = -INFINITY, L = 0.f;
-        constexpr int kAhead = 8;   // sums that are requested together with the statistics
-        for (int base = 0; base < n; base += 32) {
-            const int m = min(32, n - base);
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at(base + lane));
-            float4 x[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float Mn = fmaxf(M, warp_max(ml.x));
-            const float ref = Mn == -INFINITY ? 0.f : Mn;
-            const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
-            M = Mn;
-            L = L * shrink + warp_sum(w * ml.y);
-            acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                if (i < m) acc.x += x[i].x * wi, acc.y += x[i].y * wi, acc.z += x[i].z * wi, acc.w += x[i].w * wi;
-            }
-#pragma unroll 4
-            for (int i = kAhead; i < m; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane);
-                acc.x += y.x * wi, acc.y += y.y * wi, acc.z += y.z * wi, acc.w += y.w * wi;
-            }
-        }
-        const float inv = L > 0.f ? 1.f / L : 0.f;   // a row that sees no key: zeros
-        uint2 packed;
-        packed.x = pack_bf16(acc.x * inv, acc.y * inv);
-        packed.y = pack_bf16(acc.z * inv, acc.w * inv);
-        reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(tok) * p.q_heads + head) * kD)[lane] = packed;
+    const Parts own = parts_of(j.own_first, j.own_pieces, j.own_t);
+    const int t = j.pre_t;
+    Parts pre = parts_of(j.pre_first, j.pre_pieces, t);
+    const int half = kSharedTcTile / p.group, block = t / (2 * half);   // tokens of a chain
+    if (block < j.tc_blocks) {
+        const int unit = h * j.tc_blocks + block, in_block = t - block * 2 * half, chain = in_block >= half ? 1 : 0;
+        const int from = j.tc_first + unit * j.tc_tiles, chunks = (j.tc_tiles + plan.tc_per - 1) / plan.tc_per;
+        const int c0 = plan.tc_chunked ? j.tc_cta + unit * chunks : from / plan.tc_per;
+        pre.count = plan.tc_chunked ? chunks : (from + j.tc_tiles - 1) / plan.tc_per - c0 + 1;
+        pre.first = p.tc_base + static_cast<int64_t>(j.tc_unit + unit + c0) * (2 * kSharedTcTile) + chain * kSharedTcTile +
+                    (in_block - chain * half) * p.group + hh;
+        pre.step = 2 * kSharedTcTile;
     }
+    const int n = pre.count + own.count;
+    auto at = [&](int i) { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; };
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, L = 0.f;
+    constexpr int kAhead = 8;   // sums that are requested together with the statistics
+    for (int base = 0; base < n; base += 32) {
+        const int m = min(32, n - base);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at(base + lane));
+        float4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float Mn = fmaxf(M, warp_max(ml.x));
+        const float ref = Mn == -INFINITY ? 0.f : Mn;
+        const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
+        M = Mn;
+        L = L * shrink + warp_sum(w * ml.y);
+        acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            if (i < m) acc.x += x[i].x * wi, acc.y += x[i].y * wi, acc.z += x[i].z * wi, acc.w += x[i].w * wi;
+        }
+#pragma unroll 4
+        for (int i = kAhead; i < m; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane);
+            acc.x += y.x * wi, acc.y += y.y * wi, acc.z += y.z * wi, acc.w += y.w * wi;
+        }
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;   // a row that sees no key: zeros
+    uint2 packed;
+    packed.x = pack_bf16(acc.x * inv, acc.y * inv);
+    packed.y = pack_bf16(acc.z * inv, acc.w * inv);
+    reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(tok) * p.q_heads + head) * kD)[lane] = packed;
 }
 
 int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
+// Query tokens whose heads of a KV head fill a row tile.
+int row_tokens(int64_t group) { return static_cast<int>(RT / group); }
+
 // Where the pieces of the workspace begin, in bytes; partial rows ahead of the tensor-core kernel's.
 struct SharedLayout {
-    int64_t slots, tc_slots, rows, rows_of, tc_of, rows_items, tc_items, join, ml, o, bytes;
+    int64_t slots, tc_slots, rows, tc_of, rows_items, tc_items, join, ml, o, bytes;
 };
 SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads) {
     const int64_t group = q_heads / kv_heads, rows = tokens * group, kg = kConsumerWarps / kv_heads, ctas = sm_count();
     SharedLayout x;
-    // tiles: at most one more than full ones per unit, and every row is in two units
-    x.slots = ctas + 2 * (rows / RT) + batch + groups;
+    // row tiles: at most one more than full ones per unit, and every row is in two units; items: one more than full ones per tile
+    x.slots = kSharedPieces * ctas + 2 * (tokens / row_tokens(group)) + batch + groups;
     x.rows = x.slots * kg * kv_heads * RT;
     // units of the tensor-core kernel: the same of groups that have more than kTcRows rows
     const int64_t tc_groups = groups < rows / (kTcRows + 1) ? groups : rows / (kTcRows + 1);
     x.tc_slots = rows > kTcRows && groups > 0 ? ctas + kv_heads * (tokens / (2 * (kSharedTcTile / group)) + tc_groups) : 0;
     const int64_t part_rows = x.rows + x.tc_slots * (2 * kSharedTcTile);
-    x.rows_of = round256(sizeof(PlanHead));
-    x.tc_of = x.rows_of + round256(ctas * sizeof(int2));
+    x.tc_of = round256(sizeof(PlanHead));
     x.rows_items = x.tc_of + round256(ctas * sizeof(int2));
     x.tc_items = x.rows_items + round256(x.slots * sizeof(RowsItem));
     x.join = x.tc_items + round256(x.tc_slots * sizeof(TcItem));
-    x.ml = x.join + round256(batch * sizeof(JoinItem));
+    x.ml = x.join + round256(tokens * sizeof(JoinItem));
     x.o = x.ml + round256(part_rows * 8);
     x.bytes = x.o + part_rows * kD * 4;
     return x;
@@ -434,7 +488,9 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
                    "attention_shared_prefix: q_heads must be a multiple of kv_heads with group size <= 16");
     B200_CHECK_ARG(a->page_size >= 1 && (a->page_size & (a->page_size - 1)) == 0,
                    "attention_shared_prefix: page_size must be a power of two");
-    B200_CHECK_ARG(a->q_stride_token % 2 == 0 && a->q_stride_head % 2 == 0, "attention_shared_prefix: q strides must be even");
+    B200_CHECK_ARG(a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0 && a->q_stride_token > 0 && a->q_stride_head > 0 &&
+                       a->q_stride_token < (1ll << 38) && a->q_stride_head < (1ll << 38),
+                   "attention_shared_prefix: q strides must be positive multiples of 8");
     B200_CHECK_ARG(a->num_slots > 0 && a->num_slots <= 0x7fffffff, "attention_shared_prefix: num_slots must be in [1, 2^31)");
     B200_CHECK_ARG(a->page_table_stride > 0 && a->page_table_stride <= (1 << 29),
                    "attention_shared_prefix: page_table_stride must be in [1, 2^29]");
@@ -444,8 +500,8 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     B200_CHECK_ARG(a->out && a->q && a->k_cache && a->v_cache && a->page_table && a->table_idx && a->seq_lens && a->qo_indptr &&
                        a->workspace && (a->groups == 0 || (a->group_indptr && a->prefix_lens)),
                    "attention_shared_prefix: NULL tensor");
-    B200_CHECK_ARG(reinterpret_cast<uintptr_t>(a->out) % 8 == 0 && reinterpret_cast<uintptr_t>(a->q) % 4 == 0,
-                   "attention_shared_prefix: out must be 8-byte and q 4-byte aligned");
+    B200_CHECK_ARG(reinterpret_cast<uintptr_t>(a->out) % 8 == 0 && reinterpret_cast<uintptr_t>(a->q) % 16 == 0,
+                   "attention_shared_prefix: out must be 8-byte and q 16-byte aligned");
     int err = B200_OK;
     int* status = device_status_words(&err);
     if (err != B200_OK) return err;
@@ -481,7 +537,6 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     }
     uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a->workspace) + 255) & ~uintptr_t(255));
     p.plan.head = reinterpret_cast<PlanHead*>(ws);
-    p.plan.rows_of = reinterpret_cast<int2*>(ws + x.rows_of);
     p.plan.tc_of = reinterpret_cast<int2*>(ws + x.tc_of);
     p.plan.rows = reinterpret_cast<RowsItem*>(ws + x.rows_items);
     p.plan.tc = reinterpret_cast<TcItem*>(ws + x.tc_items);
@@ -491,14 +546,14 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.tc_base = x.rows;
     p.max_slots = static_cast<int>(x.slots);
     p.tc_slots = static_cast<int>(x.tc_slots);
-    // Queries are copied by tensor maps there.
-    const bool aligned = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride_token % 8 == 0 && a->q_stride_head % 8 == 0 &&
-                         a->q_stride_token > 0 && a->q_stride_head > 0;
-    p.tc_rows = aligned ? kTcRows : 0x7fffffff;
+    p.row_tokens = row_tokens(p.group);
+    p.tc_rows = kTcRows;
     // (a group has more rows than that only if all have)
-    p.with_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > p.tc_rows;
+    p.with_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > kTcRows;
     p.ctas = sm_count();
-    CUtensorMap tk, tv;
+    CUtensorMap tk, tv, tq;
+    err = make_shared_query_tmap(&tq, p, p.q_heads, p.row_tokens);
+    if (err != B200_OK) return err;
     err = make_kv_tmap(&tk, a->k_cache, a->num_slots, a->kv_heads, a->page_size);
     if (err != B200_OK) return err;
     err = make_kv_tmap(&tv, a->v_cache, a->num_slots, a->kv_heads, a->page_size);
@@ -511,12 +566,11 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
         err = launch_shared_prefix_tc(p, a->k_cache, a->v_cache, a->page_size, s);
         if (err != B200_OK) return err;
     }
-    const int smem = kStages * kStageBytes + 1024;
+    const int smem = kStages * kStageBytes + kQueryBytes + 1024;
     B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(p.ctas), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, p));
-    const int turns = div_ceil(a->tokens, a->batch) < 64 ? div_ceil(a->tokens, a->batch) : 64;
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(div_ceil(a->q_heads, kMergeWarps), a->batch, turns),
-                                  dim3(kMergeWarps * 32), 0, s, dim3(1, 1, 1), p));
+    B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(p.ctas), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, tq, p));
+    B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(a->tokens, div_ceil(a->q_heads, kMergeWarps)), dim3(kMergeWarps * 32),
+                                  0, s, dim3(1, 1, 1), p));
     return B200_OK;
 }
 

@@ -45,7 +45,7 @@ constexpr float kLazyLog2 = 8.0f;
 // How K and V tiles are copied ([0] K, [1] V), into 16 groups of 8 keys, each both halves of the head dimension.
 struct SharedKvMaps {
     CUtensorMap q;         // half rows of a chain's tokens, all heads of a KV head
-    CUtensorMap rows[2];   // half rows of min(page, 8) keys: any slot
+    CUtensorMap rows[2];   // half rows of single keys, four to a copy: any slots
     CUtensorMap page[2];   // whole rows of min(page, 128) keys from a slot that 8 divides
     CUtensorMap tile[2];   // whole rows of 128 keys: tiles whose pages are consecutive slots
     int whole_pages, whole_tiles;   // are the latter two there?
@@ -73,6 +73,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Half rows of four slots, one behind the other in shared memory.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int column, int r0, int r1, int r2, int r3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(column), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -95,6 +103,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&maps.q);
         for (int kv = 0; kv < 2; ++kv) {
+            if (maps.kpc < 8) tma_prefetch_desc(&maps.rows[kv]);
             if (maps.whole_pages) tma_prefetch_desc(&maps.page[kv]);
             if (maps.whole_tiles) tma_prefetch_desc(&maps.tile[kv]);
         }
@@ -149,14 +158,15 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
         for (int i = items.x; i < items.y && !failed; ++i) {
             const TcItem it = get_item(i);
             const int32_t* pt_row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride;
-            auto copies_of = [&](int kt) { return (min(kTile, it.keys - kt * kTile) + kpc - 1) / kpc; };
+            // This lane's slots, fetched a tile ahead (the table's trip to L2 would stand between a slot's release and its copy): of keys
+            // lane * 4 .. + 3 where pages are smaller than a group of 8, else of the first keys of pages lane and lane + 32 ...
+            const bool small = kpc < 8;
             int next[4];
-            auto fetch_slots = [&](int kt) {   // a tile ahead: the table's trip to L2 would stand between a slot's release and its copy
-                const int n = copies_of(kt);
+            auto fetch_slots = [&](int kt) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int copy = i * 32 + lane;
-                    next[i] = copy < n ? pt_row[kt * kTile + copy * kpc] : 0;
+                    const int key = kt * kTile + (small ? lane * 4 + i : (i * 32 + lane) * kpc);
+                    next[i] = key < it.keys && (small || (i * 32 + lane) * kpc < kTile) ? pt_row[key] : 0;
                 }
             };
             fetch_slots(it.t0);
@@ -174,54 +184,58 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
             }
             for (int kt = it.t0; kt < it.t1; ++kt) {
                 // A tile whose pages are consecutive slots is one copy; so is a page, unless it is smaller than a group of 8 or starts
-                // inside one.
-                const int n = copies_of(kt);
-                bool whole = it.keys - kt * kTile >= kTile && maps.whole_tiles, groups = maps.whole_pages;
+                // inside one: then every four keys are.
+                const int keys = min(kTile, it.keys - kt * kTile), n = small ? 0 : (keys + kpc - 1) / kpc;
+                const int span = small ? 1 : kpc;   // slots that a table entry stands for here
+                bool whole = keys == kTile && maps.whole_tiles, pages = !small;
                 int sl[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     sl[i] = next[i];
-                    if (sl[i] < 0 || static_cast<int64_t>(sl[i]) + kpc > p.num_slots) {
+                    if (sl[i] < 0 || static_cast<int64_t>(sl[i]) + span > p.num_slots) {
                         atomicExch(&p.status[kStatusBadIndex], sl[i] + 1);
                         sl[i] = 0;
                     }
-                    if ((sl[i] & 7) != 0) groups = false;
+                    if ((sl[i] & 7) != 0) pages = false;
                 }
                 const int first = __shfl_sync(0xffffffffu, sl[0], 0);
                 if ((first & 7) != 0) whole = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int copy = i * 32 + lane;
-                    if (copy < n && sl[i] != first + copy * kpc) whole = false;
+                    const int key = small ? lane * 4 + i : (i * 32 + lane) * kpc;
+                    if (key < kTile && sl[i] != first + key) whole = false;
                 }
                 whole = __all_sync(0xffffffffu, whole);
-                groups = __all_sync(0xffffffffu, groups);
+                pages = __all_sync(0xffffffffu, pages) && (maps.whole_pages || whole);
                 if (kt + 1 < it.t1) fetch_slots(kt + 1);
                 if (!__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(&empty[slot]), phase, p.status, 331))) {
                     failed = true;
                     break;
                 }
                 const uint32_t bar = smem_u32(&full[slot]), base = smem_base + kKVOff + slot * kSlotBytes;
-                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n * kpc) * kD * 2u);
+                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(whole || !pages ? kTile : n * kpc) * kD * 2u);
                 __syncwarp();
                 if (whole) {
                     if (lane == 0) tma_load_5d(base, &maps.tile[kv], 0, 0, 0, first >> 3, it.h, bar);
-                } else {
+                } else if (pages) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int copy = i * 32 + lane;
-                        if (copy >= n) continue;
-                        if (groups) {
-                            tma_load_5d(base + copy * kpc * (kD * 2), &maps.page[kv], 0, 0, 0, sl[i] >> 3, it.h, bar);
-                            continue;
-                        }
-                        for (int key = copy * kpc; key < (copy + 1) * kpc; key += 8) {
-                            const uint32_t dst = base + (key >> 3) * 2048 + (key & 7) * 128;
-                            const int from = sl[i] + key - copy * kpc;
-                            tma_load_3d(dst, &maps.rows[kv], 0, it.h, from, bar);
-                            tma_load_3d(dst + 1024, &maps.rows[kv], 64, it.h, from, bar);
+                        if (copy < n) tma_load_5d(base + copy * kpc * (kD * 2), &maps.page[kv], 0, 0, 0, sl[i] >> 3, it.h, bar);
+                    }
+                } else {
+                    if (!small) {   // pages that start inside a group: their keys' slots
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = kt * kTile + lane * 4 + i;
+                            sl[i] = key < it.keys ? pt_row[key] : 0;
+                            if (sl[i] < 0 || sl[i] >= p.num_slots) sl[i] = 0;
                         }
                     }
+                    // (keys behind the prefix: slot 0's, of which nothing is used)
+                    const uint32_t dst = base + (lane >> 1) * 2048 + (lane & 1) * 512;
+                    tma_gather4(dst, &maps.rows[kv], it.h * kD, sl[0], sl[1], sl[2], sl[3], bar);
+                    tma_gather4(dst + 1024, &maps.rows[kv], it.h * kD + 64, sl[0], sl[1], sl[2], sl[3], bar);
                 }
                 if (++slot == ring_end) {
                     slot = ring;
@@ -515,10 +529,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
 
 }  // namespace
 
-namespace {
-
-// Half rows (64 elements) of the queries [tokens][heads][128]: a KV head's heads of as many tokens as a chain has.
-int make_query_tmap(CUtensorMap* out, const SharedPrefixParams& p) {
+int make_shared_query_tmap(CUtensorMap* out, const SharedPrefixParams& p, int heads, int tokens) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) {
         set_last_error("cuTensorMapEncodeTiled is not available from this driver");
@@ -526,7 +537,7 @@ int make_query_tmap(CUtensorMap* out, const SharedPrefixParams& p) {
     }
     const cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(p.q_heads), static_cast<cuuint64_t>(p.tokens)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.q_sh) * 2, static_cast<cuuint64_t>(p.q_st) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(kTile / p.group)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(tokens)};
     const cuuint32_t es[3] = {1, 1, 1};
     CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(p.q), dims, strides, box, es,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -538,18 +549,17 @@ int make_query_tmap(CUtensorMap* out, const SharedPrefixParams& p) {
     return B200_OK;
 }
 
-}  // namespace
-
 int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream) {
     SharedKvMaps maps = {};
-    int err = make_query_tmap(&maps.q, p);
+    int err = make_shared_query_tmap(&maps.q, p, p.group, kTile / p.group);
     if (err != B200_OK) return err;
     maps.kpc = page_size < kTile ? page_size : kTile;
     maps.whole_pages = maps.kpc >= 8 && p.num_slots >= 8 ? 1 : 0;
-    maps.whole_tiles = maps.kpc < kTile && p.num_slots >= kTile ? 1 : 0;
+    maps.whole_tiles = p.num_slots >= kTile ? 1 : 0;
     for (int kv = 0; kv < 2; ++kv) {
         const void* cache = kv == 0 ? k_cache : v_cache;
-        err = make_kv_tile_tmap(&maps.rows[kv], cache, p.num_slots, p.kv_heads, maps.kpc < 8 ? maps.kpc : 8);
+        const uint64_t width = static_cast<uint64_t>(p.kv_heads) * kD;
+        err = make_tmap_2d_bf16_sw128(&maps.rows[kv], cache, width, static_cast<uint64_t>(p.num_slots), width * 2, 64, 1);
         if (err == B200_OK && maps.whole_pages) err = make_kv_groups_tmap(&maps.page[kv], cache, p.num_slots, p.kv_heads, maps.kpc);
         if (err == B200_OK && maps.whole_tiles) err = make_kv_groups_tmap(&maps.tile[kv], cache, p.num_slots, p.kv_heads, kTile);
         if (err != B200_OK) return err;

@@ -4,12 +4,14 @@
 // rows; the rows kernel over everything else; and the kernel that joins a row's parts.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace b200 {
 
 constexpr int kSharedMaxBatch = 1024;
-constexpr int kSharedRowTile = 16;     // query rows of a tile of the rows kernel
+constexpr int kSharedPieces = 4;       // items of the rows kernel per CTA, about
 constexpr int kSharedTcTile = 128;     // keys of a tile of the tensor-core kernel, and query rows of one of its chains
 
 // Units are the groups' prefixes (0 .. groups) and the requests' own keys (groups .. groups + batch).
@@ -24,7 +26,7 @@ struct __align__(16) RowsItem {
     int tile;          // row tile
     int s_begin, s_end;
     int reread;        // other row tiles read the same keys
-    int pad;
+    int slot;          // of its partial results; -1: there are no more items
 };
 
 // ... and of the tensor-core kernel: tiles [t0, t1) of a prefix for a block of rows.
@@ -37,31 +39,33 @@ struct __align__(16) TcItem {
     int pad;
 };
 
-// Where the parts of a request's rows are.  A row tile's stages (a unit's key tiles) are spread over neighbouring CTAs, and parts lie
-// at tile + CTA (unit + CTA).
+// Where the parts of a token's rows are.  A row tile has `pieces` parts one behind the other in the rows kernel's slots; in the
+// tensor-core kernel's a unit's parts lie at unit + CTA.
 struct __align__(16) JoinItem {
-    int row0, row1;                      // query rows
-    int own_tile, own_tiles, own_first, own_stages;   // tiles before, tiles, stages before, stages per tile
-    int pre_row0;                        // first query row of the group
-    int pre_tile, pre_tiles, pre_first, pre_stages;   // the group's prefix in the rows kernel, or ...
+    int owned;                                        // 0: by no request, nothing is written
+    int own_t, own_first, own_pieces;                 // its place among the request's tokens, the request's own keys
+    int pre_t;                                        // its place among the group's tokens
+    int pre_first, pre_pieces;                        // the group's prefix in the rows kernel, or ...
     int tc_unit, tc_blocks, tc_first, tc_tiles, tc_cta;   // ... in the tensor-core kernel: units before, blocks per KV head, tiles before,
                                                           // tiles per unit, first CTA
+    int pad[4];
 };
 
 struct __align__(16) PlanHead {
-    int fits;                     // 0: index arrays ask for more room than the host has counted; nothing is written
-    int early, early_stages, late_stages;   // rows kernel: stages of each of the first `early` CTAs, and of each of the others
+    int fits;                     // 0: the index arrays are no such arrays; nothing is written
+    int rows_items;
     int tc_per, tc_chunked;       // tensor-core kernel: tiles per CTA, in chunks of one unit or in runs
+    int next;                     // rows kernel: the first item that nobody has taken yet
+    int rows_lead;                // ... and how many a CTA takes ahead of the one it copies
     int pad[2];
 };
 
 struct SharedPlan {
     PlanHead* head;
-    int2* rows_of;       // [CTAs] items of a CTA of the rows kernel
-    int2* tc_of;         // [CTAs] ... of the tensor-core kernel
-    RowsItem* rows;      // [max_slots], item = slot of its partial results
-    TcItem* tc;          // [tc_slots]
-    JoinItem* join;      // [batch]
+    int2* tc_of;         // [CTAs] items of a CTA of the tensor-core kernel
+    RowsItem* rows;      // [max_slots]
+    TcItem* tc;          // [tc_slots], item = slot of its partial results
+    JoinItem* join;      // [tokens]
 };
 
 struct SharedPrefixParams {
@@ -74,6 +78,7 @@ struct SharedPrefixParams {
     int tokens, batch, groups;
     int q_heads, kv_heads, group;   // group: query heads per KV head
     int stage_keys, kpc;            // rows kernel: keys per stage and per copy
+    int row_tokens;                 // ... and query tokens per row tile: 16 / group
     int64_t num_slots;
     float scale_log2;
     float *ws_ml, *ws_o;            // partial rows, (maximum, sum) and x 128: the rows kernel's [max_slots, key groups, kv_heads, row tile],
@@ -86,6 +91,8 @@ struct SharedPrefixParams {
     int* status;
 };
 
+// Half rows (64 elements) of the queries [tokens][heads][128]: `heads` heads of `tokens` tokens per copy.
+int make_shared_query_tmap(CUtensorMap* out, const SharedPrefixParams& p, int heads, int tokens);
 int launch_shared_prefix_plan(const SharedPrefixParams& p, cudaStream_t stream);
 int launch_shared_prefix_tc(const SharedPrefixParams& p, const void* k_cache, const void* v_cache, int page_size, cudaStream_t stream);
 

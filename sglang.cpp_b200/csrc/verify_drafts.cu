@@ -83,19 +83,54 @@ verify_drafts_kernel(const VerifyParams p) {
     const int without = refused && p.draft == nullptr ? p.draft_tokens[start + a] : -1;   // a draft that was certain
     const int run = ((p.vocab + C * kWarps - 1) / (C * kWarps) + 127) / 128 * 128;
     const int first = min((rank * kWarps + warp) * run, p.vocab), last = min(first + run, p.vocab);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(prow) | reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
     bool rest = refused;   // p - q; or p, where no entry of p exceeds q
-    auto weight = [&](int i) -> double {
-        const float x = entry(__ldg(prow + i));
-        if (!rest) return x;
-        if (qrow == nullptr) return i == without ? static_cast<double>(fmaxf(x - 1.f, 0.f)) : static_cast<double>(x);
-        return fmax(static_cast<double>(x) - static_cast<double>(entry(__ldg(qrow + i))), 0.0);
+    auto weigh = [&](float x, float y, int i) -> double {
+        const float px = entry(x);
+        if (!rest) return px;
+        if (qrow == nullptr) return i == without ? fmaxf(px - 1.f, 0.f) : px;
+        return fmax(static_cast<double>(px) - static_cast<double>(entry(y)), 0.0);
+    };
+    // Sum of entries [from, to), lanes next to one another; the loads of a round before its sums.
+    auto sum_of = [&](int from, int to) {
+        const bool both = rest && qrow != nullptr;
+        double sum = 0.0;
+        if (aligned && ((from | to) & 3) == 0) {
+            constexpr int kRound = 4;
+            for (int base = from; base < to; base += kRound * 128) {
+                float4 x[kRound], y[kRound];
+#pragma unroll
+                for (int k = 0; k < kRound; ++k) {
+                    const int i = base + k * 128 + lane * 4;
+                    x[k] = i < to ? __ldg(reinterpret_cast<const float4*>(prow + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    y[k] = both && i < to ? __ldg(reinterpret_cast<const float4*>(qrow + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < kRound; ++k) {
+                    const int i = base + k * 128 + lane * 4;
+                    sum += (weigh(x[k].x, y[k].x, i) + weigh(x[k].y, y[k].y, i + 1)) + (weigh(x[k].z, y[k].z, i + 2) + weigh(x[k].w, y[k].w, i + 3));
+                }
+            }
+        } else {
+            constexpr int kRound = 8;
+            for (int base = from; base < to; base += kRound * 32) {
+                float x[kRound], y[kRound];
+#pragma unroll
+                for (int k = 0; k < kRound; ++k) {
+                    const int i = base + k * 32 + lane;
+                    x[k] = i < to ? __ldg(prow + i) : 0.f;
+                    y[k] = both && i < to ? __ldg(qrow + i) : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < kRound; ++k) sum += weigh(x[k], y[k], base + k * 32 + lane);
+            }
+        }
+        return sum;
     };
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     double total = 0.0, before = 0.0, mine = 0.0;   // of the row, of the runs before this warp's, of this run
     for (int pass = 0; pass < 2; ++pass) {
-        double sum = 0.0;
-#pragma unroll 8
-        for (int i = first + lane; i < last; i += 32) sum += weight(i);
+        double sum = sum_of(first, last);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s_sum[warp] = sum;
@@ -139,24 +174,37 @@ verify_drafts_kernel(const VerifyParams p) {
     }
     const double goal = unit_interval(p.draw[b]) * total;
     if (!(mine > 0.0) || goal < before || goal >= before + mine) return;
-    double ahead = before;
-    int pick = -1, positive = -1;
-    for (int base = first; base < last && pick < 0; base += 32) {
-        const int i = base + lane;
-        const double w = i < last ? weight(i) : 0.0;
-        double incl = w;
+    // The run once more: a stretch of neighbouring entries per lane, then, of the lane whose stretch the goal is in, an entry per lane.
+    // (The sums are formed in another order than before: the last bits may put the goal behind the run's last entry.)
+    auto scan = [&](double w) {   // sums up to and with each lane's
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const double t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += t;
+            const double t = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += t;
         }
-        const uint32_t over = __ballot_sync(0xffffffffu, w > 0.0 && ahead + incl > goal);
-        const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
-        if (over != 0) pick = base + __ffs(over) - 1;
+        return w;
+    };
+    auto weight = [&](int i) { return weigh(__ldg(prow + i), rest && qrow != nullptr ? __ldg(qrow + i) : 0.f, i); };
+    const int stretch = (last - first + 31) / 32;
+    double own = 0.0;
+#pragma unroll 8
+    for (int i = 0; i < stretch; ++i)
+        if (first + lane * stretch + i < last) own += weight(first + lane * stretch + i);
+    const double upto = scan(own);
+    const uint32_t over = __ballot_sync(0xffffffffu, own > 0.0 && before + upto > goal), some = __ballot_sync(0xffffffffu, own > 0.0);
+    const int chosen = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
+    double ahead = before + __shfl_sync(0xffffffffu, upto, chosen) - __shfl_sync(0xffffffffu, own, chosen);
+    const int from = first + chosen * stretch, to = min(from + stretch, last);
+    int pick = -1, positive = -1;
+    for (int base = from; base < to && pick < 0; base += 32) {
+        const int i = base + lane;
+        const double w = i < to ? weight(i) : 0.0;
+        const double incl = scan(w);
+        const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && ahead + incl > goal), any = __ballot_sync(0xffffffffu, w > 0.0);
+        if (hit != 0) pick = base + __ffs(hit) - 1;
         if (any != 0) positive = base + 31 - __clz(any);
         ahead += __shfl_sync(0xffffffffu, incl, 31);
     }
-    // (the walk adds in another order than the sums: the last bits may put the goal behind the run's last entry)
     if (lane == 0) *out = pick >= 0 ? pick : positive;
 }
 

@@ -21,12 +21,12 @@ def _attention(pkg, **change):
     (dict(head_dim=64), "head_dim"), (dict(batch=1025), "batch"), (dict(batch=-1), "batch"), (dict(tokens=-1), "batch"),
     (dict(groups=5), "groups"), (dict(groups=-1), "groups"), (dict(kv_heads=3), "kv_heads"), (dict(kv_heads=16, q_heads=16), "kv_heads"),
     (dict(kv_heads=0), "kv_heads"), (dict(q_heads=20), "q_heads"), (dict(q_heads=0), "q_heads"), (dict(q_heads=136), "q_heads"),
-    (dict(page_size=12), "page_size"), (dict(page_size=0), "page_size"), (dict(q_stride_token=2049), "strides"),
-    (dict(q_stride_head=129), "strides"), (dict(num_slots=0), "num_slots"), (dict(num_slots=1 << 31), "num_slots"),
+    (dict(page_size=12), "page_size"), (dict(page_size=0), "page_size"), (dict(q_stride_token=2052), "strides"),
+    (dict(q_stride_head=132), "strides"), (dict(q_stride_head=0), "strides"), (dict(q_stride_token=-2048), "strides"), (dict(num_slots=0), "num_slots"), (dict(num_slots=1 << 31), "num_slots"),
     (dict(page_table_stride=0), "page_table_stride"), (dict(tokens=1 << 27), "too many"), (dict(out=None), "NULL"), (dict(q=None), "NULL"),
     (dict(group_indptr=None), "NULL"), (dict(prefix_lens=None), "NULL"), (dict(workspace=None), "NULL"), (dict(qo_indptr=None), "NULL"),
     (dict(sm_scale=0.0), "sm_scale"), (dict(sm_scale=-1.0), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"),
-    (dict(sm_scale=float("inf")), "sm_scale"), (dict(out=260), "aligned"), (dict(q=258), "aligned"),
+    (dict(sm_scale=float("inf")), "sm_scale"), (dict(out=260), "aligned"), (dict(q=264), "aligned"),
 ])
 def test_attention_refusals(pkg, change, text):
     rc, said = _attention(pkg, **change)

@@ -182,13 +182,16 @@ def test_shared_prefix_reports_slots_outside_the_pool(L):
     assert L.read_device_status() == (0, -2)
 
 
-def test_shared_prefix_refuses_overlapping_requests(L):
-    """Requests whose rows overlap want more partial results than there is room for: reported, nothing written."""
+@pytest.mark.parametrize("name,at,value", [("qo", 1, 64), ("qo", 64, 65), ("qo", 0, -1), ("qo", 30, 28), ("groups", 1, 65),
+                                           ("groups", 0, -1), ("groups", 1, 1)])
+def test_shared_prefix_reports_odd_index_arrays(L, name, at, value):
+    """Requests or groups that overlap, or lie outside the rows there are: reported, nothing written."""
     n = 64
-    s = SharedSetup([[(20, 1)] * n], [100], 16, 16, 8, seed=13)
-    s.qo = np.asarray([0, n] * (n // 2) + [n], np.int32)
+    s = SharedSetup([[(20, 1)] * 40, [(20, 1)] * 24], [100, 100], 16, 16, 8, seed=13)
+    (s.qo if name == "qo" else s.group_indptr)[at] = value
+    if (name, value) == ("groups", 1):
+        s.group_indptr[:] = (2, 1, n)
     out = torch.full((n, 16 * D), 7.0, dtype=bf16, device="cuda")
-    s.lens = [120] * n
     s.run(L, out=out)
     torch.cuda.synchronize()
     assert L.read_device_status() == (0, n + 1) and bool((out == 7).all())
