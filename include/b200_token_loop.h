@@ -357,7 +357,7 @@ B200_API int b200_sample_from_probs(int32_t* out, const float* probs, int rows, 
  * all), of those over the entries whose cumulative probability, their own included, stays within top_p[r] (never without
  * the largest; 1: all), zeros elsewhere.  A temperature of at most 1e-6 (or NaN) gives 1 at the first maximum.  top_k, top_p:
  * device arrays or NULL.  bf16 logits [rows, vocab] of row stride ld, fp32 out [rows, vocab] contiguous.  A NaN counts as
- * -inf; a row of nothing else becomes zeros.  Cuts are decided by 64-bit sums.  vocab up to 327680. */
+ * -inf; a row of nothing else becomes zeros.  Cuts are decided by 64-bit sums.  vocab up to 2^24. */
 B200_API int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, int vocab,
                                  const float* temperatures, const int32_t* top_k, const float* top_p,
                                  b200_stream_t stream);

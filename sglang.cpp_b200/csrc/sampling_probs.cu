@@ -11,20 +11,30 @@
 // them; the few entries outside are added up one by one in fp64, by class (above, between, below).  Where a border falls among those
 // it is found by bisection of the patterns instead, 16 rounds of counts or sums over the whole row.
 //
-// A cluster of CTAs owns a row and keeps it in registers: read once, written once.  The counters meet by ranges of patterns: CTA r adds
-// up all CTAs' counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which thread's
-// patterns the cut falls.  Bound by HBM, 6 bytes per entry; with filters also by the counting, an atomic per entry in shared
-// memory.  CTAs of 512 threads, two on an SM, so that one's loads and stores lie under the other's meetings.
+// A CTA, or where rows are few a cluster of them, owns a row and goes over it from memory once and from L2 once or twice more.
+//     no filter:       sums under a running maximum; results.
+//     top_k <= 256:    the lanes' maxima; of every warp's 32 the r-th largest, r = ceil(top_k / warps): the smallest of these has top_k
+//                      entries at or above it.  A second round lists all such entries (some hundreds), which are sorted, weighed and
+//                      cut; the results are zeros but for what is kept.
+//     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
+//                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
+//                      thread's patterns the cut falls.
+// Bound by HBM, 6 bytes per entry; the last kind also by the counting, an atomic per entry in shared memory.  CTAs of 256 threads, four
+// on an SM, so that one's loads and stores lie under another's sorting.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxVectors = 10;             // of 8 entries, per thread
+constexpr int kMaxVocab = 1 << 24;
+constexpr int kWaves = 4;
+constexpr int kList = 2048;                 // entries that can be listed
 constexpr int kBins = 8192;                 // counted patterns: half of them positive
 constexpr int kHalf = kBins / 2;
 constexpr uint32_t kLowMagnitude = 0x3380;  // 2^-24
@@ -68,7 +78,9 @@ constexpr int kClasses = 3;
 struct Meet {   // each CTA's copy: what the CTAs of a row tell one another
     float top[kMaxCluster];                  // the share's maximum
     int first[kMaxCluster];                  // where it is first
-    double sum[kMaxCluster];                 // weights: of the share (no filters), of the CTA's range of patterns
+    float from[kMaxCluster];                 // top_k entries of the share are at least this
+    int listed[kMaxCluster];
+    double sum[kMaxCluster];                 // weights: of the share under its maximum (no filters), of the CTA's range of patterns
     int count[kMaxCluster];                  // entries in that range
     int out_count[kMaxCluster][kClasses];
     double out_sum[kMaxCluster][kClasses];
@@ -112,20 +124,42 @@ __device__ __noinline__ double weight64(float a, float top, double per_t) {
     return e < -200.0 ? 0.0 : exp2(e);
 }
 
+// Are exponents of the form a s - max s good enough in fp32?  Not where the second term is infinite or its rounding more than a half
+// (nor, then, with a temperature of 0 or infinity).
+__device__ __forceinline__ bool fp32_does(float top, float s) { return fabsf(top * s) < 4e6f && s > 1e-30f && s < 1e30f; }
+
 // A logit: a NaN as -inf, one kind of zero.
 __device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.f, -INFINITY); }
 
-// VECTORS: of 8 entries per thread.  ALIGNED: rows of both sides are read and written 16 bytes at a time; else entry by entry, neighbours
-// by neighbouring threads.
-template <int VECTORS, bool FILTERS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, VECTORS <= 5 ? 2 : 1)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two entries, a NaN as -inf.
+__device__ __forceinline__ uint32_t number_or_low(uint32_t w) {
+    uint32_t low = 0xff80ff80u;
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w), *reinterpret_cast<__nv_bfloat162*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+// The largest of eight entries (two at a time; a NaN loses against a number).
+__device__ __forceinline__ float largest_of(const uint4& a) {
+    auto pair = [](uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(pair(a.x), pair(a.y)), __hmax2(pair(a.z), pair(a.w)));
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+    return fmaxf(fmaxf(bf16_lo(w), bf16_hi(w)) + 0.f, -INFINITY);
+}
+
+// ALIGNED: rows of both sides are read and written 16 bytes at a time; else entry by entry, neighbours by neighbouring threads.
+template <bool FILTERS, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, 4)
 sampling_probs_kernel(const ProbsParams p) {
-    constexpr int N = VECTORS * 8;
     __shared__ __align__(16) int hist[FILTERS ? kBins : 4];
     __shared__ Meet meet;
     __shared__ double s_d[kWarps];
+    __shared__ float s_f[kWarps];
     __shared__ int s_i[kWarps], s_cut;
-    __shared__ int s_count[kClasses];
+    __shared__ int s_count[kClasses], s_listed;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, row = static_cast<int>(blockIdx.x) / C;
@@ -135,40 +169,6 @@ sampling_probs_kernel(const ProbsParams p) {
     pdl_wait_prior();
     const __nv_bfloat16* x = p.logits + static_cast<int64_t>(row) * p.ld + begin;
     float* out = p.out + static_cast<int64_t>(row) * p.vocab + begin;
-    // Entry e of this thread's vector j is entry ... of the share.
-    auto place = [&](int i) { return ALIGNED ? ((i >> 3) * kThreads + tid) * 8 + (i & 7) : i * kThreads + tid; };
-
-    // ---- the share, in registers, two entries to one; what lies behind the row as -inf ----
-    uint32_t raw[N / 2];
-    if (ALIGNED) {
-#pragma unroll
-        for (int j = 0; j < VECTORS; ++j) {
-            const int at = (j * kThreads + tid) * 8;
-            uint4 a = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-            if (at + 8 <= n) a = __ldg(reinterpret_cast<const uint4*>(x + at));
-            raw[j * 4] = a.x, raw[j * 4 + 1] = a.y, raw[j * 4 + 2] = a.z, raw[j * 4 + 3] = a.w;
-        }
-#pragma unroll
-        for (int j = 0; j < VECTORS; ++j) {
-            const int at = (j * kThreads + tid) * 8;
-            if (at < n && at + 8 > n) {   // the row's last entries
-                for (int e = 0; e < n - at; ++e) {
-                    const uint32_t bits = __bfloat16_as_ushort(x[at + e]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (k == e >> 1) raw[j * 4 + k] = (e & 1) ? (raw[j * 4 + k] & 0xffffu) | bits << 16 : (raw[j * 4 + k] & 0xffff0000u) | bits;
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint32_t lo = place(i) < n ? __bfloat16_as_ushort(x[place(i)]) : 0xff80u;
-            const uint32_t hi = place(i + 1) < n ? __bfloat16_as_ushort(x[place(i + 1)]) : 0xff80u;
-            raw[i >> 1] = hi << 16 | lo;
-        }
-    }
-    auto entry = [&](int i) { return clean((i & 1) ? bf16_hi(raw[i >> 1]) : bf16_lo(raw[i >> 1])); };
     const float T = p.temperatures[row];
     const bool greedy = !(T > 1.0000001e-6f);
     int K = FILTERS && p.top_k != nullptr ? p.top_k[row] : 0;
@@ -176,68 +176,317 @@ sampling_probs_kernel(const ProbsParams p) {
     const float P = FILTERS && p.top_p != nullptr ? p.top_p[row] : 1.f;
     const bool want_k = K < p.vocab, want_p = P < 1.f;
     const bool filter = FILTERS && !greedy && (want_k || want_p);
+    const double per_t = 1.4426950408889634 / static_cast<double>(T);
+    const float s_hi = static_cast<float>(per_t);
+
+    // eight(their patterns, the first one's place) or one(entry, place) for all of the share, a round's loads ahead of its work.
+    auto all_of = [&](auto eight, auto one) {
+        if (ALIGNED) {
+            constexpr int kRound = 4;
+            const int vectors = n >> 3;
+            for (int v0 = tid; v0 < vectors; v0 += kRound * kThreads) {
+                uint4 a[kRound];
+#pragma unroll
+                for (int j = 0; j < kRound; ++j)
+                    if (v0 + j * kThreads < vectors) a[j] = __ldg(reinterpret_cast<const uint4*>(x) + v0 + j * kThreads);
+#pragma unroll
+                for (int j = 0; j < kRound; ++j) {
+                    if (v0 + j * kThreads >= vectors) break;
+                    eight(a[j], (v0 + j * kThreads) * 8);
+                }
+            }
+            if (const int i = vectors * 8 + tid; i < n) one(clean(__bfloat162float(x[i])), i);
+        } else {
+            constexpr int kRound = 8;
+            for (int i0 = tid; i0 < n; i0 += kRound * kThreads) {
+                float a[kRound];
+#pragma unroll
+                for (int j = 0; j < kRound; ++j) a[j] = i0 + j * kThreads < n ? clean(__bfloat162float(x[i0 + j * kThreads])) : -INFINITY;
+#pragma unroll
+                for (int j = 0; j < kRound; ++j) {
+                    if (i0 + j * kThreads >= n) break;
+                    one(a[j], i0 + j * kThreads);
+                }
+            }
+        }
+    };
+    // f(eight neighbouring entries, or one; how many; the first one's place); eight of which none reaches the bound go to else_f instead.
+    auto each_from = [&](float bound, auto f, auto else_f) {
+        all_of(
+            [&](const uint4& a, int at) {
+                if (bound > -INFINITY && largest_of(a) < bound) {
+                    else_f(at);
+                    return;
+                }
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = clean((e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]));
+                f(y, std::integral_constant<int, 8>{}, at);
+            },
+            [&](float a, int at) {
+                const float y[1] = {a};
+                f(y, std::integral_constant<int, 1>{}, at);
+            });
+    };
+    auto each = [&](auto f) { each_from(-INFINITY, f, [](int) {}); };
+    // This thread's largest entry.
+    auto largest = [&]() {
+        float top = -INFINITY;
+        all_of([&](const uint4& a, int) { top = fmaxf(top, largest_of(a)); }, [&](float a, int) { top = fmaxf(top, a); });
+        return top;
+    };
+    // Eight neighbouring results, whole sectors at once where rows begin with one (halves of them: 20 percent of the time).
+    const bool sectors = ALIGNED && reinterpret_cast<uintptr_t>(out) % 32 == 0;
+    auto store8 = [&](const float (&z)[8], int at) {
+        if (sectors) {
+            asm volatile("st.global.cs.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + at), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]),
+                         "f"(z[4]), "f"(z[5]), "f"(z[6]), "f"(z[7])
+                         : "memory");
+        } else {
+            __stcs(reinterpret_cast<float4*>(out + at), make_float4(z[0], z[1], z[2], z[3]));
+            __stcs(reinterpret_cast<float4*>(out + at) + 1, make_float4(z[4], z[5], z[6], z[7]));
+        }
+    };
+    // value(entry, place) to the results.
+    auto store_from = [&](float bound, auto value) {   // (entries below the bound: 0)
+        each_from(bound, [&](const auto& y, auto count, int at) {
+            if constexpr (count() == 8) {
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = value(y[e], at + e);
+                store8(z, at);
+            } else {
+                __stcs(out + at, value(y[0], at));
+            }
+        }, [&](int at) {
+            const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            store8(z, at);
+        });
+    };
+    auto store = [&](auto value) { store_from(-INFINITY, value); };
+
+    if (FILTERS && tid == 0) {
+        meet.value[0] = meet.value[1] = -INFINITY;
+        meet.ties[0] = meet.ties[1] = 0x7fffffff;
+        s_cut = 0x7fffffff;
+        s_listed = 0;
+    }
+    bool met = false;   // the first wait for the cluster is done
+    auto meet_first = [&]() {
+        if (!met) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        met = true;
+    };
+    if constexpr (FILTERS) {
+        if (filter && want_k && K <= kThreads) {
+            // ---- a bound that top_k entries reach ----
+            float top = largest();
+            const int r = (K + kWarps - 1) / kWarps;
+            float sorted = top;   // of the lanes, the largest first
+#pragma unroll
+            for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+                for (int o = size / 2; o > 0; o /= 2) {
+                    const float other = __shfl_xor_sync(0xffffffffu, sorted, o);
+                    const bool down = (lane & size) == 0 || size == 32, low = (lane & o) == 0;
+                    sorted = low == down ? fmaxf(sorted, other) : fminf(sorted, other);
+                }
+            const float reach = __shfl_sync(0xffffffffu, sorted, r - 1);
+            top = __shfl_sync(0xffffffffu, sorted, 0);
+            if (lane == 0) {
+                s_f[warp] = reach;
+                s_d[warp] = top;
+            }
+            __syncthreads();
+            float from = INFINITY;
+            for (int w = 0; w < kWarps; ++w) {
+                from = fminf(from, s_f[w]);
+                top = fmaxf(top, static_cast<float>(s_d[w]));
+            }
+            meet_first();
+            if (tid == 0) {
+                tell(&meet.top[rank], C, top);
+                tell(&meet.from[rank], C, from);
+            }
+            meet_all();
+            float xmax = -INFINITY;
+            for (int i = 0; i < C; ++i) {
+                from = fmaxf(from, meet.from[i]);
+                xmax = fmaxf(xmax, meet.top[i]);
+            }
+            // ---- the entries that reach it, by value and place in one word, the larger value and the earlier place the smaller word ----
+            uint64_t* list = reinterpret_cast<uint64_t*>(hist) + kList;   // this share's; all of them sorted ahead of it
+            uint64_t* all = reinterpret_cast<uint64_t*>(hist);
+            if (from > -INFINITY)
+                each_from(from, [&](const auto& y, auto count, int at) {
+#pragma unroll
+                    for (int e = 0; e < count(); ++e)
+                        if (y[e] >= from) {
+                            const int i = atomicAdd(&s_listed, 1);
+                            if (i < kList) list[i] = static_cast<uint64_t>(0xffffu - key_of(y[e])) << 32 | static_cast<uint32_t>(begin + at + e);
+                        }
+                }, [](int) {});
+            __syncthreads();
+            if (tid == 0) tell(&meet.listed[rank], C, from > -INFINITY ? s_listed : kList + 1);
+            meet_all();
+            int total = 0, before = 0;
+            for (int i = 0; i < C; ++i) {
+                if (i < rank) before += min(meet.listed[i], kList + 1);
+                total += min(meet.listed[i], kList + 1);
+            }
+            if (total <= kList) {
+                int size = 32;
+                while (size < total) size *= 2;
+                for (int i = tid; i < size; i += kThreads) {
+                    uint64_t word = ~0ull;
+                    int at = i, who = 0;
+                    while (who < C - 1 && at >= meet.listed[who]) at -= meet.listed[who++];
+                    if (i < total) {
+                        if (C == 1) word = list[i];
+                        else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(word) : "r"(remote(list + at, who)));
+                    }
+                    all[i] = word;
+                }
+                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (nothing remote is read any more; waited for at the end)
+                __syncthreads();
+                for (int run = 2; run <= size; run *= 2)
+                    for (int o = run / 2; o > 0; o /= 2) {
+                        for (int i = tid; i < size / 2; i += kThreads) {
+                            const int a = 2 * i - (i & (o - 1)), b = a + o;
+                            const uint64_t wa = all[a], wb = all[b];
+                            if ((wa > wb) == ((a & run) == 0)) {
+                                all[a] = wb;
+                                all[b] = wa;
+                            }
+                        }
+                        __syncthreads();
+                    }
+                // ---- weights of the first top_k, and what of them stays ----
+                const uint64_t word = all[tid];   // (at least 32; behind them whatever is there is not used)
+                const bool there = tid < K && tid < total;
+                const double w = there ? weight64(value_of(0xffffu - static_cast<uint32_t>(word >> 32)), xmax, per_t) : 0.0;
+                double upto = w;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double d = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += d;
+                }
+                if (lane == 31) s_d[warp] = upto;
+                __syncthreads();
+                double sum = 0.0, ahead = 0.0;
+                for (int i = 0; i < kWarps; ++i) {
+                    if (i == warp) ahead = sum;
+                    sum += s_d[i];
+                }
+                upto += ahead;
+                const bool stays = there && w > 0.0 && (!want_p || tid == 0 || upto <= fmax(static_cast<double>(P), 0.0) * sum);
+                double kept = stays ? w : 0.0;
+                kept = warp_sum(kept);
+                __syncthreads();
+                if (lane == 0) s_d[warp] = kept;
+                for (int i = tid; i < (ALIGNED ? n >> 2 : 0); i += kThreads) __stcs(reinterpret_cast<float4*>(out) + i, make_float4(0.f, 0.f, 0.f, 0.f));
+                for (int i = (ALIGNED ? n & ~3 : 0) + tid; i < n; i += kThreads) __stcs(out + i, 0.f);
+                __syncthreads();   // (the zeros are ahead of what is kept)
+                kept = 0.0;
+                for (int i = 0; i < kWarps; ++i) kept += s_d[i];
+                const int place = static_cast<int>(word & 0xffffffffu) - begin;
+                if (stays && place >= 0 && place < n) out[place] = static_cast<float>(w / kept);
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+                return;
+            }
+            // (too many: counted like the others.  The lists have been read by nobody.)
+        }
+    }
+    // ---- the maximum; without filters also the sum under a running one, with them the counts ----
+    float top = -INFINITY, part = 0.f, at = -INFINITY;
+    bool outside = false;
     if (FILTERS && filter) {
         for (int i = tid; i < kBins / 4; i += kThreads) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
         if (tid < kClasses) s_count[tid] = 0;
         __syncthreads();
-    }
-    float top = -INFINITY;
+        auto count_one = [&](uint32_t bits) {   // (patterns outside may be a NaN's: looked at again below)
+            const int m = static_cast<int>(bits & 0x7fffu) - static_cast<int>(kLowMagnitude);
+            const int bin = kHalf + (m ^ (static_cast<int>(bits << 16) >> 31));
+            if (static_cast<uint32_t>(m) < static_cast<uint32_t>(kHalf)) atomicAdd(&hist[bin], 1);
+            else outside = true;
+        };
+        all_of(
+            [&](const uint4& a, int) {
+                top = fmaxf(top, largest_of(a));
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, entry(i));
-    bool outside = false;
-    if (FILTERS && filter) {
+                for (int e = 0; e < 4; ++e) {
+                    count_one(w[e] & 0xffffu);
+                    count_one(w[e] >> 16);
+                }
+            },
+            [&](float a, int) {
+                top = fmaxf(top, a);
+                count_one(__float_as_uint(a) >> 16);
+            });
+    } else if (greedy) {
+        top = largest();
+    } else {
+        // 2^(y s - at), at = s times the maximum so far
+        all_of(
+            [&](const uint4& a, int) {
+                const float here = largest_of(a);
+                if (here > top) {
+                    const float now = fmaxf(here * s_hi, -3.402823466e38f);   // (nothing but a mask's lowest numbers so far)
+                    part *= exp2f(at - now);   // (the first time: nothing)
+                    top = here;
+                    at = now;
+                }
+                const uint32_t w[4] = {number_or_low(a.x), number_or_low(a.y), number_or_low(a.z), number_or_low(a.w)};
+                float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int bin = bin_of(entry(i));
-            if (bin >= 0) atomicAdd(&hist[bin], 1);
-            else if (place(i) < n) outside = true;
-        }
+                for (int e = 0; e < 8; ++e) sum += ex2(fmaf((e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]), s_hi, -at));
+                if (top > -INFINITY) part += sum;
+            },
+            [&](float a, int) {
+                if (a > top) {
+                    const float now = fmaxf(a * s_hi, -3.402823466e38f);
+                    part *= exp2f(at - now);
+                    top = a;
+                    at = now;
+                }
+                if (top > -INFINITY) part += ex2(fmaf(a, s_hi, -at));
+            });
     }
+    const float my_top = top;
     top = warp_max(top);
-    if (lane == 0) s_d[warp] = top;
-    if (tid == 0) {
-        meet.value[0] = meet.value[1] = -INFINITY;
-        meet.ties[0] = meet.ties[1] = 0x7fffffff;
-        s_cut = 0x7fffffff;
-    }
+    if (lane == 0) s_f[warp] = top;
     outside = __syncthreads_or(outside);
-    top = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, static_cast<float>(s_d[w]));
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_f[w]);
+    const bool odd = !fp32_does(top, s_hi);
+    if (!greedy && !filter) {   // this share's sum under its maximum
+        double sum = 0.0;
+        if (odd) each([&](const auto& y, auto count, int) {
+            for (int e = 0; e < count(); ++e) sum += weight64(y[e], top, per_t);
+        });
+        else if (my_top > -INFINITY) sum = static_cast<double>(part) * exp2(static_cast<double>(at) - static_cast<double>(top) * s_hi);
+        sum = warp_sum(sum);
+        if (lane == 0) s_d[warp] = sum;
+        __syncthreads();
+        sum = 0.0;
+        for (int w = 0; w < kWarps; ++w) sum += s_d[w];
+        meet_first();
+        if (tid == 0) tell(&meet.sum[rank], C, sum);
+    } else {
+        meet_first();
+    }
     if (tid == 0) tell(&meet.top[rank], C, top);
     meet_all();   // also: everyone's counters are complete
     float xmax = -INFINITY;
     for (int r = 0; r < C; ++r) xmax = fmaxf(xmax, meet.top[r]);
 
-    auto store = [&](auto value) {   // value(i) to entry i
-        if (ALIGNED) {
-#pragma unroll
-            for (int j = 0; j < VECTORS; ++j) {
-                const int at = (j * kThreads + tid) * 8;
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = value(j * 8 + e);
-                if (at + 8 <= n) {
-                    reinterpret_cast<float4*>(out + at)[0] = make_float4(y[0], y[1], y[2], y[3]);
-                    reinterpret_cast<float4*>(out + at)[1] = make_float4(y[4], y[5], y[6], y[7]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (at + e < n) out[at + e] = y[e];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (place(i) < n) out[place(i)] = value(i);
-        }
-    };
-
     if (greedy) {   // one-hot at the first maximum of all shares
         int at = 0x7fffffff;
+        each([&](const auto& y, auto count, int place) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (entry(i) == xmax) at = min(at, begin + place(i));
+            for (int e = 0; e < count(); ++e)
+                if (y[e] == xmax) at = min(at, begin + place + e);
+        });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) s_i[warp] = at;
         __syncthreads();
@@ -246,76 +495,65 @@ sampling_probs_kernel(const ProbsParams p) {
         meet_all();
         int first = 0x7fffffff;
         for (int r = 0; r < C; ++r) first = min(first, meet.first[r]);
-        store([&](int i) { return begin + place(i) == first ? 1.f : 0.f; });
+        store([&](float, int place) { return begin + place == first ? 1.f : 0.f; });
         return;
     }
     if (xmax == -INFINITY) {   // nothing but -inf and NaN
-        store([](int) { return 0.f; });
+        store([](float, int) { return 0.f; });
         return;
     }
 
-    // Weights.  fp64 for the sums that decide; for the entries fp32, with what the exponent (x - max) log2(e) / T loses when it is
-    // rounded put back as a factor 2^lost = 1 + lost ln 2, so that a far tail keeps its digits.
-    const double per_t = 1.4426950408889634 / static_cast<double>(T);
-    const float s_hi = static_cast<float>(per_t), s_lo = static_cast<float>(per_t - static_cast<double>(s_hi));
-    const bool plain = xmax < INFINITY && s_hi > 1e-30f && s_hi < 1e30f;   // no infinities but -inf, whose exponent is -inf
-    auto weight = [&](float a) -> float {
-        const float d = a - xmax, hi = d * s_hi;
-        float y;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(hi));
-        const float lost = fmaf(d, s_lo, fmaf(d, s_hi, -hi));
-        if (plain) return hi < -126.f ? 0.f : fmaf(y, lost * 0.693147182f, y);
-        return static_cast<float>(weight64(a, xmax, per_t));
+    // Weights.  fp64 for the sums that decide; for the results fp32: 2^(a s - c) with c = max s rounded, whose rounding, the same for all,
+    // is part of the factor behind it.  s is rounded too: an entry 2^e below the largest is off by |e| 2^-23 of itself.
+    const float c = xmax * s_hi;
+    const bool plain = fp32_does(xmax, s_hi);
+    // Results of the entries above or at `bound` for which keeps(entry, place); 0 elsewhere.
+    auto finish = [&](double kept, float bound, auto keeps) {
+        if (plain) {
+            const float factor = static_cast<float>(exp2(static_cast<double>(c) - static_cast<double>(xmax) * s_hi) / kept);
+            store_from(bound, [&](float a, int place) { return keeps(a, place) ? ex2(fmaf(a, s_hi, -c)) * factor : 0.f; });
+        } else {
+            store_from(bound, [&](float a, int place) { return keeps(a, place) ? static_cast<float>(weight64(a, xmax, per_t) / kept) : 0.f; });
+        }
     };
 
     if (!filter) {
-        float w[N];   // (where there are filters too, registers are short: weights are formed a second time)
         double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < N; i += 8) {
-            float part = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[i + e] = weight(entry(i + e));
-                part += w[i + e];
-            }
-            sum += part;
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) s_d[warp] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int w = 0; w < kWarps; ++w) sum += s_d[w];
-        if (tid == 0) tell(&meet.sum[rank], C, sum);
-        meet_all();
-        sum = 0.0;
-        for (int r = 0; r < C; ++r) sum += meet.sum[r];
-        const float inv = static_cast<float>(1.0 / sum);
-        if (FILTERS) store([&](int i) { return weight(entry(i)) * inv; });
-        else store([&](int i) { return w[i] * inv; });
+        for (int r = 0; r < C; ++r)
+            sum += plain ? meet.sum[r] * exp2((static_cast<double>(meet.top[r]) - static_cast<double>(xmax)) * s_hi)
+                         : meet.sum[r] * weight64(meet.top[r], xmax, per_t);
+        finish(sum, -INFINITY, [](float, int) { return true; });
         return;
     }
     if constexpr (FILTERS) {
         // ---- entries that are not counted ----
         double out_sum[kClasses] = {0.0, 0.0, 0.0};
-        if (outside) {
-#pragma unroll 1
-            for (int c = 0; c < kClasses; ++c) {
-                double sum = 0.0;
-                int count = 0;
-                for (int i = tid; i < n; i += kThreads) {
-                    const float a = clean(__bfloat162float(x[i]));
-                    if (bin_of(a) >= 0 || c != (a >= 256.f ? 0 : a <= -256.f ? 2 : 1)) continue;
-                    sum += weight64(a, xmax, per_t);
-                    ++count;
+        if (outside) {   // (a round of its own: one row in hundreds has any)
+            int out_count[kClasses] = {0, 0, 0};
+            each([&](const auto& y, auto count, int) {
+#pragma unroll
+                for (int e = 0; e < count(); ++e) {
+                    if (bin_of(y[e]) >= 0) continue;
+                    const double w = weight64(y[e], xmax, per_t);
+                    const int c = y[e] >= 256.f ? 0 : y[e] <= -256.f ? 2 : 1;
+#pragma unroll
+                    for (int i = 0; i < kClasses; ++i)
+                        if (i == c) {
+                            out_sum[i] += w;
+                            ++out_count[i];
+                        }
                 }
-                sum = warp_sum(sum);
-                count = __reduce_add_sync(0xffffffffu, count);
+            });
+#pragma unroll
+            for (int c = 0; c < kClasses; ++c) {
+                const double sum = warp_sum(out_sum[c]);
+                const int count = __reduce_add_sync(0xffffffffu, out_count[c]);
                 if (lane == 0) {
                     s_d[warp] = sum;
                     atomicAdd(&s_count[c], count);
                 }
                 __syncthreads();
+                out_sum[c] = 0.0;
                 for (int w = 0; w < kWarps; ++w) out_sum[c] += s_d[w];
                 __syncthreads();
             }
@@ -325,11 +563,12 @@ sampling_probs_kernel(const ProbsParams p) {
             tell(&meet.out_sum[rank][tid], C, tid == 0 ? out_sum[0] : tid == 1 ? out_sum[1] : out_sum[2]);
         }
         // ---- this CTA's range of patterns, a run of them per thread, from the top down ----
-        const int each = kBins / C / kThreads;   // 2 .. 16
-        const int bin_top = kBins - 1 - (rank * kThreads + tid) * each;
+        const int bins = kBins / C / kThreads;   // 4 .. 32
+        const int bin_top = kBins - 1 - (rank * kThreads + tid) * bins;
         int my_count = 0;
         double my_sum = 0.0;
         auto count_of = [&](int bin) {
+            if (C == 1) return hist[bin];
             int c[kMaxCluster], sum = 0;
 #pragma unroll
             for (int r = 0; r < kMaxCluster; ++r) {
@@ -341,7 +580,7 @@ sampling_probs_kernel(const ProbsParams p) {
             return sum;
         };
 #pragma unroll 1
-        for (int i = 0; i < each; ++i) {
+        for (int i = 0; i < bins; ++i) {
             const int c = count_of(bin_top - i);
             if (c == 0) continue;
             my_count += c;
@@ -414,7 +653,7 @@ sampling_probs_kernel(const ProbsParams p) {
                 int c_run = above;
                 double s_run = lower;
 #pragma unroll 1
-                for (int i = 0; i < each; ++i) {
+                for (int i = 0; i < bins; ++i) {
                     const int c = count_of(bin_top - i);
                     if (c == 0) continue;
                     const float a = value_of_bin(bin_top - i);
@@ -443,7 +682,7 @@ sampling_probs_kernel(const ProbsParams p) {
                 int c_run = above;
                 double s_run = lower;
 #pragma unroll 1
-                for (int i = 0; i < each; ++i) {
+                for (int i = 0; i < bins; ++i) {
                     const float a = value_of_bin(bin_top - i);
                     int c = count_of(bin_top - i);
                     if (a < last) break;
@@ -557,17 +796,24 @@ sampling_probs_kernel(const ProbsParams p) {
         }
         // ---- of the last kept value, the first `ties` by index: those of the shares before this one first ----
         {
+            const int bin = bin_of(last);   // (counted, or found by bisection: then by counting)
             int count = 0;
+            if (bin >= 0 && !missed) {
+                if (tid == 0) tell(&meet.equal[rank], C, hist[bin]);
+            } else {
+                each([&](const auto& y, auto c, int) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) count += place(i) < n && entry(i) == last ? 1 : 0;
-            count = __reduce_add_sync(0xffffffffu, count);
-            __syncthreads();
-            if (lane == 0) s_i[warp] = count;
-            __syncthreads();
-            if (tid == 0) {
-                count = 0;
-                for (int w = 0; w < kWarps; ++w) count += s_i[w];
-                tell(&meet.equal[rank], C, count);
+                    for (int e = 0; e < c(); ++e) count += y[e] == last ? 1 : 0;
+                });
+                count = __reduce_add_sync(0xffffffffu, count);
+                __syncthreads();
+                if (lane == 0) s_i[warp] = count;
+                __syncthreads();
+                if (tid == 0) {
+                    count = 0;
+                    for (int w = 0; w < kWarps; ++w) count += s_i[w];
+                    tell(&meet.equal[rank], C, count);
+                }
             }
             meet_all();   // (nothing remote is touched behind this)
         }
@@ -575,50 +821,51 @@ sampling_probs_kernel(const ProbsParams p) {
         for (int r = 0; r < rank; ++r) before += meet.equal[r];
         const int room = max(ties - before, 0);
         if (room < meet.equal[rank]) {
-            // Some of this share's do not fit.  A bit per entry, where the counters were: the first that does not.
-            constexpr int kWords = (N * kThreads + 31) / 32, kEach = (kWords + kThreads - 1) / kThreads;
-            static_assert(kWords <= kBins, "");
-            for (int i = tid; i < kWords; i += kThreads) hist[i] = 0;
-            __syncthreads();
+            // Some of this share's do not fit: the first that does not.  By blocks of as many entries as there are bits where the counters
+            // were.
+            constexpr int kBlock = kBins * 32;
+            int passed = 0;   // equal entries of the blocks before
+            for (int base = 0; base < n; base += kBlock) {
+                const int words = min(kBins, (n - base + 31) / 32), mine_words = (words + kThreads - 1) / kThreads;
+                __syncthreads();
+                for (int i = tid; i < words; i += kThreads) hist[i] = 0;
+                __syncthreads();
+                each([&](const auto& y, auto c, int at) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (place(i) < n && entry(i) == last) atomicOr(&hist[place(i) >> 5], 1 << (place(i) & 31));
-            __syncthreads();
-            int mine = 0;
+                    for (int e = 0; e < c(); ++e)
+                        if (y[e] == last && at + e >= base && at + e - base < kBlock)
+                            atomicOr(&hist[(at + e - base) >> 5], 1 << ((at + e - base) & 31));
+                });
+                __syncthreads();
+                int mine = 0;
+                for (int i = tid * mine_words; i < min((tid + 1) * mine_words, words); ++i) mine += __popc(hist[i]);
+                int to = mine;
 #pragma unroll
-            for (int i = 0; i < kEach; ++i)
-                if (tid * kEach + i < kWords) mine += __popc(hist[tid * kEach + i]);
-            int to = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int c = __shfl_up_sync(0xffffffffu, to, o);
-                if (lane >= o) to += c;
-            }
-            if (lane == 31) s_i[warp] = to;
-            __syncthreads();
-            for (int w = 0; w < warp; ++w) to += s_i[w];
-            int from = to - mine;
-            if (from <= room && room < to)
-                for (int i = 0; i < kEach; ++i) {
-                    const int word = hist[tid * kEach + i], here = __popc(word);
-                    if (from <= room && room < from + here) s_cut = (tid * kEach + i) * 32 + __fns(word, 0, room - from + 1);
-                    from += here;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int c = __shfl_up_sync(0xffffffffu, to, o);
+                    if (lane >= o) to += c;
                 }
+                if (lane == 31) s_i[warp] = to;
+                __syncthreads();
+                int total = 0;
+                for (int w = 0; w < kWarps; ++w) {
+                    if (w < warp) to += s_i[w];
+                    total += s_i[w];
+                }
+                int from = passed + to - mine;
+                if (from <= room && room < passed + to)
+                    for (int i = tid * mine_words; i < min((tid + 1) * mine_words, words); ++i) {
+                        const int here = __popc(hist[i]);
+                        if (from <= room && room < from + here) s_cut = base + i * 32 + __fns(hist[i], 0, room - from + 1);
+                        from += here;
+                    }
+                passed += total;
+            }
             __syncthreads();
         }
         const int cut = s_cut;
-        const float inv = static_cast<float>(1.0 / kept);
-        store([&](int i) {
-            const float a = entry(i);
-            return a > last || (a == last && place(i) < cut) ? weight(a) * inv : 0.f;
-        });
+        finish(kept, last, [&](float a, int place) { return a > last || (a == last && place < cut); });
     }
-}
-
-template <int VECTORS>
-auto kernel_for(bool filters, bool aligned) {
-    return filters ? (aligned ? sampling_probs_kernel<VECTORS, true, true> : sampling_probs_kernel<VECTORS, true, false>)
-                   : (aligned ? sampling_probs_kernel<VECTORS, false, true> : sampling_probs_kernel<VECTORS, false, false>);
 }
 
 }  // namespace
@@ -630,9 +877,8 @@ int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, in
                         const int32_t* top_k, const float* top_p, b200_stream_t stream) {
     using namespace b200;
     B200_CHECK_ARG(rows >= 0 && vocab > 0 && ld >= vocab, "sampling_probs: bad shape");
-    constexpr int most = kMaxCluster * kThreads * kMaxVectors * 8;
-    if (vocab > most) {
-        set_last_error("sampling_probs: vocab %d is above %d", vocab, most);
+    if (vocab > kMaxVocab) {
+        set_last_error("sampling_probs: vocab %d is above %d", vocab, kMaxVocab);
         return B200_ERR_UNSUPPORTED;
     }
     B200_CHECK_ARG(rows <= (1 << 27), "sampling_probs: too many rows");
@@ -640,16 +886,13 @@ int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, in
     B200_CHECK_ARG(out && logits && temperatures, "sampling_probs: NULL tensor");
     const bool filters = top_k != nullptr || top_p != nullptr;
     const bool aligned = (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && ld % 8 == 0 && vocab % 4 == 0;
-    // CTAs per row: as few as hold it at five vectors a thread, and more while rows are few and shares large.
+    // CTAs per row: one, and more while the SMs have room for them and shares are large.
     int cluster = 1;
-    while (cluster < kMaxCluster && vocab > cluster * kThreads * 5 * 8) cluster *= 2;
-    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= 2 * sm_count() && vocab / cluster > kThreads * 8) cluster *= 2;
-    const int vectors = div_ceil(vocab, cluster * kThreads * 8);
+    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= kWaves * 4 * sm_count() && vocab / cluster > kThreads * 64) cluster *= 2;
     ProbsParams p = {out, static_cast<const __nv_bfloat16*>(logits), ld, rows, vocab, div_ceil(div_ceil(vocab, cluster), 8) * 8, cluster,
                      temperatures, top_k, top_p};
-    auto kernel = vectors <= 1 ? kernel_for<1>(filters, aligned) : vectors <= 2 ? kernel_for<2>(filters, aligned)
-                : vectors <= 3 ? kernel_for<3>(filters, aligned) : vectors <= 4 ? kernel_for<4>(filters, aligned)
-                : vectors <= 5 ? kernel_for<5>(filters, aligned) : kernel_for<kMaxVectors>(filters, aligned);
+    auto kernel = filters ? (aligned ? sampling_probs_kernel<true, true> : sampling_probs_kernel<true, false>)
+                          : (aligned ? sampling_probs_kernel<false, true> : sampling_probs_kernel<false, false>);
     B200_CHECK_CUDA(launch_kernel(kernel, dim3(static_cast<unsigned>(rows) * cluster), dim3(kThreads), 0, static_cast<cudaStream_t>(stream),
                                   dim3(cluster, 1, 1), p));
     return B200_OK;

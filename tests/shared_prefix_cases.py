@@ -138,11 +138,15 @@ def probs_oracle(logits, temperatures, top_k=None, top_p=None):
 
 
 def assert_probs(got, want):
-    """Zero where it should be, and elsewhere within 2^-19: exponentials of 2 ulp (twice 2^-22), their exponents' last place, three
-    roundings (2^-24 each), and the sum they are divided by: the same errors of the weights, 16 fp32 additions (2^-20)."""
+    """Zero where it should be, and elsewhere right to 2^-19 of itself and 2^-23 for every power of two that it lies below the
+    row's largest.  The exponent e = (x - max) log2(e) / T is formed in fp32: half a last place of it and of the factor, 2 * 2^-24 |e|, so
+    ln 2 of that of the weight; a weight's exponential is right to 2^-22, the sum that it is divided by as its terms (nearly all
+    of it within 2^-10 of the largest: 2^-21) and 8 additions (2^-21), products and quotient 3 * 2^-24: below 2^-20 together."""
     got = got.double().cpu()
     assert bool(((got > 0) <= (want > 0)).all()), "probability outside the kept set"
-    bad = ~((got - want).abs() <= 2.0 ** -19 * want + 2.0 ** -126)
+    largest = want.amax(-1, keepdim=True).clamp_min(1e-300)
+    below = -torch.log2(want.clamp_min(1e-300) / largest)
+    bad = ~((got - want).abs() <= (2.0 ** -19 + 2.0 ** -23 * below) * want + 2.0 ** -126)
     assert not bool(bad.any()), f"{int(bad.sum())} off, relative {float(((got - want).abs() / want.clamp_min(1e-300))[bad].max())}"
 
 

@@ -50,7 +50,7 @@ def test_attention_workspace_sizes(pkg):
 
 
 @pytest.mark.parametrize("change,rc,text", [
-    (dict(rows=-1), 1, "shape"), (dict(vocab=0), 1, "shape"), (dict(ld=99), 1, "shape"), (dict(vocab=327681, ld=400000), 4, "327680"),
+    (dict(rows=-1), 1, "shape"), (dict(vocab=0), 1, "shape"), (dict(ld=99), 1, "shape"), (dict(vocab=(1 << 24) + 1, ld=1 << 25), 4, "16777216"),
     (dict(out=None), 1, "NULL"), (dict(logits=None), 1, "NULL"), (dict(temperatures=None), 1, "NULL"), (dict(rows=1 << 28), 1, "rows"),
 ])
 def test_sampling_probs_refusals(pkg, change, rc, text):

@@ -276,6 +276,23 @@ def test_sampling_probs_odd_values(L, filtered):
     assert_probs(extreme, want)
 
 
+@pytest.mark.parametrize("vocab", [9000, 9001, 70000])
+def test_sampling_probs_masked_vocabulary(L, vocab):
+    """Most of the vocabulary at the type's lowest number, or at -inf; all of it; and temperatures from nearly 0 to nearly infinite."""
+    low = float(torch.finfo(bf16).min)
+    for mask in (low, -float("inf"), -1e4):
+        x = _logits(7, vocab, vocab)
+        keep = torch.zeros(vocab, dtype=torch.bool)
+        keep[5::vocab // 40] = True
+        x[:, ~keep] = mask
+        x[6] = mask
+        t = [0.7, 1.0, 2e-6, 1e-5, 1e6, 1e38, 1.0]
+        for k, p in ((None, None), ([50] * 7, None), ([3] * 7, [0.9] * 7), (None, [0.6] * 7), ([1000] * 7, [0.95] * 7)):
+            got = L.sampling_probs(x.cuda(), _f32(t), None if k is None else _i32(k), None if p is None else _f32(p))
+            want = probs_oracle(x, np.asarray(t, np.float32), k, None if p is None else np.asarray(p, np.float32))
+            assert_probs(got, want)
+
+
 def test_sampling_probs_is_what_sample_draws_from(L):
     """The kept set is b200_sample's candidate set (rows whose border is not within its 40-bit sums' reach)."""
     rows, vocab = 32, 32000
