@@ -13,8 +13,8 @@
 //
 // A CTA, or where rows are few a cluster of them, owns a row and goes over it from memory once and from L2 once or twice more.
 //     no filter:       sums under a running maximum; results.
-//     top_k <= 256:    the lanes' maxima; of every warp's 32 the r-th largest, r = ceil(top_k / warps): the smallest of these has top_k
-//                      entries at or above it.  A second round lists all such entries (some hundreds), which are sorted, weighed and
+//     top_k <= 256:    the lanes' maxima; of every warp's 32 the r-th largest, r = ceil(top_k / warps of the row): the smallest of these
+//                      has top_k entries at or above it.  A second round lists all such entries (some hundreds), which are sorted, weighed and
 //                      cut; the results are zeros but for what is kept.
 //     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
 //                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
@@ -78,7 +78,7 @@ constexpr int kClasses = 3;
 struct Meet {   // each CTA's copy: what the CTAs of a row tell one another
     float top[kMaxCluster];                  // the share's maximum
     int first[kMaxCluster];                  // where it is first
-    float from[kMaxCluster];                 // top_k entries of the share are at least this
+    float from[kMaxCluster];                 // its part of the top_k entries, by number, is at least this
     int listed[kMaxCluster];
     double sum[kMaxCluster];                 // weights: of the share under its maximum (no filters), of the CTA's range of patterns
     int count[kMaxCluster];                  // entries in that range
@@ -281,7 +281,7 @@ sampling_probs_kernel(const ProbsParams p) {
         if (filter && want_k && K <= kThreads) {
             // ---- a bound that top_k entries reach ----
             float top = largest();
-            const int r = (K + kWarps - 1) / kWarps;
+            const int r = (K + kWarps * C - 1) / (kWarps * C);
             float sorted = top;   // of the lanes, the largest first
 #pragma unroll
             for (int size = 2; size <= 32; size *= 2)
@@ -311,7 +311,7 @@ sampling_probs_kernel(const ProbsParams p) {
             meet_all();
             float xmax = -INFINITY;
             for (int i = 0; i < C; ++i) {
-                from = fmaxf(from, meet.from[i]);
+                from = fminf(from, meet.from[i]);
                 xmax = fmaxf(xmax, meet.top[i]);
             }
             // ---- the entries that reach it, by value and place in one word, the larger value and the earlier place the smaller word ----
@@ -349,7 +349,9 @@ sampling_probs_kernel(const ProbsParams p) {
                 }
                 asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (nothing remote is read any more; waited for at the end)
                 __syncthreads();
-                for (int run = 2; run <= size; run *= 2)
+                // (Thread i's pair lies in the 64 words of its warp as long as they are at most 32 apart: no need to wait for other warps.)
+                for (int run = 2; run <= size; run *= 2) {
+                    if (run > 64) __syncthreads();
                     for (int o = run / 2; o > 0; o /= 2) {
                         for (int i = tid; i < size / 2; i += kThreads) {
                             const int a = 2 * i - (i & (o - 1)), b = a + o;
@@ -359,8 +361,11 @@ sampling_probs_kernel(const ProbsParams p) {
                                 all[b] = wa;
                             }
                         }
-                        __syncthreads();
+                        if (o > 32) __syncthreads();
+                        else __syncwarp();
                     }
+                }
+                __syncthreads();
                 // ---- weights of the first top_k, and what of them stays ----
                 const uint64_t word = all[tid];   // (at least 32; behind them whatever is there is not used)
                 const bool there = tid < K && tid < total;

@@ -33,6 +33,21 @@ def _check(cond: bool, msg: str) -> None:
         raise B200Error(1, msg)
 
 
+def _launch(index: int, name: str, *args) -> None:
+    """The call on device ``index`` and its current stream.  (Without torch.cuda's own guard and stream object where the device is the
+    current one: they take longer than a small call.)"""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, stream)
+
+
+def _fail(msg: str) -> None:
+    raise B200Error(1, msg)
+
+
 def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.size(0) > 1 else t.size(1)   # (a single row's says nothing)
 
@@ -340,6 +355,10 @@ class SharedPrefixAttention:
         _check(nbytes > 0, "unsupported head configuration or size for attention over a shared prefix")
         _check(kv_cache.kv_heads_ == num_kv_heads and kv_cache.head_dim_ == head_dim, "KV cache layout mismatch")
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=kv_cache.kv_buffer_.device)
+        self.args_ = _lib.SharedPrefixArgs(
+            num_slots=kv_cache.total_slots, q_heads=num_qo_heads, kv_heads=num_kv_heads, head_dim=head_dim, page_size=kv_cache.page_size_,
+            sm_scale=self.sm_scale, workspace=self.workspace.data_ptr(), workspace_bytes=nbytes)
+        self.args_ref_ = ctypes.byref(self.args_)
 
     def forward(self, q: torch.Tensor, layer_id: int, page_table: torch.Tensor, table_idx: torch.Tensor, seq_lens: torch.Tensor,
                 qo_indptr: torch.Tensor, group_indptr: torch.Tensor, prefix_lens: torch.Tensor,
@@ -347,37 +366,42 @@ class SharedPrefixAttention:
         """q [tokens, q_heads, head_dim]; request b owns rows [qo_indptr[b], qo_indptr[b + 1]), the last positions of its
         seq_lens[b] keys.  Group g is requests [group_indptr[g], group_indptr[g + 1]), whose page-table rows agree in their first
         prefix_lens[g] positions.  Rows that no request owns are not written."""
-        kc = self.kv_cache_
-        _cuda_bf16(q, "q")
-        _check(q.dim() == 3 and q.size(1) == self.num_qo_heads_ and q.size(2) == self.head_dim_, "q must be [tokens, q_heads, head_dim]")
-        _check(q.stride(2) == 1, "Last dimension must be contiguous")
-        index = {"page_table": page_table, "table_idx": table_idx, "seq_lens": seq_lens, "qo_indptr": qo_indptr,
-                 "group_indptr": group_indptr, "prefix_lens": prefix_lens}
-        for name, t in index.items():
-            _check(t.is_cuda and t.dtype == torch.int32, f"{name} must be a CUDA int32 tensor")
-            _check(t.device == q.device, f"{name} must be on the device of q")
-            _check(t.stride(-1) == 1 or t.size(-1) <= 1, f"{name} must be contiguous")
-        _check(q.device == kc.kv_buffer_.device == self.workspace.device, "q and the KV cache must be on one device")
-        batch, groups = table_idx.numel(), prefix_lens.numel()
-        _check(page_table.dim() == 2, "page_table must be rank 2")
-        _check(seq_lens.numel() == batch and qo_indptr.numel() == batch + 1, "seq_lens [batch], qo_indptr [batch + 1]")
-        _check(group_indptr.numel() == groups + 1, "group_indptr must be [groups + 1]")
-        _check(q.size(0) <= self.max_tokens_ and batch <= self.max_batch_, "more query rows or requests than the workspace is made for")
-        shape = (q.size(0), self.num_qo_heads_ * self.head_dim_)
+        kc, args, dev = self.kv_cache_, self.args_, q.get_device()
+        if dev < 0 or q.dtype is not bf16:
+            _fail("q must be a CUDA tensor of bfloat16")
+        if q.dim() != 3 or q.size(1) != self.num_qo_heads_ or q.size(2) != self.head_dim_ or q.stride(2) != 1:
+            _fail("q must be [tokens, q_heads, head_dim] with a contiguous last dimension")
+        tokens, batch, groups = q.size(0), table_idx.numel(), prefix_lens.numel()
+        for name, t, count in (("page_table", page_table, -1), ("table_idx", table_idx, batch), ("seq_lens", seq_lens, batch),
+                               ("qo_indptr", qo_indptr, batch + 1), ("group_indptr", group_indptr, groups + 1),
+                               ("prefix_lens", prefix_lens, groups)):
+            if t.get_device() != dev or t.dtype is not torch.int32:
+                _fail(f"{name} must be a CUDA int32 tensor on the device of q")
+            if count < 0:
+                if t.dim() != 2 or (t.stride(1) != 1 and t.size(1) > 1):
+                    _fail(f"{name} must be rank 2 with contiguous rows")
+            elif t.dim() != 1 or t.numel() != count or (count > 1 and t.stride(0) != 1):
+                _fail(f"{name} must be contiguous [{count}]: table_idx and seq_lens [batch], qo_indptr [batch + 1], prefix_lens [groups], "
+                      "group_indptr [groups + 1]")
+        if kc.kv_buffer_.get_device() != dev or self.workspace.get_device() != dev:
+            _fail("q, the KV cache and the workspace must be on one device")
+        if tokens > self.max_tokens_ or batch > self.max_batch_:
+            _fail("more query rows or requests than the workspace is made for")
+        if not 0 <= layer_id < kc.num_layers_:
+            _fail("no such layer")
         if out is None:
-            out = torch.empty(shape, dtype=bf16, device=q.device)
-        _cuda_bf16(out, "out")
-        _check(tuple(out.shape) == shape and out.is_contiguous() and out.device == q.device, "out must be contiguous [tokens, q_heads * head_dim]")
-        args = _lib.SharedPrefixArgs(
-            out=out.data_ptr(), q=q.data_ptr(), q_stride_token=q.stride(0), q_stride_head=q.stride(1),
-            k_cache=kc.k_cache(layer_id).data_ptr(), v_cache=kc.v_cache(layer_id).data_ptr(), num_slots=kc.total_slots,
-            page_table=page_table.data_ptr(), page_table_stride=page_table.stride(0), table_idx=table_idx.data_ptr(),
-            seq_lens=seq_lens.data_ptr(), qo_indptr=qo_indptr.data_ptr(), group_indptr=group_indptr.data_ptr(),
-            prefix_lens=prefix_lens.data_ptr(), tokens=q.size(0), batch=batch, groups=groups, q_heads=self.num_qo_heads_,
-            kv_heads=self.num_kv_heads_, head_dim=self.head_dim_, page_size=kc.page_size_, sm_scale=self.sm_scale,
-            workspace=self.workspace.data_ptr(), workspace_bytes=self.workspace.numel())
-        with torch.cuda.device(q.device):
-            call("b200_attention_shared_prefix", ctypes.byref(args), _stream())
+            out = torch.empty(tokens, self.num_qo_heads_ * self.head_dim_, dtype=bf16, device=q.device)
+        elif (out.get_device() != dev or out.dtype is not bf16 or tuple(out.shape) != (tokens, self.num_qo_heads_ * self.head_dim_)
+              or not out.is_contiguous()):
+            _fail("out must be contiguous bfloat16 [tokens, q_heads * head_dim] on the device of q")
+        layer = layer_id * kc.total_slots * kc.kv_heads_ * kc.head_dim_ * 2
+        args.out, args.q, args.q_stride_token, args.q_stride_head = out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1)
+        args.k_cache, args.v_cache = kc.k_buffer_.data_ptr() + layer, kc.v_buffer_.data_ptr() + layer
+        args.page_table, args.page_table_stride = page_table.data_ptr(), _row_stride(page_table)
+        args.table_idx, args.seq_lens, args.qo_indptr = table_idx.data_ptr(), seq_lens.data_ptr(), qo_indptr.data_ptr()
+        args.group_indptr, args.prefix_lens = group_indptr.data_ptr(), prefix_lens.data_ptr()
+        args.tokens, args.batch, args.groups = tokens, batch, groups
+        _launch(dev, "b200_attention_shared_prefix", self.args_ref_)
         return out
 
 
@@ -508,17 +532,20 @@ def sample_from_probs(probs: torch.Tensor, uniform: torch.Tensor, top_k: Optiona
 def sampling_probs(logits: torch.Tensor, temperatures: torch.Tensor, top_k: Optional[torch.Tensor] = None,
                    top_p: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The distribution that ``sample`` draws from, with the same arguments: float32 [rows, vocab], zeros outside the kept set."""
-    _cuda_bf16(logits, "logits")
-    _check(logits.dim() == 2 and (logits.stride(1) == 1 or logits.size(1) == 1), "logits must be rank 2 with contiguous rows")
+    dev = logits.get_device()
+    if dev < 0 or logits.dtype is not bf16:
+        _fail("logits must be a CUDA tensor of bfloat16")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.size(1) != 1):
+        _fail("logits must be rank 2 with contiguous rows")
     rows, vocab = logits.shape
     for name, t, dtype in (("temperatures", temperatures, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32)):
-        if t is not None:
-            _check(t.device == logits.device and t.dtype == dtype and t.numel() == rows and t.is_contiguous(),
-                   f"{name} must be {dtype} [rows] on the device of logits")
+        if t is None and name != "temperatures":
+            continue
+        if t.get_device() != dev or t.dtype is not dtype or t.numel() != rows or not t.is_contiguous():
+            _fail(f"{name} must be contiguous {dtype} [rows] on the device of logits")
     out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
-    with torch.cuda.device(logits.device):
-        call("b200_sampling_probs", out.data_ptr(), logits.data_ptr(), _row_stride(logits), rows, vocab,
-             temperatures.data_ptr(), _ptr(top_k), _ptr(top_p), _stream())
+    _launch(dev, "b200_sampling_probs", out.data_ptr(), logits.data_ptr(), _row_stride(logits), rows, vocab,
+            temperatures.data_ptr(), _ptr(top_k), _ptr(top_p))
     return out
 
 
@@ -529,26 +556,32 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_
     [drafts + batch, vocab]: request b's rows begin at draft_indptr[b] + b and are one more than its drafts; draft_probs [drafts,
     vocab], or None where drafts were certain.  Returns int32 tokens [batch, max_drafts + 1] (accepted drafts, the token behind
     them, -1) and int32 accepted [batch]."""
-    dev = target_probs.device
-    _check(target_probs.is_cuda and target_probs.dtype == torch.float32 and target_probs.dim() == 2
-           and (target_probs.stride(1) == 1 or target_probs.size(1) == 1), "target_probs must be CUDA float32 [rows, vocab] with contiguous rows")
+    dev = target_probs.get_device()
+    if dev < 0 or target_probs.dtype is not torch.float32:
+        _fail("target_probs must be a CUDA tensor of float32")
+    if target_probs.dim() != 2 or (target_probs.stride(1) != 1 and target_probs.size(1) != 1):
+        _fail("target_probs must be rank 2 with contiguous rows")
     vocab, batch, drafts = target_probs.size(1), draw_uniform.numel(), draft_tokens.numel()
     for name, t, dtype in (("draft_tokens", draft_tokens, torch.int32), ("draft_indptr", draft_indptr, torch.int32),
                            ("accept_uniform", accept_uniform, torch.float32), ("draw_uniform", draw_uniform, torch.float32)):
-        _check(t.device == dev and t.dtype == dtype and t.is_contiguous(), f"{name} must be contiguous {dtype} on the device of target_probs")
-    _check(max_drafts >= 0, "max_drafts must not be negative")
-    _check(draft_indptr.numel() == batch + 1, "draft_indptr must be [batch + 1]")
-    _check(target_probs.size(0) == drafts + batch, "target_probs must have one row per draft and one per request")
-    _check(accept_uniform.numel() == drafts, "accept_uniform must have one number per draft")
-    if draft_probs is not None:
-        _check(draft_probs.device == dev and draft_probs.dtype == torch.float32 and tuple(draft_probs.shape) == (drafts, vocab)
-               and (draft_probs.stride(1) == 1 or vocab == 1), "draft_probs must be float32 [drafts, vocab] with contiguous rows")
-    tokens = torch.empty(batch, max_drafts + 1, dtype=torch.int32, device=dev)
-    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        call("b200_verify_drafts", tokens.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(), _row_stride(target_probs),
-             _ptr(draft_probs), vocab if draft_probs is None else _row_stride(draft_probs), draft_tokens.data_ptr(),
-             draft_indptr.data_ptr(), accept_uniform.data_ptr(), draw_uniform.data_ptr(), batch, drafts, max_drafts, vocab, _stream())
+        if t.get_device() != dev or t.dtype is not dtype or not t.is_contiguous():
+            _fail(f"{name} must be contiguous {dtype} on the device of target_probs")
+    if max_drafts < 0:
+        _fail("max_drafts must not be negative")
+    if draft_indptr.numel() != batch + 1:
+        _fail("draft_indptr must be [batch + 1]")
+    if target_probs.size(0) != drafts + batch:
+        _fail("target_probs must have one row per draft and one per request")
+    if accept_uniform.numel() != drafts:
+        _fail("accept_uniform must have one number per draft")
+    if draft_probs is not None and (draft_probs.get_device() != dev or draft_probs.dtype is not torch.float32
+                                    or tuple(draft_probs.shape) != (drafts, vocab) or (draft_probs.stride(1) != 1 and vocab != 1)):
+        _fail("draft_probs must be float32 [drafts, vocab] with contiguous rows on the device of target_probs")
+    tokens = torch.empty(batch, max_drafts + 1, dtype=torch.int32, device=target_probs.device)
+    accepted = torch.empty(batch, dtype=torch.int32, device=target_probs.device)
+    _launch(dev, "b200_verify_drafts", tokens.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(), _row_stride(target_probs),
+            _ptr(draft_probs), vocab if draft_probs is None else _row_stride(draft_probs), draft_tokens.data_ptr(),
+            draft_indptr.data_ptr(), accept_uniform.data_ptr(), draw_uniform.data_ptr(), batch, drafts, max_drafts, vocab)
     return tokens, accepted
 
 
