@@ -6,10 +6,12 @@
 // and the parts of a row join exactly: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.  Everything up to the output is fp32 but
 // the probabilities, which are rounded to bf16 as the other attention kernels here do (their products run on the tensor cores).
 //
-// Rows kernel (bound by HBM): an item is a run of stages of a group's prefix or of what a request has of its own, for a tile of 16 of
-// its rows, (token, head of the KV head's group) pairs.  Items are cut by shared_prefix_plan.cu; a CTA takes the next one that nobody
+// Rows kernel (bound by HBM): an item is a run of stages of a group's prefix or of what a request has of its own, for a tile of up to
+// 8 * NT of its rows, (token, head of the KV head's group) pairs.  Items are cut by shared_prefix_plan.cu; a CTA takes the next one that nobody
 // has taken (which CTA does an item changes no result), two ahead of the one it works on.  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages, a warp for each
-// half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with mma.sync.
+// half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with mma.sync: S^T = K Q^T and O^T = V^T P^T, so that
+// the rows are the products' short side (eight of them; with the rows on the long side a step of one token and two heads per KV head
+// filled 2 of 16, and a stage took 1.05 us).
 #include "common.cuh"
 #include "kernels.h"
 #include "shared_prefix.cuh"
@@ -25,19 +27,18 @@ constexpr int kThreads = (kConsumerWarps + kProducerWarps) * 32;
 constexpr int kStageRows = 128;
 constexpr uint32_t kHalfBytes = kStageRows * 128;    // 64 of the 128 elements of every row
 constexpr uint32_t kStageBytes = 4 * kHalfBytes;
-constexpr int kStages = 3;
 constexpr uint32_t kItems = 4;                       // places for items that have been taken
-constexpr uint32_t kQueryBytes = 2 * kHalfBytes;     // 16 rows of each of 8 heads
-constexpr int RT = 16;                               // rows of a tile's products; as many whole tokens as fit are used
+constexpr int kSmallPage = 8;                        // pages of fewer slots are copied 16 bytes at a time
 constexpr int kMergeWarps = 4;
 constexpr int kTcRows = 32;
 
+constexpr int kStages = 3;   // in the ring, beside the queries of 8 * NT rows of every KV head
 // Values of keys behind limit0 that hold an infinity or NaN: weight times value for the rows that see the key, then zeros in
 // the key's place.  Weights x and sums o as the products' registers hold them.
-template <typename Addr>
-__device__ __forceinline__ void add_odd_values(uint32_t base, int key0, int valid, int limit0, const int (&limit)[2],
-                                               const float (&x)[8], float (&o)[16][4], const Addr& value_addr) {
-    const int lane = threadIdx.x & 31, t = lane & 3;
+template <int NT, typename Addr>
+__device__ __forceinline__ void add_odd_values(uint32_t base, int key0, int valid, int limit0, const int (&limit)[NT][2],
+                                               const float (&x)[NT][4], float (&o)[NT][8][4], const Addr& value_addr) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint32_t odd = 0;
     for (int i = lane; i < 16 * 16; i += 32) {
         const int j = i >> 4;
@@ -54,26 +55,33 @@ __device__ __forceinline__ void add_odd_values(uint32_t base, int key0, int vali
     for (int j = 0; j < 16; ++j) {
         if ((odd >> j & 1) == 0) continue;
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-            const float even = (j & 8) ? x[4 + 2 * rr] : x[2 * rr], next = (j & 8) ? x[5 + 2 * rr] : x[1 + 2 * rr];
-            const float w = round_bf16(__shfl_sync(0xffffffffu, (j & 1) ? next : even, (lane & ~3) | (j & 7) >> 1));
-            if (key0 + j <= limit[rr]) {
+        for (int m = 0; m < NT; ++m)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    uint32_t v;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(value_addr(base, j, i) + 4u * t));
-                    o[i][2 * rr] += w * bf16_lo(v);
-                    o[i][2 * rr + 1] += w * bf16_hi(v);
+            for (int rr = 0; rr < 2; ++rr) {
+                const float w = round_bf16(__shfl_sync(0xffffffffu, (j & 8) ? x[m][2 + rr] : x[m][rr], (j & 7) << 2 | t));
+                if (key0 + j <= limit[m][rr]) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {   // of the values, elements i * 8 + g
+                        uint32_t v;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(value_addr(base, j, i) + (g >> 1) * 4u));
+                        o[m][i >> 1][(i & 1) * 2 + rr] += w * ((g & 1) ? bf16_hi(v) : bf16_lo(v));
+                    }
                 }
+                __syncwarp();
             }
-            __syncwarp();
-        }
         if (lane < 16) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(value_addr(base, j, lane)), "r"(0u) : "memory");
     }
     fence_proxy_async_smem();
     __syncwarp();
 }
+// An 8 x 8 matrix of 16-bit elements, rows to columns.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
+template <int NT, bool SMALL>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                           const __grid_constant__ CUtensorMap tmap_q, const SharedPrefixParams p) {
@@ -85,7 +93,12 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t query_base = smem_base + kStages * kStageBytes;
+    // Large pages: K lo, K hi, V lo, V hi in swizzled rows of 128 bytes.  Small ones: K and V of a slot in one piece, all heads, 16 bytes
+    // further apart than they are long, which spreads eight keys over all banks.
+    const uint32_t slot_bytes = static_cast<uint32_t>(p.kv_heads) * kD * 2 + 16;
+    const uint32_t values_at = SMALL ? static_cast<uint32_t>(p.stage_keys) * slot_bytes : 2 * kHalfBytes;
+    const uint32_t stage_bytes = SMALL ? 2 * values_at : kStageBytes;
+    const uint32_t query_base = smem_base + (kStages * stage_bytes + 127u & ~127u);
     const int Hkv = p.kv_heads, G = p.group, SK = p.stage_keys;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -143,19 +156,25 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         const void* map = which < 2 ? &tmap_k : &tmap_v;
         const bool leads = which == 0 && lane == 0;
         if (leads) {
-            const int taken = atomicAdd(&p.plan.head->next, static_cast<int>(lead));
-            for (uint32_t i = 0; i < lead; ++i) hand_on(i, taken + static_cast<int>(i));
+            const bool first = static_cast<int>(blockIdx.x) < p.plan.head->rows_first;
+            if (first) hand_on(0, static_cast<int>(blockIdx.x));
+            for (uint32_t i = first ? 1 : 0; i < lead; ++i) hand_on(i, atomicAdd(&p.plan.head->next, 1));
         }
         __syncwarp();
         auto copies_of = [&](const RowsItem& it, int st) { return (min(SK, it.hi - it.start - st * SK) + p.kpc - 1) / p.kpc; };
+        // Pages of fewer than 8 slots: a slot's row of all heads by one plain copy, by two warps for K and two for V, every other key each.
+        // (Tensor copies of a slot or two take 17 ns each whatever their size: stages of pages of one slot 2.2 us.  16 bytes per lane,
+        // by cp.async: 2.5 us, the instructions that form 4096 addresses.)
+        const int span = SMALL ? 1 : p.kpc;   // slots that a table entry stands for here
+        const __nv_bfloat16* cache = which < 2 ? p.k_cache : p.v_cache;
         int next[4];   // this lane's slots of a stage's copies, fetched a stage ahead
         auto fetch_slots = [&](const RowsItem& it, int st) {
             const int32_t* row = p.page_table + static_cast<int64_t>(it.table) * p.pt_stride + it.start + st * SK;
-            const int n = copies_of(it, st);
+            const int n = SMALL ? min(SK, it.hi - it.start - st * SK) : copies_of(it, st);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int copy = c * 32 + lane;
-                next[c] = copy < n ? row[copy * p.kpc] : 0;
+                next[c] = copy < n ? row[copy * span] : 0;
             }
         };
         RowsItem it = get_item(0);
@@ -182,7 +201,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     sl[c] = next[c];
-                    if (sl[c] < 0 || static_cast<int64_t>(sl[c]) + p.kpc > p.num_slots) {
+                    if (sl[c] < 0 || static_cast<int64_t>(sl[c]) + span > p.num_slots) {
                         atomicExch(&p.status[kStatusBadIndex], sl[c] + 1);
                         sl[c] = 0;
                     }
@@ -194,15 +213,31 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                     break;
                 }
                 const uint32_t bar = smem_u32(&full_bar[slot]);
-                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * copy_bytes);
-                __syncwarp();
-                const uint32_t base = smem_base + slot * kStageBytes + which * kHalfBytes;
+                if (SMALL) {
+                    const uint32_t base = smem_base + slot * stage_bytes + (which >> 1) * values_at, bytes = slot_bytes - 16;
+                    const int keys = min(SK, it.hi - it.start - st * SK);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>((keys + 1 - (which & 1)) >> 1) * bytes);
+                    __syncwarp();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int copy = c * 32 + lane;
-                    if (copy >= n) continue;
-                    if (it.reread) tma_load_3d(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar);
-                    else tma_load_3d_hint(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar, once);
+                    for (int c = 0; c < 4; ++c) {
+                        const int key = c * 32 + lane;
+                        if (key < keys && (key & 1) == (which & 1))
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                             base + static_cast<uint32_t>(key) * slot_bytes),
+                                         "l"(cache + static_cast<int64_t>(sl[c]) * Hkv * kD), "r"(bytes), "r"(bar)
+                                         : "memory");
+                    }
+                } else {
+                    if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(n) * copy_bytes);
+                    __syncwarp();
+                    const uint32_t base = smem_base + slot * stage_bytes + which * kHalfBytes;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int copy = c * 32 + lane;
+                        if (copy >= n) continue;
+                        if (it.reread) tma_load_3d(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar);
+                        else tma_load_3d_hint(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar, once);
+                    }
                 }
                 if (st == it.s_begin) {
                     if (leads) hand_on(turn + lead, taken);
@@ -226,43 +261,61 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         const int js = kg * 16 + j;
         return static_cast<uint32_t>((js & ~(p.kpc - 1)) * Hkv + h * p.kpc + (js & (p.kpc - 1)));
     };
-    auto value_addr = [&](uint32_t base, int j, int c16) { return swz128(base + (2 + (c16 >> 3)) * kHalfBytes + tile_row(j) * 128u, c16 & 7); };
-    const int QT = p.row_tokens;   // query tokens of a row tile
-    // Shared-memory row of a tile's row r: queries lie as [token][head].
-    auto query_row = [&](int r) -> uint32_t {
-        const int tok = min(r / G, QT - 1);
-        return static_cast<uint32_t>(tok * p.q_heads + h * G + min(r - tok * G, G - 1));
+    // 16 bytes of that key and head.
+    auto key_addr = [&](uint32_t base, int j, int c16) -> uint32_t {
+        if (SMALL) return base + static_cast<uint32_t>(kg * 16 + j) * slot_bytes + static_cast<uint32_t>(h * 16 + c16) * 16u;
+        return swz128(base + (c16 >> 3) * kHalfBytes + tile_row(j) * 128u, c16 & 7);
     };
-    const uint32_t query_addr = query_base + query_row((mi & 1) * 8 + r8) * 128u;
+    auto value_addr = [&](uint32_t base, int j, int c16) { return key_addr(base + values_at, j, c16); };
+    const int QT = p.row_tokens;   // query tokens of a row tile
+    // Queries lie as [token][head] in shared memory: the rows of this lane's addresses (row r8 of each eight), and the tokens of its
+    // products' columns.
+    uint32_t query_row[NT];
+    int row_tok[NT][2];
+#pragma unroll
+    for (int m = 0; m < NT; ++m) {
+        const int r = m * 8 + r8, tok = min(r / G, QT - 1);
+        query_row[m] = query_base + static_cast<uint32_t>(tok * p.q_heads + h * G + min(r - tok * G, G - 1)) * 128u;
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) row_tok[m][rr] = (m * 8 + 2 * t + rr) / G;
+    }
     const uint32_t query_half = static_cast<uint32_t>(QT * p.q_heads + 7 & ~7) * 128u;
-    const int row_tok[2] = {g / G, (g + 8) / G};   // of this lane's two rows
     for (uint32_t turn = 0;; ++turn) {
         const RowsItem un = get_item(turn);
         if (un.slot < 0) break;
         const int rows = min(un.ntok - un.tile * QT, QT) * G;   // of this tile, at least one
-        // Query fragments, and the last key that each of this lane's two rows sees.
-        uint32_t qa[8][4];
-        int limit[2];
+        // Query fragments (columns are rows of the tile), and the last key that each of this lane's rows sees.
+        uint32_t qb[NT][8][2];
+        int limit[NT][2];
         if (!failed && !mbar_wait_warp(smem_u32(&query_full), turn & 1u, p.status, 225)) failed = true;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-            const int c16 = ks * 2 + (mi >> 1);
-            ldmatrix_x4(swz128(query_addr + (c16 >> 3) * query_half, c16 & 7), qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
-        }
+        for (int m = 0; m < NT; ++m)
+#pragma unroll
+            for (int ks = 0; ks < 8; ks += 2) {   // four 8 x 8 matrices: 32 elements of the head dimension
+                const int c16 = ks * 2 + mi;
+                ldmatrix_x4(swz128(query_row[m] + (c16 >> 3) * query_half, c16 & 7), qb[m][ks][0], qb[m][ks][1], qb[m][ks + 1][0], qb[m][ks + 1][1]);
+            }
         mbar_release_stage(smem_u32(&query_empty), lane);
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr)
-            limit[rr] = rr * 8 + g < rows ? min(un.limit0 + un.tile * QT + row_tok[rr], un.hi - 1) : -1;
-        float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[16][4];
+        for (int m = 0; m < NT; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            for (int rr = 0; rr < 2; ++rr)
+                limit[m][rr] = m * 8 + 2 * t + rr < rows ? min(un.limit0 + un.tile * QT + row_tok[m][rr], un.hi - 1) : -1;
+        float mx[NT][2], l[NT][2], o[NT][8][4];
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            mx[m][0] = mx[m][1] = -INFINITY;
+            l[m][0] = l[m][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[m][i][0] = o[m][i][1] = o[m][i][2] = o[m][i][3] = 0.f;
+        }
         for (int st = un.s_begin; st < un.s_end; ++st, ++it_count) {
             const uint32_t slot = it_count % kStages;
             if (!failed && !mbar_wait_warp(smem_u32(&full_bar[slot]), (it_count / kStages) & 1u, p.status, 222)) failed = true;
             const int key0 = un.start + st * SK + kg * 16;
             const int skip = un.lo - key0, valid = un.hi - key0;   // keys [skip, valid) of the 16 belong to the unit
             if (!failed && valid > 0 && skip < 16) {
-                const uint32_t base = smem_base + slot * kStageBytes;
+                const uint32_t base = smem_base + slot * stage_bytes;
                 if (valid < 16 || skip > 0) {
                     // Rows outside the unit hold whatever the page (or an earlier stage) has there: 0 * NaN would stay.
                     for (int i = lane; i < 16 * 16; i += 32) {
@@ -273,81 +326,84 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
-                // ---- S = Q K^T ----
-                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-                {
-                    const uint32_t rowoff = tile_row((mi >> 1) * 8 + r8) * 128u;
+                // ---- S^T = K Q^T: keys g and g + 8, rows 2 t and 2 t + 1 of every eight ----
+                float x[NT][4];
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const int c16 = ks * 2 + (mi & 1);
-                        uint32_t b00, b01, b10, b11;
-                        ldmatrix_x4(swz128(base + (c16 >> 3) * kHalfBytes + rowoff, c16 & 7), b00, b01, b10, b11);
-                        mma_bf16_16816(s0, qa[ks], b00, b01);
-                        mma_bf16_16816(s1, qa[ks], b10, b11);
-                    }
-                }
-                // ---- softmax, with the running maximum ----
-                float x[8], top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = key0 + (e >> 2) * 8 + 2 * t + (e & 1), rr = e >> 1 & 1;
-                    x[e] = key >= un.lo && key <= limit[rr] ? (e < 4 ? s0[e] : s1[e - 4]) * p.scale_log2 : -INFINITY;
-                    top[rr] = fmaxf(top[rr], x[e]);
-                }
-#pragma unroll
-                for (int rr = 0; rr < 2; ++rr) {
-                    top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xffffffffu, top[rr], 1));
-                    top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xffffffffu, top[rr], 2));
-                    const float now = fmaxf(mx[rr], top[rr]);
-                    const float ref = now == -INFINITY ? 0.f : now;   // no key seen yet: every weight is 2^-inf = 0
-                    const float shrink = exp2f(mx[rr] - ref);
-                    mx[rr] = now;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if ((e >> 1 & 1) == rr) {
-                            x[e] = exp2f(x[e] - ref);
-                            sum += x[e];
-                        }
-                    l[rr] = l[rr] * shrink + sum;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        o[i][2 * rr] *= shrink;
-                        o[i][2 * rr + 1] *= shrink;
-                    }
-                }
-                const uint32_t pa[4] = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-                // Keys that later rows see and earlier ones do not: an infinity or NaN in their values must not reach the earlier
-                // rows as 0 times it.  Such keys are added by hand for the rows that see them.
-                if (un.ntok > 1 && un.limit0 + 1 < key0 + min(valid, 16)) add_odd_values(base, key0, valid, un.limit0, limit, x, o, value_addr);
-                // ---- O += P V ----
+                for (int m = 0; m < NT; ++m) x[m][0] = x[m][1] = x[m][2] = x[m][3] = 0.f;
                 {
                     const int j = (mi & 1) * 8 + r8;
 #pragma unroll
-                    for (int np = 0; np < 8; ++np) {
-                        uint32_t v0, v1, v2, v3;
-                        ldmatrix_x4_trans(value_addr(base, j, np * 2 + (mi >> 1)), v0, v1, v2, v3);
-                        mma_bf16_16816(o[2 * np], pa, v0, v1);
-                        mma_bf16_16816(o[2 * np + 1], pa, v2, v3);
+                    for (int ks = 0; ks < 8; ++ks) {
+                        uint32_t ka[4];
+                        ldmatrix_x4(key_addr(base, j, ks * 2 + (mi >> 1)), ka[0], ka[1], ka[2], ka[3]);
+#pragma unroll
+                        for (int m = 0; m < NT; ++m) mma_bf16_16816(x[m], ka, qb[m][ks][0], qb[m][ks][1]);
+                    }
+                }
+                // ---- softmax, with the running maximum ----
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int m = 0; m < NT; ++m) {
+                    float top[2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + g + (e >> 1) * 8;
+                        x[m][e] = key >= un.lo && key <= limit[m][e & 1] ? x[m][e] * p.scale_log2 : -INFINITY;
+                    }
+#pragma unroll
+                    for (int rr = 0; rr < 2; ++rr) {
+                        top[rr] = fmaxf(x[m][rr], x[m][2 + rr]);
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) top[rr] = fmaxf(top[rr], __shfl_xor_sync(0xffffffffu, top[rr], d));
+                        const float now = fmaxf(mx[m][rr], top[rr]);
+                        const float ref = now == -INFINITY ? 0.f : now;   // no key seen yet: every weight is 2^-inf = 0
+                        const float shrink = exp2f(mx[m][rr] - ref);
+                        mx[m][rr] = now;
+                        x[m][rr] = exp2f(x[m][rr] - ref);
+                        x[m][2 + rr] = exp2f(x[m][2 + rr] - ref);
+                        l[m][rr] = l[m][rr] * shrink + (x[m][rr] + x[m][2 + rr]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            o[m][i][rr] *= shrink;
+                            o[m][i][2 + rr] *= shrink;
+                        }
+                    }
+                    pb[m][0] = transpose_8x8(pack_bf16(x[m][0], x[m][1]));
+                    pb[m][1] = transpose_8x8(pack_bf16(x[m][2], x[m][3]));
+                }
+                // Keys that later rows see and earlier ones do not: an infinity or NaN in their values must not reach the earlier
+                // rows as 0 times it.  Such keys are added by hand for the rows that see them.
+                if (un.ntok > 1 && un.limit0 + 1 < key0 + min(valid, 16)) add_odd_values<NT>(base, key0, valid, un.limit0, limit, x, o, value_addr);
+                // ---- O^T += V^T P^T ----
+                {
+                    const int j = (mi >> 1) * 8 + r8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t va[4];
+                        ldmatrix_x4_trans(value_addr(base, j, i * 2 + (mi & 1)), va[0], va[1], va[2], va[3]);
+#pragma unroll
+                        for (int m = 0; m < NT; ++m) mma_bf16_16816(o[m][i], va, pb[m][0], pb[m][1]);
                     }
                 }
             }
             mbar_release_stage(smem_u32(&empty_bar[slot]), lane);
         }
         // ---- the part's statistics and sums ----
-        const int64_t part = (static_cast<int64_t>(un.slot) * KG + kg) * Hkv + h;
+        const int64_t part = ((static_cast<int64_t>(un.slot) * KG + kg) * Hkv + h) * (8 * NT);
 #pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-            float sum = l[rr];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (rr * 8 + g >= rows) continue;
-            const int64_t at = part * RT + rr * 8 + g;
-            float* dst = p.ws_o + at * kD + 2 * t;
+        for (int m = 0; m < NT; ++m)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * rr], o[i][2 * rr + 1]);
-            if (t == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(mx[rr], sum);
-        }
+            for (int rr = 0; rr < 2; ++rr) {
+                float sum = l[m][rr];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int r = m * 8 + 2 * t + rr;
+                if (r >= rows) continue;
+                float* dst = p.ws_o + (part + r) * kD + g;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dst[i * 8] = o[m][i >> 1][(i & 1) * 2 + rr];
+                if (g == 0) *reinterpret_cast<float2*>(p.ws_ml + (part + r) * 2) = make_float2(mx[m][rr], sum);
+            }
     }
     if (p.with_tc) pdl_wait_prior();
 }
@@ -373,7 +429,7 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     const int h = head / p.group, hh = head - h * p.group, KG = kConsumerWarps / p.kv_heads;
     auto parts_of = [&](int first, int pieces, int t) {   // of token t of the unit
         const int tile = t / p.row_tokens, r = (t - tile * p.row_tokens) * p.group + hh;
-        return Parts{(static_cast<int64_t>(first + tile * pieces) * KG * p.kv_heads + h) * RT + r, static_cast<int64_t>(p.kv_heads) * RT,
+        return Parts{(static_cast<int64_t>(first + tile * pieces) * KG * p.kv_heads + h) * p.tile_rows + r, static_cast<int64_t>(p.kv_heads) * p.tile_rows,
                      pieces * KG};
     };
     const Parts own = parts_of(j.own_first, j.own_pieces, j.own_t);
@@ -429,19 +485,24 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
 
 int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-// Query tokens whose heads of a KV head fill a row tile.
-int row_tokens(int64_t group) { return static_cast<int>(RT / group); }
+// Eights of rows of a row tile: as few as hold what a request brings on average, or a group whose prefix is read here.
+int row_eights(int64_t tokens, int64_t batch, int64_t groups, int64_t group) {
+    int64_t rows = div_ceil64(tokens * group, batch);
+    if (groups > 0 && tokens * group <= kTcRows * groups) rows = div_ceil64(tokens * group, groups);
+    if (rows < group) rows = group;
+    return rows <= 8 ? 1 : 2;
+}
 
 // Where the pieces of the workspace begin, in bytes; partial rows ahead of the tensor-core kernel's.
 struct SharedLayout {
     int64_t slots, tc_slots, rows, tc_of, rows_items, tc_items, join, ml, o, bytes;
 };
-SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads) {
+SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads, int nt) {
     const int64_t group = q_heads / kv_heads, rows = tokens * group, kg = kConsumerWarps / kv_heads, ctas = sm_count();
     SharedLayout x;
     // row tiles: at most one more than full ones per unit, and every row is in two units; items: one more than full ones per tile
-    x.slots = kSharedPieces * ctas + 2 * (tokens / row_tokens(group)) + batch + groups;
-    x.rows = x.slots * kg * kv_heads * RT;
+    x.slots = kSharedPieces * ctas + 2 * (tokens / (8 * nt / group)) + batch + groups;
+    x.rows = x.slots * kg * kv_heads * 8 * nt;
     // units of the tensor-core kernel: the same of groups that have more than kTcRows rows
     const int64_t tc_groups = groups < rows / (kTcRows + 1) ? groups : rows / (kTcRows + 1);
     x.tc_slots = rows > kTcRows && groups > 0 ? ctas + kv_heads * (tokens / (2 * (kSharedTcTile / group)) + tc_groups) : 0;
@@ -463,6 +524,16 @@ struct FollowOn {
     ~FollowOn() { set_pdl_launches(was); }
 };
 
+template <int NT>
+int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const SharedPrefixParams& p, cudaStream_t stream) {
+    const int stage = kStageBytes + (p.small ? 2 * p.stage_keys * 16 : 0);
+    const int smem = (kStages * stage + 127 & ~127) + NT * 8 * p.kv_heads * kD * 2 + 1024;
+    auto kernel = p.small ? shared_prefix_rows_kernel<NT, true> : shared_prefix_rows_kernel<NT, false>;
+    B200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    B200_CHECK_CUDA(launch_kernel(kernel, dim3(p.ctas), dim3(kThreads), smem, stream, dim3(1, 1, 1), tk, tv, tq, p));
+    return B200_OK;
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -473,7 +544,12 @@ int64_t b200_attention_shared_prefix_workspace_bytes(int max_tokens, int max_bat
     if (max_tokens <= 0 || max_batch <= 0 || max_batch > kSharedMaxBatch || q_heads <= 0 || head_dim != kD) return -1;
     if (kv_heads < 1 || kv_heads > 8 || 8 % kv_heads != 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > 16) return -1;
     if (static_cast<int64_t>(max_tokens) * q_heads > (1 << 28)) return -1;
-    return shared_layout(max_tokens, max_batch, max_batch, q_heads, kv_heads).bytes + 256;
+    int64_t most = 0;
+    for (int nt = q_heads / kv_heads <= 8 ? 1 : 2; nt <= 2; ++nt) {
+        const int64_t bytes = shared_layout(max_tokens, max_batch, max_batch, q_heads, kv_heads, nt).bytes;
+        if (bytes > most) most = bytes;
+    }
+    return most + 256;
 }
 
 int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t stream) {
@@ -525,11 +601,16 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.kv_heads = a->kv_heads;
     p.group = a->q_heads / a->kv_heads;
     p.stage_keys = kStageRows / a->kv_heads;
-    p.kpc = a->page_size < p.stage_keys ? a->page_size : p.stage_keys;
+    p.small = a->page_size < kSmallPage;
+    p.kpc = !p.small && a->page_size < p.stage_keys ? a->page_size : p.stage_keys;
+    p.align = p.small ? 1 : p.kpc;
+    p.k_cache = static_cast<const __nv_bfloat16*>(a->k_cache);
+    p.v_cache = static_cast<const __nv_bfloat16*>(a->v_cache);
     p.num_slots = a->num_slots;
     p.scale_log2 = a->sm_scale * 1.4426950408889634f;
     p.status = status;
-    const SharedLayout x = shared_layout(a->tokens, a->batch, a->groups, a->q_heads, a->kv_heads);
+    const int nt = row_eights(a->tokens, a->batch, a->groups, p.group);
+    const SharedLayout x = shared_layout(a->tokens, a->batch, a->groups, a->q_heads, a->kv_heads, nt);
     if (a->workspace_bytes < x.bytes + 256) {
         set_last_error("attention_shared_prefix: workspace of %lld bytes is too small (need %lld)",
                        static_cast<long long>(a->workspace_bytes), static_cast<long long>(x.bytes + 256));
@@ -546,7 +627,8 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.tc_base = x.rows;
     p.max_slots = static_cast<int>(x.slots);
     p.tc_slots = static_cast<int>(x.tc_slots);
-    p.row_tokens = row_tokens(p.group);
+    p.tile_rows = 8 * nt;
+    p.row_tokens = p.tile_rows / p.group;
     p.tc_rows = kTcRows;
     // (a group has more rows than that only if all have)
     p.with_tc = a->groups > 0 && static_cast<int64_t>(a->tokens) * p.group > kTcRows;
@@ -566,9 +648,8 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
         err = launch_shared_prefix_tc(p, a->k_cache, a->v_cache, a->page_size, s);
         if (err != B200_OK) return err;
     }
-    const int smem = kStages * kStageBytes + kQueryBytes + 1024;
-    B200_CHECK_CUDA(cudaFuncSetAttribute(shared_prefix_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_rows_kernel, dim3(p.ctas), dim3(kThreads), smem, s, dim3(1, 1, 1), tk, tv, tq, p));
+    err = nt == 1 ? launch_rows<1>(tk, tv, tq, p, s) : launch_rows<2>(tk, tv, tq, p, s);
+    if (err != B200_OK) return err;
     B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(a->tokens, div_ceil(a->q_heads, kMergeWarps)), dim3(kMergeWarps * 32),
                                   0, s, dim3(1, 1, 1), p));
     return B200_OK;

@@ -57,7 +57,8 @@ struct __align__(16) PlanHead {
     int tc_per, tc_chunked;       // tensor-core kernel: tiles per CTA, in chunks of one unit or in runs
     int next;                     // rows kernel: the first item that nobody has taken yet
     int rows_lead;                // ... and how many a CTA takes ahead of the one it copies
-    int pad[2];
+    int rows_first;               // ... and the CTAs that begin with the item of their own number
+    int pad;
 };
 
 struct SharedPlan {
@@ -77,8 +78,10 @@ struct SharedPrefixParams {
     const int32_t *table_idx, *seq_lens, *qo_indptr, *group_indptr, *prefix_lens;
     int tokens, batch, groups;
     int q_heads, kv_heads, group;   // group: query heads per KV head
-    int stage_keys, kpc;            // rows kernel: keys per stage and per copy
-    int row_tokens;                 // ... and query tokens per row tile: 16 / group
+    int stage_keys, kpc;            // rows kernel: keys per stage, and those that lie together in it (a copy's, with its pages)
+    int small, align;               // ... whether pages are too small for copies of them; keys are read from a multiple of this
+    int tile_rows, row_tokens;      // ... rows of a row tile, and the query tokens whose heads fill it: tile_rows / group
+    const __nv_bfloat16 *k_cache, *v_cache;
     int64_t num_slots;
     float scale_log2;
     float *ws_ml, *ws_o;            // partial rows, (maximum, sum) and x 128: the rows kernel's [max_slots, key groups, kv_heads, row tile],

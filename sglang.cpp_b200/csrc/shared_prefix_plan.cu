@@ -33,7 +33,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     __shared__ int s_first[kMaxUnits + 1];                                      // items before a unit, in the rows kernel
     __shared__ int s_tc[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];      // tiles and units before a group, in the other
     __shared__ int4 s_warp[32];
-    __shared__ int s_per;
+    __shared__ int s_per, s_chunks;   // tiles per chunk, chunks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = static_cast<int>(blockDim.x);
     const int G = p.group, Hkv = p.kv_heads, SK = p.stage_keys, QB = kSharedTcTile / G, QT = p.row_tokens, U = p.groups + p.batch, ctas = p.ctas;
     pdl_launch_dependents();
@@ -81,7 +81,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     __syncthreads();
 
     // ---- sizes ----
-    auto start_of = [&](int lo) { return lo & ~(p.kpc - 1); };
+    auto start_of = [&](int lo) { return lo & ~(p.align - 1); };
     auto stages_of = [&](int lo, int hi) { return (max(hi - start_of(lo), 0) + SK - 1) / SK; };
     // a group's prefix: row tiles and stages of the rows kernel, or units and key tiles of the other
     int g_tiles = 0, g_stages = 0, g_units = 0, g_tc = 0;
@@ -115,8 +115,10 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     sum = lane < threads >> 5 ? s_warp[lane] : make_int4(0, 0, 0, 0);
     const int stages = __reduce_add_sync(0xffffffffu, sum.x), tc_tiles = __reduce_add_sync(0xffffffffu, sum.y);
     const int units = __reduce_add_sync(0xffffffffu, sum.z), longest = __reduce_max_sync(0xffffffffu, sum.w);
-    // Items of equal stages, few enough for the room there is for partial results.
-    const int piece = max((stages + kSharedPieces * ctas - 1) / (kSharedPieces * ctas), kMinStages);
+    // Stages per item: about an item per CTA where that makes short ones (every item costs a microsecond of queries and results, and its
+    // parts have to be joined: 64 requests of up to 512 keys of their own 34.8 us with 2 stages, 31.4 with 6), several where they
+    // would be long, and no more of them than there is room for.
+    const int piece = max(max((stages + kSharedPieces * ctas - 1) / (kSharedPieces * ctas), min((stages + ctas - 1) / ctas, kLongPiece)), kMinStages);
     const int g_pieces = (g_stages + piece - 1) / piece, b_pieces = (b_stages + piece - 1) / piece;
 
     // ---- sums over what comes before: x the groups' items, y the requests'; z key tiles, w units ----
@@ -156,7 +158,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     const bool chunked = units > 0 && 2 * units <= ctas;
     if (warp == 0) {
         const int least = max((tc_tiles + ctas - 1) / ctas, kMinTiles), most = max(longest, least);
-        int per = least;
+        int per = least, chunks = 0;
         if (chunked) {
             per = lane == 31 ? most : min(static_cast<int>(least * exp2f(log2f(static_cast<float>(most) / least) * (lane / 31.f)) + 0.5f), most);
             int count = 0;
@@ -178,13 +180,18 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
                 }
             }
             per = __shfl_sync(0xffffffffu, per, best);
+            chunks = __shfl_sync(0xffffffffu, count, best);
         }
         if (lane == 0) {
             s_per = per;
+            s_chunks = chunks;
             PlanHead h = {};
             h.fits = fits;
             h.rows_items = fits ? items : 0;
-            h.rows_lead = piece < kLongPiece ? 2 : 1;
+            // CTAs that find an SM free begin with the item of their own number.
+            h.rows_first = chunked || units == 0 ? max(ctas - s_chunks, 0) : 0;
+            h.next = min(h.rows_first, h.rows_items);
+            h.rows_lead = piece < kLongPiece && items > 2 * ctas ? 2 : 1;
             h.tc_per = per;
             h.tc_chunked = chunked;
             *p.plan.head = h;

@@ -32,6 +32,11 @@ ATTENTION = {
     "many rows": ([[(70, 64), (100, 90), (50, 1)]], [400], 16, 16, 8),
     "wide group": ([[(3 + i % 50, 1) for i in range(150)]], [2100], 16, 16, 8),
     "wide groups of drafts": ([[(6 + i % 40, 1 + i % 5) for i in range(40)], [(9, 3)] * 30, [(5, 1)] * 3], [1500, 129, 777], 16, 32, 4),
+    "pages of one token, every layout": ([[(40, 2), (17, 1), (3, 3)], [(21, 1), (90, 1)]], [75, 310], 1, 32, 8),
+    "pages of two, two KV heads": ([[(40, 3), (17, 1), (300, 1)]], [211], 2, 8, 2),
+    "pages of four, one KV head, many heads": ([[(40, 2), (17, 1), (300, 5)]], [1021], 4, 14, 1),
+    "pages of one token, wide group": ([[(3 + i % 20, 1 + i % 3) for i in range(40)]], [515], 1, 16, 4),
+    "pages of eight": ([[(40, 2), (17, 1), (3, 3)], [(21, 1), (90, 1)]], [75, 310], 8, 32, 8),
     "long": ([[(40, 1), (5, 1), (600, 1)] * 8], [9000], 16, 16, 8),
 }
 
