@@ -10,17 +10,20 @@
 // that a border is missed by no more than that.  Sums are formed in a fixed order: equal calls, equal tokens.
 //
 // Bound by HBM: one row of p, and one of q where a draft was refused, 8 bytes per vocabulary entry and request, read once; the
-// other rows are looked at in one place each.  A cluster of CTAs shares a row: every warp sums a run of consecutive entries, the
-// CTAs exchange their sums, and the warp in whose run the target lies walks it once more (a few KB from L2).
+// other rows are looked at in one place each.  A cluster of CTAs shares a row: every warp sums a run of consecutive entries in
+// rounds of 512 (their loads before their sums), the CTAs exchange their sums, and the warp in whose run the target lies finds
+// the round by the sums that its lanes kept and reads that round once more.
 #include "common.cuh"
 #include "kernels.h"
 
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxThreads = 1024, kMaxPerSm = 4;   // an SM's threads are shared by one, two or four CTAs
+constexpr int kMaxWarps = kMaxThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kEach = 16;            // entries of a lane in a round
+constexpr int kRound = 32 * kEach;
 
 struct VerifyParams {
     int32_t *tokens, *accepted;
@@ -33,14 +36,14 @@ struct VerifyParams {
 };
 
 // What an entry counts for: nothing unless it is a positive number.
-__device__ __forceinline__ float entry(float p) { return p > 0.f ? fminf(p, 3.402823466e38f) : 0.f; }
+__device__ __forceinline__ float entry(float p) { return fminf(fmaxf(p, 0.f), 3.402823466e38f); }   // (a NaN is 0: the other of the two)
 __device__ __forceinline__ float unit_interval(float u) { return u > 0.f ? fminf(u, 0.99999994f) : 0.f; }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMaxThreads)
 verify_drafts_kernel(const VerifyParams p) {
-    __shared__ double s_sum[kWarps], s_cta[kMaxCluster];
+    __shared__ double s_sum[kMaxWarps], s_cta[kMaxCluster];
     __shared__ int s_accepted;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, b = static_cast<int>(blockIdx.x) / C;
     if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (waited for ahead of the first remote store)
     pdl_launch_dependents();
@@ -72,7 +75,7 @@ verify_drafts_kernel(const VerifyParams p) {
     __syncthreads();
     const int a = s_accepted;
     if (rank == 0)
-        for (int j = threadIdx.x; j <= p.most; j += kThreads)
+        for (int j = threadIdx.x; j <= p.most; j += blockDim.x)
             if (j != a) p.tokens[static_cast<int64_t>(b) * (p.most + 1) + j] = j < a ? p.draft_tokens[start + j] : -1;
     if (rank == 0 && threadIdx.x == 0) p.accepted[b] = a;
 
@@ -81,9 +84,10 @@ verify_drafts_kernel(const VerifyParams p) {
     const bool refused = a < n;
     const float* qrow = refused && p.draft != nullptr ? p.draft + (start + a) * p.draft_ld : nullptr;
     const int without = refused && p.draft == nullptr ? p.draft_tokens[start + a] : -1;   // a draft that was certain
-    const int run = ((p.vocab + C * kWarps - 1) / (C * kWarps) + 127) / 128 * 128;
-    const int first = min((rank * kWarps + warp) * run, p.vocab), last = min(first + run, p.vocab);
-    const bool aligned = ((reinterpret_cast<uintptr_t>(prow) | reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
+    const int run = (p.vocab + C * warps * kRound - 1) / (C * warps * kRound) * kRound;
+    const int first = static_cast<int>(min(static_cast<int64_t>(rank * warps + warp) * run, static_cast<int64_t>(p.vocab)));
+    const int last = first + min(run, p.vocab - first);
+    const int per = (run / kRound + 31) / 32, part = per * kRound;   // a part: rounds, entries whose sum one lane keeps
     bool rest = refused;   // p - q; or p, where no entry of p exceeds q
     auto weigh = [&](float x, float y, int i) -> double {
         const float px = entry(x);
@@ -91,52 +95,81 @@ verify_drafts_kernel(const VerifyParams p) {
         if (qrow == nullptr) return i == without ? fmaxf(px - 1.f, 0.f) : px;
         return fmax(static_cast<double>(px) - static_cast<double>(entry(y)), 0.0);
     };
-    // Sum of entries [from, to), lanes next to one another; the loads of a round before its sums.
-    auto sum_of = [&](int from, int to) {
-        const bool both = rest && qrow != nullptr;
+    // Sums of a lane's entries of a round.  p - q is taken as the rounded fp32 difference and what its rounding left out (an fp32
+    // number too, as p >= q >= 0), and the small parts are summed in fp32: sixteen of them are off by 2^-20 of theirs, 2^-45 of
+    // the difference, and a conversion to fp64 per entry is saved (they run at a quarter of fp64's rate).
+    auto difference = [&](const float (&x)[kEach], const float (&y)[kEach]) {
         double sum = 0.0;
-        if (aligned && ((from | to) & 3) == 0) {
-            constexpr int kRound = 4;
-            for (int base = from; base < to; base += kRound * 128) {
-                float4 x[kRound], y[kRound];
+        float small = 0.f;
 #pragma unroll
-                for (int k = 0; k < kRound; ++k) {
-                    const int i = base + k * 128 + lane * 4;
-                    x[k] = i < to ? __ldg(reinterpret_cast<const float4*>(prow + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    y[k] = both && i < to ? __ldg(reinterpret_cast<const float4*>(qrow + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+        for (int k = 0; k < kEach; ++k) {
+            const float px = entry(x[k]), qx = entry(y[k]), d = px - qx;
+            if (d > 0.f) small += (px - d) - qx;
+            sum += fmaxf(d, 0.f);
+        }
+        return sum + small;
+    };
+    auto plain = [&](const float (&x)[kEach], int base, bool aligned) {   // p, less the draft that was certain
+        double sum = 0.0;
+        const int skip = rest && without >= base && without < base + kRound ? without - base : -1;
+        const int at = aligned ? skip / 128 * 4 + skip % 4 : skip / 32, of = aligned ? skip % 128 / 4 : skip % 32;
+        const bool here = skip >= 0 && lane == of;
 #pragma unroll
-                for (int k = 0; k < kRound; ++k) {
-                    const int i = base + k * 128 + lane * 4;
-                    sum += (weigh(x[k].x, y[k].x, i) + weigh(x[k].y, y[k].y, i + 1)) + (weigh(x[k].z, y[k].z, i + 2) + weigh(x[k].w, y[k].w, i + 3));
-                }
-            }
-        } else {
-            constexpr int kRound = 8;
-            for (int base = from; base < to; base += kRound * 32) {
-                float x[kRound], y[kRound];
-#pragma unroll
-                for (int k = 0; k < kRound; ++k) {
-                    const int i = base + k * 32 + lane;
-                    x[k] = i < to ? __ldg(prow + i) : 0.f;
-                    y[k] = both && i < to ? __ldg(qrow + i) : 0.f;
-                }
-#pragma unroll
-                for (int k = 0; k < kRound; ++k) sum += weigh(x[k], y[k], base + k * 32 + lane);
-            }
+        for (int k = 0; k < kEach; ++k) {
+            const float px = entry(x[k]);
+            sum += here && k == at ? fmaxf(px - 1.f, 0.f) : px;
         }
         return sum;
+    };
+    // Sum of this warp's run, the same in every lane; kept: lane c's, of the run's c-th part.
+    double kept = 0.0;
+    auto sum_run = [&]() {
+        const bool both = rest && qrow != nullptr;
+        const bool aligned = ((reinterpret_cast<uintptr_t>(prow) | (both ? reinterpret_cast<uintptr_t>(qrow) : 0) | (p.vocab & 3)) & 15) == 0;
+        auto fetch = [&](float (&x)[kEach], const float* row, int round) {
+            const int base = first + round * kRound;
+            if (aligned) {
+#pragma unroll
+                for (int k = 0; k < kEach / 4; ++k) {
+                    const int i = base + k * 128 + lane * 4;
+                    reinterpret_cast<float4*>(x)[k] = i < last ? __ldg(reinterpret_cast<const float4*>(row + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    const int i = base + k * 32 + lane;
+                    x[k] = i < last ? __ldg(row + i) : 0.f;
+                }
+            }
+        };
+        double all = 0.0, sum = 0.0;
+        kept = 0.0;
+        const int rounds = (last - first + kRound - 1) / kRound;
+        auto add = [&](double w, int round) {
+            sum += w;
+            if ((round + 1) % per != 0 && round + 1 < rounds) return;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == round / per) kept = sum;
+            all += sum;
+            sum = 0.0;
+        };
+        for (int r = 0; r < rounds; ++r) {
+            float x[kEach], y[kEach];
+            fetch(x, prow, r);
+            if (both) fetch(y, qrow, r);
+            add(both ? difference(x, y) : plain(x, first + r * kRound, aligned), r);
+        }
+        return all;
     };
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     double total = 0.0, before = 0.0, mine = 0.0;   // of the row, of the runs before this warp's, of this run
     for (int pass = 0; pass < 2; ++pass) {
-        double sum = sum_of(first, last);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double sum = sum_run();
         if (lane == 0) s_sum[warp] = sum;
         __syncthreads();
         double cta = 0.0, ahead = 0.0;
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             if (w == warp) ahead = cta;
             cta += s_sum[w];
         }
@@ -174,8 +207,8 @@ verify_drafts_kernel(const VerifyParams p) {
     }
     const double goal = unit_interval(p.draw[b]) * total;
     if (!(mine > 0.0) || goal < before || goal >= before + mine) return;
-    // The run once more: a stretch of neighbouring entries per lane, then, of the lane whose stretch the goal is in, an entry per lane.
-    // (The sums are formed in another order than before: the last bits may put the goal behind the run's last entry.)
+    // The part of the run, by the sums that the lanes kept; then that part once more, neighbouring entries in a lane.  (The sums
+    // are formed in another order than before: the last bits may put the goal behind the part's last entry.)
     auto scan = [&](double w) {   // sums up to and with each lane's
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -184,28 +217,45 @@ verify_drafts_kernel(const VerifyParams p) {
         }
         return w;
     };
-    auto weight = [&](int i) { return weigh(__ldg(prow + i), rest && qrow != nullptr ? __ldg(qrow + i) : 0.f, i); };
-    const int stretch = (last - first + 31) / 32;
-    double own = 0.0;
-#pragma unroll 8
-    for (int i = 0; i < stretch; ++i)
-        if (first + lane * stretch + i < last) own += weight(first + lane * stretch + i);
-    const double upto = scan(own);
-    const uint32_t over = __ballot_sync(0xffffffffu, own > 0.0 && before + upto > goal), some = __ballot_sync(0xffffffffu, own > 0.0);
-    const int chosen = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
-    double ahead = before + __shfl_sync(0xffffffffu, upto, chosen) - __shfl_sync(0xffffffffu, own, chosen);
-    const int from = first + chosen * stretch, to = min(from + stretch, last);
-    int pick = -1, positive = -1;
-    for (int base = from; base < to && pick < 0; base += 32) {
-        const int i = base + lane;
-        const double w = i < to ? weight(i) : 0.0;
-        const double incl = scan(w);
-        const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && ahead + incl > goal), any = __ballot_sync(0xffffffffu, w > 0.0);
-        if (hit != 0) pick = base + __ffs(hit) - 1;
-        if (any != 0) positive = base + 31 - __clz(any);
-        ahead += __shfl_sync(0xffffffffu, incl, 31);
+    auto choose = [&](double own, double ahead, double& upto) {   // the first lane whose sum passes the goal, or -1
+        upto = scan(own);
+        return __ffs(__ballot_sync(0xffffffffu, own > 0.0 && ahead + upto > goal)) - 1;
+    };
+    double upto;
+    int chosen = choose(kept, before, upto);
+    if (chosen < 0) chosen = 31 - __clz(__ballot_sync(0xffffffffu, kept > 0.0));
+    double ahead = before + __shfl_sync(0xffffffffu, upto, chosen) - __shfl_sync(0xffffffffu, kept, chosen);
+    const int from = first + chosen * part, to = min(from + part, last);
+    int pick = -1;   // the last positive entry so far, until one passes the goal
+    for (int base = from; base < to; base += kRound) {
+        double w[kEach], own = 0.0;
+        const int at = base + lane * kEach;
+        float x[kEach], y[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            x[k] = at + k < to ? __ldg(prow + at + k) : 0.f;
+            y[k] = rest && qrow != nullptr && at + k < to ? __ldg(qrow + at + k) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) own += w[k] = weigh(x[k], y[k], at + k);
+        const int hit = choose(own, ahead, upto);
+        const uint32_t positive = __ballot_sync(0xffffffffu, own > 0.0);
+        const int who = hit >= 0 ? hit : 31 - __clz(positive);
+        if (who >= 0) {
+            double sum = ahead + upto - own;
+            int mine = -1;
+            bool passed = false;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                sum += w[k];
+                if (w[k] > 0.0 && !passed) mine = at + k, passed = hit >= 0 && sum > goal;
+            }
+            pick = __shfl_sync(0xffffffffu, mine, who);
+        }
+        if (hit >= 0) break;
+        ahead += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) *out = pick >= 0 ? pick : positive;
+    if (lane == 0) *out = pick;
 }
 
 }  // namespace
@@ -226,12 +276,14 @@ int b200_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_p
     int err = B200_OK;
     int* status = device_status_words(&err);
     if (err != B200_OK) return err;
-    // CTAs per row: enough to fill the device, and no fewer than 4096 entries each.
-    int cluster = 1;
-    while (cluster < kMaxCluster && static_cast<int64_t>(batch) * cluster < 2 * sm_count() && vocab / (2 * cluster) >= 4096) cluster *= 2;
+    // CTAs per row: enough to fill the device, and no fewer than 4096 entries each.  Their threads: all that an SM has room for.
+    const int64_t sms = sm_count();
+    int cluster = 1, threads = kMaxThreads;
+    while (cluster < kMaxCluster && static_cast<int64_t>(batch) * 2 * cluster <= kMaxPerSm * sms && vocab / (2 * cluster) >= 4096) cluster *= 2;
+    while (threads > kMaxThreads / kMaxPerSm && static_cast<int64_t>(batch) * cluster * threads > sms * kMaxThreads) threads /= 2;
     VerifyParams p = {tokens,       accepted,       target_probs, draft_probs, target_ld,    draft_ld, draft_tokens, draft_indptr,
                       accept_uniform, draw_uniform, batch,        total_drafts, max_drafts, vocab,    cluster,      status};
-    B200_CHECK_CUDA(launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(batch) * cluster), dim3(kThreads), 0,
+    B200_CHECK_CUDA(launch_kernel(verify_drafts_kernel, dim3(static_cast<unsigned>(batch) * cluster), dim3(threads), 0,
                                   static_cast<cudaStream_t>(stream), dim3(cluster, 1, 1), p));
     return B200_OK;
 }
