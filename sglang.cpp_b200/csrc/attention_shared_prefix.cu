@@ -180,9 +180,6 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         RowsItem it = get_item(0);
         if (it.slot >= 0) fetch_slots(it, it.s_begin);
         for (uint32_t turn = 0; it.slot >= 0 && !failed; ++turn) {
-            int taken = 0;
-            if (leads) taken = atomicAdd(&p.plan.head->next, 1);
-            __syncwarp();
             if (which == 3) {   // the queries, when the consumers have taken the last item's to registers
                 if (!mbar_wait_warp(smem_u32(&query_empty), (turn & 1u) ^ 1u, p.status, 226)) break;
                 const uint32_t half = static_cast<uint32_t>(p.row_tokens * p.q_heads) * 128u, bar = smem_u32(&query_full);
@@ -195,6 +192,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
             }
             RowsItem after;
             after.slot = -1;
+            const int take_at = lead > 1 ? it.s_begin : max(it.s_end - 1, it.s_begin);
             for (int st = it.s_begin; st < it.s_end; ++st, ++it_count) {
                 const int n = copies_of(it, st);
                 int sl[4];
@@ -239,8 +237,8 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                         else tma_load_3d_hint(base + copy * copy_bytes, map, (which & 1) * 64, sl[c], 0, bar, once);
                     }
                 }
-                if (st == it.s_begin) {
-                    if (leads) hand_on(turn + lead, taken);
+                if (st == take_at) {
+                    if (leads) hand_on(turn + lead, atomicAdd(&p.plan.head->next, 1));
                     __syncwarp();
                     after = get_item(turn + 1);
                 }
