@@ -124,6 +124,13 @@ __device__ __noinline__ double weight64(float a, float top, double per_t) {
     return e < -200.0 ? 0.0 : exp2(e);
 }
 
+// The weight of a, and by what factor the weight of a - step is smaller.
+__device__ __noinline__ double2 weight_and_ratio(float a, float top, double per_t, float step) {
+    const double e = (static_cast<double>(a) - static_cast<double>(top)) * per_t, d = -static_cast<double>(step) * per_t;
+    const double w = exp2(e), ratio = exp2(d);
+    return make_double2(a == top ? 1.0 : e >= -200.0 ? w : 0.0, ratio);
+}
+
 // Are exponents of the form a s - max s good enough in fp32?  Not where the second term is infinite or its rounding more than a half
 // (nor, then, with a temperature of 0 or infinity).
 __device__ __forceinline__ bool fp32_does(float top, float s) { return fabsf(top * s) < 4e6f && s > 1e-30f && s < 1e30f; }
@@ -159,7 +166,7 @@ sampling_probs_kernel(const ProbsParams p) {
     __shared__ double s_d[kWarps];
     __shared__ float s_f[kWarps];
     __shared__ int s_i[kWarps], s_cut;
-    __shared__ int s_count[kClasses], s_listed;
+    __shared__ int s_count[kClasses], s_listed, s_owners;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, row = static_cast<int>(blockIdx.x) / C;
@@ -270,7 +277,7 @@ sampling_probs_kernel(const ProbsParams p) {
         meet.value[0] = meet.value[1] = -INFINITY;
         meet.ties[0] = meet.ties[1] = 0x7fffffff;
         s_cut = 0x7fffffff;
-        s_listed = 0;
+        s_listed = s_owners = 0;
     }
     bool met = false;   // the first wait for the cluster is done
     auto meet_first = [&]() {
@@ -281,6 +288,7 @@ sampling_probs_kernel(const ProbsParams p) {
         if (filter && want_k && K <= kThreads) {
             // ---- a bound that top_k entries reach ----
             float top = largest();
+            const float own_top = top;
             const int r = (K + kWarps * C - 1) / (kWarps * C);
             float sorted = top;   // of the lanes, the largest first
 #pragma unroll
@@ -317,15 +325,50 @@ sampling_probs_kernel(const ProbsParams p) {
             // ---- the entries that reach it, by value and place in one word, the larger value and the earlier place the smaller word ----
             uint64_t* list = reinterpret_cast<uint64_t*>(hist) + kList;   // this share's; all of them sorted ahead of it
             uint64_t* all = reinterpret_cast<uint64_t*>(hist);
-            if (from > -INFINITY)
-                each_from(from, [&](const auto& y, auto count, int at) {
+            auto take = [&](const auto& y, auto count, int at) {
 #pragma unroll
-                    for (int e = 0; e < count(); ++e)
-                        if (y[e] >= from) {
-                            const int i = atomicAdd(&s_listed, 1);
-                            if (i < kList) list[i] = static_cast<uint64_t>(0xffffu - key_of(y[e])) << 32 | static_cast<uint32_t>(begin + at + e);
+                for (int e = 0; e < count(); ++e)
+                    if (y[e] >= from) {
+                        const int i = atomicAdd(&s_listed, 1);
+                        if (i < kList) list[i] = static_cast<uint64_t>(0xffffu - key_of(y[e])) << 32 | static_cast<uint32_t>(begin + at + e);
+                    }
+            };
+            // They lie with the threads whose maximum reaches it: where these are few, all go over those threads' entries together (a
+            // round over everything took 8.6 us of a CTA's 31).
+            int* owner = hist;   // (ahead of the list)
+            if (ALIGNED && own_top >= from && from > -INFINITY) owner[atomicAdd(&s_owners, 1)] = tid;
+            __syncthreads();
+            if (from > -INFINITY) {
+                if (ALIGNED && s_owners * 2 <= kThreads) {
+                    constexpr int kRound = 4;
+                    const int vectors = n >> 3, each_has = (vectors + kThreads - 1) / kThreads, items = s_owners * each_has;
+                    for (int i0 = tid; i0 < items; i0 += kRound * kThreads) {
+                        uint4 a[kRound];
+                        int v[kRound];
+#pragma unroll
+                        for (int j = 0; j < kRound; ++j) {
+                            const int i = i0 + j * kThreads, o = i / each_has;
+                            v[j] = i < items ? owner[o] + (i - o * each_has) * kThreads : vectors;
+                            if (v[j] < vectors) a[j] = __ldg(reinterpret_cast<const uint4*>(x) + v[j]);
                         }
-                }, [](int) {});
+#pragma unroll
+                        for (int j = 0; j < kRound; ++j) {
+                            if (v[j] >= vectors || largest_of(a[j]) < from) continue;
+                            const uint32_t w[4] = {a[j].x, a[j].y, a[j].z, a[j].w};
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = clean((e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]));
+                            take(y, std::integral_constant<int, 8>{}, v[j] * 8);
+                        }
+                    }
+                    if (const int i = vectors * 8 + tid; i < n) {
+                        const float y[1] = {clean(__bfloat162float(x[i]))};
+                        take(y, std::integral_constant<int, 1>{}, i);
+                    }
+                } else {
+                    each_from(from, take, [](int) {});
+                }
+            }
             __syncthreads();
             if (tid == 0) tell(&meet.listed[rank], C, from > -INFINITY ? s_listed : kList + 1);
             meet_all();
@@ -572,24 +615,42 @@ sampling_probs_kernel(const ProbsParams p) {
         const int bin_top = kBins - 1 - (rank * kThreads + tid) * bins;
         int my_count = 0;
         double my_sum = 0.0;
-        auto count_of = [&](int bin) {
-            if (C == 1) return hist[bin];
-            int c[kMaxCluster], sum = 0;
+        // Four patterns at a time, the CTAs' counts in one load each: their counts and weights in descending order.  (Four lie in one
+        // binade: their values are a step apart and their weights a factor.  A load and an exponential for each took 21 us of a CTA's 67.)
+        auto four = [&](int top, int (&c)[4]) {
+            int4 v = make_int4(0, 0, 0, 0);
+            if (C == 1) {
+                v = *reinterpret_cast<const int4*>(&hist[top - 3]);
+            } else {
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {
-                c[r] = 0;
-                if (r < C) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[r]) : "r"(remote(&hist[bin], r)));
+                for (int r = 0; r < kMaxCluster; ++r) {
+                    int4 u = make_int4(0, 0, 0, 0);
+                    if (r < C)
+                        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(remote(&hist[top - 3], r)));
+                    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                }
             }
+            c[0] = v.w, c[1] = v.z, c[2] = v.y, c[3] = v.x;
+            return (v.x | v.y | v.z | v.w) != 0;
+        };
+        auto weights = [&](int top, double (&w)[4]) {
+            int k = 0;   // (those above the maximum do not occur)
+            while (k < 3 && value_of_bin(top - k) > xmax) ++k;
+            const double2 f = weight_and_ratio(value_of_bin(top - k), xmax, per_t, value_of_bin(top) - value_of_bin(top - 1));
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) sum += c[r];
-            return sum;
+            for (int i = 0; i < 4; ++i) w[i] = i < k ? 0.0 : i == k ? f.x : w[i - 1] * f.y;
         };
 #pragma unroll 1
-        for (int i = 0; i < bins; ++i) {
-            const int c = count_of(bin_top - i);
-            if (c == 0) continue;
-            my_count += c;
-            my_sum += c * weight64(value_of_bin(bin_top - i), xmax, per_t);
+        for (int i = 0; i < bins; i += 4) {
+            int c[4];
+            if (!four(bin_top - i, c)) continue;
+            double w[4];
+            weights(bin_top - i, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                my_count += c[k];
+                my_sum += c[k] * w[k];
+            }
         }
         // Counts and sums of the threads before this one.  `lower` of a thread is `upper` of the one before it to the last bit, so
         // that exactly one thread's run holds a border.
@@ -657,20 +718,24 @@ sampling_probs_kernel(const ProbsParams p) {
             if (above < K && K <= above + my_count) {
                 int c_run = above;
                 double s_run = lower;
+                bool found = false;
 #pragma unroll 1
-                for (int i = 0; i < bins; ++i) {
-                    const int c = count_of(bin_top - i);
-                    if (c == 0) continue;
-                    const float a = value_of_bin(bin_top - i);
-                    const double w = weight64(a, xmax, per_t);
-                    if (K <= c_run + c) {
-                        tell(&meet.value[0], C, a);
-                        tell(&meet.ties[0], C, K - c_run);
-                        tell(&meet.kept[0], C, s_run + (K - c_run) * w);
-                        break;
+                for (int i = 0; i < bins && !found; i += 4) {
+                    int c[4];
+                    if (!four(bin_top - i, c)) continue;
+                    double w[4];
+                    weights(bin_top - i, w);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (!found && K <= c_run + c[k]) {
+                            tell(&meet.value[0], C, value_of_bin(bin_top - i - k));
+                            tell(&meet.ties[0], C, K - c_run);
+                            tell(&meet.kept[0], C, s_run + (K - c_run) * w[k]);
+                            found = true;
+                        }
+                        c_run += c[k];
+                        s_run += c[k] * w[k];
                     }
-                    c_run += c;
-                    s_run += c * w;
                 }
             }
             meet_all();
@@ -686,25 +751,30 @@ sampling_probs_kernel(const ProbsParams p) {
             if (my_count > 0 && value_of_bin(bin_top) >= last && (lower <= budget || above == 0) && upper > budget) {
                 int c_run = above;
                 double s_run = lower;
+                bool found = false;
 #pragma unroll 1
-                for (int i = 0; i < bins; ++i) {
-                    const float a = value_of_bin(bin_top - i);
-                    int c = count_of(bin_top - i);
-                    if (a < last) break;
-                    if (c == 0) continue;
-                    if (a == last) c = min(c, ties);
-                    const double w = weight64(a, xmax, per_t);
-                    if (s_run + c * w > budget) {
-                        const double fit = fmin(fmax(floor((budget - s_run) / w), 0.0), static_cast<double>(c));
-                        int j = static_cast<int>(fit);
-                        if (c_run == 0 && j == 0) j = 1;
-                        tell(&meet.value[1], C, a);
-                        tell(&meet.ties[1], C, j);
-                        tell(&meet.kept[1], C, s_run + j * w);
-                        break;
+                for (int i = 0; i < bins && !found; i += 4) {
+                    int c[4];
+                    if (!four(bin_top - i, c)) continue;
+                    double w[4];
+                    weights(bin_top - i, w);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float a = value_of_bin(bin_top - i - k);
+                        if (found || a < last || c[k] == 0) continue;
+                        if (a == last) c[k] = min(c[k], ties);
+                        if (s_run + c[k] * w[k] > budget) {
+                            const double fit = fmin(fmax(floor((budget - s_run) / w[k]), 0.0), static_cast<double>(c[k]));
+                            int j = static_cast<int>(fit);
+                            if (c_run == 0 && j == 0) j = 1;
+                            tell(&meet.value[1], C, a);
+                            tell(&meet.ties[1], C, j);
+                            tell(&meet.kept[1], C, s_run + j * w[k]);
+                            found = true;
+                        }
+                        c_run += c[k];
+                        s_run += c[k] * w[k];
                     }
-                    c_run += c;
-                    s_run += c * w;
                 }
             }
             meet_all();
@@ -825,7 +895,7 @@ sampling_probs_kernel(const ProbsParams p) {
         int before = 0;
         for (int r = 0; r < rank; ++r) before += meet.equal[r];
         const int room = max(ties - before, 0);
-        if (room < meet.equal[rank]) {
+        if (room > 0 && room < meet.equal[rank]) {
             // Some of this share's do not fit: the first that does not.  By blocks of as many entries as there are bits where the counters
             // were.
             constexpr int kBlock = kBins * 32;
@@ -835,12 +905,12 @@ sampling_probs_kernel(const ProbsParams p) {
                 __syncthreads();
                 for (int i = tid; i < words; i += kThreads) hist[i] = 0;
                 __syncthreads();
-                each([&](const auto& y, auto c, int at) {
+                each_from(last, [&](const auto& y, auto c, int at) {
 #pragma unroll
                     for (int e = 0; e < c(); ++e)
                         if (y[e] == last && at + e >= base && at + e - base < kBlock)
                             atomicOr(&hist[(at + e - base) >> 5], 1 << ((at + e - base) & 31));
-                });
+                }, [](int) {});
                 __syncthreads();
                 int mine = 0;
                 for (int i = tid * mine_words; i < min((tid + 1) * mine_words, words); ++i) mine += __popc(hist[i]);
@@ -868,7 +938,7 @@ sampling_probs_kernel(const ProbsParams p) {
             }
             __syncthreads();
         }
-        const int cut = s_cut;
+        const int cut = room > 0 ? s_cut : 0;
         finish(kept, last, [&](float a, int place) { return a > last || (a == last && place < cut); });
     }
 }
