@@ -961,9 +961,13 @@ int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, in
     B200_CHECK_ARG(out && logits && temperatures, "sampling_probs: NULL tensor");
     const bool filters = top_k != nullptr || top_p != nullptr;
     const bool aligned = (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && ld % 8 == 0 && vocab % 4 == 0;
-    // CTAs per row: one, and more while the SMs have room for them and shares are large.
+    // CTAs per row: one, and more while that makes no more than four rounds of them on the device, so that the SMs stay full to the end
+    // (320 rows of 151936, filters mixed: up to one round 164 us, two 130, four 109, nine 133; 512 rows without filters 98, 92, 85, 96),
+    // and while shares are large enough to pay for the CTAs' meetings: 64 entries a thread, or 32 where no row lists its largest (8 rows
+    // of 32000: 8.3 us at 64 and 6.3 at 32 without filters, 28.7 and 24.6 with top_p, but 14.4 and 16.5 for 64 rows with top_k 40).
     int cluster = 1;
-    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= kWaves * 4 * sm_count() && vocab / cluster > kThreads * 64) cluster *= 2;
+    const int least = kThreads * (top_k != nullptr ? 64 : 32);
+    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= kWaves * 4 * sm_count() && vocab / cluster > least) cluster *= 2;
     ProbsParams p = {out, static_cast<const __nv_bfloat16*>(logits), ld, rows, vocab, div_ceil(div_ceil(vocab, cluster), 8) * 8, cluster,
                      temperatures, top_k, top_p};
     auto kernel = filters ? (aligned ? sampling_probs_kernel<true, true> : sampling_probs_kernel<true, false>)
