@@ -28,9 +28,12 @@ constexpr int kStageRows = 128;
 constexpr uint32_t kHalfBytes = kStageRows * 128;    // 64 of the 128 elements of every row
 constexpr uint32_t kStageBytes = 4 * kHalfBytes;
 constexpr uint32_t kItems = 4;                       // places for items that have been taken
-constexpr int kSmallPage = 8;                        // pages of fewer slots are copied 16 bytes at a time
-constexpr int kMergeWarps = 4;
-constexpr int kTcRows = 32;
+constexpr int kSmallPage = 8;                        // pages of fewer slots are copied slot by slot (of 4: 40.7 us, 40.9 by pages)
+constexpr int merge_warps(int w) { return w < 4 ? 4 : w; }   // of a CTA of the merge, w of them for a row
+// Rows of a group above which its prefix may be the tensor-core kernel's (shared_prefix_plan.cu has the rest of the rule).  Up to 16 the
+// rows kernel is no slower: 4 requests of 4 heads per KV head behind 300, 2000 and 32768 keys 14.9, 16.4 and 45.1 us, there 20.5, 20.5
+// and 43.1; 16 requests behind 4096 keys 37 and 22.6.
+constexpr int kTcRows = 16;
 
 constexpr int kStages = 3;   // in the ring, beside the queries of 8 * NT rows of every KV head
 // Values of keys behind limit0 that hold an infinity or NaN: weight times value for the rows that see the key, then zeros in
@@ -412,12 +415,16 @@ struct Parts {
     int count;
 };
 
-// Joins the parts of every row, a warp per (token, head); rows that no request owns stay as they were.  Bound by the trips to L2:
-// where the parts are, then their statistics and the first of their sums.
-__global__ void __launch_bounds__(kMergeWarps * 32)
+// Joins the parts of every row, W warps per (token, head); rows that no request owns stay as they were.  Bound by the trips to L2:
+// where the parts are, then their statistics and the first of their sums, then the other sums.
+template <int W>
+__global__ void __launch_bounds__(merge_warps(W) * 32)
 shared_prefix_merge_kernel(const SharedPrefixParams p) {
+    __shared__ float2 s_ml[W > 1 ? W : 1];
+    __shared__ float4 s_acc[W > 1 ? W : 1][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = static_cast<int>(blockIdx.y) * kMergeWarps + warp;
+    const int share = W > 1 ? warp : 0;   // of the parts: this one and every W-th behind it
+    const int head = W > 1 ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * merge_warps(W) + warp;
     const int tok = static_cast<int>(blockIdx.x);
     pdl_launch_dependents();
     // The plan stands before the parts do: the kernel ahead is launched behind the end of the plan's, and this one behind that
@@ -453,14 +460,15 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
     constexpr int kAhead = 8;   // sums that are requested together with the statistics
-    for (int base = 0; base < n; base += 32) {
-        const int m = min(32, n - base);
+    const int mine = (n - share + W - 1) / W;
+    for (int base = 0; base < mine; base += 32) {
+        const int m = min(32, mine - base);
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at(base + lane));
+        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at((base + lane) * W + share));
         float4 x[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-            x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + i) * W + share) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
         const float Mn = fmaxf(M, warp_max(ml.x));
         const float ref = Mn == -INFINITY ? 0.f : Mn;
         const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
@@ -475,8 +483,26 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
 #pragma unroll 4
         for (int i = kAhead; i < m; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at(base + i) * kD) + lane);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + i) * W + share) * kD) + lane);
             acc.x += y.x * wi, acc.y += y.y * wi, acc.z += y.z * wi, acc.w += y.w * wi;
+        }
+    }
+    if (W > 1) {
+        s_acc[share][lane] = acc;
+        if (lane == 0) s_ml[share] = make_float2(M, L);
+        __syncthreads();
+        if (share > 0) return;
+#pragma unroll
+        for (int i = 1; i < W; ++i) M = fmaxf(M, s_ml[i].x);
+        const float ref = M == -INFINITY ? 0.f : M;
+        L = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float w = exp2f(s_ml[i].x - ref);
+            const float4 y = s_acc[i][lane];
+            L += w * s_ml[i].y;
+            acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
         }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;   // a row that sees no key: zeros
@@ -488,7 +514,8 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
 
 int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-// Eights of rows of a row tile: as few as hold what a request brings on average, or a group whose prefix is read here.
+// Eights of rows of a row tile: as few as hold what a request brings on average, or a group whose prefix is read here.  (64 requests of
+// 8 rows and up to 1000 keys each: 38.5 us with one, 42.4 with two; of 12 rows: 59.6 and 46.3.)
 int row_eights(int64_t tokens, int64_t batch, int64_t groups, int64_t group) {
     int64_t rows = div_ceil64(tokens * group, batch);
     if (groups > 0 && tokens * group <= kTcRows * groups) rows = div_ceil64(tokens * group, groups);
@@ -534,6 +561,17 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
     auto kernel = p.small ? shared_prefix_rows_kernel<NT, true> : shared_prefix_rows_kernel<NT, false>;
     B200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     B200_CHECK_CUDA(launch_kernel(kernel, dim3(p.ctas), dim3(kThreads), smem, stream, dim3(1, 1, 1), tk, tv, tq, p));
+    return B200_OK;
+}
+
+// Warps per row: as many as are on the device at once (7 CTAs of 4 on an SM).  Few rows behind a long prefix have hundreds of parts
+// each: two requests behind 32768 keys 107 us with a warp per row, 54 with four, 39 with sixteen.
+int launch_merge(const SharedPrefixParams& p, cudaStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, warps = 28 * static_cast<int64_t>(sm_count());
+    const int w = rows * 16 <= warps ? 16 : rows * 4 <= warps ? 4 : 1;
+    auto kernel = w == 16 ? shared_prefix_merge_kernel<16> : w == 4 ? shared_prefix_merge_kernel<4> : shared_prefix_merge_kernel<1>;
+    const int heads = w > 1 ? 1 : merge_warps(w);   // of a CTA
+    B200_CHECK_CUDA(launch_kernel(kernel, dim3(p.tokens, div_ceil(p.q_heads, heads)), dim3(merge_warps(w) * 32), 0, stream, dim3(1, 1, 1), p));
     return B200_OK;
 }
 
@@ -653,9 +691,7 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     }
     err = nt == 1 ? launch_rows<1>(tk, tv, tq, p, s) : launch_rows<2>(tk, tv, tq, p, s);
     if (err != B200_OK) return err;
-    B200_CHECK_CUDA(launch_kernel(shared_prefix_merge_kernel, dim3(a->tokens, div_ceil(a->q_heads, kMergeWarps)), dim3(kMergeWarps * 32),
-                                  0, s, dim3(1, 1, 1), p));
-    return B200_OK;
+    return launch_merge(p, s);
 }
 
 }  // extern "C"

@@ -22,6 +22,9 @@ static_assert(kMaxThreads >= kSharedMaxBatch, "a thread per request");
 constexpr int kMaxUnits = 2 * kSharedMaxBatch;
 constexpr int kMinStages = 2, kMinTiles = 2;   // per item
 constexpr int kLongPiece = 6;                  // stages of an item that covers the fetching of the next
+// Groups of up to kTcAlways rows are the tensor-core kernel's only where they are that many stages per CTA: 8 requests of 4 heads per KV
+// head behind 300 keys (0.5 stages) 18.5 us without and 21.3 with it, behind 4096 (7) 28.7 and 22.6, behind 32768 106 and 46.8.
+constexpr int kTcAlways = 32, kTcWorth = 6;
 // Microseconds: a tile of two chains' rows, one of a single chain's, the rest of a chunk; a stage of a CTA among few, and of all at once.
 constexpr float kTileTwo = 1.8f, kTileOne = 0.85f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
 
@@ -32,7 +35,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
     __shared__ int s_first[kMaxUnits + 1];                                      // items before a unit, in the rows kernel
     __shared__ int s_tc[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];      // tiles and units before a group, in the other
-    __shared__ int4 s_warp[32];
+    __shared__ int4 s_warp[32], s_open[32];
     __shared__ int s_per, s_chunks;   // tiles per chunk, chunks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = static_cast<int>(blockDim.x);
     const int G = p.group, Hkv = p.kv_heads, SK = p.stage_keys, QB = kSharedTcTile / G, QT = p.row_tokens, U = p.groups + p.batch, ctas = p.ctas;
@@ -83,16 +86,19 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     // ---- sizes ----
     auto start_of = [&](int lo) { return lo & ~(p.align - 1); };
     auto stages_of = [&](int lo, int hi) { return (max(hi - start_of(lo), 0) + SK - 1) / SK; };
-    // a group's prefix: row tiles and stages of the rows kernel, or units and key tiles of the other
+    // a group's prefix: row tiles and stages of the rows kernel, or units and key tiles of the other; or both ways, where that is
+    // still open
     int g_tiles = 0, g_stages = 0, g_units = 0, g_tc = 0;
-    bool two = false;
+    bool two = false, open = false;
     if (tid < p.groups && s_prefix[tid] > 0) {
         const int n = max(s_row[s_bound[tid + 1]] - s_row[s_bound[tid]], 0);
+        open = n * G > p.tc_rows && n * G <= kTcAlways;
         if (n * G > p.tc_rows) {
             g_units = Hkv * ((n + 2 * QB - 1) / (2 * QB));
             g_tc = (s_prefix[tid] + kSharedTcTile - 1) / kSharedTcTile;
             two = n > QB;
-        } else if (n > 0) {
+        }
+        if (n > 0 && n * G <= kTcAlways) {
             g_tiles = (n + QT - 1) / QT;
             g_stages = stages_of(0, s_prefix[tid]);
         }
@@ -104,17 +110,29 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
         b_stages = stages_of(lo, len);
         b_tiles = (ntok + QT - 1) / QT;
     }
-    // sums over all: stages, key tiles, units, longest prefix
-    int4 sum = make_int4(g_tiles * g_stages + b_tiles * b_stages, g_units * g_tc, g_units, g_tc);
-    sum.x = __reduce_add_sync(0xffffffffu, sum.x);
-    sum.y = __reduce_add_sync(0xffffffffu, sum.y);
-    sum.z = __reduce_add_sync(0xffffffffu, sum.z);
-    sum.w = __reduce_max_sync(0xffffffffu, sum.w);
-    if (lane == 0) s_warp[warp] = sum;
+    // sums over all: stages, key tiles, units, longest prefix; what is open apart
+    int4 sum = make_int4((open ? 0 : g_tiles * g_stages) + b_tiles * b_stages, open ? 0 : g_units * g_tc, open ? 0 : g_units, open ? 0 : g_tc);
+    int4 also = open ? make_int4(g_tiles * g_stages, g_units * g_tc, g_units, g_tc) : make_int4(0, 0, 0, 0);
+    auto add_up = [](int4 v) {
+        return make_int4(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y), __reduce_add_sync(0xffffffffu, v.z),
+                         __reduce_max_sync(0xffffffffu, v.w));
+    };
+    sum = add_up(sum);
+    also = add_up(also);
+    if (lane == 0) {
+        s_warp[warp] = sum;
+        s_open[warp] = also;
+    }
     const bool any_two = __syncthreads_or(two);
-    sum = lane < threads >> 5 ? s_warp[lane] : make_int4(0, 0, 0, 0);
-    const int stages = __reduce_add_sync(0xffffffffu, sum.x), tc_tiles = __reduce_add_sync(0xffffffffu, sum.y);
-    const int units = __reduce_add_sync(0xffffffffu, sum.z), longest = __reduce_max_sync(0xffffffffu, sum.w);
+    sum = add_up(lane < threads >> 5 ? s_warp[lane] : make_int4(0, 0, 0, 0));
+    also = add_up(lane < threads >> 5 ? s_open[lane] : make_int4(0, 0, 0, 0));
+    const bool by_tc = also.x > kTcWorth * ctas;
+    if (open) {
+        if (by_tc) g_tiles = g_stages = 0;
+        else g_units = g_tc = 0;
+    }
+    const int stages = sum.x + (by_tc ? 0 : also.x), tc_tiles = sum.y + (by_tc ? also.y : 0);
+    const int units = sum.z + (by_tc ? also.z : 0), longest = by_tc ? max(sum.w, also.w) : sum.w;
     // Stages per item: about an item per CTA where that makes short ones (every item costs a microsecond of queries and results, and its
     // parts have to be joined: 64 requests of up to 512 keys of their own 34.8 us with 2 stages, 31.4 with 6), several where they
     // would be long, and no more of them than there is room for.
