@@ -416,17 +416,12 @@ struct Parts {
 };
 
 // Joins the parts of every row, W warps per (token, head); rows that no request owns stay as they were.  Bound by the trips to L2:
-// where the parts are, then their statistics and the first of their sums, then the other sums.
+// where the parts are, then their statistics and the first of their sums, then the other sums.  Among many rows (W = 1) those of
+// dozens of parts are joined by the grid's first CTAs, a CTA each (with all alike, two requests behind 26298 keys kept 158 others
+// waiting for 60 us).
 template <int W>
-__global__ void __launch_bounds__(merge_warps(W) * 32)
-shared_prefix_merge_kernel(const SharedPrefixParams p) {
-    __shared__ float2 s_ml[W > 1 ? W : 1];
-    __shared__ float4 s_acc[W > 1 ? W : 1][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int share = W > 1 ? warp : 0;   // of the parts: this one and every W-th behind it
-    const int head = W > 1 ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * merge_warps(W) + warp;
-    const int tok = static_cast<int>(blockIdx.x);
-    pdl_launch_dependents();
+__device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, int head, int share, bool waited, bool by_cta, float2* s_ml, float4 (*s_acc)[32]) {
+    const int lane = threadIdx.x & 31;   // share: of the parts, that one and every W-th behind it
     // The plan stands before the parts do: the kernel ahead is launched behind the end of the plan's, and this one behind that
     // launch.  (Where the parts are, found ahead of the wait: 0.9 us of divisions and a trip to L2 while the last parts are formed.)
     JoinItem j;
@@ -453,41 +448,43 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
                     (in_block - chain * half) * p.group + hh;
         pre.step = 2 * kSharedTcTile;
     }
-    pdl_wait_prior();   // (by every CTA: what follows this kernel waits for it alone)
-    if (head >= p.q_heads || !j.owned) return;
+    if (!waited) pdl_wait_prior();   // (by every CTA: what follows this kernel waits for it alone)
+    if (head >= p.q_heads || !j.owned || (j.many != 0 && !by_cta)) return;
     const int n = pre.count + own.count;
     auto at = [&](int i) { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; };
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
-    constexpr int kAhead = 8;   // sums that are requested together with the statistics
+    constexpr int kAhead = 8;   // sums that are requested at a time, the first together with the statistics
     const int mine = (n - share + W - 1) / W;
     for (int base = 0; base < mine; base += 32) {
         const int m = min(32, mine - base);
         float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at((base + lane) * W + share));
         float4 x[kAhead];
+        auto fetch = [&](int from) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            x[i] = i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + i) * W + share) * kD) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < kAhead; ++i)
+                x[i] = from + i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + from + i) * W + share) * kD) + lane)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        fetch(0);
         const float Mn = fmaxf(M, warp_max(ml.x));
         const float ref = Mn == -INFINITY ? 0.f : Mn;
         const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
         M = Mn;
         L = L * shrink + warp_sum(w * ml.y);
         acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
+        for (int from = 0; from < m; from += kAhead) {
+            if (from > 0) fetch(from);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (i < m) acc.x += x[i].x * wi, acc.y += x[i].y * wi, acc.z += x[i].z * wi, acc.w += x[i].w * wi;
-        }
-#pragma unroll 4
-        for (int i = kAhead; i < m; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + i) * W + share) * kD) + lane);
-            acc.x += y.x * wi, acc.y += y.y * wi, acc.z += y.z * wi, acc.w += y.w * wi;
+            for (int i = 0; i < kAhead; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, from + i);
+                if (from + i < m) acc.x += x[i].x * wi, acc.y += x[i].y * wi, acc.z += x[i].z * wi, acc.w += x[i].w * wi;
+            }
         }
     }
     if (W > 1) {
+        if (waited) __syncthreads();   // (the last row's have been read)
         s_acc[share][lane] = acc;
         if (lane == 0) s_ml[share] = make_float2(M, L);
         __syncthreads();
@@ -512,6 +509,29 @@ shared_prefix_merge_kernel(const SharedPrefixParams p) {
     reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(tok) * p.q_heads + head) * kD)[lane] = packed;
 }
 
+template <int W>
+__global__ void __launch_bounds__(merge_warps(W) * 32)
+shared_prefix_merge_kernel(const SharedPrefixParams p, int first_ctas) {
+    constexpr int kWarps = merge_warps(W);
+    __shared__ float2 s_ml[kWarps];
+    __shared__ float4 s_acc[kWarps][32];
+    const int warp = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    if constexpr (W > 1) {
+        join_row<W>(p, static_cast<int>(blockIdx.x) / p.q_heads, static_cast<int>(blockIdx.x) % p.q_heads, warp, false, true, s_ml, s_acc);
+    } else {
+        const int cta = static_cast<int>(blockIdx.x) - first_ctas, per_token = (p.q_heads + kWarps - 1) / kWarps;
+        if (cta >= 0) {
+            join_row<1>(p, cta / per_token, cta % per_token * kWarps + warp, 0, false, false, nullptr, nullptr);
+        } else {
+            const int rows = __ldcg(&p.plan.head->many) * p.q_heads;
+            pdl_wait_prior();
+            for (int i = blockIdx.x; i < rows; i += first_ctas)
+                join_row<kWarps>(p, __ldcg(p.plan.many + i / p.q_heads), i % p.q_heads, warp, true, true, s_ml, s_acc);
+        }
+    }
+}
+
 int64_t round256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
 // Eights of rows of a row tile: as few as hold what a request brings on average, or a group whose prefix is read here.  (64 requests of
@@ -525,7 +545,7 @@ int row_eights(int64_t tokens, int64_t batch, int64_t groups, int64_t group) {
 
 // Where the pieces of the workspace begin, in bytes; partial rows ahead of the tensor-core kernel's.
 struct SharedLayout {
-    int64_t slots, tc_slots, rows, tc_of, rows_items, tc_items, join, ml, o, bytes;
+    int64_t slots, tc_slots, rows, tc_of, rows_items, tc_items, join, many, ml, o, bytes;
 };
 SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_heads, int kv_heads, int nt) {
     const int64_t group = q_heads / kv_heads, rows = tokens * group, kg = kConsumerWarps / kv_heads, ctas = sm_count();
@@ -541,7 +561,8 @@ SharedLayout shared_layout(int64_t tokens, int64_t batch, int64_t groups, int q_
     x.rows_items = x.tc_of + round256(ctas * sizeof(int2));
     x.tc_items = x.rows_items + round256(x.slots * sizeof(RowsItem));
     x.join = x.tc_items + round256(x.tc_slots * sizeof(TcItem));
-    x.ml = x.join + round256(tokens * sizeof(JoinItem));
+    x.many = x.join + round256(tokens * sizeof(JoinItem));
+    x.ml = x.many + round256(tokens * sizeof(int));
     x.o = x.ml + round256(part_rows * 8);
     x.bytes = x.o + part_rows * kD * 4;
     return x;
@@ -564,14 +585,16 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
     return B200_OK;
 }
 
-// Warps per row: as many as are on the device at once (7 CTAs of 4 on an SM).  Few rows behind a long prefix have hundreds of parts
-// each: two requests behind 32768 keys 107 us with a warp per row, 54 with four, 39 with sixteen.
+// Warps per row: many where few rows behind a long prefix have hundreds of parts each (two requests behind 32768 keys: 107 us with a
+// warp per row, 54 with four, 39 with sixteen), as far as they are on the device at once (28 on an SM); four only up to half of that
+// (64 requests of 16 heads behind 2051 keys: 28.8 us with a warp, 30.8 with four).
 int launch_merge(const SharedPrefixParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, warps = 28 * static_cast<int64_t>(sm_count());
-    const int w = rows * 16 <= warps ? 16 : rows * 4 <= warps ? 4 : 1;
+    const int w = rows * 16 <= warps ? 16 : rows * 8 <= warps ? 4 : 1;
     auto kernel = w == 16 ? shared_prefix_merge_kernel<16> : w == 4 ? shared_prefix_merge_kernel<4> : shared_prefix_merge_kernel<1>;
-    const int heads = w > 1 ? 1 : merge_warps(w);   // of a CTA
-    B200_CHECK_CUDA(launch_kernel(kernel, dim3(p.tokens, div_ceil(p.q_heads, heads)), dim3(merge_warps(w) * 32), 0, stream, dim3(1, 1, 1), p));
+    const int first = w > 1 ? 0 : 2 * sm_count(), per_token = w > 1 ? p.q_heads : div_ceil(p.q_heads, merge_warps(w));
+    B200_CHECK_CUDA(launch_kernel(kernel, dim3(first + static_cast<unsigned>(p.tokens) * per_token), dim3(merge_warps(w) * 32), 0, stream,
+                                  dim3(1, 1, 1), p, first));
     return B200_OK;
 }
 
@@ -663,6 +686,8 @@ int b200_attention_shared_prefix(const b200_shared_prefix_args* a, b200_stream_t
     p.plan.rows = reinterpret_cast<RowsItem*>(ws + x.rows_items);
     p.plan.tc = reinterpret_cast<TcItem*>(ws + x.tc_items);
     p.plan.join = reinterpret_cast<JoinItem*>(ws + x.join);
+    p.plan.many = reinterpret_cast<int*>(ws + x.many);
+    p.parts = kConsumerWarps / p.kv_heads;
     p.ws_ml = reinterpret_cast<float*>(ws + x.ml);
     p.ws_o = reinterpret_cast<float*>(ws + x.o);
     p.tc_base = x.rows;

@@ -14,6 +14,8 @@ constexpr int kSharedMaxBatch = 1024;
 constexpr int kSharedPieces = 4;       // items of the rows kernel per CTA, about
 constexpr int kSharedTcTile = 128;     // keys of a tile of the tensor-core kernel, and query rows of one of its chains
 
+constexpr int kSharedMany = 32;        // parts of a row that are too many for one warp, among rows of a few
+
 // Units are the groups' prefixes (0 .. groups) and the requests' own keys (groups .. groups + batch).
 
 // What a CTA of the rows kernel does in one go: stages [s_begin, s_end) of a unit's keys for a tile of its rows.
@@ -48,7 +50,8 @@ struct __align__(16) JoinItem {
     int pre_first, pre_pieces;                        // the group's prefix in the rows kernel, or ...
     int tc_unit, tc_blocks, tc_first, tc_tiles, tc_cta;   // ... in the tensor-core kernel: units before, blocks per KV head, tiles before,
                                                           // tiles per unit, first CTA
-    int pad[4];
+    int many;                                         // 1: more than kSharedMany parts in all
+    int pad[3];
 };
 
 struct __align__(16) PlanHead {
@@ -58,7 +61,7 @@ struct __align__(16) PlanHead {
     int next;                     // rows kernel: the first item that nobody has taken yet
     int rows_lead;                // ... and how many a CTA takes ahead of the one it copies
     int rows_first;               // ... and the CTAs that begin with the item of their own number
-    int pad;
+    int many;                     // tokens whose rows have more than kSharedMany parts
 };
 
 struct SharedPlan {
@@ -67,6 +70,7 @@ struct SharedPlan {
     RowsItem* rows;      // [max_slots]
     TcItem* tc;          // [tc_slots], item = slot of its partial results
     JoinItem* join;      // [tokens]
+    int* many;           // [tokens] those of many parts
 };
 
 struct SharedPrefixParams {
@@ -90,6 +94,7 @@ struct SharedPrefixParams {
     int tc_rows;                    // groups of more query rows (tokens x group) than this: their prefixes by the tensor-core kernel
     int with_tc;                    // is that kernel launched at all?
     int ctas;                       // of either kernel
+    int parts;                      // of a stage in the rows kernel: warps that share the keys of a KV head
     SharedPlan plan;
     int* status;
 };

@@ -25,8 +25,9 @@ constexpr int kLongPiece = 6;                  // stages of an item that covers 
 // Groups of up to kTcAlways rows are the tensor-core kernel's only where they are that many stages per CTA: 8 requests of 4 heads per KV
 // head behind 300 keys (0.5 stages) 18.5 us without and 21.3 with it, behind 4096 (7) 28.7 and 22.6, behind 32768 106 and 46.8.
 constexpr int kTcAlways = 32, kTcWorth = 6;
-// Microseconds: a tile of two chains' rows, one of a single chain's, the rest of a chunk; a stage of a CTA among few, and of all at once.
-constexpr float kTileTwo = 1.8f, kTileOne = 0.85f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
+// Microseconds: a tile of two chains' rows, one of a single chain's, one of small pages (128 copies), the rest of a chunk; a stage of a CTA among few, and of all at once.
+// (kTileSmall as large as kTileOne: 105 requests in pages of four tokens 150 us, so 105.)
+constexpr float kTileTwo = 1.8f, kTileOne = 0.85f, kTileSmall = 3.1f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
 
 __global__ void __launch_bounds__(kMaxThreads)
 shared_prefix_plan_kernel(const SharedPrefixParams p) {
@@ -184,7 +185,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
                 const int k = s_unit[g + 1] - s_unit[g];
                 if (k > 0) count += k * (((s_tc[g + 1] - s_tc[g]) / k + per - 1) / per);
             }
-            const float time = per * (any_two ? kTileTwo : kTileOne) + kChunk;
+            const float time = per * (p.small ? kTileSmall : any_two ? kTileTwo : kTileOne) + kChunk;
             const float left = fmaxf(stages - (ctas - count) * (time * (1.f / kStageAlone)), 0.f);
             float cost = count <= ctas ? time + left * (kStageAll / ctas) : 3e38f;
             int best = lane;
@@ -337,6 +338,8 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
                     j.pre_pieces = (s_first[g + 1] - s_first[g]) / ((s_row[s_bound[g + 1]] - first + QT - 1) / QT);
                 }
             }
+            j.many = (j.own_pieces + j.pre_pieces) * p.parts + (j.tc_blocks > 0 ? (j.tc_tiles + per - 1) / per : 0) > kSharedMany;
+            if (j.many != 0) p.plan.many[atomicAdd(&p.plan.head->many, 1)] = tok;
         }
         p.plan.join[tok] = j;
     }
