@@ -293,8 +293,8 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
  * seq_lens[b] keys, as for b200_attention_prefill (a decode step: one each; drafted tokens: a few each).  Rows of no
  * request are left as they were; a row that sees no key becomes zeros.  out [tokens, q_heads * head_dim] contiguous.
  * Everything per request and group is read on the device: a captured call follows what the arrays hold at its replay,
- * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words.  A
- * qo_indptr or group_indptr that decreases or leaves [0, tokens] or [0, batch] is reported as tokens + 1, and nothing is
+ * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words
+ * (-1 as -2^31).  A qo_indptr or group_indptr that decreases or leaves [0, tokens] or [0, batch] is reported as tokens + 1, and nothing is
  * written.
  * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head; q 16-byte aligned, its strides multiples of
  * 8 elements.  workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
@@ -370,7 +370,7 @@ B200_API int b200_sampling_probs(float* out, const void* logits, int64_t ld, int
  * drawn with draw_uniform[b] by inverse CDF in index order: from max(target - draft, 0) at the first draft that was not
  * accepted (from target where that is zero throughout), from the last row where all were.  Negative numbers and NaN among
  * the probabilities count as 0; a row without a positive number gives token 0.  A drafted token outside [0, vocab) is not
- * accepted and reported in the status words.
+ * accepted and reported in the status words (-1 as -2^31).
  * tokens int32 [batch, max_drafts + 1]: the accepted drafts, the token behind them, then -1; accepted int32 [batch].  Of
  * more than max_drafts drafts the first max_drafts are looked at.  All probabilities fp32, rows target_ld and draft_ld
  * apart; uniform numbers fp32 in [0, 1).  total_drafts = draft_indptr[batch].  Decisions and sums in 64 bits, in a fixed

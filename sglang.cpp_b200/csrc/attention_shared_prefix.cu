@@ -121,7 +121,8 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     }
     __syncthreads();
     // Behind the tensor-core kernel nothing here waits for what that writes, and the plan is complete: it has waited for it.  The wait
-    // is made up for at the end, since the kernel that joins the parts waits for this one alone.
+    // is made up for at the end, since the kernel that joins the parts waits for this one alone.  (What other kernels wrote is read
+    // from L2 here: the plan, the page table, and by copies queries, keys and values.)
     if (!p.with_tc) pdl_wait_prior();
     pdl_launch_dependents();
     // Item number `turn` of this CTA, for the whole warp; a slot of -1 ends it.
@@ -137,13 +138,18 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
     };
     // By one lane of the first producer warp: items are handed on one or two ahead of the one whose copies are made (long and short
     // ones: an item's description, its pages' slots and its first copies are three trips to memory, which short ones do not cover).
-    const int count = p.plan.head->rows_items;
-    const uint32_t lead = static_cast<uint32_t>(p.plan.head->rows_lead);
+    const int count = __ldcg(&p.plan.head->rows_items);
+    const uint32_t lead = static_cast<uint32_t>(__ldcg(&p.plan.head->rows_lead));
     auto hand_on = [&](uint32_t turn, int taken) {
         const uint32_t at = turn % kItems;
         RowsItem it;
         it.slot = -1;
-        if (taken < count) it = p.plan.rows[taken];
+        if (taken < count) {
+            static_assert(sizeof(RowsItem) % 16 == 0, "read in 16-byte loads");
+#pragma unroll
+            for (unsigned i = 0; i < sizeof(RowsItem) / 16; ++i)
+                reinterpret_cast<int4*>(&it)[i] = __ldcg(reinterpret_cast<const int4*>(p.plan.rows + taken) + i);
+        }
         if (!mbar_wait_bounded(smem_u32(&item_empty[at]), (turn / kItems & 1u) ^ 1u, p.status, 224)) return;
         s_item[at] = it;
         mbar_arrive(smem_u32(&item_full[at]));
@@ -159,7 +165,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
         const void* map = which < 2 ? &tmap_k : &tmap_v;
         const bool leads = which == 0 && lane == 0;
         if (leads) {
-            const bool first = static_cast<int>(blockIdx.x) < p.plan.head->rows_first;
+            const bool first = static_cast<int>(blockIdx.x) < __ldcg(&p.plan.head->rows_first);
             if (first) hand_on(0, static_cast<int>(blockIdx.x));
             for (uint32_t i = first ? 1 : 0; i < lead; ++i) hand_on(i, atomicAdd(&p.plan.head->next, 1));
         }
@@ -177,7 +183,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int copy = c * 32 + lane;
-                next[c] = copy < n ? row[copy * span] : 0;
+                next[c] = copy < n ? __ldcg(row + copy * span) : 0;
             }
         };
         RowsItem it = get_item(0);
@@ -203,7 +209,7 @@ shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __gr
                 for (int c = 0; c < 4; ++c) {
                     sl[c] = next[c];
                     if (sl[c] < 0 || static_cast<int64_t>(sl[c]) + span > p.num_slots) {
-                        atomicExch(&p.status[kStatusBadIndex], sl[c] + 1);
+                        atomicExch(&p.status[kStatusBadIndex], bad_index_word(sl[c]));
                         sl[c] = 0;
                     }
                 }

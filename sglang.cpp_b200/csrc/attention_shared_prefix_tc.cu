@@ -193,7 +193,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 for (int i = 0; i < 4; ++i) {
                     sl[i] = next[i];
                     if (sl[i] < 0 || static_cast<int64_t>(sl[i]) + span > p.num_slots) {
-                        atomicExch(&p.status[kStatusBadIndex], sl[i] + 1);
+                        atomicExch(&p.status[kStatusBadIndex], bad_index_word(sl[i]));
                         sl[i] = 0;
                     }
                     if ((sl[i] & 7) != 0) pages = false;

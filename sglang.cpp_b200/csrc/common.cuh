@@ -100,6 +100,9 @@ enum StatusWord : int {
     kStatusBadIndex = 1,  // an index check failed (value: the offending index + 1)
 };
 
+// That value, where -1 is to be reported too (0 says that all is well): as the lowest number.
+__device__ __forceinline__ int bad_index_word(int index) { return index == -1 || index == 0x7fffffff ? static_cast<int>(0x80000000u) : index + 1; }
+
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 

@@ -61,7 +61,7 @@ verify_drafts_kernel(const VerifyParams p) {
             if (j < n) {
                 const int x = p.draft_tokens[start + j];
                 const bool known = x >= 0 && x < p.vocab;
-                if (!known && rank == 0) atomicExch(&p.status[kStatusBadIndex], x + 1);
+                if (!known && rank == 0) atomicExch(&p.status[kStatusBadIndex], bad_index_word(x));
                 const double px = known ? entry(target[j * p.target_ld + x]) : 0.0;
                 const double qx = p.draft == nullptr ? 1.0 : known ? entry(p.draft[(start + j) * p.draft_ld + x]) : 0.0;
                 refused = !(unit_interval(p.accept[start + j]) * qx < px);
@@ -163,17 +163,17 @@ verify_drafts_kernel(const VerifyParams p) {
         return all;
     };
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    double total = 0.0, before = 0.0, mine = 0.0;   // of the row, of the runs before this warp's, of this run
+    double total = 0.0, before = 0.0, upto_end = 0.0;   // of the row, of the runs before this warp's, with this one
     for (int pass = 0; pass < 2; ++pass) {
         const double sum = sum_run();
         if (lane == 0) s_sum[warp] = sum;
         __syncthreads();
-        double cta = 0.0, ahead = 0.0;
+        double cta = 0.0, ahead = 0.0, with = 0.0;
         for (int w = 0; w < warps; ++w) {
             if (w == warp) ahead = cta;
             cta += s_sum[w];
+            if (w == warp) with = cta;
         }
-        mine = sum;
         if (C > 1) {
             if (threadIdx.x < static_cast<unsigned>(C)) {
                 uint32_t at;
@@ -188,7 +188,8 @@ verify_drafts_kernel(const VerifyParams p) {
         }
         total = 0.0;
         for (int r = 0; r < C; ++r) {
-            if (r == rank) before = total + ahead;
+            // (One run's end is the next one's beginning to the last bit, so that exactly one of them holds the goal.)
+            if (r == rank) before = total + ahead, upto_end = total + with;
             total += s_cta[r];
         }
         if (total > 0.0 || !rest) break;   // (the same in every CTA of the cluster)
@@ -206,7 +207,7 @@ verify_drafts_kernel(const VerifyParams p) {
         return;
     }
     const double goal = unit_interval(p.draw[b]) * total;
-    if (!(mine > 0.0) || goal < before || goal >= before + mine) return;
+    if (goal < before || goal >= upto_end) return;
     // The part of the run, by the sums that the lanes kept; then that part once more, neighbouring entries in a lane.  (The sums
     // are formed in another order than before: the last bits may put the goal behind the part's last entry.)
     auto scan = [&](double w) {   // sums up to and with each lane's

@@ -400,7 +400,7 @@ class SharedPrefixAttention:
         args.page_table, args.page_table_stride = page_table.data_ptr(), _row_stride(page_table)
         args.table_idx, args.seq_lens, args.qo_indptr = table_idx.data_ptr(), seq_lens.data_ptr(), qo_indptr.data_ptr()
         args.group_indptr, args.prefix_lens = group_indptr.data_ptr(), prefix_lens.data_ptr()
-        args.tokens, args.batch, args.groups = tokens, batch, groups
+        args.tokens, args.batch, args.groups, args.sm_scale = tokens, batch, groups, self.sm_scale
         _launch(dev, "b200_attention_shared_prefix", self.args_ref_)
         return out
 

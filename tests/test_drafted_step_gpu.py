@@ -190,6 +190,11 @@ def test_shared_prefix_reports_slots_outside_the_pool(L):
     s.table[s.table_idx[1], 112:128] = -3
     s.run(L)
     assert L.read_device_status() == (0, -2)
+    for own in (20, 700):   # the prefix by either kernel
+        s = SharedSetup([[(own, 1)] * 20], [100], 16, 16, 8, seed=12)
+        s.table[s.table_idx[3], 112:128] = -1
+        s.run(L)
+        assert L.read_device_status() == (0, -2 ** 31)
 
 
 @pytest.mark.parametrize("name,at,value", [("qo", 1, 64), ("qo", 64, 65), ("qo", 0, -1), ("qo", 30, 28), ("groups", 1, 65),
@@ -382,6 +387,18 @@ def test_verify_drafts_draws_at_the_ends(L):
     assert got[0][0, 0] == 7 and got[0][1, 0] == vocab - 10
 
 
+@pytest.mark.parametrize("vocab", [4096, 131072])
+def test_verify_drafts_draws_between_runs_of_the_row(L, vocab):
+    """1, 2^-53, 2^-53, 1 at places all over the row and u = 1/2: the goal is 1 + 2^-53, or 1 where the sum of all is rounded to 2.
+    However the sums are grouped, one of the four places is drawn."""
+    for step in (1, 33, 128, 512, 520, 1024, vocab // 8):
+        at = [5, vocab // 8, vocab // 8 + step, vocab // 8 + 2 * step]
+        p = torch.zeros(1, vocab)
+        p[0, at] = torch.tensor([1.0, 2.0 ** -53, 2.0 ** -53, 1.0])
+        tokens, accepted = L.verify_drafts(p.cuda(), _i32([]), _i32([0, 0]), _f32([]), _f32([0.5]), 0)
+        assert int(accepted[0]) == 0 and int(tokens[0, 0]) in at, (step, tokens)
+
+
 def test_verify_drafts_odd_values(L):
     vocab = 600
     s = _drafted([2, 3, 1], vocab, 7)
@@ -398,6 +415,9 @@ def test_verify_drafts_tokens_outside_the_vocabulary(L):
         s["accept"][:] = 0.0
         _same(_verify(L, s), verify_oracle(**s))
         assert L.read_device_status()[1] in (401, -6)
+        s["tokens"][1], s["tokens"][3] = -1, 2
+        _same(_verify(L, s), verify_oracle(**s))
+        assert L.read_device_status()[1] == -2 ** 31
 
 
 def test_verify_drafts_strides_and_fewer_than_brought(L):
