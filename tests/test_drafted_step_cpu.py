@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 P = ctypes.c_void_p(256)   # never dereferenced: the calls below are refused
 
@@ -100,3 +101,13 @@ def test_oracles_on_known_answers():
     assert run(0, 0.99, 0.5) == [[[0, 2]], [1]]          # p > q: always accepted
     assert run(1, 0.49, 0.15) == [[[1, 1]], [1]]
     assert run(1, 0.51, 0.7) == [[[0, -1]], [0]]         # refused: the rest is all on token 0
+
+
+def test_python_calls_take_no_cpu_tensors(pkg):
+    """There is no path without the device."""
+    from sglang_cpp_b200 import layers as L
+    f, i = torch.ones(2), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: L.sampling_probs(torch.zeros(2, 8, dtype=torch.bfloat16), f),
+                 lambda: L.verify_drafts(torch.ones(2, 8), i[:0], i, f[:0], f, 0)):
+        with pytest.raises(L.B200Error, match="CUDA"):
+            call()

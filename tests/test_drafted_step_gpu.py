@@ -219,6 +219,70 @@ def test_shared_prefix_in_a_pool_beyond_32_bits(L):
     assert_attention(s.run(L), *s.want())
 
 
+def test_shared_prefix_most_requests(L):
+    """As many requests as there may be: groups of two and of hundreds, some of nobody's rows, in pages of any order."""
+    members = [[(1 + (7 * i) % 30, 1), (3, (i % 4) // 2)] for i in range(300)] + [[(2 + i % 9, 1) for i in range(400)]] + [[(5, 1)] for _ in range(24)]
+    s = SharedSetup(members, [(13 * i) % 90 for i in range(300)] + [700] + [40] * 24, 16, 16, 8, seed=15)
+    assert len(s.reqs) == 1024
+    got = s.run(L)
+    assert_attention(got, *s.want())
+    assert L.read_device_status() == (0, 0)
+
+
+def test_shared_prefix_on_two_streams(L):
+    """Two objects at once: calls of one change nothing for the other's."""
+    setups = [SharedSetup([[(60, 2)] * 30, [(9, 1)]], [1700, 20], 16, 16, 8, seed=16), SharedSetup([[(700, 1), (30, 3)]] * 9, [260] * 9, 16, 32, 4, seed=17)]
+    streams = [torch.cuda.Stream() for _ in setups]
+    work = [(s, L.SharedPrefixAttention(s.cache(L), s.heads, s.kv_heads, D, s.q.shape[0], len(s.reqs)), s.q.cuda(),
+             s.index(s.table, s.table_idx, s.lens, s.qo, s.group_indptr, s.prefixes)) for s in setups]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, attn, q, index) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(attn.forward(q, 0, *index))
+    torch.cuda.synchronize()
+    for s, outs in zip(setups, got):
+        assert_attention(outs[0], *s.want())
+        assert all(torch.equal(outs[0], o) for o in outs)
+
+
+def test_shared_prefix_checks_its_arguments(L):
+    s = SharedSetup([[(20, 1), (30, 2)]], [100], 16, 16, 8, seed=18)
+    attn = L.SharedPrefixAttention(s.cache(L), 16, 8, D, 3, 2)
+    q, index = s.q.cuda(), s.index(s.table, s.table_idx, s.lens, s.qo, s.group_indptr, s.prefixes)
+    good = attn.forward(q, 0, *index)
+    assert_attention(good, *s.want())
+
+    def refused(q=q, layer=0, out=None, **change):
+        names = ("page_table", "table_idx", "seq_lens", "qo_indptr", "group_indptr", "prefix_lens")
+        with pytest.raises(L.B200Error):
+            attn.forward(q, layer, *[change.get(n, t) for n, t in zip(names, index)], out=out)
+
+    refused(q=q.float())
+    refused(q=q.cpu())
+    refused(q=q[:, :8])
+    refused(q=q.transpose(0, 1))
+    refused(q=torch.zeros(3, 16, D + 4, dtype=bf16, device="cuda")[:, :, 4:])      # rows that are not 16-byte aligned
+    refused(q=torch.zeros(4, 16, D, dtype=bf16, device="cuda"))                     # more rows than the workspace is for
+    refused(layer=1)
+    refused(layer=-1)
+    refused(out=good[:2])
+    refused(out=good.float())
+    refused(page_table=index[0].long())
+    refused(page_table=index[0].t())
+    refused(table_idx=index[1][:1])
+    refused(seq_lens=index[2].cpu())
+    refused(qo_indptr=index[3][:2])
+    refused(group_indptr=index[4][:1])
+    refused(prefix_lens=index[5].expand(2).contiguous())
+    with pytest.raises(L.B200Error):
+        L.SharedPrefixAttention(s.cache(L), 16, 4, D, 3, 2)
+    with pytest.raises(L.B200Error):
+        L.SharedPrefixAttention(s.cache(L), 16, 8, D, 3, 1025)
+    assert torch.equal(attn.forward(q, 0, *index), good)
+
+
 # ---- probabilities ----------------------------------------------------------------------------------------------
 
 def _logits(rows, vocab, seed, spread=2.0, step=0.0):
