@@ -19,8 +19,9 @@
 //     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
 //                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
 //                      thread's patterns the cut falls.
-// Bound by HBM, 6 bytes per entry; the last kind also by the counting, an atomic per entry in shared memory.  CTAs of 256 threads, four
-// on an SM, so that one's loads and stores lie under another's sorting.
+// Bound by HBM, 6 bytes per entry; the last kind also by the counting, an atomic per entry in shared memory.  CTAs of 256 threads, five
+// on an SM, so that one's loads and stores lie under another's sorting (320 rows of 151936 at top_p 0.9: 160 us with four, 141 with
+// five, 155 with six, whose registers do not suffice).
 #include <type_traits>
 
 #include "common.cuh"
@@ -33,7 +34,8 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 24;
-constexpr int kWaves = 4;
+constexpr int kPerSm = 5;                   // CTAs on an SM at once ...
+constexpr int kMostPerSm = 16;              // ... and all in all, as far as clusters make them more
 constexpr int kList = 2048;                 // entries that can be listed
 constexpr int kBins = 8192;                 // counted patterns: half of them positive
 constexpr int kHalf = kBins / 2;
@@ -159,7 +161,7 @@ __device__ __forceinline__ float largest_of(const uint4& a) {
 
 // ALIGNED: rows of both sides are read and written 16 bytes at a time; else entry by entry, neighbours by neighbouring threads.
 template <bool FILTERS, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, kPerSm)
 sampling_probs_kernel(const ProbsParams p) {
     __shared__ __align__(16) int hist[FILTERS ? kBins : 4];
     __shared__ Meet meet;
@@ -961,13 +963,13 @@ int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, in
     B200_CHECK_ARG(out && logits && temperatures, "sampling_probs: NULL tensor");
     const bool filters = top_k != nullptr || top_p != nullptr;
     const bool aligned = (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 && ld % 8 == 0 && vocab % 4 == 0;
-    // CTAs per row: one, and more while that makes no more than four rounds of them on the device, so that the SMs stay full to the end
-    // (320 rows of 151936, filters mixed: up to one round 164 us, two 130, four 109, nine 133; 512 rows without filters 98, 92, 85, 96),
+    // CTAs per row: one, and more while that makes no more than 16 for an SM, three rounds of them, so that the SMs stay full to the end
+    // (320 rows of 151936, filters mixed: up to 4 for an SM 164 us, 8: 130, 16: 109, 36: 133; 512 rows without filters 98, 92, 85, 96),
     // and while shares are large enough to pay for the CTAs' meetings: 64 entries a thread, or 32 where no row lists its largest (8 rows
     // of 32000: 8.3 us at 64 and 6.3 at 32 without filters, 28.7 and 24.6 with top_p, but 14.4 and 16.5 for 64 rows with top_k 40).
     int cluster = 1;
     const int least = kThreads * (top_k != nullptr ? 64 : 32);
-    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= kWaves * 4 * sm_count() && vocab / cluster > least) cluster *= 2;
+    while (cluster < kMaxCluster && static_cast<int64_t>(rows) * cluster * 2 <= kMostPerSm * sm_count() && vocab / cluster > least) cluster *= 2;
     ProbsParams p = {out, static_cast<const __nv_bfloat16*>(logits), ld, rows, vocab, div_ceil(div_ceil(vocab, cluster), 8) * 8, cluster,
                      temperatures, top_k, top_p};
     auto kernel = filters ? (aligned ? sampling_probs_kernel<true, true> : sampling_probs_kernel<true, false>)
