@@ -296,9 +296,10 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
  * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words
  * (-1 as -2^31).  A qo_indptr or group_indptr that decreases or leaves [0, tokens] or [0, batch] is reported as tokens + 1, and nothing is
  * written.
- * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head; q 16-byte aligned, its strides multiples of
- * 8 elements.  workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
- * run one after another. */
+ * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head, up to 1024 requests; q 16-byte aligned, its
+ * strides multiples of 8 elements.  For a few rows per request: thousands of rows of one prompt are b200_attention_prefill's.
+ * workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
+ * run one after another (so does the replay of graphs that captured them). */
 typedef struct b200_shared_prefix_args {
     void* out;
     const void* q;

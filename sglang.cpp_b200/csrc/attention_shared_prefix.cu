@@ -7,11 +7,19 @@
 // the probabilities, which are rounded to bf16 as the other attention kernels here do (their products run on the tensor cores).
 //
 // Rows kernel (bound by HBM): an item is a run of stages of a group's prefix or of what a request has of its own, for a tile of up to
-// 8 * NT of its rows, (token, head of the KV head's group) pairs.  Items are cut by shared_prefix_plan.cu; a CTA takes the next one that nobody
-// has taken (which CTA does an item changes no result), two ahead of the one it works on.  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA boxes of whole pages, a warp for each
-// half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with mma.sync: S^T = K Q^T and O^T = V^T P^T, so that
-// the rows are the products' short side (eight of them; with the rows on the long side a step of one token and two heads per KV head
-// filled 2 of 16, and a stage took 1.05 us).
+// 8 * NT of its rows, (token, head of the KV head's group) pairs.  Items are cut by shared_prefix_plan.cu; a CTA takes the next one that
+// nobody has taken (which CTA does an item changes no result): short ones two ahead, since their description, slots and first copies
+// are three trips to memory, long ones with the last copies of the one before, so that late CTAs find some (taken with the first
+// copies: 48 drafted requests behind 16001 keys 80 us, so 74.5).  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA
+// boxes of whole pages, a warp for each half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with
+// mma.sync: S^T = K Q^T and O^T = V^T P^T, so that the rows are the products' short side (eight of them; with the rows on the long side a
+// step of one token and two heads per KV head filled 2 of 16).  64 KB of a stage take a CTA 0.8 to 1 us where all are at work
+// (1.05 the other way round), 1.2 to 1.4 with two eights of rows; 128 requests of 1 row with up to 2048 keys of their own behind 32768
+// shared ones: 667 MB in 138 us with the tensor-core kernel beside it, 0.74 of the copy bandwidth.
+//
+// Few launches, no wait between them that is not needed: the kernels are launched early (programmatic dependent launches), the
+// rows kernel does not wait for the tensor-core kernel, whose SMs its last CTAs take over, and the merge finds its parts ahead of
+// its wait.
 #include "common.cuh"
 #include "kernels.h"
 #include "shared_prefix.cuh"
@@ -426,20 +434,22 @@ struct Parts {
 // dozens of parts are joined by the grid's first CTAs, a CTA each (with all alike, two requests behind 26298 keys kept 158 others
 // waiting for 60 us).
 template <int W>
-__device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, int head, int share, bool waited, bool by_cta, float2* s_ml, float4 (*s_acc)[32]) {
+__device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, int head, int share, bool waited, bool by_cta,
+                                         float2* s_ml, float4 (*s_acc)[32]) {
     const int lane = threadIdx.x & 31;   // share: of the parts, that one and every W-th behind it
     // The plan stands before the parts do: the kernel ahead is launched behind the end of the plan's, and this one behind that
     // launch.  (Where the parts are, found ahead of the wait: 0.9 us of divisions and a trip to L2 while the last parts are formed.)
     JoinItem j;
     static_assert(sizeof(JoinItem) % 16 == 0, "read in 16-byte loads");
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(JoinItem) / 16; ++i) reinterpret_cast<int4*>(&j)[i] = __ldcg(reinterpret_cast<const int4*>(p.plan.join + tok) + i);
+    for (unsigned i = 0; i < sizeof(JoinItem) / 16; ++i)
+        reinterpret_cast<int4*>(&j)[i] = __ldcg(reinterpret_cast<const int4*>(p.plan.join + tok) + i);
     const int tc_per = __ldcg(&p.plan.head->tc_per), tc_chunked = __ldcg(&p.plan.head->tc_chunked);
     const int h = head / p.group, hh = head - h * p.group, KG = kConsumerWarps / p.kv_heads;
     auto parts_of = [&](int first, int pieces, int t) {   // of token t of the unit
         const int tile = t / p.row_tokens, r = (t - tile * p.row_tokens) * p.group + hh;
-        return Parts{(static_cast<int64_t>(first + tile * pieces) * KG * p.kv_heads + h) * p.tile_rows + r, static_cast<int64_t>(p.kv_heads) * p.tile_rows,
-                     pieces * KG};
+        return Parts{(static_cast<int64_t>(first + tile * pieces) * KG * p.kv_heads + h) * p.tile_rows + r,
+                     static_cast<int64_t>(p.kv_heads) * p.tile_rows, pieces * KG};
     };
     const Parts own = parts_of(j.own_first, j.own_pieces, j.own_t);
     const int t = j.pre_t;

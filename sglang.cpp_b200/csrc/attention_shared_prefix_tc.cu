@@ -17,6 +17,9 @@
 // chains' softmax.  Every role walks the same items; the rings and the chains go on across them, so the next item's tiles are under
 // way while one is finished.  Barriers are tested by parity: whoever tests one knows that the phase before it is over (the rings
 // are filled and emptied in order, and a chain's barriers alternate between its two sides).
+// A tile of two chains (16.8 MFLOP) takes 1.65 to 1.9 us, 0.8 to 0.9 of the rate of large library products, whose power limit it
+// meets as well; a tile of one chain 0.85.  In pages of fewer than eight slots a tile is 128 copies of four half rows and takes 3.1 us.
+// The softmax is bound by its instructions: an eighth of the exponentials on the FMA pipe cost 12 percent.
 #include <type_traits>
 
 #include "common.cuh"

@@ -14,8 +14,8 @@
 // A CTA, or where rows are few a cluster of them, owns a row and goes over it from memory once and from L2 once or twice more.
 //     no filter:       sums under a running maximum; results.
 //     top_k <= 256:    the lanes' maxima; of every warp's 32 the r-th largest, r = ceil(top_k / warps of the row): the smallest of these
-//                      has top_k entries at or above it.  A second round lists all such entries (some hundreds), which are sorted, weighed and
-//                      cut; the results are zeros but for what is kept.
+//                      has top_k entries at or above it.  All such entries (some hundreds) are listed, from the threads whose maximum
+//                      reaches it, sorted, weighed and cut; the results are zeros but for what is kept.
 //     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
 //                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
 //                      thread's patterns the cut falls.
@@ -434,7 +434,8 @@ sampling_probs_kernel(const ProbsParams p) {
                 kept = warp_sum(kept);
                 __syncthreads();
                 if (lane == 0) s_d[warp] = kept;
-                for (int i = tid; i < (ALIGNED ? n >> 2 : 0); i += kThreads) __stcs(reinterpret_cast<float4*>(out) + i, make_float4(0.f, 0.f, 0.f, 0.f));
+                for (int i = tid; i < (ALIGNED ? n >> 2 : 0); i += kThreads)
+                    __stcs(reinterpret_cast<float4*>(out) + i, make_float4(0.f, 0.f, 0.f, 0.f));
                 for (int i = (ALIGNED ? n & ~3 : 0) + tid; i < n; i += kThreads) __stcs(out + i, 0.f);
                 __syncthreads();   // (the zeros are ahead of what is kept)
                 kept = 0.0;
@@ -628,7 +629,9 @@ sampling_probs_kernel(const ProbsParams p) {
                 for (int r = 0; r < kMaxCluster; ++r) {
                     int4 u = make_int4(0, 0, 0, 0);
                     if (r < C)
-                        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(remote(&hist[top - 3], r)));
+                        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                                     : "r"(remote(&hist[top - 3], r)));
                     v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
                 }
             }

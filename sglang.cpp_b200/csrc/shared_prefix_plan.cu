@@ -1,10 +1,10 @@
 // Attention over a shared prefix: how the work of a call is cut into items (attention_shared_prefix.cu has the formulas).
 //
 // Lengths are known on the device alone, so that a captured call follows them.  One CTA, a thread per request and per group (no more
-// warps than that takes: 32 of them for 64 requests cost 2 us), counts
-// row tiles and stages (rows kernel) or KV heads x blocks and key tiles (tensor-core kernel), adds these up, and writes the items that
-// the kernels begin with one load.  (Every CTA counting for itself: 2.5 to 4.5 us ahead of each of the two kernels, and five dependent
-// loads per item.)
+// warps than that takes: 32 of them for 64 requests cost 2 us), counts row tiles and stages (rows kernel) or KV heads x blocks and
+// key tiles (tensor-core kernel), adds these up, and writes the items that the kernels begin with one load.  Bound by its trips to memory
+// and barriers: 3.5 us for 4 requests, 4.2 for 64, 6 for 48 of 168 rows, 9 for 158 of 474.  (Every CTA counting for itself: 2.5 to
+// 4.5 us ahead of each of the two kernels, and five dependent loads per item.)
 //
 // The tensor-core kernel is bound by products and exponentials, the rows kernel by HBM, and a CTA of either fills an SM.  Both
 // therefore run at once on different SMs: with chunks of `per` tiles the first takes so many CTAs, the rows kernel's first CTAs begin
@@ -25,7 +25,8 @@ constexpr int kLongPiece = 6;                  // stages of an item that covers 
 // Groups of up to kTcAlways rows are the tensor-core kernel's only where they are that many stages per CTA: 8 requests of 4 heads per KV
 // head behind 300 keys (0.5 stages) 18.5 us without and 21.3 with it, behind 4096 (7) 28.7 and 22.6, behind 32768 106 and 46.8.
 constexpr int kTcAlways = 32, kTcWorth = 6;
-// Microseconds: a tile of two chains' rows, one of a single chain's, one of small pages (128 copies), the rest of a chunk; a stage of a CTA among few, and of all at once.
+// Microseconds: a tile of two chains' rows, one of a single chain's, one of small pages (128 copies), the rest of a chunk; a stage of a
+// CTA among few, and of all at once.
 // (kTileSmall as large as kTileOne: 105 requests in pages of four tokens 150 us, so 105.)
 constexpr float kTileTwo = 1.8f, kTileOne = 0.85f, kTileSmall = 3.1f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
 
