@@ -37,7 +37,9 @@ constexpr uint32_t kHalfBytes = kStageRows * 128;    // 64 of the 128 elements o
 constexpr uint32_t kStageBytes = 4 * kHalfBytes;
 constexpr uint32_t kItems = 4;                       // places for items that have been taken
 constexpr int kSmallPage = 8;                        // pages of fewer slots are copied slot by slot (of 4: 40.7 us, 40.9 by pages)
-constexpr int merge_warps(int w) { return w < 4 ? 4 : w; }   // of a CTA of the merge, w of them for a row
+// Warps of a CTA of the merge, w of them for a row.  (With a warp per row as many as join a row of many parts: 158 requests, two of them
+// behind 26298 keys, 97 us with four, 86 with eight, 83 with sixteen, which cost others 2 to 5 percent.)
+constexpr int merge_warps(int w) { return w < 2 ? 8 : w; }
 // Rows of a group above which its prefix may be the tensor-core kernel's (shared_prefix_plan.cu has the rest of the rule).  Up to 16 the
 // rows kernel is no slower: 4 requests of 4 heads per KV head behind 300, 2000 and 32768 keys 14.9, 16.4 and 45.1 us, there 20.5, 20.5
 // and 43.1; 16 requests behind 4096 keys 37 and 22.6.
@@ -608,7 +610,7 @@ int launch_merge(const SharedPrefixParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, warps = 28 * static_cast<int64_t>(sm_count());
     const int w = rows * 16 <= warps ? 16 : rows * 8 <= warps ? 4 : 1;
     auto kernel = w == 16 ? shared_prefix_merge_kernel<16> : w == 4 ? shared_prefix_merge_kernel<4> : shared_prefix_merge_kernel<1>;
-    const int first = w > 1 ? 0 : 2 * sm_count(), per_token = w > 1 ? p.q_heads : div_ceil(p.q_heads, merge_warps(w));
+    const int first = w > 1 ? 0 : sm_count(), per_token = w > 1 ? p.q_heads : div_ceil(p.q_heads, merge_warps(w));
     B200_CHECK_CUDA(launch_kernel(kernel, dim3(first + static_cast<unsigned>(p.tokens) * per_token), dim3(merge_warps(w) * 32), 0, stream,
                                   dim3(1, 1, 1), p, first));
     return B200_OK;
