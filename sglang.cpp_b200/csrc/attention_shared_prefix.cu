@@ -431,16 +431,15 @@ struct Parts {
     int count;
 };
 
-// Joins the parts of every row, W warps per (token, head); rows that no request owns stay as they were.  Bound by the trips to L2:
-// where the parts are, then their statistics and the first of their sums, then the other sums.  Among many rows (W = 1) those of
-// dozens of parts are joined by the grid's first CTAs, a CTA each (with all alike, two requests behind 26298 keys kept 158 others
-// waiting for 60 us).
-template <int W>
-__device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, int head, int share, bool waited, bool by_cta,
-                                         float2* s_ml, float4 (*s_acc)[32]) {
-    const int lane = threadIdx.x & 31;   // share: of the parts, that one and every W-th behind it
-    // The plan stands before the parts do: the kernel ahead is launched behind the end of the plan's, and this one behind that
-    // launch.  (Where the parts are, found ahead of the wait: 0.9 us of divisions and a trip to L2 while the last parts are formed.)
+// Where a row's parts are: of the group's prefix, and of the request's own keys.  The plan stands before the parts do: the kernel
+// ahead of the merge is launched behind the end of the plan's, and the merge behind that launch.  (Found ahead of the wait: 0.9 us of
+// divisions and a trip to L2 while the last parts are formed.)
+struct RowParts {
+    Parts pre, own;
+    bool owned, many;
+    __device__ __forceinline__ int64_t at(int i) const { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; }
+};
+__device__ __forceinline__ RowParts find_parts(const SharedPrefixParams& p, int tok, int head) {
     JoinItem j;
     static_assert(sizeof(JoinItem) % 16 == 0, "read in 16-byte loads");
 #pragma unroll
@@ -466,10 +465,18 @@ __device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, i
                     (in_block - chain * half) * p.group + hh;
         pre.step = 2 * kSharedTcTile;
     }
+    return RowParts{pre, own, j.owned != 0, j.many != 0};
+}
+
+// Joins the parts of a row by W warps, this one those of number `share` and every W-th behind it.  Bound by the trips to L2: where the
+// parts are, then their statistics and the first of their sums, then the other sums.
+template <int W>
+__device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, int head, int share, bool waited, float2* s_ml, float4 (*s_acc)[32]) {
+    const int lane = threadIdx.x & 31;
+    const RowParts parts = find_parts(p, tok, head);
     if (!waited) pdl_wait_prior();   // (by every CTA: what follows this kernel waits for it alone)
-    if (head >= p.q_heads || !j.owned || (j.many != 0 && !by_cta)) return;
-    const int n = pre.count + own.count;
-    auto at = [&](int i) { return i < pre.count ? pre.first + i * pre.step : own.first + (i - pre.count) * own.step; };
+    if (!parts.owned) return;
+    const int n = parts.pre.count + parts.own.count;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
     constexpr int kAhead = 8;   // sums that are requested at a time, the first together with the statistics
@@ -477,12 +484,12 @@ __device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, i
     for (int base = 0; base < mine; base += 32) {
         const int m = min(32, mine - base);
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at((base + lane) * W + share));
+        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + parts.at((base + lane) * W + share));
         float4 x[kAhead];
         auto fetch = [&](int from) {
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                x[i] = from + i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + at((base + from + i) * W + share) * kD) + lane)
+                x[i] = from + i < m ? __ldcg(reinterpret_cast<const float4*>(p.ws_o + parts.at((base + from + i) * W + share) * kD) + lane)
                                     : make_float4(0.f, 0.f, 0.f, 0.f);
         };
         fetch(0);
@@ -501,24 +508,22 @@ __device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, i
             }
         }
     }
-    if (W > 1) {
-        if (waited) __syncthreads();   // (the last row's have been read)
-        s_acc[share][lane] = acc;
-        if (lane == 0) s_ml[share] = make_float2(M, L);
-        __syncthreads();
-        if (share > 0) return;
+    if (waited) __syncthreads();   // (the last row's have been read)
+    s_acc[share][lane] = acc;
+    if (lane == 0) s_ml[share] = make_float2(M, L);
+    __syncthreads();
+    if (share > 0) return;
 #pragma unroll
-        for (int i = 1; i < W; ++i) M = fmaxf(M, s_ml[i].x);
-        const float ref = M == -INFINITY ? 0.f : M;
-        L = 0.f;
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 1; i < W; ++i) M = fmaxf(M, s_ml[i].x);
+    const float ref = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const float w = exp2f(s_ml[i].x - ref);
-            const float4 y = s_acc[i][lane];
-            L += w * s_ml[i].y;
-            acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
-        }
+    for (int i = 0; i < W; ++i) {
+        const float w = exp2f(s_ml[i].x - ref);
+        const float4 y = s_acc[i][lane];
+        L += w * s_ml[i].y;
+        acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;   // a row that sees no key: zeros
     uint2 packed;
@@ -527,6 +532,71 @@ __device__ __forceinline__ void join_row(const SharedPrefixParams& p, int tok, i
     reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(tok) * p.q_heads + head) * kD)[lane] = packed;
 }
 
+// ... of two rows, neighbouring heads of a token, by half a warp each: 8 elements of the head dimension per lane.  (A warp each: 48 drafted
+// requests of 5376 rows 75.5 us, so 72.4; 256 requests behind 50 keys 34.8 and 32.0.)
+__device__ __forceinline__ void join_two(const SharedPrefixParams& p, int tok, int pair) {
+    const int lane = threadIdx.x & 15, head = pair * 2 + (threadIdx.x >> 4 & 1);
+    const RowParts parts = find_parts(p, tok, min(head, p.q_heads - 1));
+    pdl_wait_prior();
+    if (!parts.owned || parts.many) return;   // (the same for both)
+    const int n = parts.pre.count + parts.own.count, most = __reduce_max_sync(0xffffffffu, n);
+    float4 acc[2] = {};
+    float M = -INFINITY, L = 0.f;
+    constexpr int kAhead = 4;
+    for (int base = 0; base < most; base += 16) {
+        const int m = min(16, n - base);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < m) ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + parts.at(base + lane));
+        float4 x[kAhead][2];
+        auto fetch = [&](int from) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (from + i >= m) continue;
+                const float4* src = reinterpret_cast<const float4*>(p.ws_o + parts.at(base + from + i) * kD) + lane;
+                x[i][0] = __ldcg(src);
+                x[i][1] = __ldcg(src + 16);
+            }
+        };
+        fetch(0);
+        float top = ml.x;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float Mn = fmaxf(M, top);
+        const float ref = Mn == -INFINITY ? 0.f : Mn;
+        const float shrink = exp2f(M - ref), w = exp2f(ml.x - ref);
+        M = Mn;
+        float sum = w * ml.y;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        L = L * shrink + sum;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) acc[e].x *= shrink, acc[e].y *= shrink, acc[e].z *= shrink, acc[e].w *= shrink;
+        for (int from = 0; from < min(16, most - base); from += kAhead) {
+            if (from > 0) fetch(from);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, from + i, 16);
+                if (from + i >= m) continue;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    acc[e].x += x[i][e].x * wi, acc[e].y += x[i][e].y * wi, acc[e].z += x[i][e].z * wi, acc[e].w += x[i][e].w * wi;
+            }
+        }
+    }
+    if (head >= p.q_heads) return;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        uint2 packed;
+        packed.x = pack_bf16(acc[e].x * inv, acc[e].y * inv);
+        packed.y = pack_bf16(acc[e].z * inv, acc[e].w * inv);
+        reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(tok) * p.q_heads + head) * kD)[lane + e * 16] = packed;
+    }
+}
+
+// Rows that no request owns stay as they were.  Many rows (W = 1): half a warp each, but those of dozens of parts by the grid's first
+// CTAs, a CTA each (with all alike, two requests behind 26298 keys kept 158 others waiting for 60 us).
 template <int W>
 __global__ void __launch_bounds__(merge_warps(W) * 32)
 shared_prefix_merge_kernel(const SharedPrefixParams p, int first_ctas) {
@@ -536,16 +606,18 @@ shared_prefix_merge_kernel(const SharedPrefixParams p, int first_ctas) {
     const int warp = threadIdx.x >> 5;
     pdl_launch_dependents();
     if constexpr (W > 1) {
-        join_row<W>(p, static_cast<int>(blockIdx.x) / p.q_heads, static_cast<int>(blockIdx.x) % p.q_heads, warp, false, true, s_ml, s_acc);
+        join_row<W>(p, static_cast<int>(blockIdx.x) / p.q_heads, static_cast<int>(blockIdx.x) % p.q_heads, warp, false, s_ml, s_acc);
     } else {
-        const int cta = static_cast<int>(blockIdx.x) - first_ctas, per_token = (p.q_heads + kWarps - 1) / kWarps;
+        const int cta = static_cast<int>(blockIdx.x) - first_ctas, pairs = (p.q_heads + 1) / 2;
         if (cta >= 0) {
-            join_row<1>(p, cta / per_token, cta % per_token * kWarps + warp, 0, false, false, nullptr, nullptr);
+            const int id = cta * kWarps + warp, tok = id / pairs;
+            if (tok < p.tokens) join_two(p, tok, id - tok * pairs);
+            else pdl_wait_prior();
         } else {
             const int rows = __ldcg(&p.plan.head->many) * p.q_heads;
             pdl_wait_prior();
             for (int i = blockIdx.x; i < rows; i += first_ctas)
-                join_row<kWarps>(p, __ldcg(p.plan.many + i / p.q_heads), i % p.q_heads, warp, true, true, s_ml, s_acc);
+                join_row<kWarps>(p, __ldcg(p.plan.many + i / p.q_heads), i % p.q_heads, warp, true, s_ml, s_acc);
         }
     }
 }
@@ -605,14 +677,14 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
 
 // Warps per row: many where few rows behind a long prefix have hundreds of parts each (two requests behind 32768 keys: 107 us with a
 // warp per row, 54 with four, 39 with sixteen), as far as they are on the device at once (28 on an SM); four only up to half of that
-// (64 requests of 16 heads behind 2051 keys: 28.8 us with a warp, 30.8 with four).
+// (64 requests of 16 heads behind 2051 keys: 28.8 us with fewer, 30.8 with four); half a warp for all others.
 int launch_merge(const SharedPrefixParams& p, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, warps = 28 * static_cast<int64_t>(sm_count());
     const int w = rows * 16 <= warps ? 16 : rows * 8 <= warps ? 4 : 1;
     auto kernel = w == 16 ? shared_prefix_merge_kernel<16> : w == 4 ? shared_prefix_merge_kernel<4> : shared_prefix_merge_kernel<1>;
-    const int first = w > 1 ? 0 : sm_count(), per_token = w > 1 ? p.q_heads : div_ceil(p.q_heads, merge_warps(w));
-    B200_CHECK_CUDA(launch_kernel(kernel, dim3(first + static_cast<unsigned>(p.tokens) * per_token), dim3(merge_warps(w) * 32), 0, stream,
-                                  dim3(1, 1, 1), p, first));
+    const int first = w > 1 ? 0 : sm_count();
+    const int64_t ctas = w > 1 ? rows : div_ceil64(static_cast<int64_t>(p.tokens) * div_ceil(p.q_heads, 2), merge_warps(w));
+    B200_CHECK_CUDA(launch_kernel(kernel, dim3(first + static_cast<unsigned>(ctas)), dim3(merge_warps(w) * 32), 0, stream, dim3(1, 1, 1), p, first));
     return B200_OK;
 }
 
