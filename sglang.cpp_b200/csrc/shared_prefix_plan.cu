@@ -37,6 +37,8 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     __shared__ int s_bound[kSharedMaxBatch + 1], s_prefix[kSharedMaxBatch];
     __shared__ int s_first[kMaxUnits + 1];                                      // items before a unit, in the rows kernel
     __shared__ int s_tc[kSharedMaxBatch + 1], s_unit[kSharedMaxBatch + 1];      // tiles and units before a group, in the other
+    __shared__ short s_pieces[kMaxUnits];                                       // items of a row tile of a unit, in the rows kernel
+    __shared__ int s_cta[kSharedMaxBatch + 1];                                  // chunks before a group, in the other
     __shared__ int4 s_warp[32], s_open[32];
     __shared__ int s_per, s_chunks;   // tiles per chunk, chunks
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = static_cast<int>(blockDim.x);
@@ -164,8 +166,12 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
         s_first[tid] = at.x;
         s_tc[tid] = at.z;
         s_unit[tid] = at.w;
+        s_pieces[tid] = static_cast<short>(g_pieces);   // (kSharedPieces * ctas and one at most)
     }
-    if (tid < p.batch) s_first[p.groups + tid] = at.y;
+    if (tid < p.batch) {
+        s_first[p.groups + tid] = at.y;
+        s_pieces[p.groups + tid] = static_cast<short>(b_pieces);
+    }
     if (tid == 0) {
         s_first[U] = items;
         s_tc[p.groups] = tc_tiles;
@@ -173,6 +179,11 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     }
     __syncthreads();
     const bool fits = !odd && items <= p.max_slots && (units == 0 || ctas + units <= p.tc_slots);
+
+    // tiles of a unit, and units per KV head, of a group in the tensor-core kernel
+    const int kv_shift = 31 - __clz(Hkv);
+    auto tiles_of = [&](int g) { return (s_prefix[g] + kSharedTcTile - 1) / kSharedTcTile; };
+    auto blocks_of = [&](int g) { return (s_unit[g + 1] - s_unit[g]) >> kv_shift; };
 
     // ---- chunks of the tensor-core kernel: a lane per candidate, from an equal share for every CTA to a CTA per unit ----
     const bool chunked = units > 0 && 2 * units <= ctas;
@@ -184,7 +195,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             int count = 0;
             for (int g = 0; g < p.groups; ++g) {
                 const int k = s_unit[g + 1] - s_unit[g];
-                if (k > 0) count += k * (((s_tc[g + 1] - s_tc[g]) / k + per - 1) / per);
+                if (k > 0) count += k * ((tiles_of(g) + per - 1) / per);
             }
             const float time = per * (p.small ? kTileSmall : any_two ? kTileTwo : kTileOne) + kChunk;
             const float left = fmaxf(stages - (ctas - count) * (time * (1.f / kStageAlone)), 0.f);
@@ -201,6 +212,19 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             }
             per = __shfl_sync(0xffffffffu, per, best);
             chunks = __shfl_sync(0xffffffffu, count, best);
+            int before = 0;
+            for (int base = 0; base < p.groups; base += 32) {
+                const int g = base + lane, mine = g < p.groups ? (s_unit[g + 1] - s_unit[g]) * ((tiles_of(g) + per - 1) / per) : 0;
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                if (g < p.groups) s_cta[g] = before + upto - mine;
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) s_cta[p.groups] = before;
         }
         if (lane == 0) {
             s_per = per;
@@ -245,10 +269,10 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             }
             it.table = s_table[b];
             it.start = start_of(it.lo);
-            const int n = stages_of(it.lo, it.hi), pieces = (n + piece - 1) / piece, off = i - s_first[u];
+            const int pieces = s_pieces[u], off = i - s_first[u];
             it.tile = off / pieces;
             it.s_begin = (off - it.tile * pieces) * piece;
-            it.s_end = min(it.s_begin + piece, n);
+            it.s_end = min(it.s_begin + piece, stages_of(it.lo, it.hi));
             it.reread = it.ntok > QT;
             it.slot = i;
             p.plan.rows[i] = it;
@@ -261,18 +285,16 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
     if (p.with_tc && cta < ctas) {
         int begin = 0, end = 0;
         if (chunked) {
-            int before = 0;
-            for (int g = 0; g < p.groups && before <= cta; ++g) {
-                const int k = s_unit[g + 1] - s_unit[g];
-                if (k == 0) continue;
-                const int of_unit = (s_tc[g + 1] - s_tc[g]) / k, chunk = (of_unit + per - 1) / per;
-                if (cta < before + k * chunk) {
-                    const int unit = (cta - before) / chunk, t = (cta - before - unit * chunk) * per;
-                    begin = s_tc[g] + unit * of_unit + t;
-                    end = s_tc[g] + unit * of_unit + min(t + per, of_unit);
-                    break;
+            if (cta < s_cta[p.groups]) {
+                int g = 0, hi = p.groups;   // the last group that does not begin behind it (those without chunks are skipped)
+                while (hi - g > 1) {
+                    const int mid = (g + hi) >> 1;
+                    if (s_cta[mid] <= cta) g = mid; else hi = mid;
                 }
-                before += k * chunk;
+                const int of_unit = tiles_of(g), chunk = (of_unit + per - 1) / per, unit = (cta - s_cta[g]) / chunk;
+                const int t = (cta - s_cta[g] - unit * chunk) * per;
+                begin = s_tc[g] + unit * of_unit + t;
+                end = s_tc[g] + unit * of_unit + min(t + per, of_unit);
             }
         } else if (units > 0) {
             begin = static_cast<int>(min(static_cast<int64_t>(cta) * per, static_cast<int64_t>(tc_tiles)));
@@ -288,10 +310,10 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             bool first = true;
             for (int pos = begin; pos < end;) {
                 while (pos >= s_tc[g + 1]) ++g;
-                const int k = s_unit[g + 1] - s_unit[g], of_unit = (s_tc[g + 1] - s_tc[g]) / k, off = pos - s_tc[g], unit = off / of_unit;
+                const int of_unit = tiles_of(g), off = pos - s_tc[g], unit = off / of_unit;
                 TcItem it;
-                it.h = unit / (k / Hkv);
-                it.tok0 = s_row[s_bound[g]] + (unit - it.h * (k / Hkv)) * 2 * QB;
+                it.h = unit / blocks_of(g);
+                it.tok0 = s_row[s_bound[g]] + (unit - it.h * blocks_of(g)) * 2 * QB;
                 it.ntok = min(s_row[s_bound[g + 1]] - it.tok0, 2 * QB);
                 it.keys = s_prefix[g];
                 it.t0 = off - unit * of_unit;
@@ -321,22 +343,18 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             j.owned = 1;
             j.own_t = tok - s_row[b];
             j.own_first = s_first[u];
-            j.own_pieces = (s_first[u + 1] - s_first[u]) / ((s_row[b + 1] - s_row[b] + QT - 1) / QT);
+            j.own_pieces = s_pieces[u];
             if (g >= 0) {
-                const int first = s_row[s_bound[g]], k = s_unit[g + 1] - s_unit[g];
-                j.pre_t = tok - first;
-                if (k > 0) {
+                j.pre_t = tok - s_row[s_bound[g]];
+                if (blocks_of(g) > 0) {
                     j.tc_unit = s_unit[g];
-                    j.tc_blocks = k / Hkv;
+                    j.tc_blocks = blocks_of(g);
                     j.tc_first = s_tc[g];
-                    j.tc_tiles = (s_tc[g + 1] - s_tc[g]) / k;
-                    for (int e = 0; chunked && e < g; ++e) {
-                        const int kk = s_unit[e + 1] - s_unit[e];
-                        if (kk > 0) j.tc_cta += kk * (((s_tc[e + 1] - s_tc[e]) / kk + per - 1) / per);
-                    }
+                    j.tc_tiles = tiles_of(g);
+                    if (chunked) j.tc_cta = s_cta[g];
                 } else if (s_first[g + 1] > s_first[g]) {
                     j.pre_first = s_first[g];
-                    j.pre_pieces = (s_first[g + 1] - s_first[g]) / ((s_row[s_bound[g + 1]] - first + QT - 1) / QT);
+                    j.pre_pieces = s_pieces[g];
                 }
             }
             j.many = (j.own_pieces + j.pre_pieces) * p.parts + (j.tc_blocks > 0 ? (j.tc_tiles + per - 1) / per : 0) > kSharedMany;
