@@ -92,6 +92,7 @@ struct Meet {   // each CTA's copy: what the CTAs of a row tell one another
     float value[2];                          // last kept value after top_k, after top_p ...
     int ties[2];                             // ... how many of it are kept ...
     double kept[2];                          // ... and the sum of the kept
+    unsigned long long cut;                  // the last entry of the sorted list that is kept
 };
 
 __device__ __forceinline__ uint32_t remote(const void* p, int r) {
@@ -107,6 +108,9 @@ __device__ __forceinline__ void tell(const float* p, int ctas, float v) {
 }
 __device__ __forceinline__ void tell(const double* p, int ctas, double v) {
     for (int r = 0; r < ctas; ++r) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote(p, r)), "d"(v) : "memory");
+}
+__device__ __forceinline__ void tell(const unsigned long long* p, int ctas, unsigned long long v) {
+    for (int r = 0; r < ctas; ++r) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, r)), "l"(v) : "memory");
 }
 __device__ __forceinline__ void meet_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -380,69 +384,87 @@ sampling_probs_kernel(const ProbsParams p) {
                 total += min(meet.listed[i], kList + 1);
             }
             if (total <= kList) {
-                int size = 32;
-                while (size < total) size *= 2;
-                for (int i = tid; i < size; i += kThreads) {
-                    uint64_t word = ~0ull;
-                    int at = i, who = 0;
-                    while (who < C - 1 && at >= meet.listed[who]) at -= meet.listed[who++];
-                    if (i < total) {
-                        if (C == 1) word = list[i];
-                        else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(word) : "r"(remote(list + at, who)));
-                    }
-                    all[i] = word;
+                // Zeros everywhere, while the first CTA sorts all the lists.  (Every CTA sorting them: 64 rows of 128256 28.4 us, so 24.7; 320
+                // of 151936 79.3 and 76.6; but 6 of 32000 12.1 and 12.6.)
+                if (ALIGNED) {
+                    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    for (int v = tid; v < n >> 3; v += kThreads) store8(z, v * 8);
                 }
-                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (nothing remote is read any more; waited for at the end)
-                __syncthreads();
-                // (Thread i's pair lies in the 64 words of its warp as long as they are at most 32 apart: no need to wait for other warps.)
-                for (int run = 2; run <= size; run *= 2) {
-                    if (run > 64) __syncthreads();
-                    for (int o = run / 2; o > 0; o /= 2) {
-                        for (int i = tid; i < size / 2; i += kThreads) {
-                            const int a = 2 * i - (i & (o - 1)), b = a + o;
-                            const uint64_t wa = all[a], wb = all[b];
-                            if ((wa > wb) == ((a & run) == 0)) {
-                                all[a] = wb;
-                                all[b] = wa;
-                            }
+                for (int i = (ALIGNED ? n & ~7 : 0) + tid; i < n; i += kThreads) __stcs(out + i, 0.f);
+                if (rank == 0) {
+                    int size = 32;
+                    while (size < total) size *= 2;
+                    for (int i = tid; i < size; i += kThreads) {
+                        uint64_t word = ~0ull;
+                        int at = i, who = 0;
+                        while (who < C - 1 && at >= meet.listed[who]) at -= meet.listed[who++];
+                        if (i < total) {
+                            if (C == 1) word = list[i];
+                            else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(word) : "r"(remote(list + at, who)));
                         }
-                        if (o > 32) __syncthreads();
-                        else __syncwarp();
+                        all[i] = word;
+                    }
+                    __syncthreads();
+                    // (Thread i's pair lies in the 64 words of its warp as long as they are at most 32 apart: no need to wait for other
+                    // warps.)
+                    for (int run = 2; run <= size; run *= 2) {
+                        if (run > 64) __syncthreads();
+                        for (int o = run / 2; o > 0; o /= 2) {
+                            for (int i = tid; i < size / 2; i += kThreads) {
+                                const int a = 2 * i - (i & (o - 1)), b = a + o;
+                                const uint64_t wa = all[a], wb = all[b];
+                                if ((wa > wb) == ((a & run) == 0)) {
+                                    all[a] = wb;
+                                    all[b] = wa;
+                                }
+                            }
+                            if (o > 32) __syncthreads();
+                            else __syncwarp();
+                        }
+                    }
+                    __syncthreads();
+                    // ---- weights of the first top_k, and how many of them stay ----
+                    const uint64_t word = all[tid];   // (at least 32; behind them whatever is there is not used)
+                    const bool there = tid < K && tid < total;
+                    const double w = there ? weight64(value_of(0xffffu - static_cast<uint32_t>(word >> 32)), xmax, per_t) : 0.0;
+                    double upto = w;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double d = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += d;
+                    }
+                    if (lane == 31) s_d[warp] = upto;
+                    __syncthreads();
+                    double sum = 0.0, ahead = 0.0;
+                    for (int i = 0; i < kWarps; ++i) {
+                        if (i == warp) ahead = sum;
+                        sum += s_d[i];
+                    }
+                    upto += ahead;
+                    const bool stays = there && w > 0.0 && (!want_p || tid == 0 || upto <= fmax(static_cast<double>(P), 0.0) * sum);
+                    const uint32_t ends = __ballot_sync(0xffffffffu, !stays);
+                    if (lane == 0) s_i[warp] = ends != 0 ? warp * 32 + __ffs(ends) - 1 : kThreads;
+                    __syncthreads();
+                    int stay = kThreads;
+                    for (int i = 0; i < kWarps; ++i) stay = min(stay, s_i[i]);
+                    double kept = warp_sum(tid < stay ? w : 0.0);
+                    if (lane == 0) s_d[warp] = kept;
+                    __syncthreads();
+                    kept = 0.0;
+                    for (int i = 0; i < kWarps; ++i) kept += s_d[i];
+                    if (tid == 0) {
+                        tell(&meet.kept[0], C, kept);
+                        tell(&meet.cut, C, all[max(stay - 1, 0)]);
                     }
                 }
-                __syncthreads();
-                // ---- weights of the first top_k, and what of them stays ----
-                const uint64_t word = all[tid];   // (at least 32; behind them whatever is there is not used)
-                const bool there = tid < K && tid < total;
-                const double w = there ? weight64(value_of(0xffffu - static_cast<uint32_t>(word >> 32)), xmax, per_t) : 0.0;
-                double upto = w;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double d = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += d;
+                meet_all();   // (also: the zeros of this CTA are ahead of what is kept, and nothing remote is touched behind this)
+                const double kept = meet.kept[0];
+                for (int i = tid; i < min(s_listed, kList); i += kThreads) {
+                    const uint64_t word = list[i];
+                    if (word <= meet.cut)
+                        out[static_cast<int>(word & 0xffffffffu) - begin] =
+                            static_cast<float>(weight64(value_of(0xffffu - static_cast<uint32_t>(word >> 32)), xmax, per_t) / kept);
                 }
-                if (lane == 31) s_d[warp] = upto;
-                __syncthreads();
-                double sum = 0.0, ahead = 0.0;
-                for (int i = 0; i < kWarps; ++i) {
-                    if (i == warp) ahead = sum;
-                    sum += s_d[i];
-                }
-                upto += ahead;
-                const bool stays = there && w > 0.0 && (!want_p || tid == 0 || upto <= fmax(static_cast<double>(P), 0.0) * sum);
-                double kept = stays ? w : 0.0;
-                kept = warp_sum(kept);
-                __syncthreads();
-                if (lane == 0) s_d[warp] = kept;
-                for (int i = tid; i < (ALIGNED ? n >> 2 : 0); i += kThreads)
-                    __stcs(reinterpret_cast<float4*>(out) + i, make_float4(0.f, 0.f, 0.f, 0.f));
-                for (int i = (ALIGNED ? n & ~3 : 0) + tid; i < n; i += kThreads) __stcs(out + i, 0.f);
-                __syncthreads();   // (the zeros are ahead of what is kept)
-                kept = 0.0;
-                for (int i = 0; i < kWarps; ++i) kept += s_d[i];
-                const int place = static_cast<int>(word & 0xffffffffu) - begin;
-                if (stays && place >= 0 && place < n) out[place] = static_cast<float>(w / kept);
-                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
                 return;
             }
             // (too many: counted like the others.  The lists have been read by nobody.)
