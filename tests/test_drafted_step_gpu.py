@@ -42,6 +42,8 @@ ATTENTION = {
     "some rows behind short prefixes": ([[(5, 1), (20, 1)] * 3, [(7, 2), (9, 3)], [(4, 1)] * 30], [100, 130, 300], 16, 32, 8),
     "few rows, hundreds of parts": ([[(1, 1), (2, 1)], [(12000, 1)]], [30000, 0], 16, 16, 8),
     "a few of many rows with hundreds of parts": ([[(9, 2), (20, 1)], [(5, 1)] * 70, [(11000, 3)]], [20000, 100, 0], 16, 16, 8),
+    "many rows of an odd number of heads": ([[(3 + i % 50, 1) for i in range(110)]], [400], 16, 5, 1),
+    "many rows, seven heads per KV head": ([[(1 + i % 70, 1 + i % 2) for i in range(50)], [(300, 9)]], [130, 0], 8, 14, 2),
     "hundreds of rows, dozens of parts": ([[(2000 + 100 * i, 1 + i % 2) for i in range(12)]], [1200], 16, 32, 8),
 }
 
