@@ -28,7 +28,7 @@ constexpr int kTcAlways = 32, kTcWorth = 6;
 // Microseconds: a tile of two chains' rows, one of a single chain's, one of small pages (128 copies), the rest of a chunk; a stage of a
 // CTA among few, and of all at once.
 // (kTileSmall as large as kTileOne: 105 requests in pages of four tokens 150 us, so 105.  kTileTwo 1.65 to 1.9 where the memory has
-// little else to do; 128 requests behind 32768 keys 145 to 149 us with 1.8, 141 to 143 with 2.0; kStageAlone 1.0 instead 142 to 145.)
+// little else to do; 128 requests behind 32768 keys 145 to 149 us with 1.8, 141 to 146 with 2.0; kStageAlone 1.0 instead 142 to 145.)
 constexpr float kTileTwo = 2.0f, kTileOne = 0.85f, kTileSmall = 3.1f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
 
 __global__ void __launch_bounds__(kMaxThreads)
