@@ -295,7 +295,7 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
  * Everything per request and group is read on the device: a captured call follows what the arrays hold at its replay,
  * up to its tokens, batch and groups.  Slots outside the pool are read as slot 0 and reported in the status words
  * (-1 as -2^31).  A qo_indptr or group_indptr that decreases or leaves [0, tokens] or [0, batch] is reported as tokens + 1, and nothing is
- * written.
+ * written; so are prefixes of 2^30 or more tiles (of 128 keys, 256 query rows and one KV head) in all.
  * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head, up to 1024 requests; q 16-byte aligned, its
  * strides multiples of 8 elements.  For a few rows per request: thousands of rows of one prompt are b200_attention_prefill's.
  * workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one

@@ -15,6 +15,30 @@ constexpr int kSharedPieces = 4;       // items of the rows kernel per CTA, abou
 constexpr int kSharedTcTile = 128;     // keys of a tile of the tensor-core kernel, and query rows of one of its chains
 
 constexpr int kSharedMany = 32;        // parts of a row that are too many for one warp, among rows of a few
+constexpr int kSharedMinStages = 2;    // of an item of the rows kernel
+constexpr int kSharedLongPiece = 6;    // stages of an item that covers the fetching of the next
+
+// Stages of the rows kernel, and tiles of the tensor-core kernel, of one unit: row tiles (or blocks of rows) times what each goes over.
+// 64 bits: 32768 row tiles behind 2^20 keys of 8 heads are 2^31 stages.
+__host__ __device__ inline int64_t shared_unit_work(int tiles, int each) { return static_cast<int64_t>(tiles) * each; }
+
+// Stages per item: about an item per CTA where that makes short ones (every item costs a microsecond of queries and results, and its
+// parts have to be joined: 64 requests of up to 512 keys of their own 34.8 us with 2 stages, 31.4 with 6), several where they
+// would be long, and no more of them than there is room for: kSharedPieces per CTA and one per row tile.  (Counts beyond 32-bit division
+// are shifted: up to twice as many stages.  A row tile has no more than 2^26.)
+__host__ __device__ inline int shared_stages_per_item(int64_t stages, int ctas) {
+    const int many = kSharedPieces * ctas;
+    if (stages > 0x40000000) {
+        int shift = 0;
+        while (2 << shift <= many) ++shift;
+        const int64_t n = (stages >> shift) + 1;
+        return n < (1 << 26) ? static_cast<int>(n) : 1 << 26;
+    }
+    const int all = static_cast<int>(stages), least = (all + many - 1) / many, one = (all + ctas - 1) / ctas;
+    const int n = one < kSharedLongPiece ? one : kSharedLongPiece;
+    const int piece = least > n ? least : n;
+    return piece > kSharedMinStages ? piece : kSharedMinStages;
+}
 
 // Units are the groups' prefixes (0 .. groups) and the requests' own keys (groups .. groups + batch).
 

@@ -20,8 +20,8 @@ namespace {
 constexpr int kMaxThreads = 1024, kMinThreads = 256;
 static_assert(kMaxThreads >= kSharedMaxBatch, "a thread per request");
 constexpr int kMaxUnits = 2 * kSharedMaxBatch;
-constexpr int kMinStages = 2, kMinTiles = 2;   // per item
-constexpr int kLongPiece = 6;                  // stages of an item that covers the fetching of the next
+constexpr int kMinTiles = 2;                   // per item
+constexpr int kLarge = 1 << 19;                // stages or tiles of a unit that are added up in 64 bits
 // Groups of up to kTcAlways rows are the tensor-core kernel's only where they are that many stages per CTA: 8 requests of 4 heads per KV
 // head behind 300 keys (0.5 stages) 18.5 us without and 21.3 with it, behind 4096 (7) 28.7 and 22.6, behind 32768 106 and 46.8.
 constexpr int kTcAlways = 32, kTcWorth = 6;
@@ -31,7 +31,14 @@ constexpr int kTcAlways = 32, kTcWorth = 6;
 // little else to do; 128 requests behind 32768 keys 145 to 149 us with 1.8, 141 to 146 with 2.0; kStageAlone 1.0 instead 142 to 145.)
 constexpr float kTileTwo = 2.0f, kTileOne = 0.85f, kTileSmall = 3.1f, kChunk = 5.f, kStageAlone = 1.2f, kStageAll = 1.45f;
 
-__global__ void __launch_bounds__(kMaxThreads)
+// A warp's sum of numbers that add up to less than 2^54: 32 of 27 bits are a 32-bit sum.
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+    const uint32_t low = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0x7ffffffu);
+    const uint32_t high = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 27));
+    return (static_cast<int64_t>(high) << 27) + low;
+}
+
+__global__ void __launch_bounds__(kMaxThreads, 1)
 shared_prefix_plan_kernel(const SharedPrefixParams p) {
     __shared__ int s_row[kSharedMaxBatch + 1], s_len[kSharedMaxBatch], s_table[kSharedMaxBatch];
     __shared__ short s_group[kSharedMaxBatch];                                  // of a request, -1: none
@@ -115,9 +122,11 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
         b_stages = stages_of(lo, len);
         b_tiles = (ntok + QT - 1) / QT;
     }
-    // sums over all: stages, key tiles, units, longest prefix; what is open apart
-    int4 sum = make_int4((open ? 0 : g_tiles * g_stages) + b_tiles * b_stages, open ? 0 : g_units * g_tc, open ? 0 : g_units, open ? 0 : g_tc);
-    int4 also = open ? make_int4(g_tiles * g_stages, g_units * g_tc, g_units, g_tc) : make_int4(0, 0, 0, 0);
+    // sums over all: stages, key tiles, units, longest prefix; what is open apart.  (2048 units of up to kLarge are a 32-bit sum.)
+    auto counted = [](int tiles, int each) { return static_cast<int>(min(shared_unit_work(tiles, each), static_cast<int64_t>(kLarge))); };
+    const int g_work = counted(g_tiles, g_stages), g_tc_work = counted(g_units, g_tc);
+    int4 sum = make_int4((open ? 0 : g_work) + counted(b_tiles, b_stages), open ? 0 : g_tc_work, open ? 0 : g_units, open ? 0 : g_tc);
+    int4 also = open ? make_int4(g_work, g_tc_work, g_units, g_tc) : make_int4(0, 0, 0, 0);
     auto add_up = [](int4 v) {
         return make_int4(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y), __reduce_add_sync(0xffffffffu, v.z),
                          __reduce_max_sync(0xffffffffu, v.w));
@@ -136,12 +145,23 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
         if (by_tc) g_tiles = g_stages = 0;
         else g_units = g_tc = 0;
     }
-    const int stages = sum.x + (by_tc ? 0 : also.x), tc_tiles = sum.y + (by_tc ? also.y : 0);
+    int64_t stages = sum.x + (by_tc ? 0 : also.x), all_tiles = sum.y + (by_tc ? also.y : 0);
     const int units = sum.z + (by_tc ? also.z : 0), longest = by_tc ? max(sum.w, also.w) : sum.w;
-    // Stages per item: about an item per CTA where that makes short ones (every item costs a microsecond of queries and results, and its
-    // parts have to be joined: 64 requests of up to 512 keys of their own 34.8 us with 2 stages, 31.4 with 6), several where they
-    // would be long, and no more of them than there is room for.
-    const int piece = max(max((stages + kSharedPieces * ctas - 1) / (kSharedPieces * ctas), min((stages + ctas - 1) / ctas, kLongPiece)), kMinStages);
+    if (stages >= kLarge || all_tiles >= kLarge) {   // (the same in every thread; otherwise no unit has so many)
+        __syncthreads();   // (the sums have been read)
+        stages = warp_sum64(shared_unit_work(g_tiles, g_stages) + shared_unit_work(b_tiles, b_stages));
+        all_tiles = warp_sum64(shared_unit_work(g_units, g_tc));
+        longlong2* s_large = reinterpret_cast<longlong2*>(s_open);
+        if (lane == 0) s_large[warp] = make_longlong2(stages, all_tiles);
+        __syncthreads();
+        const longlong2 part = lane < threads >> 5 ? s_large[lane] : make_longlong2(0, 0);
+        stages = warp_sum64(part.x);
+        all_tiles = warp_sum64(part.y);
+    }
+    // (Tiles are numbered in 32 bits: so many, a quarter of a minute's work, are refused.)
+    const bool countable = all_tiles < 0x40000000;
+    const int tc_tiles = countable ? static_cast<int>(all_tiles) : 0;
+    const int piece = shared_stages_per_item(stages, ctas);
     const int g_pieces = (g_stages + piece - 1) / piece, b_pieces = (b_stages + piece - 1) / piece;
 
     // ---- sums over what comes before: x the groups' items, y the requests'; z key tiles, w units ----
@@ -179,7 +199,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
         s_unit[p.groups] = units;
     }
     __syncthreads();
-    const bool fits = !odd && items <= p.max_slots && (units == 0 || ctas + units <= p.tc_slots);
+    const bool fits = !odd && countable && items <= p.max_slots && (units == 0 || ctas + units <= p.tc_slots);
 
     // tiles of a unit, and units per KV head, of a group in the tensor-core kernel
     const int kv_shift = 31 - __clz(Hkv);
@@ -236,7 +256,7 @@ shared_prefix_plan_kernel(const SharedPrefixParams p) {
             // CTAs that find an SM free begin with the item of their own number.
             h.rows_first = chunked || units == 0 ? max(ctas - s_chunks, 0) : 0;
             h.next = min(h.rows_first, h.rows_items);
-            h.rows_lead = piece < kLongPiece && items > 2 * ctas ? 2 : 1;
+            h.rows_lead = piece < kSharedLongPiece && items > 2 * ctas ? 2 : 1;
             h.tc_per = per;
             h.tc_chunked = chunked;
             *p.plan.head = h;
