@@ -222,50 +222,73 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k,
         }
     } else if (warp == 1) {
         // ================= MMA issuer =================
-        if (lane == 0) {
-            const uint32_t idesc_s = idesc_128x128(false);
-            const uint32_t idesc_pv = idesc_128x128(true);
-            const uint32_t q_addr = smem_base + kQOff, p_addr = smem_base + kPOff;
-            bool failed = false;
-            auto issue_s = [&](int kt) {
-                const uint32_t slot = kt % kStages;
-                if (!mbar_wait_bounded(smem_u32(&k_full[slot]), static_cast<uint32_t>(kt / kStages) & 1u,
-                                       p.status, 312)) {
-                    failed = true;
-                    return;
-                }
-                tc_fence_after();
-                const uint32_t k_addr = smem_base + kKVOff + slot * kStageBytes;
-                const uint32_t d = tmem_base + kColS + static_cast<uint32_t>(kt & 1) * 128u;
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t off = (ks >> 2) * kAtomBytes + (ks & 3) * 32;
-                    tc_mma_bf16(d, kmajor_sw128_desc(q_addr + off), kmajor_sw128_desc(k_addr + off), idesc_s,
-                                ks > 0 ? 1u : 0u);
-                }
-                tc_commit(smem_u32(&s_full[kt & 1]));
-                tc_commit(smem_u32(&k_empty[slot]));
-            };
-            issue_s(0);
-            for (int kt = 0; kt < ntiles && !failed; ++kt) {
-                if (kt + 1 < ntiles) issue_s(kt + 1);
-                if (failed) break;
-                const uint32_t slot = kt % kStages;
-                if (!mbar_wait_bounded(smem_u32(&v_full[slot]), static_cast<uint32_t>(kt / kStages) & 1u, p.status, 316))
-                    break;
-                if (!mbar_wait_bounded(smem_u32(&p_full), static_cast<uint32_t>(kt) & 1u, p.status, 313)) break;
-                tc_fence_after();
-                const uint32_t v_addr = smem_base + kKVOff + slot * kStageBytes + 2 * kAtomBytes;
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    // keys ks*16 .. +15: P columns inside atom ks/4; V rows 2048 bytes further per step
-                    const uint32_t p_off = (ks >> 2) * kAtomBytes + (ks & 3) * 32;
-                    tc_mma_bf16(tmem_base + kColPV, kmajor_sw128_desc(p_addr + p_off),
-                                mnmajor_sw128_desc(v_addr + ks * 2048), idesc_pv, ks > 0 ? 1u : 0u);
-                }
-                tc_commit(smem_u32(&pv_full));
-                tc_commit(smem_u32(&v_empty[slot]));
+        const uint32_t idesc_s = idesc_128x128(false);
+        const uint32_t idesc_pv = idesc_128x128(true);
+        const uint32_t q_addr = smem_base + kQOff, p_addr = smem_base + kPOff;
+        bool failed = false;
+        auto issue_s = [&](int kt) {
+            const uint32_t slot = kt % kStages;
+            if (!mbar_wait_bounded(smem_u32(&k_full[slot]), static_cast<uint32_t>(kt / kStages) & 1u,
+                                   p.status, 312)) {
+                failed = true;
+                return;
             }
+            tc_fence_after();
+            const uint32_t k_addr = smem_base + kKVOff + slot * kStageBytes;
+            const uint32_t d = tmem_base + kColS + static_cast<uint32_t>(kt & 1) * 128u;
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                const uint32_t off = (ks >> 2) * kAtomBytes + (ks & 3) * 32;
+                tc_mma_bf16(d, kmajor_sw128_desc(q_addr + off), kmajor_sw128_desc(k_addr + off), idesc_s,
+                            ks > 0 ? 1u : 0u);
+            }
+            tc_commit(smem_u32(&s_full[kt & 1]));
+            tc_commit(smem_u32(&k_empty[slot]));
+        };
+        auto issue_pv = [&](int kt) {
+            const uint32_t slot = kt % kStages;
+            if (!mbar_wait_bounded(smem_u32(&v_full[slot]), static_cast<uint32_t>(kt / kStages) & 1u, p.status, 316) ||
+                !mbar_wait_bounded(smem_u32(&p_full), static_cast<uint32_t>(kt) & 1u, p.status, 313)) {
+                failed = true;
+                return;
+            }
+            tc_fence_after();
+            const uint32_t v_addr = smem_base + kKVOff + slot * kStageBytes + 2 * kAtomBytes;
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                // keys ks*16 .. +15: P columns inside atom ks/4; V rows 2048 bytes further per step
+                const uint32_t p_off = (ks >> 2) * kAtomBytes + (ks & 3) * 32;
+                tc_mma_bf16(tmem_base + kColPV, kmajor_sw128_desc(p_addr + p_off),
+                            mnmajor_sw128_desc(v_addr + ks * 2048), idesc_pv, ks > 0 ? 1u : 0u);
+            }
+            tc_commit(smem_u32(&pv_full));
+            tc_commit(smem_u32(&v_empty[slot]));
+        };
+        const int in_page = kv_end & (p.kpc - 1);
+        const int clean = in_page != 0 ? ntiles - 1 : ntiles;   // tiles whose last page ends with them
+        if (lane == 0) {
+            issue_s(0);
+            for (int kt = 0; kt < clean && !failed; ++kt) {
+                if (kt + 1 < ntiles) issue_s(kt + 1);
+                if (!failed) issue_pv(kt);
+            }
+        }
+        __syncwarp();
+        if (clean < ntiles) {
+            // Behind the last key the last page holds whatever was there before: as values, these have to be numbers for their weights of
+            // 0.  The whole warp clears them while the last tile's softmax runs.
+            const uint32_t slot = clean % kStages;
+            if (mbar_wait_warp(smem_u32(&v_full[slot]), static_cast<uint32_t>(clean / kStages) & 1u, p.status, 317)) {
+                const uint32_t base = smem_base + kKVOff + slot * kStageBytes + 2 * kAtomBytes;
+                for (int i = lane; i < (p.kpc - in_page) * 16; i += 32) {
+                    const int key = kv_end - clean * kTile + (i >> 4), c = i & 15;
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(base + (c >> 3) * kAtomBytes + key * 128 + (c & 7) * 16), "r"(0u)
+                                 : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && !failed) issue_pv(clean);
         }
     } else {
         // ================= softmax / output rows =================

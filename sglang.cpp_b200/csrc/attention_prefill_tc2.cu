@@ -357,15 +357,20 @@ attention_prefill_tc2_kernel(const __grid_constant__ KvMaps maps, const PrefillT
         }
     } else if (warp == 3) {
         // ================= issuer of O_i += P_i V =================
-        if (elect_one()) {
+        const uint32_t leader = elect_one();
+        // Behind the last key the last page holds whatever was there before: as values, these have to be numbers for their weights of 0.
+        // The whole warp clears them while the last tile's softmax runs.  (The softmax warps themselves: spills in their loop, 1024
+        // tokens of 16 heads 19.9 -> 20.4 us; V's producer, which handed the tile on behind its copies: 21.8.)
+        const int in_page = kv_end & (p.kpc - 1);
+        uint32_t slot = kKSlots, phase = 0;
+        bool failed = false;
+        auto add_tiles = [&](int begin, int end) {
             const uint32_t idesc = idesc_bf16_128x128(true);
             const uint64_t v_desc = grouped_keys_desc(smem_base + kKVOff, 1024);   // second half of the head dimension 1024 bytes on
-            uint32_t slot = kKSlots, phase = 0;
-            bool failed = false;
             auto wait = [&](uint32_t bar, uint32_t parity, int site) {
                 if (!failed && !mbar_wait_mostly_ready(bar, parity, p.status, site)) failed = true;
             };
-            for (int kt = 0; kt < ntiles && !failed; ++kt) {
+            for (int kt = begin; kt < end && !failed; ++kt) {
                 const uint64_t v = v_desc + slot * (kSlotBytes >> 4);
                 const uint32_t parity = static_cast<uint32_t>(kt) & 1u;
                 wait(smem_u32(&full[slot]), phase, 326);
@@ -388,6 +393,23 @@ attention_prefill_tc2_kernel(const __grid_constant__ KvMaps maps, const PrefillT
                     phase ^= 1;
                 }
             }
+        };
+        const int clean = in_page != 0 ? ntiles - 1 : ntiles;   // tiles without such a page
+        if (leader) add_tiles(0, clean);
+        __syncwarp();
+        if (clean < ntiles) {
+            const uint32_t at = kKSlots + static_cast<uint32_t>(clean % kVSlots);
+            if (mbar_wait_warp(smem_u32(&full[at]), static_cast<uint32_t>(clean / kVSlots) & 1u, p.status, 329)) {
+                const uint32_t base = smem_base + kKVOff + at * kSlotBytes;
+                for (int i = lane; i < (p.kpc - in_page) * 16; i += 32) {
+                    const int key = kv_end - first_key(clean) + (i >> 4), c = i & 15;
+                    const uint32_t a = base + (key >> 3) * 2048 + (c >> 3) * 1024 + (key & 7) * 128 + (c & 7) * 16;
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (leader) add_tiles(clean, ntiles);
         }
     } else if (warp >= 4) {
         // ================= softmax / output rows =================

@@ -166,3 +166,59 @@ def test_prefill_from_a_cache_smaller_than_a_page(L, pkg, page_size, num_slots):
     assert torch.isfinite(out).all()
     status = L.read_device_status()
     assert status[0] == 0 and status[1] != 0
+
+
+@pytest.mark.parametrize("page_size", [1, 4, 16, 64, 256])
+@pytest.mark.parametrize("seq_lens,extend_lens,hq,hkv", [
+    ([1, 21, 130, 200], [1, 21, 30, 40], 16, 8),          # one tile of query rows: extensions up to 128 / group
+    ([700, 385], [64, 1], 16, 8),                          # ... more tiles of keys than V's ring has places
+    ([1, 100, 129, 513, 300], [1, 100, 129, 70, 299], 16, 8),   # two
+    ([1000, 257], [65, 257], 32, 4),
+])
+def test_prefill_ignores_what_a_page_holds_behind_the_last_key(L, page_size, seq_lens, extend_lens, hq, hkv):
+    """A recycled page's slots behind the last key: infinities and NaN there reach no row."""
+    from tests.shared_prefix_cases import SharedSetup, assert_attention
+
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        s = SharedSetup([[(n, e)] for n, e in zip(seq_lens, extend_lens)], [0] * len(seq_lens), page_size, hq, hkv, seed=page_size + len(seq_lens))
+        for pool in (s.k, s.v):
+            pool[pool[:, 0, 0].isnan()] = bad
+        attn = L.PagedAttention(s.cache(L), hq, hkv, 128, max_batch=len(seq_lens))
+        got = attn.prefill(s.q.cuda(), 0, *s.index(s.table, s.table_idx, s.lens, s.qo), max(extend_lens))
+        assert_attention(got, *s.want())
+    assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("page_size,window,keep_first", [(16, 100, 0), (64, 70, 5), (256, 2 ** 31 - 1, 0)])
+def test_window_prefill_ignores_what_a_page_holds_behind_the_last_key(L, page_size, window, keep_first):
+    """The same with a sliding window, whose prompts run on the two-tile kernel."""
+    import ctypes
+    import math
+
+    from sglang_cpp_b200 import _lib
+    from tests.shared_prefix_cases import SharedSetup, assert_attention
+
+    ext, hq, hkv = [130, 21, 300], 16, 8
+    s = SharedSetup([[(n, e)] for n, e in zip([130, 517, 300], ext)], [0] * 3, page_size, hq, hkv, seed=page_size)
+    cache, q = s.cache(L), s.q.cuda()
+    table, idx, lens, qo = s.index(s.table, s.table_idx, s.lens, s.qo)
+    of_row = [(b, n - e + i + 1) for b, (n, e) in enumerate(zip(s.lens, ext)) for i in range(e)]
+    row_table, row_len = s.index([s.table_idx[b] for b, _ in of_row], [n for _, n in of_row])
+    out = torch.empty(len(of_row), hq * 128, dtype=torch.bfloat16, device="cuda")
+    workspace = torch.zeros(_lib.load().b200_attention_decode_workspace_bytes(3, hq, hkv, 128), dtype=torch.uint8, device="cuda")
+    a = _lib.WindowAttentionArgs(
+        out=out.data_ptr(), q=q.data_ptr(), q_stride=q.stride(0), k_cache=cache.k_cache(0).data_ptr(), v_cache=cache.v_cache(0).data_ptr(),
+        num_slots=cache.total_slots, page_table=table.data_ptr(), page_table_stride=table.stride(0), table_idx=idx.data_ptr(),
+        seq_lens=lens.data_ptr(), qo_indptr=qo.data_ptr(), row_table=row_table.data_ptr(), row_len=row_len.data_ptr(), tokens=len(of_row),
+        batch=3, max_extend=max(ext), heads=hq, kv_heads=hkv, padded_dim=128, padded_value_dim=128, page_size=page_size,
+        scale=1 / math.sqrt(128), window=window, keep_first=keep_first, workspace=workspace.data_ptr(), workspace_bytes=workspace.numel())
+    _lib.call("b200_window_attention", ctypes.byref(a), 0, torch.cuda.current_stream().cuda_stream)
+    want, size = (torch.zeros(len(of_row), hq, 128, dtype=torch.float64) for _ in range(2))
+    for r, (b, n) in enumerate(of_row):
+        seen = [j for j in range(n) if n - 1 - j < window or j < keep_first]
+        slots = torch.from_numpy(s.table[s.table_idx[b], seen].astype("int64"))
+        k, v = s.k[slots].double(), s.v[slots].double()
+        w = torch.softmax(torch.einsum("hgd,khd->hgk", s.q[r].double().reshape(hkv, -1, 128), k) / math.sqrt(128), -1)
+        want[r] = torch.einsum("hgk,khd->hgd", w, v).reshape(hq, 128)
+        size[r] = torch.einsum("hgk,khd->hgd", w, v.abs()).reshape(hq, 128)
+    assert_attention(out, want.reshape(len(of_row), -1), size.reshape(len(of_row), -1))
