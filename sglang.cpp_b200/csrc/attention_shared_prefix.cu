@@ -675,12 +675,13 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
     return B200_OK;
 }
 
-// Warps per row: many where few rows behind a long prefix have hundreds of parts each (two requests behind 32768 keys: 107 us with a
-// warp per row, 54 with four, 39 with sixteen), as far as they are on the device at once (28 on an SM); four only up to half of that
-// (64 requests of 16 heads behind 2051 keys: 28.8 us with fewer, 30.8 with four); half a warp for all others.
+// Warps per row: sixteen as long as there is a row per SM, whose registers hold one such CTA (128 rows of 8 KV heads behind 304, 4096 and
+// 32768 keys 13.4, 16.4 and 42.3 us, with four 13.6, 20.7 and 56.1; 160 rows 16.3, 21.0 and 43.0, with four 14.0, 20.4 and 40.0; 256 rows
+// 17.7, 22.2 and 44.7, with four 14.2, 18.9 and 40.8).  Four up to three and a half rows per SM (512 rows 18.4, 19.7 and 42.2, with half a
+// warp 17.7, 21.1 and 43.7; 64 requests of 16 heads behind 2051 keys 30.8 and 28.8); half a warp for all others.
 int launch_merge(const SharedPrefixParams& p, cudaStream_t stream) {
-    const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, warps = 28 * static_cast<int64_t>(sm_count());
-    const int w = rows * 16 <= warps ? 16 : rows * 8 <= warps ? 4 : 1;
+    const int64_t rows = static_cast<int64_t>(p.tokens) * p.q_heads, sms = sm_count();
+    const int w = rows <= sms ? 16 : rows * 2 <= sms * 7 ? 4 : 1;
     auto kernel = w == 16 ? shared_prefix_merge_kernel<16> : w == 4 ? shared_prefix_merge_kernel<4> : shared_prefix_merge_kernel<1>;
     const int first = w > 1 ? 0 : sm_count();
     const int64_t ctas = w > 1 ? rows : div_ceil64(static_cast<int64_t>(p.tokens) * div_ceil(p.q_heads, 2), merge_warps(w));
