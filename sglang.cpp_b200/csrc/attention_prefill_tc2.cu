@@ -101,24 +101,6 @@ struct KvMaps {
     CUtensorMap tile[2];   // whole rows of 128 keys: tiles whose pages are consecutive slots
 };
 
-// Two fp32 operations per instruction, and the maximum of three.
-__device__ __forceinline__ uint64_t as_pair(float2 x) { return *reinterpret_cast<uint64_t*>(&x); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
-    return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)));
-    return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 template <bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prefill_tc2_kernel(const __grid_constant__ KvMaps maps, const PrefillTc2Params p) {
@@ -357,7 +339,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ KvMaps maps, const PrefillT
         }
     } else if (warp == 3) {
         // ================= issuer of O_i += P_i V =================
-        const uint32_t leader = elect_one();
+        const bool leader = elect_one();
         // Behind the last key the last page holds whatever was there before: as values, these have to be numbers for their weights of 0.
         // The whole warp clears them while the last tile's softmax runs.  (The softmax warps themselves: spills in their loop, 1024
         // tokens of 16 heads 19.9 -> 20.4 us; V's producer, which handed the tile on behind its copies: 21.8.)

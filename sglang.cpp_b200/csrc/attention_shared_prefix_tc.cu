@@ -55,27 +55,6 @@ struct SharedKvMaps {
     int kpc;                        // keys of a page in a tile
 };
 
-__device__ __forceinline__ uint64_t as_pair(float2 x) { return *reinterpret_cast<uint64_t*>(&x); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
-    return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)));
-    return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Half rows of four slots, one behind the other in shared memory.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int column, int r0, int r1, int r2, int r3, uint32_t bar) {
     asm volatile(
@@ -413,7 +392,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 tc_fence_after();
                 float alpha = 1.f;
                 if (mx != -INFINITY && (m_ref == -INFINITY || (mx - m_ref) * sc > kLazyLog2)) {
-                    if (m_ref != -INFINITY) alpha = ex2((m_ref - mx) * sc);
+                    if (m_ref != -INFINITY) alpha = ex2_approx((m_ref - mx) * sc);
                     m_ref = mx;
                 }
                 if (__any_sync(0xffffffffu, alpha != 1.f)) {
@@ -437,7 +416,7 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 e = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, mb2);
-                        const float2 pr = make_float2(ex2(e.x), ex2(e.y));
+                        const float2 pr = make_float2(ex2_approx(e.x), ex2_approx(e.y));
                         sum = add2(sum, pr);
                         packed[i >> 1] = pack_bf16(pr.x, pr.y);
                     }
@@ -487,8 +466,8 @@ shared_prefix_tc_kernel(const __grid_constant__ SharedKvMaps maps, const SharedP
                 if (join) {
                     const float2 b = s_ml[r];
                     const float top = fmaxf(m, b.x), ref = top == -INFINITY ? 0.f : top;
-                    mine = ex2(m - ref);
-                    other = ex2(b.x - ref);
+                    mine = ex2_approx(m - ref);
+                    other = ex2_approx(b.x - ref);
                     l = l * mine + b.y * other;
                     m = top;
                 }

@@ -144,11 +144,6 @@ __device__ __forceinline__ bool fp32_does(float top, float s) { return fabsf(top
 // A logit: a NaN as -inf, one kind of zero.
 __device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.f, -INFINITY); }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Two entries, a NaN as -inf.
 __device__ __forceinline__ uint32_t number_or_low(uint32_t w) {
     uint32_t low = 0xff80ff80u;
@@ -378,11 +373,8 @@ sampling_probs_kernel(const ProbsParams p) {
             __syncthreads();
             if (tid == 0) tell(&meet.listed[rank], C, from > -INFINITY ? s_listed : kList + 1);
             meet_all();
-            int total = 0, before = 0;
-            for (int i = 0; i < C; ++i) {
-                if (i < rank) before += min(meet.listed[i], kList + 1);
-                total += min(meet.listed[i], kList + 1);
-            }
+            int total = 0;
+            for (int i = 0; i < C; ++i) total += min(meet.listed[i], kList + 1);
             if (total <= kList) {
                 // Zeros everywhere, while the first CTA sorts all the lists.  (Every CTA sorting them: 64 rows of 128256 28.4 us, so 24.7; 320
                 // of 151936 79.3 and 76.6; but 6 of 32000 12.1 and 12.6.)
@@ -513,7 +505,7 @@ sampling_probs_kernel(const ProbsParams p) {
                 const uint32_t w[4] = {number_or_low(a.x), number_or_low(a.y), number_or_low(a.z), number_or_low(a.w)};
                 float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum += ex2(fmaf((e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]), s_hi, -at));
+                for (int e = 0; e < 8; ++e) sum += ex2_approx(fmaf((e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]), s_hi, -at));
                 if (top > -INFINITY) part += sum;
             },
             [&](float a, int) {
@@ -523,7 +515,7 @@ sampling_probs_kernel(const ProbsParams p) {
                     top = a;
                     at = now;
                 }
-                if (top > -INFINITY) part += ex2(fmaf(a, s_hi, -at));
+                if (top > -INFINITY) part += ex2_approx(fmaf(a, s_hi, -at));
             });
     }
     const float my_top = top;
@@ -584,7 +576,7 @@ sampling_probs_kernel(const ProbsParams p) {
     auto finish = [&](double kept, float bound, auto keeps) {
         if (plain) {
             const float factor = static_cast<float>(exp2(static_cast<double>(c) - static_cast<double>(xmax) * s_hi) / kept);
-            store_from(bound, [&](float a, int place) { return keeps(a, place) ? ex2(fmaf(a, s_hi, -c)) * factor : 0.f; });
+            store_from(bound, [&](float a, int place) { return keeps(a, place) ? ex2_approx(fmaf(a, s_hi, -c)) * factor : 0.f; });
         } else {
             store_from(bound, [&](float a, int place) { return keeps(a, place) ? static_cast<float>(weight64(a, xmax, per_t) / kept) : 0.f; });
         }

@@ -29,6 +29,23 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                  : "memory");
 }
+// Two fp32 operations per instruction, and the maximum of three.
+__device__ __forceinline__ uint64_t as_pair(float2 x) { return *reinterpret_cast<uint64_t*>(&x); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(as_pair(a)), "l"(as_pair(b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // One lane of a converged warp.  A role's whole issue loop goes behind one such test: the compiler then knows
 // the loop to be warp-uniform and forms the descriptors in uniform registers (44 against 62 cycles per
 // small MMA behind `lane == 0`).
