@@ -285,6 +285,44 @@ def test_shared_prefix_checks_its_arguments(L):
     assert torch.equal(attn.forward(q, 0, *index), good)
 
 
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_shared_prefix_most_heads(L, page, rows):
+    """Sixteen query heads on each of eight KV heads: the rows kernel's largest shared memory."""
+    s = SharedSetup([[(9, rows), (130, 1)], [(40, rows)]], [300, 0], page, 128, 8, seed=19)
+    assert_attention(s.run(L), *s.want())
+    assert L.read_device_status() == (0, 0)
+
+
+def test_shared_prefix_queries_of_any_strides(L):
+    """Heads outside, tokens inside; and rows that are part of wider ones, heads too."""
+    s = SharedSetup([[(20, 2), (30, 5), (9, 3)], [(700, 1)]], [140, 0], 16, 16, 8, seed=20)
+    want = s.want()
+    attn = L.SharedPrefixAttention(s.cache(L), 16, 8, D, s.q.shape[0], 4)
+    turned = s.q.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+    assert turned.stride(0) < turned.stride(1)
+    wide = torch.full((s.q.shape[0] + 1, 18, D + 8), float("nan"), dtype=bf16, device="cuda")
+    wide[1:, 1:17, 8:] = s.q.cuda()
+    for q in (turned, wide[1:, 1:17, 8:]):
+        assert_attention(s.run(L, attn, q=q), *want)
+
+
+def test_shared_prefix_calls_repeat_themselves(L):
+    """Which CTA does which item changes from call to call, the result does not."""
+    for groups, prefixes, heads, kv_heads in (([[(1 + 13 * i % 300, 1 + i % 4) for i in range(60)]], [3000], 32, 8),
+                                              ([[(1, 1), (900, 2)], [(5000, 1)]], [9000, 0], 8, 1)):
+        s = SharedSetup(groups, prefixes, 16, heads, kv_heads, seed=22)
+        attn = L.SharedPrefixAttention(s.cache(L), heads, kv_heads, D, s.q.shape[0], len(s.reqs))
+        q, index = s.q.cuda(), s.index(s.table, s.table_idx, s.lens, s.qo, s.group_indptr, s.prefixes)
+        other, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+        first = attn.forward(q, 0, *index)
+        for i in range(20):
+            if i % 3 == 1:   # other work holds some of the SMs
+                with torch.cuda.stream(other):
+                    torch.mm(busy, busy)
+            assert torch.equal(attn.forward(q, 0, *index), first)
+
+
 # ---- probabilities ----------------------------------------------------------------------------------------------
 
 def _logits(rows, vocab, seed, spread=2.0, step=0.0):
