@@ -298,8 +298,11 @@ B200_API int b200_attention_prefill(void* out, const void* q, int64_t q_stride_t
  * written; so are prefixes of 2^30 or more tiles (of 128 keys, 256 query rows and one KV head) in all.
  * bf16, head_dim 128, kv_heads 1, 2, 4 or 8, up to 16 query heads per KV head, up to 1024 requests; q 16-byte aligned, its
  * strides multiples of 8 elements.  For a few rows per request: thousands of rows of one prompt are b200_attention_prefill's.
- * workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests, not initialised; calls that share one
- * run one after another (so does the replay of graphs that captured them). */
+ * With one row each b200_attention_decode is faster (9 to 19 us against 11 to 22) as long as what it reads again stays below some 64 MB:
+ * the sum over groups of (requests - 1) * prefix * kv_heads * 512 bytes; at 1 KV head below some 40.
+ * workspace: b200_attention_shared_prefix_workspace_bytes for the most tokens and requests (38 MiB for 4 and 4 of 16 / 8 heads, 83 for
+ * 64 and 64 of 32 / 8, 382 for 1024 and 256), not initialised; calls that share one run one after another (so does the
+ * replay of graphs that captured them). */
 typedef struct b200_shared_prefix_args {
     void* out;
     const void* q;
@@ -358,7 +361,8 @@ B200_API int b200_sample_from_probs(int32_t* out, const float* probs, int rows, 
  * all), of those over the entries whose cumulative probability, their own included, stays within top_p[r] (never without
  * the largest; 1: all), zeros elsewhere.  A temperature of at most 1e-6 (or NaN) gives 1 at the first maximum.  top_k, top_p:
  * device arrays or NULL.  bf16 logits [rows, vocab] of row stride ld, fp32 out [rows, vocab] contiguous.  A NaN counts as
- * -inf; a row of nothing else becomes zeros.  Cuts are decided by 64-bit sums.  vocab up to 2^24. */
+ * -inf; a row of nothing else becomes zeros (at such a temperature: 1 at index 0).  Cuts are decided by 64-bit sums.  vocab up to
+ * 2^24. */
 B200_API int b200_sampling_probs(float* out, const void* logits, int64_t ld, int rows, int vocab,
                                  const float* temperatures, const int32_t* top_k, const float* top_p,
                                  b200_stream_t stream);
@@ -374,8 +378,8 @@ B200_API int b200_sampling_probs(float* out, const void* logits, int64_t ld, int
  * accepted and reported in the status words (-1 as -2^31).
  * tokens int32 [batch, max_drafts + 1]: the accepted drafts, the token behind them, then -1; accepted int32 [batch].  Of
  * more than max_drafts drafts the first max_drafts are looked at.  All probabilities fp32, rows target_ld and draft_ld
- * apart; uniform numbers fp32 in [0, 1).  total_drafts = draft_indptr[batch].  Decisions and sums in 64 bits, in a fixed
- * order. */
+ * apart; uniform numbers fp32 in [0, 1).  total_drafts = draft_indptr[batch].  Drafts are tested in 64 bits; sums are right to
+ * 1e-13, in a fixed order. */
 B200_API int b200_verify_drafts(int32_t* tokens, int32_t* accepted, const float* target_probs, int64_t target_ld,
                                 const float* draft_probs, int64_t draft_ld, const int32_t* draft_tokens,
                                 const int32_t* draft_indptr, const float* accept_uniform, const float* draw_uniform,

@@ -13,9 +13,9 @@
 // copies: 48 drafted requests behind 16001 keys 80 us, so 74.5).  A stage is 128 (key, KV head) rows of K and of V, copied by 3-D TMA
 // boxes of whole pages, a warp for each half of K and of V; eight warps each own 16 keys of one KV head in it and multiply with
 // mma.sync: S^T = K Q^T and O^T = V^T P^T, so that the rows are the products' short side (eight of them; with the rows on the long side a
-// step of one token and two heads per KV head filled 2 of 16).  64 KB of a stage take a CTA 0.8 to 1 us where all are at work
-// (1.05 the other way round), 1.2 to 1.4 with two eights of rows; 128 requests of 1 row with up to 2048 keys of their own behind 32768
-// shared ones: 668 MB in 141 us with the tensor-core kernel beside it, 0.72 of the copy bandwidth.
+// step of one token and two heads per KV head filled 2 of 16).  64 KB of a stage, with all CTAs at work, take one 1.07 us from L2 and
+// 1.39 us from memory (7.0 TB/s; copies 6.5), with two eights of rows 1.47; 128 requests of 1 row with up to 2048 keys of their own
+// behind 32768 shared ones: 668 MB in 142 us with the tensor-core kernel beside it, 0.72 of the copy bandwidth.
 //
 // Few launches, no wait between them that is not needed: the kernels are launched early (programmatic dependent launches), the
 // rows kernel does not wait for the tensor-core kernel, whose SMs its last CTAs take over, and the merge finds its parts ahead of

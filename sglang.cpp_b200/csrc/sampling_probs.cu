@@ -19,9 +19,14 @@
 //     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
 //                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
 //                      thread's patterns the cut falls.
-// Bound by HBM, 6 bytes per entry; the last kind also by the counting, an atomic per entry in shared memory.  CTAs of 256 threads, five
-// on an SM, so that one's loads and stores lie under another's sorting (320 rows of 151936 at top_p 0.9: 160 us with four, 141 with
-// five, 155 with six, whose registers do not suffice).
+// What bounds it: no filter, HBM (512 rows of 128256, 6 bytes per entry: 85 us, 0.71 of the copy bandwidth; second reads are L2's).
+// The others wait for one another's meetings, sorts and counts, an atomic per entry in shared memory (320 rows of 151936: 65 us
+// without filters, 77 with top_k 40, 133 to 138 with top_p 0.9; DRAM at 31 percent with all kinds mixed).  CTAs of 256 threads, five on an
+// SM, so that one's loads and stores lie under another's sorting (at top_p 0.9 160 us with four, 141 with five, 155 with six,
+// whose registers do not suffice).
+// Far from these: a mask that leaves fewer entries than top_k, whose border is found by bisection (20 of 151936, top_k 40: 320 rows 710
+// us, with top_p 1730; 8 rows 123 and 384); rows of an odd length, read 2 and written 4 bytes at a time (320 of 151935: 123 us
+// without filters, 124 with top_k 40, 171 with top_p).
 #include <type_traits>
 
 #include "common.cuh"
@@ -593,7 +598,7 @@ sampling_probs_kernel(const ProbsParams p) {
     if constexpr (FILTERS) {
         // ---- entries that are not counted ----
         double out_sum[kClasses] = {0.0, 0.0, 0.0};
-        if (outside) {   // (a round of its own: one row in hundreds has any)
+        if (outside) {   // (a round of its own: one row in hundreds has any, but every one with a mask: 320 rows at top_p 0.9 133 us, so 164)
             int out_count[kClasses] = {0, 0, 0};
             each([&](const auto& y, auto count, int) {
 #pragma unroll

@@ -6,8 +6,9 @@
 // from the target's own distribution.  The draw is the inverse of the summed probabilities in index order: the first index whose
 // running sum exceeds u * (sum of all).
 //
-// Everything is decided in fp64: a product of two fp32 numbers is exact there, and a sum of a row's is right to 1e-13 or so, so
-// that a border is missed by no more than that.  Sums are formed in a fixed order: equal calls, equal tokens.
+// Drafts are tested in fp64, where a product of two fp32 numbers is exact.  A row's sum is right to 1e-13 or so (fp64, but for what the
+// rounding of sixteen differences left out, which is added up in fp32: 2^-45 of them), so that a border is missed by no more
+// than that.  Sums are formed in a fixed order: equal calls, equal tokens.
 //
 // Bound by HBM: one row of p, and one of q where a draft was refused, 8 bytes per vocabulary entry and request, read once; the
 // other rows are looked at in one place each.  A cluster of CTAs shares a row: every warp sums a run of consecutive entries in
