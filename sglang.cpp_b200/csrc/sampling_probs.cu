@@ -11,7 +11,7 @@
 // them; the few entries outside are added up one by one in fp64, by class (above, between, below).  Where a border falls among those
 // it is found by bisection of the patterns instead, 16 rounds of counts or sums over the whole row.
 //
-// A CTA, or where rows are few a cluster of them, owns a row and goes over it from memory once and from L2 once or twice more.
+// A CTA, or where rows are few a cluster of them, owns a row and goes over it from memory once and once or twice more, mostly from L2.
 //     no filter:       sums under a running maximum; results.
 //     top_k <= 256:    the lanes' maxima; of every warp's 32 the r-th largest, r = ceil(top_k / warps of the row): the smallest of these
 //                      has top_k entries at or above it.  All such entries (some hundreds) are listed, from the threads whose maximum
@@ -19,7 +19,8 @@
 //     other filters:   maximum and counts; results.  In a cluster the counters meet by ranges of patterns: CTA r adds up all CTAs'
 //                      counts of the r-th range from the top, weighs them, and the sums of the ranges before decide in which
 //                      thread's patterns the cut falls.
-// What bounds it: no filter, HBM (512 rows of 128256, 6 bytes per entry: 85 us, 0.71 of the copy bandwidth; second reads are L2's).
+// What bounds it: no filter, HBM (512 rows of 128256, 6 bytes per entry: 85 us, 0.71 of the copy bandwidth; of the 131 MB
+// that are read twice, 82 come from memory again).
 // The others wait for one another's meetings, sorts and counts, an atomic per entry in shared memory (320 rows of 151936: 65 us
 // without filters, 77 with top_k 40, 133 to 138 with top_p 0.9; DRAM at 31 percent with all kinds mixed).  CTAs of 256 threads, five on an
 // SM, so that one's loads and stores lie under another's sorting (at top_p 0.9 160 us with four, 141 with five, 155 with six,
