@@ -264,7 +264,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k,
             tc_commit(smem_u32(&pv_full));
             tc_commit(smem_u32(&v_empty[slot]));
         };
-        const int in_page = kv_end & (p.kpc - 1);
+        const int in_page = max(kv_end, 0) & (p.kpc - 1);
         const int clean = in_page != 0 ? ntiles - 1 : ntiles;   // tiles whose last page ends with them
         if (lane == 0) {
             issue_s(0);

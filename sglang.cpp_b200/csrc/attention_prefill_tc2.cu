@@ -343,7 +343,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ KvMaps maps, const PrefillT
         // Behind the last key the last page holds whatever was there before: as values, these have to be numbers for their weights of 0.
         // The whole warp clears them while the last tile's softmax runs.  (The softmax warps themselves: spills in their loop, 1024
         // tokens of 16 heads 19.9 -> 20.4 us; V's producer, which handed the tile on behind its copies: 21.8.)
-        const int in_page = kv_end & (p.kpc - 1);
+        const int in_page = max(kv_end, 0) & (p.kpc - 1);
         uint32_t slot = kKSlots, phase = 0;
         bool failed = false;
         auto add_tiles = [&](int begin, int end) {
