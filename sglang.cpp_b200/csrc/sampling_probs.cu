@@ -498,12 +498,14 @@ sampling_probs_kernel(const ProbsParams p) {
     } else if (greedy) {
         top = largest();
     } else {
-        // 2^(y s - at), at = s times the maximum so far
+        // 2^(y s - at), at = s times the maximum so far.  Where that is below -2^30 there is nothing but a mask's low numbers so far, which
+        // are nothing beside a maximum that fp32 does for: as its own reference at would be off by more than an exponent's range.
+        constexpr float kLowest = -1073741824.f;
         all_of(
             [&](const uint4& a, int) {
                 const float here = largest_of(a);
                 if (here > top) {
-                    const float now = fmaxf(here * s_hi, -3.402823466e38f);   // (nothing but a mask's lowest numbers so far)
+                    const float now = fmaxf(here * s_hi, kLowest);
                     part *= exp2f(at - now);   // (the first time: nothing)
                     top = here;
                     at = now;
@@ -516,7 +518,7 @@ sampling_probs_kernel(const ProbsParams p) {
             },
             [&](float a, int) {
                 if (a > top) {
-                    const float now = fmaxf(a * s_hi, -3.402823466e38f);
+                    const float now = fmaxf(a * s_hi, kLowest);
                     part *= exp2f(at - now);
                     top = a;
                     at = now;

@@ -412,6 +412,21 @@ def test_sampling_probs_masked_vocabulary(L, vocab):
             assert_probs(got, want)
 
 
+@pytest.mark.parametrize("vocab", [70, 430, 9000, 9001, 70000])
+@pytest.mark.parametrize("mask", [-3.3895313892515355e38, -3e33, -1e30, -1e12, -1e10, -5e9, -1e8])
+def test_sampling_probs_masked_by_low_numbers_at_any_temperature(L, vocab, mask):
+    """Stretches of low numbers ahead of the row's largest, whose scaled values are far from any fp32 exponent; some rows all of
+    them."""
+    t = [1.0, 1.2, 1.45, 1.5, 1.6, 1.7, 1.9, 2.0, 2.5, 3.0, 5.0, 10.0, 33.0, 1e3, 1e4, 3e5, 0.7, 2e-6]
+    x = _logits(len(t), vocab, vocab)
+    x[:, :-vocab // 40] = mask
+    x[::5] = mask
+    x[1::5, vocab // 2] = 3.0
+    want = probs_oracle(x, np.asarray(t, np.float32))
+    assert_probs(L.sampling_probs(x.cuda(), _f32(t)), want)
+    assert_probs(L.sampling_probs(x.cuda(), _f32(t), _i32([0] * len(t)), _f32([1.0] * len(t))), want)
+
+
 def test_sampling_probs_is_what_sample_draws_from(L):
     """The kept set is b200_sample's candidate set (rows whose border is not within its 40-bit sums' reach)."""
     rows, vocab = 32, 32000
