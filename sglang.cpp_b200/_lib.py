@@ -96,6 +96,12 @@ PROTOTYPES: dict[str, tuple] = {
     "b200_verify_drafts": (_I, [_P, _P, _P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "b200_attention_shared_prefix_workspace_bytes": (_L, [_I, _I, _I, _I, _I]),
     "b200_attention_shared_prefix": (_I, [_P, _P]),
+    "b200_attention_prompt": (_I, [_P, _P]),
+    "b200_pages_workspace_bytes": (_L, [_I]),
+    "b200_copy_pages": (_I, [_P, _P, _P, _P, _I, _P, _L, _P]),
+    "b200_fork_rows": (_I, [_P, _P, _L, _L, _L, _P, _P, _P, _P, _I, _P]),
+    "b200_count_pages": (_I, [_P, _P, _P, _P, _L, _L, _L, _P, _P, _I, _P, _I, _I, _I, _P, _L, _P]),
+    "b200_compact_pages": (_I, [_P, _P, _L, _P, _P, _P, _L, _L, _L, _P, _P, _I, _P, _I, _P, _L, _P]),
     "b200_comm_create": (_I, [_I, _I, _L, POINTER(c_void_p)]),
     "b200_comm_handle_bytes": (_I, []),
     "b200_comm_export": (_I, [_P, _P]),
@@ -236,6 +242,24 @@ class SharedPrefixArgs(ctypes.Structure):
         ("group_indptr", _P), ("prefix_lens", _P), ("tokens", c_int32), ("batch", c_int32), ("groups", c_int32),
         ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("page_size", c_int32), ("sm_scale", c_float),
         ("workspace", _P), ("workspace_bytes", _L),
+    ]
+
+
+class PromptAttentionArgs(ctypes.Structure):
+    """b200_prompt_attention_args."""
+    _fields_ = [
+        ("out", _P), ("lse", _P), ("q", _P), ("k", _P), ("v", _P), ("q_stride_token", _L), ("q_stride_head", _L),
+        ("k_stride_token", _L), ("k_stride_head", _L), ("v_stride_token", _L), ("v_stride_head", _L), ("indptr", _P),
+        ("tokens", c_int32), ("batch", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+        ("sm_scale", c_float),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    """b200_page_pool."""
+    _fields_ = [
+        ("planes", _P), ("plane_stride", _L), ("num_planes", c_int32), ("slot_bytes", c_int32), ("page_size", c_int32),
+        ("num_pages", c_int32),
     ]
 
 

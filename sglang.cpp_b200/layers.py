@@ -297,6 +297,85 @@ class MHAKVCache:
              k.stride(0), v.stride(0), self.total_slots, _stream())
 
 
+# --------------------------------------------------------------------------- pages
+class CachePages:
+    """Pages of a KV cache copied, shared, counted and moved (the reference's pages are shared by its prefix cache only and never
+    move).  ``pages``: how many of the cache's pages take part, the first ones (a dummy request's page behind them does not).
+    Page numbers, rows and lengths are int32 tensors on the cache's device.  One object's calls run one after another (they share its
+    workspace): use an object per stream, and per captured graph that may be replayed beside another."""
+
+    def __init__(self, kv_cache: MHAKVCache, pages: Optional[int] = None):
+        self.kv_cache_ = kv_cache
+        self.pages_ = kv_cache.num_pages_ if pages is None else pages
+        _check(0 < self.pages_ <= kv_cache.num_pages_, "no such number of pages in the cache")
+        buf = kv_cache.kv_buffer_
+        self.device_ = buf.get_device()
+        _check(self.device_ >= 0, "the cache must be on a CUDA device")
+        slot = kv_cache.kv_heads_ * kv_cache.head_dim_ * buf.element_size()
+        self.pool_ = _lib.PagePool(buf.data_ptr(), kv_cache.total_slots * slot, 2 * kv_cache.num_layers_, slot, kv_cache.page_size_,
+                                   self.pages_)
+        self.pool_ref_ = ctypes.byref(self.pool_)
+        nbytes = _lib.load().b200_pages_workspace_bytes(self.pages_)
+        _check(nbytes > 0, "no such number of pages")
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=buf.device)
+
+    def _index(self, name: str, t: torch.Tensor, count: int = -1) -> int:
+        if t.get_device() != self.device_ or t.dtype is not torch.int32 or t.dim() != 1 or (t.size(0) > 1 and t.stride(0) != 1):
+            _fail(f"{name} must be a contiguous int32 tensor of rank 1 on the device of the cache")
+        if 0 <= count != t.size(0):
+            _fail(f"{name} must have {count} numbers")
+        return t.data_ptr()
+
+    def _table(self, name: str, t: torch.Tensor) -> None:
+        if t.get_device() != self.device_ or t.dtype is not torch.int32 or t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1):
+            _fail(f"{name} must be int32 of rank 2 with contiguous rows on the device of the cache")
+
+    def copy(self, src: torch.Tensor, dst: torch.Tensor, tokens: Optional[torch.Tensor] = None) -> None:
+        """Page src[i] (or the first tokens[i] slots of it) to page dst[i] in every layer; a negative page: nothing."""
+        n = src.numel()
+        _launch(self.device_, "b200_copy_pages", self.pool_ref_, self._index("src", src), self._index("dst", dst, n),
+                None if tokens is None else self._index("tokens", tokens, n), n, self.workspace.data_ptr(), self.workspace.numel())
+
+    def fork(self, page_table: torch.Tensor, parents: torch.Tensor, children: torch.Tensor, lens: torch.Tensor,
+             new_pages: torch.Tensor) -> None:
+        """Row children[i] of the page table goes on from the first lens[i] positions of row parents[i]: whole pages are shared, the
+        tokens of a last part page are copied to page new_pages[i]."""
+        n = parents.numel()
+        self._table("page_table", page_table)
+        _launch(self.device_, "b200_fork_rows", self.pool_ref_, page_table.data_ptr(), page_table.size(0), _row_stride(page_table),
+                page_table.size(1), self._index("parents", parents), self._index("children", children, n), self._index("lens", lens, n),
+                self._index("new_pages", new_pages, n), n)
+
+    def count(self, page_table: torch.Tensor, rows: torch.Tensor, lens: torch.Tensor, held: Optional[torch.Tensor] = None):
+        """(refs [pages]: how many of the rows, and of ``held``, hold each page; the free pages in ascending order, then -1 [pages]; their
+        number [1])."""
+        n = rows.numel()
+        self._table("page_table", page_table)
+        refs, free, number = torch.empty(2 * self.pages_ + 1, dtype=torch.int32, device=page_table.device).split((self.pages_, self.pages_, 1))
+        _launch(self.device_, "b200_count_pages", refs.data_ptr(), free.data_ptr(), number.data_ptr(), page_table.data_ptr(),
+                page_table.size(0), _row_stride(page_table), page_table.size(1), self._index("rows", rows), self._index("lens", lens, n), n,
+                None if held is None else self._index("held", held), 0 if held is None else held.numel(), self.pool_.page_size, self.pages_,
+                self.workspace.data_ptr(), self.workspace.numel())
+        return refs, free, number
+
+    def compact(self, page_table: torch.Tensor, rows: torch.Tensor, lens: torch.Tensor, held: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None):
+        """Moves the pages that the rows and ``held`` name to the front of the pool and renames them in the rows of ``out`` (the page
+        table itself where None).  Returns (map [pages]: where each page is now, -1 for free ones; how many are in use [1])."""
+        n = rows.numel()
+        self._table("page_table", page_table)
+        if out is None:
+            out = page_table
+        self._table("out", out)
+        _check(out.shape == page_table.shape, "out must have the shape of page_table")
+        where, used = torch.empty(self.pages_ + 1, dtype=torch.int32, device=page_table.device).split((self.pages_, 1))
+        _launch(self.device_, "b200_compact_pages", self.pool_ref_, out.data_ptr(), _row_stride(out), where.data_ptr(), used.data_ptr(),
+                page_table.data_ptr(), page_table.size(0), _row_stride(page_table), page_table.size(1), self._index("rows", rows),
+                self._index("lens", lens, n), n, None if held is None else self._index("held", held), 0 if held is None else held.numel(),
+                self.workspace.data_ptr(), self.workspace.numel())
+        return where, used
+
+
 # --------------------------------------------------------------------------- attention
 class PagedAttention:
     """Stands where FlashInferBackend::forward does (src/attention/flashinfer_backend.cu:522-682),
@@ -404,6 +483,39 @@ class SharedPrefixAttention:
         args.tokens, args.batch, args.groups, args.sm_scale = tokens, batch, groups, self.sm_scale
         _launch(dev, "b200_attention_shared_prefix", self.args_ref_)
         return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indptr: torch.Tensor, sm_scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Causal attention over whole prompts that lie behind one another, without a cache (b200_attention_prompt): sequence s is rows
+    [indptr[s], indptr[s + 1]) of q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], which may be columns of wider rows.
+    Returns [tokens, q_heads * head_dim], with return_lse also the logarithms of the rows' sums, float32 [tokens, q_heads].  Rows that
+    no sequence owns are not written."""
+    dev = q.get_device()
+    if dev < 0 or q.dtype is not bf16 or q.dim() != 3:
+        _fail("q must be a CUDA tensor of bfloat16 [tokens, q_heads, head_dim]")
+    tokens, heads, dim = q.shape
+    for name, t in (("k", k), ("v", v)):
+        if t.get_device() != dev or t.dtype is not bf16 or t.dim() != 3 or t.size(0) != tokens or t.size(2) != dim or t.size(1) != k.size(1):
+            _fail(f"{name} must be bfloat16 [tokens, kv_heads, head_dim] on the device of q")
+    if dim > 1 and not q.stride(2) == k.stride(2) == v.stride(2) == 1:
+        _fail("the last dimensions of q, k and v must be contiguous")
+    if indptr.get_device() != dev or indptr.dtype is not torch.int32 or indptr.dim() != 1 or indptr.numel() < 1 or not indptr.is_contiguous():
+        _fail("indptr must be contiguous int32 [sequences + 1] on the device of q")
+    if out is None:
+        out = torch.empty(tokens, heads * dim, dtype=bf16, device=q.device)
+    elif out.get_device() != dev or out.dtype is not bf16 or tuple(out.shape) != (tokens, heads * dim) or not out.is_contiguous():
+        _fail("out must be contiguous bfloat16 [tokens, q_heads * head_dim] on the device of q")
+    lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
+
+    def strides(t):   # (those of a dimension of one say nothing)
+        return t.stride(0) if t.size(0) > 1 else t.size(1) * dim, t.stride(1) if t.size(1) > 1 else dim
+
+    args = _lib.PromptAttentionArgs(
+        out.data_ptr(), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides(q), *strides(k), *strides(v), indptr.data_ptr(),
+        tokens, indptr.numel() - 1, heads, k.size(1), dim, 1.0 / math.sqrt(dim) if sm_scale is None else sm_scale)
+    _launch(dev, "b200_attention_prompt", ctypes.byref(args))
+    return (out, lse) if return_lse else out
 
 
 def qknorm_rope_store(qkv: torch.Tensor, q_norm: Optional[RMSNorm], k_norm: Optional[RMSNorm],

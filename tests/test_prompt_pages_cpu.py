@@ -1,0 +1,139 @@
+"""What attention over whole prompts and the operators on cache pages refuse (checked before any CUDA call), and their plain forms on cases
+worked out by hand."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.prompt_pages_cases import PromptSetup, compact_oracle, copy_oracle, count_oracle, fork_oracle
+
+P = ctypes.c_void_p(256)   # never dereferenced: the calls below are refused
+
+
+def _prompt(pkg, **change):
+    from sglang_cpp_b200 import _lib
+    a = dict(out=256, lse=None, q=256, k=256, v=256, q_stride_token=4096, q_stride_head=128, k_stride_token=4096, k_stride_head=128,
+             v_stride_token=4096, v_stride_head=128, indptr=256, tokens=9, batch=2, q_heads=16, kv_heads=8, head_dim=128, sm_scale=0.1)
+    a.update(change)
+    lib = pkg.load_library()
+    rc = lib.b200_attention_prompt(ctypes.byref(_lib.PromptAttentionArgs(**a)), None)
+    return rc, lib.b200_last_error().decode()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(head_dim=136), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(head_dim=60), "head_dim"), (dict(batch=1025), "batch"),
+    (dict(batch=-1), "batch"), (dict(tokens=-1), "tokens"), (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=3), "q_heads"), (dict(q_heads=0), "q_heads"),
+    (dict(q_heads=129, kv_heads=1), "q_heads"), (dict(q_stride_token=4100), "strides"), (dict(q_stride_head=0), "strides"),
+    (dict(k_stride_token=-4096), "strides"), (dict(k_stride_head=4), "strides"), (dict(v_stride_token=1 << 40), "strides"), (dict(v_stride_head=129), "strides"),
+    (dict(sm_scale=0.0), "sm_scale"), (dict(sm_scale=-1.0), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"), (dict(sm_scale=float("inf")), "sm_scale"),
+    (dict(tokens=1 << 28), "too many"), (dict(out=None), "NULL"), (dict(q=None), "NULL"), (dict(k=None), "NULL"), (dict(v=None), "NULL"),
+    (dict(indptr=None), "NULL"), (dict(out=264), "aligned"), (dict(q=264), "aligned"), (dict(k=258), "aligned"), (dict(v=260), "aligned"),
+])
+def test_prompt_attention_refusals(pkg, change, text):
+    rc, said = _prompt(pkg, **change)
+    assert rc == 1 and text in said, (rc, said)
+
+
+def test_prompt_attention_null_arguments_and_nothing_to_do(pkg):
+    assert pkg.load_library().b200_attention_prompt(None, None) == 1
+    assert _prompt(pkg, batch=0)[0] == 0
+    assert _prompt(pkg, tokens=0)[0] == 0
+
+
+POOL = dict(planes=256, plane_stride=1 << 20, num_planes=4, slot_bytes=256, page_size=16, num_pages=64)
+
+
+def _pool(**change):
+    from sglang_cpp_b200 import _lib
+    return ctypes.byref(_lib.PagePool(**{**POOL, **change}))
+
+
+def _calls(lib, pool, **change):
+    """Each of the calls on a pool, with arguments that it would take."""
+    a = dict(src=P, dst=P, tokens=None, copies=4, table=P, rows=8, stride=128, cols=100, parents=P, children=P, lens=P, new=P, count=4, which=P,
+             held=None, held_count=0, out=P, out_stride=128, map=P, used=P, refs=P, free=P, free_count=P, page_size=16, num_pages=64, ws=P,
+             ws_bytes=1 << 20)
+    a.update(change)
+    g = lambda names: [a[n] for n in names.split()]
+    return {
+        "copy": lambda: lib.b200_copy_pages(pool, *g("src dst tokens copies ws ws_bytes"), None),
+        "fork": lambda: lib.b200_fork_rows(pool, *g("table rows stride cols parents children lens new count"), None),
+        "count": lambda: lib.b200_count_pages(*g("refs free free_count table rows stride cols which lens count held held_count page_size num_pages ws ws_bytes"), None),
+        "compact": lambda: lib.b200_compact_pages(pool, *g("out out_stride map used table rows stride cols which lens count held held_count ws ws_bytes"), None),
+    }
+
+
+@pytest.mark.parametrize("call", ["copy", "fork", "compact"])
+@pytest.mark.parametrize("change,text", [
+    (dict(planes=None), "planes"), (dict(planes=264), "aligned"), (dict(plane_stride=(1 << 20) + 8), "plane_stride"), (dict(plane_stride=16 * 64 * 256 - 16), "plane_stride"),
+    (dict(num_planes=0), "num_planes"), (dict(num_planes=1 << 26), "num_planes"), (dict(slot_bytes=0), "slot_bytes"), (dict(slot_bytes=24), "slot_bytes"),
+    (dict(page_size=0), "page_size"), (dict(num_pages=0), "num_pages"), (dict(page_size=1 << 26), "2^31"),
+])
+def test_pool_refusals(pkg, call, change, text):
+    lib = pkg.load_library()
+    assert _calls(lib, _pool(**change))[call]() == 1 and text in lib.b200_last_error().decode()
+    assert _calls(lib, None)[call]() == 1 and "NULL pool" in lib.b200_last_error().decode()
+
+
+@pytest.mark.parametrize("call,change,text", [
+    ("copy", dict(copies=-1), "count"), ("copy", dict(copies=65), "count"), ("copy", dict(src=None), "NULL"), ("copy", dict(dst=None), "NULL"),
+    ("copy", dict(ws=None), "workspace"), ("copy", dict(ws_bytes=100), "workspace"),
+    ("fork", dict(count=-1), "count"), ("fork", dict(count=1025), "count"), ("fork", dict(table=None), "NULL"), ("fork", dict(parents=None), "NULL"),
+    ("fork", dict(children=None), "NULL"), ("fork", dict(lens=None), "NULL"), ("fork", dict(new=None), "NULL"), ("fork", dict(stride=99), "overlap"),
+    ("fork", dict(rows=-1), "table"), ("fork", dict(cols=-1), "table"), ("fork", dict(cols=1 << 31, stride=1 << 31), "table"),
+    ("count", dict(refs=None), "NULL"), ("count", dict(free=None), "NULL"), ("count", dict(free_count=None), "NULL"), ("count", dict(table=None), "NULL"),
+    ("count", dict(which=None), "NULL"), ("count", dict(lens=None), "NULL"), ("count", dict(count=-1), "count"), ("count", dict(held_count=-1), "count"),
+    ("count", dict(held_count=3), "NULL"), ("count", dict(page_size=0), "page_size"), ("count", dict(num_pages=0), "num_pages"),
+    ("count", dict(num_pages=1 << 28), "2^31"), ("count", dict(ws=None), "workspace"), ("count", dict(ws_bytes=64), "workspace"), ("count", dict(stride=50), "overlap"),
+    ("compact", dict(map=None), "NULL"), ("compact", dict(used=None), "NULL"), ("compact", dict(out=None), "NULL"), ("compact", dict(out_stride=99), "overlap"),
+    ("compact", dict(table=None), "NULL"), ("compact", dict(which=None), "NULL"), ("compact", dict(lens=None), "NULL"), ("compact", dict(count=-1), "count"),
+    ("compact", dict(held_count=2), "NULL"), ("compact", dict(ws=None), "workspace"), ("compact", dict(ws_bytes=512), "workspace"),
+])
+def test_page_refusals(pkg, call, change, text):
+    lib = pkg.load_library()
+    assert _calls(lib, _pool(), **change)[call]() == 1 and text in lib.b200_last_error().decode(), lib.b200_last_error()
+
+
+def test_page_calls_of_nothing(pkg):
+    lib = pkg.load_library()
+    assert _calls(lib, _pool(), copies=0, src=None, dst=None)["copy"]() == 0
+    assert _calls(lib, _pool(), count=0, parents=None, children=None)["fork"]() == 0
+
+
+def test_pages_workspace_sizes(pkg):
+    size = pkg.load_library().b200_pages_workspace_bytes
+    assert size(1) > 0 and size(0) == -1 and size(-5) == -1
+    sizes = [size(n) for n in (1, 31, 32, 33, 1000, 1 << 20)]
+    assert sizes == sorted(sizes) and size(1 << 20) < 32 << 20
+
+
+def test_oracles_on_known_answers():
+    s = PromptSetup([1, 2], 2, 1, 8, seed=1)
+    out, size, lse, _ = s.want()
+    q, k, v = (x.double() for x in s.parts(s.rows))
+    assert torch.allclose(out[0], v[0].expand(2, 8)) and torch.allclose(lse[0], (q[0] * k[0]).sum(-1) / math.sqrt(8))
+    assert torch.allclose(out[1], v[1].expand(2, 8))
+    a, b = ((q[2] * k[j]).sum(-1) / math.sqrt(8) for j in (1, 2))
+    w = torch.sigmoid(a - b)[:, None]
+    assert torch.allclose(out[2], w * v[1] + (1 - w) * v[2]) and torch.allclose(lse[2], torch.logaddexp(a, b))
+
+    kv = torch.arange(12).reshape(1, 1, 12, 1, 1).expand(2, 1, 12, 1, 1).clone()
+    # page 0 -> 2; 1 -> 3 twice named; 4 -> 5 whose page is read by the last pair, which writes page 1 (read by the second and third)
+    got, left = copy_oracle(kv, 2, 6, [0, 1, 1, 4, 5, -1, 7], [2, 3, 3, 5, 1, 0, 0])
+    assert got[0, 0, :, 0, 0].tolist() == [0, 1, 2, 3, 0, 1, 6, 7, 8, 9, 10, 11] and left == {3, 5, 1}
+    got, left = copy_oracle(kv, 2, 6, [0, 1], [2, 3], [1, 0])
+    assert got[0, 0, :, 0, 0].tolist() == [0, 1, 2, 3, 0, 5, 6, 7, 8, 9, 10, 11] and not left
+
+    table = np.full((4, 6), -1, np.int32)
+    table[0, :4] = [4, 5, 0, 1]                    # pages 2 and 0
+    got, t, left = fork_oracle(kv, table, 2, 6, [0, 0], [1, 3], [3, 2], [4, 9])
+    assert t[1].tolist() == [4, 5, 8, 9, -1, -1] and t[3].tolist() == [4, 5, -1, -1, -1, -1] and not left
+    assert got[0, 0, 8:10, 0, 0].tolist() == [0, 9]
+
+    refs, free, n = count_oracle(t, [0, 1, 3], [4, 3, 1], 2, 6, held=[5, 0])
+    assert refs.tolist() == [2, 0, 3, 0, 1, 1] and free.tolist() == [1, 3, -1, -1, -1, -1] and n == 2
+    got, t2, where, used = compact_oracle(got, t, [0, 1, 3], [4, 3, 1], 2, 6, held=[5, 0])
+    assert used == 4 and where.tolist() == [0, -1, 2, -1, 1, 3]
+    assert t2[1].tolist() == [4, 5, 2, 3, -1, -1] and got[0, 0, 2:4, 0, 0].tolist() == [0, 9] and got[0, 0, 6:8, 0, 0].tolist() == [10, 11]
