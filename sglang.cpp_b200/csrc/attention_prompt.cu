@@ -17,11 +17,9 @@
 // items and fetches Q and K, warp 2 V, one thread of warp 1 issues S, one of warp 3 P V, warps 4-7 and 8-11 are the softmax of the two tiles.
 // Each goes on to its next item by itself, so that an item's output is written while the next one's first products run.
 //
-// Keys behind a row are masked as scores; as values they meet weights of 0, which is right for numbers only.  Warp 2 therefore looks
-// through the tiles that some row of the item does not see in full: rows behind the sequence become zeros, and an infinity or NaN
-// becomes 0 and is added in the end to the rows that see it.
-#include <type_traits>
-
+// Keys behind a row are masked as scores; as values they meet weights of 0, which is right for numbers only.  Rows behind a sequence
+// become zeros in shared memory; where a row's result is no number, values that it does not see are looked through, and if one is to
+// blame the row is summed up once more without them.
 #include "common.cuh"
 #include "kernels.h"
 #include "tcgen05.cuh"
@@ -32,14 +30,14 @@ namespace {
 
 constexpr int kMaxDim = 128, kMaxBatch = 1024, kMaxGroup = 128;
 constexpr int kTile = 128;                  // keys per K/V tile and rows per query tile
-constexpr int kThreads = 384;
-// The first warpgroup leaves its registers to the others; 384 x 168 are launched.
-constexpr int kIssueRegs = 72, kSoftmaxRegs = 216;
-static_assert(128 * (kIssueRegs + 2 * kSoftmaxRegs) <= kThreads * 168, "");
+constexpr int kThreads = 512;               // warpgroups: copies and issue, softmax of either query tile, output
+// The first and the last one leave registers to the others; 512 x 128 are launched.
+constexpr int kFewRegs = 64, kSoftmaxRegs = 192;
+static_assert(128 * (2 * kFewRegs + 2 * kSoftmaxRegs) <= kThreads * 128, "");
 constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16 under the 128-byte swizzle
-constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns at a time
-constexpr float kLazyLog2 = 8.0f;           // the reference maximum moves when the true one is 2^8 ahead
-constexpr int kOddTiles = 2;                // K/V tiles of an item that some of its rows do not see in full
+constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns
+constexpr int kAgain = 2048;                // query tiles of a CTA that are noted one by one
+constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more
 
 // Sizes by the padded head dimension.
 template <int DP>
@@ -49,17 +47,43 @@ struct Shape {
     static constexpr uint32_t kSlotBytes = kHalves * kAtomBytes;
     static constexpr uint32_t kQOff = 0, kKOff = 2 * kSlotBytes, kVOff = kKOff + kKSlots * kSlotBytes;
     static constexpr uint32_t kStageOff = kVOff + kVSlots * kSlotBytes;
-    static constexpr uint32_t kSmemBytes = kStageOff + 8 * kStageBytes;
+    static constexpr uint32_t kSmemBytes = kStageOff + 4 * kStageBytes;
     // TMEM columns: S (128, of both tiles in turn where O takes 256), P0, P1 (64 each), O0, O1
     static constexpr bool kSharedS = DP == 128;
     static constexpr uint32_t kColS1 = kSharedS ? 0 : 128, kColP = kSharedS ? 128 : 256, kColO = kColP + 128;
 };
 
+// A wait for the phase of that parity in few instructions (the kernel has some thirty, and its roles share the SM's small instruction caches):
+// the hardware sleeps up to a microsecond per test, and the tests are counted.  False: reported, and nothing more is waited for.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* status, int site) {
+    const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
+    for (int i = 0; i < (1 << 21); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity & 1u)
+            : "memory");
+        if (done) return true;
+    }
+    atomicExch(&status[kStatusTimeout], site);
+    return false;
+}
+// The same for a whole warp whose lanes go on together.
+__device__ __forceinline__ bool wait_phase_warp(uint64_t* bar, uint32_t parity, int* status, int site) {
+    return __all_sync(0xffffffffu, wait_phase(bar, parity, status, site)) != 0;
+}
+
 struct PromptParams {
     __nv_bfloat16* out;
     float* lse;
-    const __nv_bfloat16* v;
-    int64_t v_st, v_sh;
+    const __nv_bfloat16 *q, *k, *v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
     const int32_t* indptr;
     int tokens, batch, q_heads, kv_heads, dim;
     int group, group_inverse;   // 65536 / group, rounded up: r / group = r * group_inverse >> 16 for r <= 128
@@ -76,23 +100,146 @@ struct Item {
     int first, len;       // row and length of the sequence (len < 0: no more items)
     int t0, head;         // first query token in it, KV head
     int tiles[2];         // K/V tiles of each query tile (0: it has no rows)
+    int keys[2];          // keys of its last one that some row sees, to a multiple of 16
+    // keys of tile kt that are multiplied with values
+    __device__ __forceinline__ int reach(int kt) const {
+        return max(kt + 1 < tiles[0] ? kTile : kt + 1 == tiles[0] ? keys[0] : 0, kt + 1 < tiles[1] ? kTile : kt + 1 == tiles[1] ? keys[1] : 0);
+    }
 };
+
+// The items of a CTA in turn.  Those of one KV head in order: blocks that are far down their sequences first; the CTAs take them one after another,
+// in turns that change direction, so that each gets long ones and short ones.  A whole warp calls.
+struct Walk {
+    const int *indptr, *blocks;
+    int batch, kv_heads, span, half, total, ctas, me;
+    int place, above, upto;       // at_least(place + 1), at_least(place): items only come nearer to the beginnings
+
+    // items of a KV head whose block is the j-th of its sequence or a later one
+    __device__ __forceinline__ int at_least(int j) const {
+        int n = 0;
+#pragma unroll 1
+        for (int s = threadIdx.x & 31; s < batch; s += 32) n += max(blocks[s] - j, 0);
+        return __reduce_add_sync(0xffffffffu, n);
+    }
+    __device__ __forceinline__ Walk(const PromptParams& p, const int* indptr_, const int* blocks_, int half_)
+        : indptr(indptr_), blocks(blocks_), batch(p.batch), kv_heads(p.kv_heads), span(p.span), half(half_), ctas(gridDim.x), me(blockIdx.x) {
+        int most = 0;
+#pragma unroll 1
+        for (int s = threadIdx.x & 31; s < batch; s += 32) most = max(most, blocks[s]);
+        place = __reduce_max_sync(0xffffffffu, most);
+        above = upto = 0;
+        total = at_least(0) * kv_heads;
+    }
+    // The n-th (n not falling).
+    __device__ __forceinline__ void find(int n, Item* it) {
+        const int lane = threadIdx.x & 31, index = n * ctas + ((n & 1) != 0 ? ctas - 1 - me : me);
+        if (index >= total) {
+            if (lane == 0) it->len = -1;
+        } else {
+            const int k = index / kv_heads;
+            while (upto <= k) {
+                above = upto;
+                upto = at_least(--place);
+            }
+            int rank = k - above;                       // that one of the sequences with a block there
+#pragma unroll 1
+            for (int base = 0; base < batch; base += 32) {
+                const bool has = base + lane < batch && blocks[base + lane] > place;
+                const uint32_t all = __ballot_sync(0xffffffffu, has);
+                if (rank < __popc(all)) {
+                    if (has && __popc(all & ((1u << lane) - 1u)) == rank) {
+                        const int first = indptr[base + lane], len = indptr[base + lane + 1] - first, t0 = place * span;
+                        it->first = first;
+                        it->len = len;
+                        it->t0 = t0;
+                        it->head = index - k * kv_heads;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int from = t0 + i * half, to = min(min(from + half, t0 + span), len), tiles = from < to ? (to + kTile - 1) / kTile : 0;
+                            it->tiles[i] = tiles;
+                            it->keys[i] = (to - (tiles - 1) * kTile + 15) & ~15;
+                        }
+                    }
+                    break;
+                }
+                rank -= __popc(all);
+            }
+        }
+        __syncwarp();
+    }
+};
+
+// A warp's rows of a query tile once more, from the keys that each row sees and no others, where a value that is no number has met the
+// weight 0 of a row before it: the values of tokens [first, end) are looked through, and if all are numbers nothing is done (the rows are what
+// their own keys make them).  tok, h: the row's token and head of the group.
+__device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, int kv_head, int first, int end, int tok, int h, bool store) {
+    const int lane = threadIdx.x & 31, vectors = p.dim >> 3;
+    const __nv_bfloat16* v = p.v + static_cast<int64_t>(seq_first) * p.v_st + kv_head * p.v_sh;
+    const __nv_bfloat16* k = p.k + static_cast<int64_t>(seq_first) * p.k_st + kv_head * p.k_sh;
+    bool found = false;
+#pragma unroll 1
+    for (int i = first * vectors + lane; i < end * vectors; i += 32) {
+        const int key = i / vectors;
+        const Vec8 x = load8(v + key * p.v_st + (i - key * vectors) * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) found = found || !isfinite(x.v[e]);
+    }
+    if (!__any_sync(0xffffffffu, found)) return;
+    const int64_t row = seq_first + tok, head = kv_head * p.group + h;
+    const __nv_bfloat16* q = p.q + row * p.q_st + head * p.q_sh;
+#pragma unroll 1
+    for (int c = 0; c < p.dim; c += 32) {
+        float o[32], m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+#pragma unroll 1
+        for (int key = 0; key <= tok; ++key) {
+            float s = 0.f;
+#pragma unroll 1
+            for (int d = 0; d < p.dim; d += 8) {
+                const Vec8 a = load8(q + d), b = load8(k + key * p.k_st + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s = fmaf(a.v[e], b.v[e], s);
+            }
+            s *= p.scale_log2;
+            const float now = fmaxf(m, s), old = now == -INFINITY ? 1.f : exp2f(m - now), w = now == -INFINITY ? 0.f : exp2f(s - now);
+            m = now;
+            sum = fmaf(sum, old, w);
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+                if (c + e >= p.dim) break;
+                const Vec8 x = load8(v + key * p.v_st + c + e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[e + i] = fmaf(w, x.v[i], o[e + i] * old);
+            }
+        }
+        const float inv = sum > 0.f ? 1.f / sum : sum;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            if (!store || c + e >= p.dim) break;
+            Vec8 x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i] = o[e + i] * inv;
+            store8(p.out + (row * p.q_heads + head) * p.dim + c + e, x);
+        }
+    }
+}
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptParams p) {
+prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_constant__ PromptParams p) {
     using X = Shape<DP>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int s_indptr[kMaxBatch + 1];
     __shared__ int s_blocks[kMaxBatch];               // items per KV head of a sequence
-    __shared__ Item s_item[2];
-    __shared__ uint32_t s_odd[2][kOddTiles][4];       // keys whose values are not all numbers, by item and tile
+    __shared__ Item s_item[2], s_redo[8];
     __shared__ __align__(8) uint64_t item_full[2], item_empty[2];
     __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[X::kKSlots], k_empty[X::kKSlots], v_full[X::kVSlots], v_empty[X::kVSlots];
-    __shared__ __align__(8) uint64_t v_ready[X::kVSlots];   // a tile that not all rows see has been looked through
-    __shared__ __align__(8) uint64_t odd_done[2];           // ... all of an item's
+    __shared__ __align__(8) uint64_t v_ready[X::kVSlots];   // a tile's rows behind the sequence have become zeros
     __shared__ __align__(8) uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
-    __shared__ __align__(8) uint64_t turn[2][4];      // a softmax warp of tile i lets its neighbour of the other tile exponentiate
+    __shared__ __align__(8) uint64_t rows_full[2][2], o_free[2];   // reference and sum of a tile's rows are there (items in turn); O has been read
+    __shared__ float2 s_rows[2][2][kTile];
+    __shared__ uint32_t s_again[kAgain / 32 + 1];   // query tiles whose rows are not all numbers, a bit each; the last word: of later items
     __shared__ __align__(8) uint64_t drain[2];
     __shared__ uint32_t tmem_base_slot;
 
@@ -108,7 +255,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
         tma_prefetch_desc(&maps.v);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&item_full[i]), 1);
-            mbar_init(smem_u32(&item_empty[i]), 3 + 8);
+            mbar_init(smem_u32(&item_empty[i]), 4 + 8 + 4);
             mbar_init(smem_u32(&q_full[i]), 1);
             mbar_init(smem_u32(&q_empty[i]), 1);
             mbar_init(smem_u32(&s_full[i]), 1);
@@ -116,8 +263,9 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
             mbar_init(smem_u32(&p_full[i]), 4);
             mbar_init(smem_u32(&pv_done[i]), 1);
             mbar_init(smem_u32(&drain[i]), 1);
-            mbar_init(smem_u32(&odd_done[i]), 1);
-            for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&turn[i][q]), 1);
+            mbar_init(smem_u32(&rows_full[i][0]), 4);
+            mbar_init(smem_u32(&rows_full[i][1]), 4);
+            mbar_init(smem_u32(&o_free[i]), 4);
         }
         for (int s = 0; s < X::kKSlots; ++s) {
             mbar_init(smem_u32(&k_full[s]), 1);
@@ -133,6 +281,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
     }
     pdl_launch_dependents();
     pdl_wait_prior();
+    for (int i = tid; i <= kAgain / 32; i += kThreads) s_again[i] = 0;
     bool odd = false;
     for (int s = tid; s < p.batch; s += kThreads) {
         const int a = p.indptr[s], b = p.indptr[s + 1];
@@ -158,113 +307,79 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_slot;
-    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
 
     if (warp == 0) {
         // ================= items, Q and K =================
-        // The items of one KV head in order: those that end a sequence's longest row of blocks first.  Of items at place j or later in their
-        // sequences there are at_least(j).
-        auto at_least = [&](int j) {
-            int n = 0;
-            for (int s = lane; s < p.batch; s += 32) n += max(s_blocks[s] - j, 0);
-            return __reduce_add_sync(0xffffffffu, n);
-        };
-        int most = 0;
-        for (int s = lane; s < p.batch; s += 32) most = max(most, s_blocks[s]);
-        int level = __reduce_max_sync(0xffffffffu, most);   // (items come in falling order)
-        const int total = at_least(0) * p.kv_heads;
-        const int ctas = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
+        Walk walk(p, s_indptr, s_blocks, QB);
         uint32_t slot = 0, phase = 1, uses[2] = {0, 0}, loads = 0;
         bool ok = true;
         const bool leader = lane == 0;
+        auto publish = [&](int n) {
+            if (!wait_phase_warp(&item_empty[n & 1], static_cast<uint32_t>(n >> 1 & 1) ^ 1u, p.status, 371)) return false;
+            walk.find(n, &s_item[n & 1]);
+            if (lane == 0) mbar_arrive(smem_u32(&item_full[n & 1]));
+            return true;
+        };
+        ok = publish(0);
         for (int n = 0; ok; ++n) {
-            const int index = n * ctas + ((n & 1) != 0 ? ctas - 1 - me : me);
-            const bool any = index < total;
-            Item it;
-            it.len = -1;
-            int ntiles = 0;
-            if (any) {
-                const int k = index / p.kv_heads;
-                int lo = 0, hi = level;                     // at_least(lo) > k >= at_least(hi)
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (at_least(mid) > k) lo = mid; else hi = mid;
-                }
-                level = hi;
-                int rank = k - at_least(hi), seq = 0;       // of the sequences with a block at place lo, that one
-                for (int base = 0; base < p.batch; base += 32) {
-                    const uint32_t has = __ballot_sync(0xffffffffu, base + lane < p.batch && s_blocks[base + lane] > lo);
-                    const int c = __popc(has);
-                    if (rank < c) {
-                        seq = base + __fns(has, 0, rank + 1);
-                        break;
-                    }
-                    rank -= c;
-                }
-                it.first = s_indptr[seq];
-                it.len = s_indptr[seq + 1] - it.first;
-                it.t0 = lo * p.span;
-                it.head = index - k * p.kv_heads;
-                for (int i = 0; i < 2; ++i) {
-                    const int from = it.t0 + i * QB, to = min(min(from + QB, it.t0 + p.span), it.len);
-                    it.tiles[i] = from < to ? (to + kTile - 1) / kTile : 0;
-                }
-                ntiles = max(it.tiles[0], it.tiles[1]);
-            }
-            ok = mbar_wait_warp(smem_u32(&item_empty[n & 1]), static_cast<uint32_t>(n >> 1 & 1) ^ 1u, p.status, 371);
-            if (leader) {
-                s_item[n & 1] = it;
-                mbar_arrive(smem_u32(&item_full[n & 1]));
-            }
-            if (!any || !ok) break;
+            const Item* it = &s_item[n & 1];
+            const int first = it->first, head = it->head, t0 = it->t0, tiles0 = it->tiles[0], tiles1 = it->tiles[1];
+            const bool end = it->len < 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
+            if (end) break;
             auto load_q = [&](int i) {
-                if (it.tiles[i] == 0) return;
-                ok = ok && mbar_wait_warp(smem_u32(&q_empty[i]), (uses[i] & 1u) ^ 1u, p.status, 372);
+                ok = ok && wait_phase_warp(&q_empty[i], (uses[i] & 1u) ^ 1u, p.status, 372);
                 ++uses[i];
                 if (ok && leader) {
                     const uint32_t bar = smem_u32(&q_full[i]), dst = smem_base + X::kQOff + i * X::kSlotBytes;
                     mbar_arrive_expect_tx(bar, static_cast<uint32_t>(X::kHalves * QB * G * 128));
-                    for (int c = 0; c < X::kHalves; ++c) tma_load_3d(dst + c * kAtomBytes, &maps.q, c * 64, it.head * G, it.first + it.t0 + i * QB, bar);
+                    for (int c = 0; c < X::kHalves; ++c) tma_load_3d(dst + c * kAtomBytes, &maps.q, c * 64, head * G, first + t0 + i * QB, bar);
                 }
             };
+            const int ntiles = max(tiles0, tiles1);
             load_q(0);
             for (int kt = 0; kt < ntiles && ok; ++kt) {
-                ok = mbar_wait_warp(smem_u32(&k_empty[slot]), phase, p.status, 373);
+                ok = wait_phase_warp(&k_empty[slot], phase, p.status, 373);
                 if (!ok) break;
                 if (leader) {
                     const uint32_t bar = smem_u32(&k_full[slot]), dst = smem_base + X::kKOff + slot * X::kSlotBytes;
                     mbar_arrive_expect_tx(bar, X::kSlotBytes);
-                    for (int c = 0; c < X::kHalves; ++c) tma_load_3d(dst + c * kAtomBytes, &maps.k, c * 64, it.head, it.first + kt * kTile, bar);
+                    for (int c = 0; c < X::kHalves; ++c) tma_load_3d(dst + c * kAtomBytes, &maps.k, c * 64, head, first + kt * kTile, bar);
                 }
                 ++loads;
                 if (++slot == X::kKSlots) {
                     slot = 0;
                     phase ^= 1;
                 }
-                if (kt == 0) load_q(1);
+                if (kt == 0) {
+                    if (tiles1 > 0) load_q(1);
+                    ok = ok && publish(n + 1);   // (while the copies are under way)
+                }
             }
         }
         // The block ends when nothing of it is under way: the releases of the last tiles, or the copies themselves.
         for (uint32_t s = 0; s < X::kKSlots; ++s) {
             const uint32_t at = (slot + s) % X::kKSlots, turns = loads / X::kKSlots + (at < loads % X::kKSlots ? 1 : 0);
-            if (turns > 0) mbar_wait_warp(smem_u32(ok ? &k_empty[at] : &k_full[at]), (turns - 1) & 1u, p.status, 374);
+            if (turns > 0) wait_phase_warp(ok ? &k_empty[at] : &k_full[at], (turns - 1) & 1u, p.status, 374);
         }
         for (int i = 0; i < 2; ++i)
-            if (uses[i] > 0) mbar_wait_warp(smem_u32(ok ? &q_empty[i] : &q_full[i]), (uses[i] - 1) & 1u, p.status, 374);
+            if (uses[i] > 0) wait_phase_warp(ok ? &q_empty[i] : &q_full[i], (uses[i] - 1) & 1u, p.status, 374);
     } else if (warp == 2) {
         // ================= V =================
         uint32_t slot = 0, phase = 1, loads = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {
-            ok = mbar_wait_warp(smem_u32(&item_full[n & 1]), static_cast<uint32_t>(n >> 1 & 1), p.status, 375);
+            ok = wait_phase_warp(&item_full[n & 1], static_cast<uint32_t>(n >> 1 & 1), p.status, 375);
             if (!ok) break;
             const Item it = s_item[n & 1];
-            if (it.len < 0) break;
-            if (lane < 4 * kOddTiles) s_odd[n & 1][lane >> 2][lane & 3] = 0;
             __syncwarp();
-            const int ntiles = max(it.tiles[0], it.tiles[1]), partly = it.t0 / kTile;
+            if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
+            if (it.len < 0) break;
+            const int ntiles = max(it.tiles[0], it.tiles[1]);
             for (int kt = 0; kt < ntiles; ++kt) {
-                ok = mbar_wait_warp(smem_u32(&v_empty[slot]), phase, p.status, 376);
+                ok = wait_phase_warp(&v_empty[slot], phase, p.status, 376);
                 if (!ok) break;
                 const uint32_t bar = smem_u32(&v_full[slot]), dst = smem_base + X::kVOff + slot * X::kSlotBytes;
                 if (lane == 0) {
@@ -272,33 +387,13 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
                     for (int c = 0; c < X::kHalves; ++c) tma_load_3d(dst + c * kAtomBytes, &maps.v, c * 64, it.head, it.first + kt * kTile, bar);
                 }
                 ++loads;
-                if (kt >= partly) {
-                    ok = mbar_wait_warp(bar, phase ^ 1u, p.status, 377);
+                const int rows = it.len - kt * kTile, reach = it.reach(kt);
+                if (kt == ntiles - 1 && rows < reach) {
+                    ok = wait_phase_warp(&v_full[slot], phase ^ 1u, p.status, 377);
                     if (!ok) break;
-                    const int rows = min(kTile, it.len - kt * kTile);
-#pragma unroll 1
-                    for (int c = 0; c < X::kHalves; ++c) {
-#pragma unroll 4
-                        for (int i = 0; i < 32; ++i) {      // four rows at a time, 16 bytes per lane
-                            const int row = i * 4 + (lane >> 3);
-                            const uint32_t a = dst + c * kAtomBytes + i * 512 + lane * 16;
-                            uint32_t x[4];
-                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
-                            uint32_t bad = 0;                // an exponent of all ones: the top bit of its half
-                            for (int k = 0; k < 4; ++k) bad |= (x[k] & 0x7f807f80u) + 0x00800080u;
-                            if (row >= rows) {
-                                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(a), "r"(0u) : "memory");
-                            } else if ((bad & 0x80008000u) != 0) {
-                                for (int k = 0; k < 4; ++k) {
-                                    const uint32_t b = (x[k] & 0x7f807f80u) + 0x00800080u;
-                                    if ((b & 0x8000u) != 0) x[k] &= 0xffff0000u;
-                                    if ((b & 0x80000000u) != 0) x[k] &= 0x0000ffffu;
-                                }
-                                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                                atomicOr(&s_odd[n & 1][kt - partly][row >> 5], 1u << (row & 31));
-                            }
-                        }
-                    }
+                    for (int c = 0; c < X::kHalves; ++c)
+                        for (int row = rows + (lane >> 3); row < reach; row += 4)
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + c * kAtomBytes + row * 128 + (lane & 7) * 16), "r"(0u) : "memory");
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&v_ready[slot]));
@@ -309,59 +404,55 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
                 }
             }
             if (!ok) break;
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&odd_done[n & 1]));
-                mbar_arrive(smem_u32(&item_empty[n & 1]));
-            }
         }
         for (uint32_t s = 0; s < X::kVSlots; ++s) {
             const uint32_t turns = loads / X::kVSlots + (s < loads % X::kVSlots ? 1 : 0);
-            if (turns > 0) mbar_wait_warp(smem_u32(ok ? &v_empty[s] : &v_full[s]), (turns - 1) & 1u, p.status, 374);
+            if (turns > 0) wait_phase_warp(ok ? &v_empty[s] : &v_full[s], (turns - 1) & 1u, p.status, 374);
         }
     } else if (warp == 1) {
         // ================= issuer of S_i = Q_i K^T =================
         if (elect_one()) {
-            const uint32_t idesc = idesc_bf16_128x128(false);
             const uint64_t q_desc = kmajor_sw128_desc(smem_base + X::kQOff), k_desc = kmajor_sw128_desc(smem_base + X::kKOff);
             const int steps = (p.dim + 15) >> 4;
-            uint32_t slot = 0, phase = 0, uses[2] = {0, 0}, heads[2] = {0, 0};
-            int last = -1;               // the tile whose scores were made last
+            // (phases: a bit per query tile)
+            uint32_t slot = 0, phase = 0, q_phase = 0, made = 0, last = 0;
             bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-                if (ok && !mbar_wait_mostly_ready(smem_u32(bar), parity & 1u, p.status, site)) ok = false;
-            };
+            auto wait = [&](uint64_t* bar, uint32_t parity, int site) { ok = ok && wait_phase(bar, parity, p.status, site); };
             for (int n = 0; ok; ++n) {
+                const Item* it = &s_item[n & 1];
                 wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 378);
-                if (!ok) break;
-                const int t[2] = {s_item[n & 1].tiles[0], s_item[n & 1].tiles[1]}, len = s_item[n & 1].len;
-                if (len < 0) break;
+                if (!ok || it->len < 0) break;
+                const int tiles0 = it->tiles[0], tiles1 = it->tiles[1], keys0 = it->keys[0], keys1 = it->keys[1];
                 mbar_arrive(smem_u32(&item_empty[n & 1]));
-                const int ntiles = max(t[0], t[1]);
+                const int ntiles = max(tiles0, tiles1);
+#pragma unroll 1
                 for (int kt = 0; kt < ntiles && ok; ++kt) {
                     const uint64_t k = k_desc + slot * (X::kSlotBytes >> 4);
                     wait(&k_full[slot], phase, 379);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (kt >= t[i]) continue;
-                        if (kt == 0) wait(&q_full[i], heads[i]++, 380);
-                        // the columns' last scores have to have been read
-                        if (X::kSharedS) {
-                            if (last >= 0) wait(&s_free[last], uses[last] - 1, 381);
-                        } else if (uses[i] > 0) {
-                            wait(&s_free[i], uses[i] - 1, 381);
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const int tiles = i == 0 ? tiles0 : tiles1;
+                        if (kt >= tiles) continue;
+                        if (kt == 0) {
+                            wait(&q_full[i], q_phase >> i, 380);
+                            q_phase ^= 1u << i;
                         }
+                        // the columns' last scores have to have been read
+                        if (!X::kSharedS) last = i;
+                        wait(&s_free[last], (made >> last) ^ 1u, 381);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t a = q_desc + static_cast<uint32_t>(i) * (X::kSlotBytes >> 4);
+                        const uint32_t idesc = idesc_bf16_m128(kt == tiles - 1 ? (i == 0 ? keys0 : keys1) : kTile);
+                        const uint64_t a = q_desc + i * (X::kSlotBytes >> 4);
+                        const uint32_t d = tmem_base + i * X::kColS1;
 #pragma unroll
                         for (int ks = 0; ks < DP / 16; ++ks)
                             if (ks < steps)
-                                tc_mma_bf16(tmem_base + (i == 1 ? X::kColS1 : 0u), a + (((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4),
-                                            k + (((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4), idesc, ks > 0 ? 1u : 0u);
+                                tc_mma_bf16(d, a + (((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4), k + (((ks >> 2) * kAtomBytes + (ks & 3) * 32) >> 4), idesc,
+                                            ks > 0 ? 1u : 0u);
                         tc_commit(smem_u32(&s_full[i]));
-                        if (kt == t[i] - 1) tc_commit(smem_u32(&q_empty[i]));
-                        ++uses[i];
+                        if (kt == tiles - 1) tc_commit(smem_u32(&q_empty[i]));
+                        made ^= 1u << i;
                         last = i;
                     }
                     if (!ok) break;
@@ -374,7 +465,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
             }
             if (!ok) {   // products under way end before the block does
                 tc_commit(smem_u32(&drain[0]));
-                mbar_wait_bounded(smem_u32(&drain[0]), 0, p.status, 374);
+                wait_phase(&drain[0], 0, p.status, 374);
             }
         }
     } else if (warp == 3) {
@@ -382,38 +473,43 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
         if (elect_one()) {
             const uint32_t idesc = idesc_bf16_128xn((p.dim + 15) & ~15, true);
             const uint64_t v_desc = mnmajor_sw128_desc(smem_base + X::kVOff);
-            uint32_t slot = 0, phase = 0, uses[2] = {0, 0}, looked = 0;
+            uint32_t slot = 0, phase = 0, p_phase = 0, o_phase = 0, looked = 0;   // (a bit per query tile; of the last: per slot)
             bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-                if (ok && !mbar_wait_mostly_ready(smem_u32(bar), parity & 1u, p.status, site)) ok = false;
-            };
+            auto wait = [&](uint64_t* bar, uint32_t parity, int site) { ok = ok && wait_phase(bar, parity, p.status, site); };
             for (int n = 0; ok; ++n) {
+                const Item* it = &s_item[n & 1];
                 wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 378);
-                if (!ok) break;
-                const int t[2] = {s_item[n & 1].tiles[0], s_item[n & 1].tiles[1]}, len = s_item[n & 1].len, partly = s_item[n & 1].t0 / kTile;
-                if (len < 0) break;
+                if (!ok || it->len < 0) break;
+                const int tiles0 = it->tiles[0], tiles1 = it->tiles[1], keys0 = it->keys[0], keys1 = it->keys[1];
+                const int ntiles = max(tiles0, tiles1);
+                const bool tail = it->len - (ntiles - 1) * kTile < it->reach(ntiles - 1);
                 mbar_arrive(smem_u32(&item_empty[n & 1]));
-                const int ntiles = max(t[0], t[1]);
+#pragma unroll 1
                 for (int kt = 0; kt < ntiles && ok; ++kt) {
                     const uint64_t v = v_desc + slot * (X::kSlotBytes >> 4);
                     wait(&v_full[slot], phase, 382);
-                    if (kt >= partly) {
+                    if (tail && kt == ntiles - 1) {
                         wait(&v_ready[slot], looked >> slot, 383);
-                        looked ^= 1u << slot;   // (its phase, a bit per slot)
+                        looked ^= 1u << slot;
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (kt >= t[i]) continue;
-                        wait(&p_full[i], uses[i], 384);
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const int tiles = i == 0 ? tiles0 : tiles1;
+                        if (kt >= tiles) continue;
+                        if (kt == 0) {
+                            wait(&o_free[i], (o_phase >> i) ^ 1u, 385);   // (of the item before)
+                            o_phase ^= 1u << i;
+                        }
+                        wait(&p_full[i], p_phase >> i, 384);
+                        p_phase ^= 1u << i;
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t prob = tmem_base + X::kColP + static_cast<uint32_t>(i) * 64u;
-                        const uint32_t d = tmem_base + X::kColO + static_cast<uint32_t>(i) * DP;
+                        const uint32_t prob = tmem_base + X::kColP + i * 64u, d = tmem_base + X::kColO + i * DP;
+                        const int keys = kt == tiles - 1 ? (i == 0 ? keys0 : keys1) : kTile;
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks)   // keys ks*16 .. +15: eight packed columns
-                            tc_mma_bf16_ts(d, prob + static_cast<uint32_t>(ks * 8), v + (ks * 2048 >> 4), idesc, (kt > 0 || ks > 0) ? 1u : 0u);
+                            if (ks * 16 < keys) tc_mma_bf16_ts(d, prob + static_cast<uint32_t>(ks * 8), v + (ks * 2048 >> 4), idesc, (kt > 0 || ks > 0) ? 1u : 0u);
                         tc_commit(smem_u32(&pv_done[i]));
-                        ++uses[i];
                     }
                     if (!ok) break;
                     tc_commit(smem_u32(&v_empty[slot]));
@@ -425,45 +521,40 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
             }
             if (!ok) {
                 tc_commit(smem_u32(&drain[1]));
-                mbar_wait_bounded(smem_u32(&drain[1]), 0, p.status, 374);
+                wait_phase(&drain[1], 0, p.status, 374);
             }
         }
-    } else {
-        // ================= softmax / output rows =================
+    } else if (warp < 12) {
+        // ================= softmax =================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int tile = (warp >> 2) - 1;         // query tile of this warp
         const int qtr = warp & 3;                 // TMEM lane quarter this warp may read
         const int r = qtr * 32 + lane;            // query row = TMEM lane
-        const int r_tok = token_of(r), r_head = r - r_tok * G;
+        const int r_tok = token_of(r);
         const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(qtr * 32) << 16);
         const uint32_t s_addr = lane_addr + (tile == 1 ? X::kColS1 : 0u);
         const uint32_t p_addr = lane_addr + X::kColP + static_cast<uint32_t>(tile) * 64u;
         const uint32_t o_addr = lane_addr + X::kColO + static_cast<uint32_t>(tile) * DP;
-        const uint32_t stage = smem_base + X::kStageOff + static_cast<uint32_t>(warp - 4) * kStageBytes;
         const float sc = p.scale_log2;
-        uint32_t uses = 0;                        // K/V tiles of this query tile so far
-        uint32_t turns = 0;                       // ... in which both tiles took part
+        uint32_t uses = 0, items = 0;             // K/V tiles of this query tile so far, items with rows in it
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-            if (ok && !__all_sync(0xffffffffu, mbar_wait_mostly_ready(smem_u32(bar), parity & 1u, p.status, site))) ok = false;
+            if (ok && !wait_phase_warp(bar, parity, p.status, site)) ok = false;
         };
-        auto low_bits = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
 
         for (int n = 0; ok; ++n) {
-            wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 385);
+            wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 386);
             if (!ok) break;
-            const Item it = s_item[n & 1];
-            if (it.len < 0) break;
-            const int mine = it.tiles[tile], both = min(it.tiles[0], it.tiles[1]);
-            const int tok = it.t0 + tile * QB + r_tok;
-            const int limit = min(tok, it.len - 1);   // last visible key of this row
-            float m_ref = -INFINITY;   // the maximum the exponentials refer to, in units of the raw scores
+            const int len = s_item[n & 1].len, t0 = s_item[n & 1].t0, mine = s_item[n & 1].tiles[tile];
+            __syncwarp();
+            if (len < 0) break;
+            if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
+            const int limit = min(t0 + tile * QB + r_tok, len - 1);   // last visible key of this row
+            float m_ref = -INFINITY;   // what the exponentials refer to, in units of the raw scores
             float l_run = 0.f;
             for (int kt = 0; kt < mine; ++kt, ++uses) {
-                wait(&s_full[tile], uses, 386);
+                wait(&s_full[tile], uses, 387);
                 tc_fence_after();
-                const int k0 = kt * kTile;
-                const bool need_mask = __any_sync(0xffffffffu, k0 + kTile - 1 > limit);
                 uint32_t s[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
@@ -471,163 +562,194 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const PromptPar
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s_free[tile]));
-                // the neighbour's exponentials first, the last product has read P and added to O
-                if (kt < both && (tile == 1 || turns > 0)) wait(&turn[tile ^ 1][qtr], tile == 1 ? turns : turns - 1, 387);
-                if (kt > 0) wait(&pv_done[tile], uses - 1, 388);
-                tc_fence_after();
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                uint32_t seen[4];   // of a masked tile: which of each 32 keys the row sees
-                float2 sum;
-                // MODE 0: no masks; 1: masks; 2: no masks, and the maximum beside
-                auto probabilities = [&](auto mode) {
-                    const float mb = m_ref == -INFINITY ? INFINITY : m_ref * sc;   // (no key seen yet: probabilities 0)
-                    const float2 sc2 = make_float2(sc, sc), mb2 = make_float2(-mb, -mb);
-                    sum = make_float2(0.f, 0.f);
+                const int seen = limit + 1 - kt * kTile;      // keys of the tile that the row sees
+                if (__any_sync(0xffffffffu, seen < kTile)) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float a = __uint_as_float(s[c][i]), b = __uint_as_float(s[c][i + 1]);
-                            const float2 e = fma2(make_float2(a, b), sc2, mb2);
-                            float2 pr = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                            if (mode == 1) {
-                                if ((seen[c] >> i & 1) == 0) pr.x = 0.f;
-                                if ((seen[c] >> (i + 1) & 1) == 0) pr.y = 0.f;
-                            }
-                            if (mode == 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], a, b);
-                            sum = add2(sum, pr);
-                            packed[i >> 1] = pack_bf16(pr.x, pr.y);
-                        }
-                        tmem_st_32x32b_x16(p_addr + c * 16, packed);
-                    }
-                };
-                // Moves the reference where the row's maximum has outgrown it; O and the sum shrink by the same factor.  (TMEM accesses are
-                // warp-wide: a warp rescales all of its rows, by 1 where nothing moved.)
-                auto outgrown = [&](float mx) { return mx != -INFINITY && (m_ref == -INFINITY || (mx - m_ref) * sc > kLazyLog2); };
-                auto move_reference = [&](float mx) {
-                    float alpha = 1.f;
-                    if (outgrown(mx)) {
-                        if (m_ref != -INFINITY) alpha = ex2_approx((m_ref - mx) * sc);
-                        m_ref = mx;
-                    }
-                    if (__any_sync(0xffffffffu, alpha != 1.f)) {
-                        l_run *= alpha;
-#pragma unroll
-                        for (int c = 0; c < DP / 16; ++c) {
-                            uint32_t ov[16];
-                            tmem_ld_32x32b_x16(o_addr + c * 16, ov);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-                            tmem_st_32x32b_x16(o_addr + c * 16, ov);
-                        }
-                    }
-                };
-                auto highest = [&]() { return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])); };
-                if (need_mask) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        seen[c] = low_bits(limit + 1 - k0 - c * 32);
+                        if (__all_sync(0xffffffffu, seen >= c * 32 + 32)) continue;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            m4[i & 3] = fmaxf(m4[i & 3], (seen[c] >> i & 1) != 0 ? __uint_as_float(s[c][i]) : -INFINITY);
+                            if (c * 32 + i >= seen) s[c][i] = 0xff800000u;
                     }
-                    move_reference(highest());
-                    probabilities(std::integral_constant<int, 1>{});
-                } else {
-                    if (kt == 0) {
+                }
+                if (uses > 0) wait(&pv_done[tile], uses - 1, 388);   // the last product has read P and added to O
+                tc_fence_after();
+                float tile_sum;
+                bool move = kt == 0;
+#pragma unroll 1
+                for (;;) {
+                    if (move) {
+                        // The reference moves to the row's maximum; O and the sum shrink by the same factor.  (TMEM accesses are warp-wide: a
+                        // warp rescales all of its rows, by 1 where nothing has moved.)
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
                             for (int i = 0; i < 32; i += 2)
                                 m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-                        m_ref = highest();
+                        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                        float alpha = 1.f;
+                        if (mx > m_ref) {
+                            if (m_ref != -INFINITY) alpha = ex2_approx((m_ref - mx) * sc);
+                            m_ref = mx;
+                        }
+                        if (kt > 0) {
+                            l_run *= alpha;
+                            tmem_st_wait();
+#pragma unroll 1
+                            for (int c = 0; c < DP / 4; ++c) {   // (rare: few registers beside the scores)
+                                uint32_t ov[4];
+                                asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                                             : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_addr + c * 4) : "memory");
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                                asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
+                                             ::"r"(o_addr + c * 4), "r"(ov[0]), "r"(ov[1]), "r"(ov[2]), "r"(ov[3]) : "memory");
+                            }
+                        }
                     }
-                    probabilities(std::integral_constant<int, 2>{});
-                    const float mx = highest();
-                    if (__any_sync(0xffffffffu, outgrown(mx))) {
-                        move_reference(mx);
-                        probabilities(std::integral_constant<int, 0>{});
+                    const float mb = m_ref == -INFINITY ? INFINITY : m_ref * sc;   // (no key seen yet: probabilities 0)
+                    const float2 sc2 = make_float2(sc, sc), mb2 = make_float2(-mb, -mb);
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 e = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, mb2);
+                            const float2 pr = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                            sum = add2(sum, pr);
+                            packed[i >> 1] = pack_bf16(pr.x, pr.y);
+                        }
+                        tmem_st_32x32b_x16(p_addr + c * 16, packed);
                     }
-                }
-                if (kt < both) {
-                    if (lane == 0) mbar_arrive(smem_u32(&turn[tile][qtr]));
-                    ++turns;
+                    tile_sum = sum.x + sum.y;
+                    if (move || !__any_sync(0xffffffffu, tile_sum > kMostSum || m_ref == -INFINITY)) break;
+                    move = true;
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&p_full[tile]));
-                l_run += sum.x + sum.y;
+                l_run += tile_sum;
             }
             if (mine > 0) {
-                // ---- the last product, then O / sum ----
-                wait(&odd_done[n & 1], static_cast<uint32_t>(n >> 1), 389);
-                wait(&pv_done[tile], uses - 1, 390);
+                s_rows[tile][items & 1][r] = make_float2(m_ref, l_run);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&rows_full[tile][items & 1]));
+                ++items;
+            }
+        }
+        // ---- rows that are no numbers, once more where that is not their own keys' doing (behind the last output) ----
+        asm volatile("bar.sync 1, 384;" ::: "memory");
+        bool any = false;
+#pragma unroll 1
+        for (int i = lane; i <= kAgain / 32; i += 32) any = any || s_again[i] != 0;
+        if (__any_sync(0xffffffffu, any) && ok) {
+            Walk walk(p, s_indptr, s_blocks, QB);
+#pragma unroll 1
+            for (int n = 0;; ++n) {
+                const uint32_t noted = n < kAgain / 2 ? s_again[n >> 4] >> (2 * n & 31) & 3u : s_again[kAgain / 32] != 0 ? 3u : 0u;
+                if (noted == 0 && n < kAgain / 2 && n * walk.ctas < walk.total) continue;
+                Item* it = &s_redo[warp - 4];
+                walk.find(n, it);
+                if (it->len < 0) break;
+                const int first = it->t0 + tile * QB, rows = min(min(QB, it->t0 + p.span - first), it->len - first);
+                if ((noted >> tile & 1u) != 0 && rows > 0)
+                    sum_up_again(p, it->first, it->head, first, min(it->len, first + 2 * kTile), first + min(r_tok, rows - 1), r - r_tok * G, r_tok < rows);
+                __syncwarp();
+            }
+        }
+    } else {
+        // ================= output: O / sum =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        const int qtr = warp & 3;
+        const int r = qtr * 32 + lane;
+        const int r_tok = token_of(r), r_head = r - r_tok * G;
+        const uint32_t stage = smem_base + X::kStageOff + static_cast<uint32_t>(qtr) * kStageBytes;
+        uint32_t uses = 0, items = 0;             // their parities, a bit per query tile; of the second: two bits each
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+            if (ok && !wait_phase_warp(bar, parity & 1u, p.status, site)) ok = false;
+        };
+        for (int n = 0; ok; ++n) {
+            wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 386);
+            if (!ok) break;
+            const Item it = s_item[n & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
+            if (it.len < 0) break;
+#pragma unroll 1
+            for (int tile = 0; tile < 2; ++tile) {
+                const int tiles = tile == 0 ? it.tiles[0] : it.tiles[1];
+                if (tiles == 0) continue;
+                uses ^= static_cast<uint32_t>(tiles & 1) << tile;
+                const uint32_t turn = items >> (2 * tile) & 3u;
+                items = (items & ~(3u << (2 * tile))) | ((turn + 1) & 3u) << (2 * tile);
+                const int first = it.t0 + tile * QB;                                        // token of the sequence
+                const int rows = min(min(QB, it.t0 + p.span - first), it.len - first);     // tokens of this tile
+                // four lanes write the 64 bytes of 32 columns of a row
+                int to[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row2 = qtr * 32 + i * 8 + (lane >> 2), tok2 = token_of(row2);
+                    to[i] = tok2 < rows ? (it.first + first + tok2) * p.q_heads + it.head * G + row2 - tok2 * G : -1;
+                }
+                wait(&rows_full[tile][turn & 1], turn >> 1, 389);
+                const float2 ml = s_rows[tile][turn & 1][r];
+                const float inv = ml.y > 0.f ? __frcp_rn(ml.y) : ml.y;      // (a sum that is no number makes the row none)
+                if (ok && r_tok < rows && p.lse != nullptr)
+                    p.lse[(it.first + first + r_tok) * p.q_heads + it.head * G + r_head] = (ml.x * p.scale_log2 + log2f(ml.y)) * 0.6931471805599453f;
+                wait(&pv_done[tile], (uses >> tile) ^ 1u, 390);
                 tc_fence_after();
-                const float inv = l_run > 0.f ? 1.f / l_run : l_run;      // (a sum that is no number makes the row none)
-                const int partly = it.t0 / kTile;
-                uint32_t any_odd = 0;
-#pragma unroll
-                for (int k = 0; k < 4 * kOddTiles; ++k) any_odd |= s_odd[n & 1][k >> 2][k & 3];
-                const bool store = ok && r_tok < QB && tok < it.len && tok < it.t0 + p.span;
-                const int64_t row0 = static_cast<int64_t>(it.first) + it.t0 + tile * QB;
-                const int head0 = it.head * G;
-                if (store && p.lse != nullptr)
-                    p.lse[(row0 + r_tok) * p.q_heads + head0 + r_head] = (m_ref * sc + log2f(l_run)) * 0.6931471805599453f;
+                const uint32_t o_addr = tmem_base + (static_cast<uint32_t>(qtr * 32) << 16) + X::kColO + static_cast<uint32_t>(tile) * DP;
+                float2 odd = make_float2(0.f, 0.f);   // 0 as long as all are numbers
 #pragma unroll 1
-                for (int c = 0; c < DP / 32; ++c) {
-                    if (c * 32 >= p.dim) break;
-                    uint32_t ov[32];
-                    tmem_ld_32x32b_x32(o_addr + c * 32, ov);
-                    tmem_ld_wait();
-                    if (any_odd != 0) {   // (rare: values of visible keys that are no numbers)
-#pragma unroll 1
-                        for (int k = 0; k < 4 * kOddTiles; ++k) {
-                            for (uint32_t bits = s_odd[n & 1][k >> 2][k & 3]; bits != 0; bits &= bits - 1) {
-                                const int key = (partly + (k >> 2)) * kTile + (k & 3) * 32 + __ffs(bits) - 1;
-                                if (key > limit) continue;
-                                const __nv_bfloat16* v = p.v + static_cast<int64_t>(it.first + key) * p.v_st + it.head * p.v_sh + c * 32;
+                for (int c = 0; c * 32 < p.dim; ++c) {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const float x = c * 32 + i < p.dim ? __bfloat162float(v[i]) : 0.f;
-                                    if (!isfinite(x)) ov[i] = __float_as_uint(__uint_as_float(ov[i]) + x);
-                                }
-                            }
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t ov[16];
+                        tmem_ld_32x32b_x16(o_addr + c * 32 + half * 16, ov);
+                        tmem_ld_wait();
+                        if (half == 1 && c * 32 + 32 >= p.dim) {   // the next item's products may have it
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(smem_u32(&o_free[tile]));
                         }
-                        __syncwarp();
-                    }
+                        if (half == 0 || c * 32 + 16 < p.dim) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t w[4];
+                            for (int i = 0; i < 16; i += 2)
+                                odd = fma2(make_float2(__uint_as_float(ov[i]), __uint_as_float(ov[i + 1])), make_float2(0.f, 0.f), odd);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            w[i] = pack_bf16(__uint_as_float(ov[j * 8 + 2 * i]) * inv, __uint_as_float(ov[j * 8 + 2 * i + 1]) * inv);
-                        const uint32_t a = stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack_bf16(__uint_as_float(ov[j * 8 + 2 * i]) * inv, __uint_as_float(ov[j * 8 + 2 * i + 1]) * inv);
+                            const uint32_t a = stage + lane * 64 + (((half * 2 + j) ^ (lane >> 1 & 3)) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        }
                     }
                     __syncwarp();
-                    // four lanes write the 64 bytes of a row
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int rr = i * 8 + (lane >> 2), row2 = qtr * 32 + rr, tok2 = token_of(row2), j = lane & 3;
-                        const uint32_t a = stage + rr * 64 + ((j ^ (rr >> 1 & 3)) << 4);
+                        const uint32_t a = stage + (i * 8 + (lane >> 2)) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
                         uint4 w;
                         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(a) : "memory");
-                        const int t = it.t0 + tile * QB + tok2;
-                        if (ok && tok2 < QB && t < it.len && t < it.t0 + p.span && c * 32 + j * 8 < p.dim)
-                            *reinterpret_cast<uint4*>(p.out + ((row0 + tok2) * p.q_heads + head0 + row2 - tok2 * G) * p.dim + c * 32 + j * 8) = w;
+                        if (ok && to[i] >= 0 && c * 32 + (lane & 3) * 8 < p.dim)
+                            *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(to[i]) * p.dim + c * 32 + (lane & 3) * 8) = w;
                     }
                     __syncwarp();
                 }
-                tc_fence_before();
-            } else {
-                wait(&odd_done[n & 1], static_cast<uint32_t>(n >> 1), 389);   // (so that this warp is never two of its phases behind)
+                if (__any_sync(0xffffffffu, !(odd.x == 0.f && odd.y == 0.f)) && lane == 0) {
+                    const int at = min(2 * n + tile, kAgain);
+                    atomicOr(&s_again[at >> 5], 1u << (at & 31));
+                }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
         }
+        asm volatile("bar.arrive 1, 384;" ::: "memory");
     }
     __syncwarp();
     tc_fence_before();
@@ -691,7 +813,13 @@ int b200_attention_prompt(const b200_prompt_attention_args* a, b200_stream_t str
     if (err != B200_OK) return err;
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.lse = a->lse;
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.k = static_cast<const __nv_bfloat16*>(a->k);
     p.v = static_cast<const __nv_bfloat16*>(a->v);
+    p.q_st = a->q_stride_token;
+    p.q_sh = a->q_stride_head;
+    p.k_st = a->k_stride_token;
+    p.k_sh = a->k_stride_head;
     p.v_st = a->v_stride_token;
     p.v_sh = a->v_stride_head;
     p.indptr = a->indptr;
