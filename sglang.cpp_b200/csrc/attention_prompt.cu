@@ -781,7 +781,8 @@ int make_rows_tmap(CUtensorMap* out, const void* base, int dim, int heads, int t
 template <int DP>
 int launch_prompt(const PromptMaps& maps, const PromptParams& p, int grid, cudaStream_t stream) {
     const int smem = Shape<DP>::kSmemBytes + 1024;
-    B200_CHECK_CUDA(cudaFuncSetAttribute(prompt_attention_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> asked{0};
+    B200_CHECK_CUDA(allow_smem(asked, reinterpret_cast<const void*>(prompt_attention_kernel<DP>), smem));
     B200_CHECK_CUDA(launch_kernel(prompt_attention_kernel<DP>, dim3(grid), dim3(kThreads), smem, stream, dim3(1, 1, 1), maps, p));
     return B200_OK;
 }

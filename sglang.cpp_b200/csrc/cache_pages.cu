@@ -6,8 +6,28 @@ namespace b200 {
 namespace {
 
 constexpr int kMaxFork = 1024;        // entries of a fork call
-constexpr int kThreads = 256;
-constexpr int kPiece = 2048;          // bytes that a warp moves at a time: four 16-byte vectors per lane
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kUnit = 512;            // bytes that a warp moves with one vector per lane; four of them at a time
+constexpr int kFewPairs = 128;        // pairs of a copy call that every CTA looks through by itself
+constexpr int kSmallPool = 40960;     // pages that one CTA counts in its shared memory ...
+constexpr int64_t kSmallHeld = 65536; // ... where no more than that many are held
+constexpr int kWords = 8;             // of 32 pages that a warp ranks where many CTAs do (32: 7 us to mark a million pages, 8: 3)
+constexpr int kChunk = kWarps * kWords * 32;
+
+// x / d for x < 2^31 by a multiplication.
+struct Divisor {
+    uint32_t d, m;
+    int shift;
+    __device__ __forceinline__ uint32_t of(uint32_t x) const { return d == 1 ? x : __umulhi(x, m) >> shift; }
+};
+Divisor divisor(uint32_t d) {
+    // m = ceil(2^(32 + shift) / d) with 2^shift < d <= 2^(shift + 1): below 2^32, and x m / 2^(32 + shift) is too large by less than x / 2^(32 + shift) < 1 / d
+    Divisor x{d, 0, 0};
+    if (d <= 1) return x;
+    while ((2u << x.shift) < d && x.shift < 31) ++x.shift;
+    x.m = static_cast<uint32_t>(((uint64_t(1) << (32 + x.shift)) + d - 1) / d);
+    return x;
+}
 
 struct Pool {
     uint8_t* planes;
@@ -22,18 +42,52 @@ struct Table {
 
 __device__ __forceinline__ void report(int* status, int index) { atomicExch(&status[kStatusBadIndex], bad_index_word(index)); }
 
-// `bytes` (a multiple of 16) from one place to another by a warp.
-__device__ __forceinline__ void move_piece(uint8_t* to, const uint8_t* from, int bytes, int lane) {
-    uint4 v[4];
+// How pages are cut into units.  A run is a page of one plane.
+struct Units {
+    int per_run;          // units of a run of kUnit bytes and more
+    int group_log;        // smaller ones: 2^group_log lanes have one
+    Divisor per_run_div, planes_div;
+};
+
+// Runs [0, pairs * planes): run r is the first slots_of(pair) slots of page src[pair] in its plane.  Warps all over the device take neighbouring
+// units.
+template <class SlotsOf>
+__device__ __forceinline__ void move_pages(const Pool& pool, const Units& units, const int32_t* src, const int32_t* dst, int pairs, SlotsOf&& slots_of) {
+    const int lane = threadIdx.x & 31;
+    const int64_t page_bytes = static_cast<int64_t>(pool.page_size) * pool.slot_bytes;
+    const int64_t runs = static_cast<int64_t>(pairs) * pool.num_planes;
+    const int runs_log = 5 - units.group_log;                                 // of a unit, where runs are small
+    const int64_t all = runs_log > 0 ? (runs + (1 << runs_log) - 1) >> runs_log : runs * units.per_run;
+    const int within = lane & ((1 << units.group_log) - 1);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps * 4;
+    for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * 4; at < all; at += step) {
+        // the first unit's run by a division, the others' by steps
+        int64_t run = at, piece = 0;
+        if (runs_log == 0) {
+            run = at < 0x7fffffff ? units.per_run_div.of(static_cast<uint32_t>(at)) : at / units.per_run;
+            piece = at - run * units.per_run;
+        }
+        uint4 v[4];
+        uint8_t* to[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int at = (k * 32 + lane) * 16;
-        if (at < bytes) v[k] = *reinterpret_cast<const uint4*>(from + at);
-    }
+        for (int k = 0; k < 4; ++k) {
+            to[k] = nullptr;
+            const int64_t r = runs_log > 0 ? (run << runs_log) + (lane >> units.group_log) : run;
+            const int64_t offset = runs_log > 0 ? within * 16 : piece * kUnit + lane * 16;
+            if (runs_log > 0 || ++piece == units.per_run) {
+                ++run;
+                piece = 0;
+            }
+            if (r >= runs) continue;
+            const uint32_t pair = units.planes_div.of(static_cast<uint32_t>(r)), plane = static_cast<uint32_t>(r) - pair * pool.num_planes;
+            if (offset >= static_cast<int64_t>(slots_of(pair)) * pool.slot_bytes) continue;
+            uint8_t* base = pool.planes + plane * pool.plane_stride + offset;
+            v[k] = __ldcs(reinterpret_cast<const uint4*>(base + src[pair] * page_bytes));
+            to[k] = base + dst[pair] * page_bytes;
+        }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int at = (k * 32 + lane) * 16;
-        if (at < bytes) *reinterpret_cast<uint4*>(to + at) = v[k];
+        for (int k = 0; k < 4; ++k)
+            if (to[k] != nullptr) __stcs(reinterpret_cast<uint4*>(to[k]), v[k]);
     }
 }
 
@@ -44,6 +98,7 @@ __global__ void __launch_bounds__(1024, 1)
 copy_check_kernel(const int32_t* src, const int32_t* dst, const int32_t* tokens, int count, int page_size, int num_pages, int words,
                   uint32_t* named, uint32_t* clash, int32_t* slots, int* status) {
     const int tid = threadIdx.x;
+    pdl_launch_dependents();
     for (int w = tid; w < words; w += 1024) named[w] = clash[w] = 0;
     __syncthreads();
     auto there = [&](int i) {
@@ -67,33 +122,44 @@ copy_check_kernel(const int32_t* src, const int32_t* dst, const int32_t* tokens,
         if (there(i)) {
             if (__ldcg(&clash[dst[i] >> 5]) >> (dst[i] & 31) & 1) report(status, dst[i]);
             else n = tokens == nullptr ? page_size : min(tokens[i], page_size);
-        } else if (src[i] >= 0 && dst[i] >= 0) {
-            if (src[i] >= num_pages) report(status, src[i]);
-            if (dst[i] >= num_pages) report(status, dst[i]);
+        } else if (src[i] >= 0 && dst[i] >= 0 && src[i] != dst[i] && (tokens == nullptr || tokens[i] > 0)) {
+            report(status, src[i] >= num_pages ? src[i] : dst[i]);
         }
         slots[i] = n;
     }
 }
 
-__device__ __forceinline__ void move_pages(const Pool& pool, const int32_t* src, const int32_t* dst, const int32_t* slots, int pairs) {
-    const int lane = threadIdx.x & 31;
-    const int64_t page_bytes = static_cast<int64_t>(pool.page_size) * pool.slot_bytes;
-    const int64_t pieces = (page_bytes + kPiece - 1) / kPiece;
-    const int64_t items = static_cast<int64_t>(pairs) * pool.num_planes * pieces;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    for (int64_t it = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items; it += warps) {
-        const int64_t run = it / pieces, at = (it - run * pieces) * kPiece;
-        const int pair = static_cast<int>(run / pool.num_planes), plane = static_cast<int>(run - static_cast<int64_t>(pair) * pool.num_planes);
-        const int64_t bytes = static_cast<int64_t>(slots != nullptr ? slots[pair] : pool.page_size) * pool.slot_bytes;
-        if (at >= bytes) continue;
-        uint8_t* base = pool.planes + plane * pool.plane_stride + at;
-        move_piece(base + dst[pair] * page_bytes, base + src[pair] * page_bytes, static_cast<int>(min(bytes - at, static_cast<int64_t>(kPiece))), lane);
-    }
-}
-
+// slots NULL: the pairs are few, and each CTA finds by itself which of its own clash with others.
 __global__ void __launch_bounds__(kThreads)
-copy_pages_kernel(const Pool pool, const int32_t* src, const int32_t* dst, const int32_t* slots, int count) {
-    move_pages(pool, src, dst, slots, count);
+copy_pages_kernel(const Pool pool, const Units units, const int32_t* src, const int32_t* dst, const int32_t* tokens, const int32_t* slots, int count,
+                  int* status) {
+    __shared__ int s_src[kFewPairs], s_dst[kFewPairs], s_slots[kFewPairs];
+    pdl_wait_prior();
+    if (slots != nullptr) {
+        move_pages(pool, units, src, dst, count, [&](uint32_t pair) { return slots[pair]; });
+        return;
+    }
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const int a = src[i], b = dst[i], n = tokens == nullptr ? pool.page_size : min(max(tokens[i], 0), pool.page_size);
+        const bool inside = a < pool.num_pages && b < pool.num_pages, wanted = a >= 0 && b >= 0 && a != b && n > 0;
+        s_src[i] = wanted && inside ? a : -1;
+        s_dst[i] = wanted && inside ? b : -2;
+        s_slots[i] = wanted && inside ? n : 0;
+        if (wanted && !inside && blockIdx.x == 0) report(status, a >= pool.num_pages ? a : b);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < count; i += kWarps) {
+        const int b = s_dst[i];
+        if (b < 0) continue;
+        bool clash = false;
+        for (int k = threadIdx.x & 31; k < count; k += 32) clash = clash || s_src[k] == b || (s_dst[k] == b && k != i);
+        if (__any_sync(0xffffffffu, clash) && (threadIdx.x & 31) == 0) {
+            s_slots[i] = 0;
+            if (blockIdx.x == 0) report(status, b);
+        }
+    }
+    __syncthreads();
+    move_pages(pool, units, src, dst, count, [&](uint32_t pair) { return s_slots[pair]; });
 }
 
 // ---- fork ----------------------------------------------------------------------------------------------------------
@@ -135,6 +201,24 @@ fork_rows_kernel(const ForkParams p) {
             return;
         }
     }
+    // 2 KB of a run per warp; its first ones are under way while the entries are compared
+    const int64_t page_bytes = static_cast<int64_t>(P) * p.pool.slot_bytes, bytes = static_cast<int64_t>(part) * p.pool.slot_bytes;
+    const int lane = tid & 31;
+    const uint32_t pieces = static_cast<uint32_t>((bytes + 4 * kUnit - 1) / (4 * kUnit)), items = pieces * p.pool.num_planes, step = gridDim.x * kWarps;
+    uint32_t it = blockIdx.x * kWarps + (tid >> 5);
+    uint4 v[4];
+    uint8_t* base = nullptr;
+    int left = 0;
+    auto load = [&]() {
+        const uint32_t plane = it / pieces;
+        const int64_t at = static_cast<int64_t>(it - plane * pieces) * (4 * kUnit);
+        base = p.pool.planes + plane * p.pool.plane_stride + at + lane * 16;
+        left = static_cast<int>(min(bytes - at, int64_t(4 * kUnit))) - lane * 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k * kUnit < left) v[k] = *reinterpret_cast<const uint4*>(base + from * page_bytes + k * kUnit);
+    };
+    if (it < items) load();
     bool bad_row = false, bad_page = false;
     for (int j = tid; j < p.count; j += kThreads) {
         if (j != i && (p.children[j] == child || p.parents[j] == child)) bad_row = true;
@@ -155,13 +239,11 @@ fork_rows_kernel(const ForkParams p) {
     const int64_t end = part > 0 ? min(static_cast<int64_t>(full) + P, p.cols) : full;
     for (int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + tid; at < end; at += static_cast<int64_t>(gridDim.x) * kThreads)
         row[at] = at < full ? old[at] : to * P + static_cast<int>(at - full);
-    if (part == 0) return;
-    const int64_t page_bytes = static_cast<int64_t>(P) * p.pool.slot_bytes, bytes = static_cast<int64_t>(part) * p.pool.slot_bytes;
-    const int64_t pieces = (bytes + kPiece - 1) / kPiece, items = pieces * p.pool.num_planes;
-    for (int64_t it = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (tid >> 5); it < items; it += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
-        const int64_t plane = it / pieces, at = (it - plane * pieces) * kPiece;
-        uint8_t* base = p.pool.planes + plane * p.pool.plane_stride + at;
-        move_piece(base + to * page_bytes, base + from * page_bytes, static_cast<int>(min(bytes - at, static_cast<int64_t>(kPiece))), tid & 31);
+    for (; it < items; it += step) {
+        if (it >= step) load();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k * kUnit < left) __stcs(reinterpret_cast<uint4*>(base + to * page_bytes + k * kUnit), v[k]);
     }
 }
 
@@ -174,14 +256,13 @@ struct HeldParams {
     int* status;
 };
 
-// The pages that entry i of the rows holds (blockIdx.x = count: those named outside the table), each once per holder.
+// The pages that entry i of the rows holds (i = count: those named outside the table), every step-th of them from the first-th on.
 template <class Each>
-__device__ __forceinline__ void each_page(const HeldParams& p, int i, Each&& each) {
-    const int first = blockIdx.y * blockDim.x + threadIdx.x, step = gridDim.y * blockDim.x;
+__device__ __forceinline__ void each_page(const HeldParams& p, int i, int first, int step, Each&& each) {
     if (i == p.count) {
         for (int k = first; k < p.held_count; k += step) {
             const int g = p.held[k];
-            if (g >= 0 && g < p.num_pages) each(g);
+            if (g >= 0 && g < p.num_pages) each(g, 1);
             else report(p.status, g);
         }
         return;
@@ -193,48 +274,90 @@ __device__ __forceinline__ void each_page(const HeldParams& p, int i, Each&& eac
     }
     const int64_t len = min(static_cast<int64_t>(max(p.lens[i], 0)), p.table.cols);
     const int32_t* row = p.table.slots + r * p.table.stride;
-    for (int64_t at = static_cast<int64_t>(first) * p.page_size; at < len; at += static_cast<int64_t>(step) * p.page_size) {
-        const int slot = row[at];
-        if (slot >= 0 && slot / p.page_size < p.num_pages && slot % p.page_size == 0) each(slot / p.page_size);
-        else report(p.status, slot);
+    const uint32_t P = static_cast<uint32_t>(p.page_size);
+    const int64_t stride = static_cast<int64_t>(step) * P;
+    for (int64_t at = static_cast<int64_t>(first) * P; at < len; at += 4 * stride) {
+        int slot[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) slot[k] = at + k * stride < len ? row[at + k * stride] : 0;
+        const bool alike = at + 3 * stride < len && slot[0] == slot[1] && slot[0] == slot[2] && slot[0] == slot[3];   // (a dummy's page throughout)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (at + k * stride >= len || (alike && k > 0)) break;
+            const uint32_t g = static_cast<uint32_t>(slot[k]) / P;
+            if (slot[k] >= 0 && g < static_cast<uint32_t>(p.num_pages) && static_cast<uint32_t>(slot[k]) == g * P) each(static_cast<int>(g), alike ? 4 : 1);
+            else report(p.status, slot[k]);
+        }
     }
 }
 
 __global__ void __launch_bounds__(kThreads)
-mark_pages_kernel(const HeldParams p, uint32_t* bits, int32_t* refs) {
-    each_page(p, blockIdx.x, [&](int g) {
-        if (refs == nullptr || atomicAdd(&refs[g], 1) == 0) atomicOr(&bits[g >> 5], 1u << (g & 31));
+count_held_kernel(const HeldParams p, int32_t* refs) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    // A row whose table names one page throughout, a dummy's for instance: one addition per warp and four places of it.  (Half a million
+    // additions to one page one by one: 300 us; by warps 17.)
+    each_page(p, blockIdx.x, blockIdx.y * kThreads + threadIdx.x, gridDim.y * kThreads, [&](int g, int n) {
+        const uint32_t with = __activemask();
+        int same;
+        __match_all_sync(with, g, &same);
+        const int all = same ? static_cast<int>(__reduce_add_sync(with, n)) : n;
+        if (!same || (threadIdx.x & 31) == __ffs(with) - 1) atomicAdd(&refs[g], all);
     });
 }
 
-// Where each page stands: `each(page, used, pages used before it, total, used below the total)` for the 8192 pages of this CTA.
-// Every CTA adds up all of the bits by itself (128 KB for a million pages).
-template <class Each>
-__device__ __forceinline__ void ranked_pages(const uint32_t* bits, int words, int num_pages, Each&& each) {
-    __shared__ int s_sum[3][kThreads / 32];
+// Which pages are held, a bit each, and how many of the CTA's kChunk.
+__global__ void __launch_bounds__(kThreads)
+mark_held_kernel(const int32_t* refs, int num_pages, uint32_t* bits, int32_t* counts) {
+    __shared__ int s_sum[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int first = blockIdx.x * kThreads;
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+        const int64_t page = static_cast<int64_t>(blockIdx.x) * kChunk + (warp * kWords + k) * 32 + lane;
+        const uint32_t word = __ballot_sync(0xffffffffu, page < num_pages && refs[page] != 0);
+        if (lane == k) mine = word;
+    }
+    if (lane < kWords) bits[(blockIdx.x * kWarps + warp) * kWords + lane] = mine;
+    const int sum = __reduce_add_sync(0xffffffffu, __popc(mine));
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        int all = 0;
+        for (int w = 0; w < kWarps; ++w) all += s_sum[w];
+        counts[blockIdx.x] = all;
+    }
+}
+
+// Where each page of the CTA's kChunk stands: each(page, held, pages held before it, all of them, those of them below that number).
+template <class Each>
+__device__ __forceinline__ void ranked_pages(const uint32_t* bits, const int32_t* counts, int chunks, int num_pages, Each&& each) {
+    __shared__ int s_sum[3][kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = blockIdx.x;
     auto all = [&](int v, int which) {
         v = __reduce_add_sync(0xffffffffu, v);
         __syncthreads();
         if (lane == 0) s_sum[which][warp] = v;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w < kThreads / 32; ++w) sum += s_sum[which][w];
+        for (int w = 0; w < kWarps; ++w) sum += s_sum[which][w];
         return sum;
     };
+    const uint32_t mine = lane < kWords ? bits[(me * kWarps + warp) * kWords + lane] : 0u;
     int before = 0, total = 0;
-    for (int w = tid; w < words; w += kThreads) {
-        const int c = __popc(bits[w]);
-        total += c;
-        if (w < first) before += c;
+    for (int c = tid; c < chunks; c += kThreads) {
+        total += counts[c];
+        if (c < me) before += counts[c];
     }
     before = all(before, 0);
     total = all(total, 1);
     int below = 0;
-    for (int w = tid; w * 32 < total; w += kThreads) below += __popc(total - w * 32 >= 32 ? bits[w] : bits[w] & ((1u << (total - w * 32)) - 1u));
+    const int edge = total / kChunk, rest = total - edge * kChunk - tid * 32;   // the chunk that the number lies in; pages below it from this word on
+    for (int c = tid; c < edge; c += kThreads) below += counts[c];
+    if (edge < chunks && tid < kChunk / 32 && rest > 0) below += __popc(bits[edge * (kChunk / 32) + tid] & (rest >= 32 ? ~0u : (1u << rest) - 1u));
     below = all(below, 2);
-    const uint32_t mine = first + tid < words ? bits[first + tid] : 0u;
     int scan = __popc(mine);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -246,20 +369,66 @@ __device__ __forceinline__ void ranked_pages(const uint32_t* bits, int words, in
     __syncthreads();
     scan += before - __popc(mine);
     for (int w = 0; w < warp; ++w) scan += s_sum[0][w];
-    for (int k = 0; k < 32; ++k) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
         const uint32_t word = __shfl_sync(0xffffffffu, mine, k);
         const int base = __shfl_sync(0xffffffffu, scan, k);
-        const int64_t page = (static_cast<int64_t>(first) + warp * 32 + k) * 32 + lane;
+        const int64_t page = static_cast<int64_t>(me) * kChunk + (warp * kWords + k) * 32 + lane;
         if (page < num_pages) each(static_cast<int>(page), (word >> lane & 1) != 0, base + __popc(word & ((1u << lane) - 1u)), total, below);
     }
 }
 
+// All of that by one CTA of 1024 threads, the counts in its shared memory.
+template <class Each>
+__device__ __forceinline__ void count_and_rank(const HeldParams& p, int* refs, Each&& each) {
+    __shared__ int s_sum[2][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int g = tid; g < p.num_pages; g += 1024) refs[g] = 0;
+    __syncthreads();
+    for (int i = warp; i < p.count; i += 32) each_page(p, i, lane, 32, [&](int g, int n) { atomicAdd(&refs[g], n); });
+    each_page(p, p.count, tid, 1024, [&](int g, int n) { atomicAdd(&refs[g], n); });
+    __syncthreads();
+    const int share = (p.num_pages + 1023) / 1024 * 32, first = warp * share, end = min(first + share, p.num_pages);   // of a warp
+    int held = 0;
+    for (int g = first + lane; g < end; g += 32) held += refs[g] != 0;
+    held = __reduce_add_sync(0xffffffffu, held);
+    if (lane == 0) s_sum[0][warp] = held;
+    __syncthreads();
+    const int others = s_sum[0][lane];
+    const int total = __reduce_add_sync(0xffffffffu, others), before0 = __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
+    int below = 0;
+    for (int g = first + lane; g < min(end, total); g += 32) below += refs[g] != 0;
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0) s_sum[1][warp] = below;
+    __syncthreads();
+    below = __reduce_add_sync(0xffffffffu, s_sum[1][lane]);
+    int before = before0;
+    for (int base = first; base < end; base += 32) {
+        const int g = base + lane, n = g < end ? refs[g] : 0;
+        const uint32_t word = __ballot_sync(0xffffffffu, n != 0);
+        if (g < end) each(g, n, before + __popc(word & ((1u << lane) - 1u)), total, below);
+        before += __popc(word);
+    }
+}
+
+__device__ __forceinline__ void list_page(int page, bool held, int before, int total, int num_pages, int32_t* free_pages, int32_t* free_count) {
+    if (held) free_pages[num_pages - total + before] = -1;
+    else free_pages[page - before] = page;
+    if (page == 0) free_count[0] = num_pages - total;
+}
 __global__ void __launch_bounds__(kThreads)
-list_free_kernel(const uint32_t* bits, int words, int num_pages, int32_t* free_pages, int32_t* free_count) {
-    ranked_pages(bits, words, num_pages, [&](int page, bool used, int before, int total, int) {
-        if (used) free_pages[num_pages - total + before] = -1;
-        else free_pages[page - before] = page;
-        if (page == 0) free_count[0] = num_pages - total;
+list_free_kernel(const uint32_t* bits, const int32_t* counts, int chunks, int num_pages, int32_t* free_pages, int32_t* free_count) {
+    pdl_wait_prior();
+    ranked_pages(bits, counts, chunks, num_pages, [&](int page, bool held, int before, int total, int) {
+        list_page(page, held, before, total, num_pages, free_pages, free_count);
+    });
+}
+__global__ void __launch_bounds__(1024, 1)
+count_small_kernel(const HeldParams p, int32_t* refs, int32_t* free_pages, int32_t* free_count) {
+    extern __shared__ int s_refs[];
+    count_and_rank(p, s_refs, [&](int page, int n, int before, int total, int) {
+        refs[page] = n;
+        list_page(page, n != 0, before, total, p.num_pages, free_pages, free_count);
     });
 }
 
@@ -267,49 +436,64 @@ list_free_kernel(const uint32_t* bits, int words, int num_pages, int32_t* free_p
 
 struct CompactParams {
     Pool pool;
+    Units units;
     HeldParams held;
     int32_t *out, *map, *used;
     int64_t out_stride;
     int32_t *src, *dst, *rank, *moves;   // pages that move, where to, the number of a page among them; how many
 };
 
+__device__ __forceinline__ void plan_page(const CompactParams& p, int page, bool held, int before, int total, int below) {
+    if (page < total) {
+        p.map[page] = held ? page : -1;
+        if (!held) p.dst[page - before] = page;
+    } else if (held) {
+        p.src[before - below] = page;
+        p.rank[page] = before - below;
+    } else {
+        p.map[page] = -1;
+    }
+    if (page == 0) {
+        p.used[0] = total;
+        p.moves[0] = total - below;
+    }
+}
 __global__ void __launch_bounds__(kThreads)
-plan_moves_kernel(const uint32_t* bits, int words, const CompactParams p) {
-    ranked_pages(bits, words, p.pool.num_pages, [&](int page, bool used, int before, int total, int below) {
-        if (page < total) {
-            p.map[page] = used ? page : -1;
-            if (!used) p.dst[page - before] = page;
-        } else if (used) {
-            p.src[before - below] = page;
-            p.rank[page] = before - below;
-        } else {
-            p.map[page] = -1;
-        }
-        if (page == 0) {
-            p.used[0] = total;
-            p.moves[0] = total - below;
-        }
+plan_moves_kernel(const uint32_t* bits, const int32_t* counts, int chunks, const CompactParams p) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    ranked_pages(bits, counts, chunks, p.pool.num_pages, [&](int page, bool held, int before, int total, int below) {
+        plan_page(p, page, held, before, total, below);
     });
+}
+__global__ void __launch_bounds__(1024, 1)
+plan_small_kernel(const CompactParams p) {
+    extern __shared__ int s_refs[];
+    pdl_launch_dependents();
+    count_and_rank(p.held, s_refs, [&](int page, int n, int before, int total, int below) { plan_page(p, page, n != 0, before, total, below); });
 }
 
 __global__ void __launch_bounds__(kThreads)
 compact_kernel(const CompactParams p) {
-    const int pairs = p.moves[0], total = p.used[0], P = p.pool.page_size;
-    for (int i = blockIdx.x * kThreads + threadIdx.x; i < pairs; i += gridDim.x * kThreads) p.map[p.src[i]] = p.dst[i];
-    // the table: a group of lanes per page, which read its first slot before they write any
-    int group = 1;
-    while (group < 32 && group * 2 <= P) group *= 2;
-    const int lane = threadIdx.x & 31, sub = lane / group, in = lane % group, per_warp = 32 / group;
+    const int P = p.pool.page_size, lane = threadIdx.x & 31;
     const Table& t = p.held.table;
-    for (int i = 0; i < p.held.count; ++i) {
+    int group = 1;                            // lanes per page of the table: they read its first slot before they write any
+    while (group < 32 && group * 2 <= P) group *= 2;
+    const int sub = lane / group, in = lane % group, per_cta = kWarps * 32 / group;
+    pdl_wait_prior();
+    const int pairs = p.moves[0], total = p.used[0];
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < pairs; i += gridDim.x * kThreads) p.map[p.src[i]] = p.dst[i];
+    // A row's table by the CTAs whose number leaves its own when divided by the number of rows.
+    const int rows = p.held.count;
+    for (int i = rows > 0 ? static_cast<int>(blockIdx.x) % rows : 0; i < rows; i += gridDim.x) {
         const int r = p.held.rows[i];
         if (r < 0 || r >= t.rows) continue;
         const int64_t len = min(static_cast<int64_t>(max(p.held.lens[i], 0)), t.cols);
-        const int pages = static_cast<int>((len + P - 1) / P);
-        const int warps = gridDim.x * (kThreads / 32);
-        for (int base = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * per_warp; base < pages; base += warps * per_warp) {
-            const int j = base + sub;
-            const int64_t at = static_cast<int64_t>(j) * P;
+        const int64_t pages = (len + P - 1) / P;
+        const int sharing = (static_cast<int>(gridDim.x) - i + rows - 1) / rows;   // CTAs of this row (0: one, in its turn)
+        const int64_t step = static_cast<int64_t>(max(sharing, 1)) * per_cta;
+        for (int64_t base = static_cast<int64_t>(blockIdx.x / rows) * per_cta + (threadIdx.x >> 5) * (32 / group); base < pages; base += step) {
+            const int64_t j = base + sub, at = j * P;
             const int slot = j < pages ? t.slots[r * t.stride + at] : -1;
             __syncwarp();
             const int g = slot / P;
@@ -318,25 +502,64 @@ compact_kernel(const CompactParams p) {
             for (int k = in; k < P && at + k < t.cols; k += group) p.out[r * p.out_stride + at + k] = to * P + k;
         }
     }
-    move_pages(p.pool, p.src, p.dst, nullptr, pairs);
+    move_pages(p.pool, p.units, p.src, p.dst, pairs, [&](uint32_t) { return p.pool.page_size; });
 }
+
+// The launches behind another one of the same call start early and wait where they need it.
+struct FollowOn {
+    const bool was = pdl_launches_enabled();
+    explicit FollowOn(bool on = true) { set_pdl_launches(on); }
+    ~FollowOn() { set_pdl_launches(was); }
+};
 
 // ---- workspace and checks ------------------------------------------------------------------------------------------
 
 struct Layout {
-    int words;                       // of a bit per page
-    int64_t bits, ints, bytes;       // two arrays of bits, then three of an int per page, then a counter
+    int chunks;                               // of kChunk pages
+    int64_t bits, counts, ints, bytes;        // two arrays of a bit per page, a count per chunk, three arrays of an int per page, a counter
 };
 Layout layout_of(int num_pages) {
     Layout x;
-    x.words = div_ceil(num_pages, 32);
-    x.bits = div_ceil64(static_cast<int64_t>(x.words) * 4, 256) * 256;
-    x.ints = div_ceil64(static_cast<int64_t>(num_pages) * 4, 256) * 256;
-    x.bytes = 2 * x.bits + 3 * x.ints + 256 + 256;
+    auto padded = [](int64_t n) { return div_ceil64(n, 256) * 256; };
+    x.chunks = div_ceil(num_pages, kChunk);
+    x.bits = padded(static_cast<int64_t>(x.chunks) * (kChunk / 8));
+    x.counts = padded(static_cast<int64_t>(x.chunks) * 4);
+    x.ints = padded(static_cast<int64_t>(num_pages) * 4);
+    x.bytes = 2 * x.bits + x.counts + 3 * x.ints + 256 + 256;
     return x;
 }
-uint8_t* aligned(void* workspace) {
-    return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+struct Scratch {
+    uint32_t *bits, *bits2;
+    int32_t *counts, *ints[3], *one;
+};
+Scratch scratch_in(void* workspace, const Layout& x) {
+    uint8_t* at = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+    Scratch s;
+    s.bits = reinterpret_cast<uint32_t*>(at);
+    s.bits2 = reinterpret_cast<uint32_t*>(at + x.bits);
+    s.counts = reinterpret_cast<int32_t*>(at + 2 * x.bits);
+    for (int i = 0; i < 3; ++i) s.ints[i] = reinterpret_cast<int32_t*>(at + 2 * x.bits + x.counts + i * x.ints);
+    s.one = reinterpret_cast<int32_t*>(at + 2 * x.bits + x.counts + 3 * x.ints);
+    return s;
+}
+Units units_of(const Pool& pool) {
+    Units u;
+    const int64_t page_bytes = static_cast<int64_t>(pool.page_size) * pool.slot_bytes;
+    u.per_run = static_cast<int>(div_ceil64(page_bytes, kUnit));
+    u.group_log = 0;
+    while (u.group_log < 5 && (16ll << u.group_log) < page_bytes) ++u.group_log;
+    u.per_run_div = divisor(static_cast<uint32_t>(u.per_run));
+    u.planes_div = divisor(static_cast<uint32_t>(pool.num_planes));
+    return u;
+}
+// CTAs for `pairs` pages: one for every 16 KB.  As long as they are known to be there, up to 128 waves of them: those that run at a time then work
+// on neighbouring pages (700 pages of 1.8 MB: 421 us with one wave, 407 with four, 398 with sixteen, 396 with all).  Where `pairs` is what there may
+// be at most, four waves, or half a one if even that is little (800 of 1600 such pages in use 170 us with one wave, 164 with four; 6 short
+// requests in a pool of 64 pages 11.7, 13, 17 us with half a wave, one, four).
+int move_grid(const Pool& pool, const Units& u, int64_t pairs, bool known) {
+    const int64_t runs = pairs * pool.num_planes, units = u.group_log < 5 ? (runs >> (5 - u.group_log)) + 1 : runs * u.per_run;
+    const int64_t wave = static_cast<int64_t>(sm_count()) * 8;
+    return static_cast<int>(min(div_ceil64(units, kWarps * 4), known ? 16 * wave : units * kUnit > (256 << 20) ? 4 * wave : wave / 2));
 }
 
 int check_pool(const b200_page_pool* pool, const char* name, Pool* out) {
@@ -373,14 +596,28 @@ int check_held(const char* name, const HeldParams& p) {
     return B200_OK;
 }
 
-// The pages held, as bits (and counted).
-int launch_mark(const HeldParams& p, uint32_t* bits, int64_t bits_bytes, int32_t* refs, cudaStream_t stream) {
-    B200_CHECK_CUDA(cudaMemsetAsync(bits, 0, bits_bytes, stream));
-    if (refs != nullptr) B200_CHECK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(p.num_pages) * 4, stream));
-    if (p.count == 0 && p.held_count == 0) return B200_OK;
-    const int64_t most = max(div_ceil64(p.table.cols, p.page_size), static_cast<int64_t>(p.held_count));
-    const int chunks = static_cast<int>(min(max(div_ceil64(most, kThreads), int64_t(1)), int64_t(64)));
-    B200_CHECK_CUDA(launch_kernel(mark_pages_kernel, dim3(p.count + 1, chunks), dim3(kThreads), 0, stream, dim3(1, 1, 1), p, bits, refs));
+// Do the pages and their holders fit one CTA?  (Lengths are on the device: rows may be as long as the table's.)
+bool small(const HeldParams& p) {
+    return p.num_pages <= kSmallPool && div_ceil64(p.table.cols, p.page_size) * p.count + p.held_count <= kSmallHeld;
+}
+// The pages held, counted and as bits, by many CTAs.
+int launch_held(const HeldParams& p, int32_t* refs, uint32_t* bits, int32_t* counts, int chunks, cudaStream_t stream) {
+    B200_CHECK_CUDA(cudaMemsetAsync(refs, 0, static_cast<size_t>(p.num_pages) * 4, stream));
+    if (p.count > 0 || p.held_count > 0) {
+        const int64_t most = max(div_ceil64(p.table.cols, p.page_size), static_cast<int64_t>(p.held_count));
+        const int y = static_cast<int>(min(max(div_ceil64(most, 4 * kThreads), int64_t(1)), int64_t(64)));
+        B200_CHECK_CUDA(launch_kernel(count_held_kernel, dim3(p.count + 1, y), dim3(kThreads), 0, stream, dim3(1, 1, 1), p, refs));
+    }
+    FollowOn follow(p.count > 0 || p.held_count > 0);
+    B200_CHECK_CUDA(launch_kernel(mark_held_kernel, dim3(chunks), dim3(kThreads), 0, stream, dim3(1, 1, 1), refs, p.num_pages, bits, counts));
+    return B200_OK;
+}
+template <class Kernel, class... Args>
+int launch_small(Kernel kernel, const HeldParams& p, cudaStream_t stream, Args... args) {
+    const int smem = p.num_pages * 4;
+    static std::atomic<uint64_t> asked{0};   // (one per kernel: their types differ)
+    B200_CHECK_CUDA(allow_smem(asked, reinterpret_cast<const void*>(kernel), kSmallPool * 4));
+    B200_CHECK_CUDA(launch_kernel(kernel, dim3(1), dim3(1024), smem, stream, dim3(1, 1, 1), args...));
     return B200_OK;
 }
 
@@ -408,15 +645,19 @@ int b200_copy_pages(const b200_page_pool* pool, const int32_t* src, const int32_
     if (err != B200_OK) return err;
     int* status = device_status_words(&err);
     if (err != B200_OK) return err;
-    uint8_t* ws = aligned(workspace);
-    int32_t* slots = reinterpret_cast<int32_t*>(ws + 2 * x.bits);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    B200_CHECK_CUDA(launch_kernel(copy_check_kernel, dim3(1), dim3(1024), 0, s, dim3(1, 1, 1), src, dst, tokens, count, p.page_size, p.num_pages,
-                                  x.words, reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + x.bits), slots, status));
-    const int64_t pieces = div_ceil64(static_cast<int64_t>(p.page_size) * p.slot_bytes, kPiece);
-    const int64_t blocks = div_ceil64(static_cast<int64_t>(count) * p.num_planes * pieces, kThreads / 32);
-    const int grid = static_cast<int>(min(blocks, static_cast<int64_t>(sm_count()) * 8));
-    B200_CHECK_CUDA(launch_kernel(copy_pages_kernel, dim3(grid), dim3(kThreads), 0, s, dim3(1, 1, 1), p, src, dst, slots, count));
+    const Units units = units_of(p);
+    const int grid = move_grid(p, units, count, true);
+    // Few pairs: each CTA compares its own with all (700 of 1.8 MB: 5 us less than with a kernel for that).  Many: one CTA, with a bit per page.
+    int32_t* slots = nullptr;
+    if (count > kFewPairs) {
+        const Scratch w = scratch_in(workspace, x);
+        slots = w.ints[0];
+        B200_CHECK_CUDA(launch_kernel(copy_check_kernel, dim3(1), dim3(1024), 0, s, dim3(1, 1, 1), src, dst, tokens, count, p.page_size, p.num_pages,
+                                      div_ceil(p.num_pages, 32), w.bits, w.bits2, slots, status));
+    }
+    FollowOn follow(count > kFewPairs);
+    B200_CHECK_CUDA(launch_kernel(copy_pages_kernel, dim3(grid), dim3(kThreads), 0, s, dim3(1, 1, 1), p, units, src, dst, tokens, slots, count, status));
     return B200_OK;
 }
 
@@ -464,12 +705,14 @@ int b200_count_pages(int32_t* refs, int32_t* free_pages, int32_t* free_count, co
     if (err != B200_OK) return err;
     p.status = device_status_words(&err);
     if (err != B200_OK) return err;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(aligned(workspace));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    err = launch_mark(p, bits, x.bits, refs, s);
+    if (small(p)) return launch_small(count_small_kernel, p, s, p, refs, free_pages, free_count);
+    const Scratch w = scratch_in(workspace, x);
+    err = launch_held(p, refs, w.bits, w.counts, x.chunks, s);
     if (err != B200_OK) return err;
-    B200_CHECK_CUDA(launch_kernel(list_free_kernel, dim3(div_ceil(x.words, kThreads)), dim3(kThreads), 0, s, dim3(1, 1, 1), bits, x.words, num_pages,
-                                  free_pages, free_count));
+    FollowOn follow;
+    B200_CHECK_CUDA(launch_kernel(list_free_kernel, dim3(x.chunks), dim3(kThreads), 0, s, dim3(1, 1, 1), w.bits, w.counts, x.chunks, num_pages, free_pages,
+                                  free_count));
     return B200_OK;
 }
 
@@ -493,21 +736,29 @@ int b200_compact_pages(const b200_page_pool* pool, int32_t* table_out, int64_t t
     if (err != B200_OK) return err;
     p.held.status = device_status_words(&err);
     if (err != B200_OK) return err;
-    uint8_t* ws = aligned(workspace);
-    uint32_t* bits = reinterpret_cast<uint32_t*>(ws);
+    const Scratch w = scratch_in(workspace, x);
+    p.units = units_of(p.pool);
     p.out = table_out;
     p.out_stride = table_out_stride;
     p.map = map;
     p.used = used;
-    p.src = reinterpret_cast<int32_t*>(ws + 2 * x.bits);
-    p.dst = reinterpret_cast<int32_t*>(ws + 2 * x.bits + x.ints);
-    p.rank = reinterpret_cast<int32_t*>(ws + 2 * x.bits + 2 * x.ints);
-    p.moves = reinterpret_cast<int32_t*>(ws + 2 * x.bits + 3 * x.ints);
+    p.rank = w.ints[0];            // (the counts of holders are not needed any more where ranks are written)
+    p.src = w.ints[1];
+    p.dst = w.ints[2];
+    p.moves = w.one;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    err = launch_mark(p.held, bits, x.bits, nullptr, s);
-    if (err != B200_OK) return err;
-    B200_CHECK_CUDA(launch_kernel(plan_moves_kernel, dim3(div_ceil(x.words, kThreads)), dim3(kThreads), 0, s, dim3(1, 1, 1), bits, x.words, p));
-    B200_CHECK_CUDA(launch_kernel(compact_kernel, dim3(sm_count() * 8), dim3(kThreads), 0, s, dim3(1, 1, 1), p));
+    if (small(p.held)) {
+        err = launch_small(plan_small_kernel, p.held, s, p);
+        if (err != B200_OK) return err;
+    } else {
+        err = launch_held(p.held, w.ints[0], w.bits, w.counts, x.chunks, s);
+        if (err != B200_OK) return err;
+        FollowOn follow;
+        B200_CHECK_CUDA(launch_kernel(plan_moves_kernel, dim3(x.chunks), dim3(kThreads), 0, s, dim3(1, 1, 1), w.bits, w.counts, x.chunks, p));
+    }
+    FollowOn follow;
+    const int grid = max(move_grid(p.pool, p.units, p.pool.num_pages / 2 + 1, false), min(count, sm_count() * 8));
+    B200_CHECK_CUDA(launch_kernel(compact_kernel, dim3(grid), dim3(kThreads), 0, s, dim3(1, 1, 1), p));
     return B200_OK;
 }
 

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/b200_token_loop.h"
 
 namespace b200 {
@@ -84,6 +86,18 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
     cfg.numAttrs = n;
     note_kernel_launch();
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// Once per kernel and device: may it have that much dynamic shared memory?  (`asked`: a static of the caller's, a bit per device.)
+inline cudaError_t allow_smem(std::atomic<uint64_t>& asked, const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if ((asked.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 static inline int div_ceil(int a, int b) { return (a + b - 1) / b; }

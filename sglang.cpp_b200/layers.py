@@ -318,6 +318,7 @@ class CachePages:
         nbytes = _lib.load().b200_pages_workspace_bytes(self.pages_)
         _check(nbytes > 0, "no such number of pages")
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=buf.device)
+        self.scratch_ = (self.workspace.data_ptr(), nbytes)
 
     def _index(self, name: str, t: torch.Tensor, count: int = -1) -> int:
         if t.get_device() != self.device_ or t.dtype is not torch.int32 or t.dim() != 1 or (t.size(0) > 1 and t.stride(0) != 1):
@@ -334,7 +335,7 @@ class CachePages:
         """Page src[i] (or the first tokens[i] slots of it) to page dst[i] in every layer; a negative page: nothing."""
         n = src.numel()
         _launch(self.device_, "b200_copy_pages", self.pool_ref_, self._index("src", src), self._index("dst", dst, n),
-                None if tokens is None else self._index("tokens", tokens, n), n, self.workspace.data_ptr(), self.workspace.numel())
+                None if tokens is None else self._index("tokens", tokens, n), n, *self.scratch_)
 
     def fork(self, page_table: torch.Tensor, parents: torch.Tensor, children: torch.Tensor, lens: torch.Tensor,
              new_pages: torch.Tensor) -> None:
@@ -351,11 +352,11 @@ class CachePages:
         number [1])."""
         n = rows.numel()
         self._table("page_table", page_table)
-        refs, free, number = torch.empty(2 * self.pages_ + 1, dtype=torch.int32, device=page_table.device).split((self.pages_, self.pages_, 1))
+        refs, free, number = page_table.new_empty(self.pages_), page_table.new_empty(self.pages_), page_table.new_empty(1)
         _launch(self.device_, "b200_count_pages", refs.data_ptr(), free.data_ptr(), number.data_ptr(), page_table.data_ptr(),
                 page_table.size(0), _row_stride(page_table), page_table.size(1), self._index("rows", rows), self._index("lens", lens, n), n,
                 None if held is None else self._index("held", held), 0 if held is None else held.numel(), self.pool_.page_size, self.pages_,
-                self.workspace.data_ptr(), self.workspace.numel())
+                *self.scratch_)
         return refs, free, number
 
     def compact(self, page_table: torch.Tensor, rows: torch.Tensor, lens: torch.Tensor, held: Optional[torch.Tensor] = None,
@@ -368,11 +369,11 @@ class CachePages:
             out = page_table
         self._table("out", out)
         _check(out.shape == page_table.shape, "out must have the shape of page_table")
-        where, used = torch.empty(self.pages_ + 1, dtype=torch.int32, device=page_table.device).split((self.pages_, 1))
+        where, used = page_table.new_empty(self.pages_), page_table.new_empty(1)
         _launch(self.device_, "b200_compact_pages", self.pool_ref_, out.data_ptr(), _row_stride(out), where.data_ptr(), used.data_ptr(),
                 page_table.data_ptr(), page_table.size(0), _row_stride(page_table), page_table.size(1), self._index("rows", rows),
                 self._index("lens", lens, n), n, None if held is None else self._index("held", held), 0 if held is None else held.numel(),
-                self.workspace.data_ptr(), self.workspace.numel())
+                *self.scratch_)
         return where, used
 
 
@@ -495,25 +496,30 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, indptr: 
     if dev < 0 or q.dtype is not bf16 or q.dim() != 3:
         _fail("q must be a CUDA tensor of bfloat16 [tokens, q_heads, head_dim]")
     tokens, heads, dim = q.shape
-    for name, t in (("k", k), ("v", v)):
-        if t.get_device() != dev or t.dtype is not bf16 or t.dim() != 3 or t.size(0) != tokens or t.size(2) != dim or t.size(1) != k.size(1):
-            _fail(f"{name} must be bfloat16 [tokens, kv_heads, head_dim] on the device of q")
-    if dim > 1 and not q.stride(2) == k.stride(2) == v.stride(2) == 1:
+    if k.dim() != 3 or v.shape != k.shape or k.size(0) != tokens or k.size(2) != dim:
+        _fail("k and v must be [tokens, kv_heads, head_dim]")
+    if k.get_device() != dev or v.get_device() != dev or k.dtype is not bf16 or v.dtype is not bf16:
+        _fail("k and v must be bfloat16 on the device of q")
+    kv_heads = k.size(1)
+    (q_st, q_sh, q_sd), (k_st, k_sh, k_sd), (v_st, v_sh, v_sd) = q.stride(), k.stride(), v.stride()
+    if not q_sd == k_sd == v_sd == 1 and dim > 1:
         _fail("the last dimensions of q, k and v must be contiguous")
     if indptr.get_device() != dev or indptr.dtype is not torch.int32 or indptr.dim() != 1 or indptr.numel() < 1 or not indptr.is_contiguous():
         _fail("indptr must be contiguous int32 [sequences + 1] on the device of q")
     if out is None:
-        out = torch.empty(tokens, heads * dim, dtype=bf16, device=q.device)
+        out = q.new_empty((tokens, heads * dim))
     elif out.get_device() != dev or out.dtype is not bf16 or tuple(out.shape) != (tokens, heads * dim) or not out.is_contiguous():
         _fail("out must be contiguous bfloat16 [tokens, q_heads * head_dim] on the device of q")
-    lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
-
-    def strides(t):   # (those of a dimension of one say nothing)
-        return t.stride(0) if t.size(0) > 1 else t.size(1) * dim, t.stride(1) if t.size(1) > 1 else dim
-
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    if tokens == 1:      # (the strides of a dimension of one say nothing)
+        q_st, k_st, v_st = heads * dim, kv_heads * dim, kv_heads * dim
+    if heads == 1:
+        q_sh = dim
+    if kv_heads == 1:
+        k_sh = v_sh = dim
     args = _lib.PromptAttentionArgs(
-        out.data_ptr(), _ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(), *strides(q), *strides(k), *strides(v), indptr.data_ptr(),
-        tokens, indptr.numel() - 1, heads, k.size(1), dim, 1.0 / math.sqrt(dim) if sm_scale is None else sm_scale)
+        out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh,
+        indptr.data_ptr(), tokens, indptr.numel() - 1, heads, kv_heads, dim, 1.0 / math.sqrt(dim) if sm_scale is None else sm_scale)
     _launch(dev, "b200_attention_prompt", ctypes.byref(args))
     return (out, lse) if return_lse else out
 
