@@ -32,7 +32,7 @@ constexpr int kMaxDim = 128, kMaxBatch = 1024, kMaxGroup = 128;
 constexpr int kTile = 128;                  // keys per K/V tile and rows per query tile
 constexpr int kThreads = 512;               // warpgroups: copies and issue, softmax of either query tile, output
 // The first and the last one leave registers to the others; 512 x 128 are launched.
-constexpr int kFewRegs = 64, kSoftmaxRegs = 192;
+constexpr int kFewRegs = 72, kSoftmaxRegs = 184;
 static_assert(128 * (2 * kFewRegs + 2 * kSoftmaxRegs) <= kThreads * 128, "");
 constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16 under the 128-byte swizzle
 constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns
@@ -545,7 +545,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
         for (int n = 0; ok; ++n) {
             wait(&item_full[n & 1], static_cast<uint32_t>(n >> 1), 386);
             if (!ok) break;
-            const int len = s_item[n & 1].len, t0 = s_item[n & 1].t0, mine = s_item[n & 1].tiles[tile];
+            const int len = s_item[n & 1].len, t0 = s_item[n & 1].t0, mine = s_item[n & 1].tiles[tile], keys16 = s_item[n & 1].keys[tile];
             __syncwarp();
             if (len < 0) break;
             if (lane == 0) mbar_arrive(smem_u32(&item_empty[n & 1]));
@@ -563,10 +563,12 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s_free[tile]));
                 const int seen = limit + 1 - kt * kTile;      // keys of the tile that the row sees
+                bool half_only = false;   // no row sees the second half of the keys
                 if (__any_sync(0xffffffffu, seen < kTile)) {
+                    half_only = __all_sync(0xffffffffu, seen <= kTile / 2);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        if (__all_sync(0xffffffffu, seen >= c * 32 + 32)) continue;
+                        if (__all_sync(0xffffffffu, seen >= c * 32 + 32) || (c >= 2 && half_only)) continue;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (c * 32 + i >= seen) s[c][i] = 0xff800000u;
@@ -615,6 +617,15 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t packed[16];
+                        if (c == 2 && half_only) {
+                            if (keys16 > 64) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) packed[i] = 0;
+                                tmem_st_32x32b_x16(p_addr + 32, packed);
+                                tmem_st_32x32b_x16(p_addr + 48, packed);
+                            }
+                            break;
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
                             const float2 e = fma2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, mb2);
@@ -832,10 +843,12 @@ int b200_attention_prompt(const b200_prompt_attention_args* a, b200_stream_t str
     p.group = a->q_heads / a->kv_heads;
     p.group_inverse = (65536 + p.group - 1) / p.group;
     p.scale_log2 = a->sm_scale * 1.4426950408889634f;
-    const int QB = kTile / p.group;
-    p.span = 2 * QB;
-    const int64_t items = static_cast<int64_t>(a->tokens / p.span + a->batch) * a->kv_heads;   // at most
-    const int grid = static_cast<int>(items < sm_count() ? items : sm_count());
+    const int QB = kTile / p.group, sms = sm_count();
+    // Where there is hardly an item per SM, an item is one query tile: its K/V tiles take two thirds of the time of a pair's (16 / 8 heads: 1 x 500
+    // tokens 18.6 us, so 14.3; 1 x 1000 22.5, 18.6; 4 x 300 14.0, 12.5; beyond: 3 x 700 of 16 / 2 heads 20.1, 22.5; 1 x 4000 of 8 / 1 59.5, 74.6).
+    auto items_of = [&](int span) { return static_cast<int64_t>(a->tokens / span + a->batch) * a->kv_heads; };   // at most
+    p.span = 2 * items_of(2 * QB) <= sms + sms / 2 ? QB : 2 * QB;
+    const int grid = static_cast<int>(min(items_of(p.span), static_cast<int64_t>(sms)));
     PromptMaps maps;
     err = make_rows_tmap(&maps.q, a->q, p.dim, p.q_heads, p.tokens, a->q_stride_token, a->q_stride_head, p.group, QB);
     if (err == B200_OK) err = make_rows_tmap(&maps.k, a->k, p.dim, p.kv_heads, p.tokens, a->k_stride_token, a->k_stride_head, 1, kTile);
