@@ -585,10 +585,12 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                         // warp rescales all of its rows, by 1 where nothing has moved.)
                         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 4; ++c) {
+                            if (c == 2 && half_only) break;   // (scores of nobody's)
 #pragma unroll
                             for (int i = 0; i < 32; i += 2)
                                 m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                        }
                         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                         float alpha = 1.f;
                         if (mx > m_ref) {
