@@ -54,16 +54,16 @@ struct Shape {
 };
 
 // A wait for the phase of that parity in few instructions (the kernel has some thirty, and its roles share the SM's small instruction caches):
-// the hardware sleeps up to a microsecond per test, and the tests are counted.  False: reported, and nothing more is waited for.
+// the hardware sleeps some 4 us per test, and the tests are counted: two seconds.  False: reported, and nothing more is waited for.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* status, int site) {
     const uint32_t addr = smem_u32(bar);
 #pragma unroll 1
-    for (int i = 0; i < (1 << 21); ++i) {
+    for (int i = 0; i < (1 << 19); ++i) {
         uint32_t done;
         asm volatile(
             "{\n\t"
             ".reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t"
             "}\n"
             : "=r"(done)

@@ -88,6 +88,7 @@ class Engine:
         self.dummy_table_idx = config.max_running_req
         self.pt_cols = (config.max_seq_len + 31) // 32 * 32   # page-table row length (src/engine/engine.cc:452-459)
         self._step_index = 0
+        self._pages = None
 
     def _create_uniform(self, model_config, c) -> None:
         m = ModelConfigStruct(
@@ -302,6 +303,38 @@ class Engine:
         """A uint8 torch view of a named device tensor (debugging and tests)."""
         ptr, n = self.tensor_info(name, layer)
         return _as_cuda_tensor(ptr, n)
+
+    def page_table(self) -> torch.Tensor:
+        """The device's page table, int32 [max_running_req + 1, columns] (the last row the dummy request's)."""
+        return self.device_view("page_table").view(torch.int32).view(self.config.max_running_req + 1, self.pt_cols)
+
+    def cache_pages(self):
+        """``layers.CachePages`` over the K/V pool of all layers, without the dummy request's page: to copy, share, count or move
+        pages between steps, on ``cuda_stream``.  (Models whose layers are listed one by one have a pool per layer.)"""
+        from .layers import CachePages, MHAKVCache
+        if self.stack:
+            raise _lib.B200Error(4, "a pool per layer: CachePages needs the K/V of all layers in one")
+        m, slots = self.model_config, (self.config.num_pages + 1) * self.page_size
+        buffer = self.device_view("kv_cache").view(torch.bfloat16).view(2, m.num_layers, slots, -1, m.head_dim)
+        return CachePages(MHAKVCache.over(buffer, self.page_size), self.config.num_pages)
+
+    def fork_rows(self, parents, children, length: int, new_pages) -> None:
+        """Rows ``children`` of the page table go on from the first ``length`` positions of rows ``parents``, and have their tokens (one more
+        than positions: the next step's).  ``new_pages``: a page for each, for the copy of the last part page."""
+        stream = self.cuda_stream()
+        if self._pages is None:
+            self._pages = self.cache_pages()
+        with torch.cuda.stream(stream):
+            old, new, page, n = torch.tensor([list(parents), list(children), list(new_pages), [length] * len(parents)], dtype=torch.int32,
+                                             device=self._pages.workspace.device)
+            self._pages.fork(self.page_table(), old, new, n, page)
+            tokens = self.device_view("token_pool").view(torch.int32).view(self.config.max_running_req + 1, self.pt_cols)
+            tokens[new.long(), :length + 1] = tokens[old.long(), :length + 1]
+            stream.synchronize()   # (the index tensors may go)
+
+    def cuda_stream(self) -> torch.cuda.Stream:
+        """The stream that steps are enqueued on."""
+        return torch.cuda.ExternalStream(_lib.load().b200_engine_stream(self._h))
 
     # ------------------------------------------------------------------ steps
     def capture_graphs(self, batch_sizes: Sequence[int]) -> None:

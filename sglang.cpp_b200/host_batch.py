@@ -582,6 +582,40 @@ class HostBatcher:
         """Insert the page-aligned prefix of a request whose prefill finished (cache_req, not finished)."""
         self.cache_manager.cache_req(req, finished=False)
 
+    def fork(self, req: Req, copies: int) -> list:
+        """``copies`` requests that go on where ``req`` stands, for several answers to one prompt (no counterpart in the reference): they
+        share the whole pages of its sequence through the prefix cache and get copies of the last part page and of its tokens, the next
+        one's included.  Between steps; ``req.input_ids`` has to hold the tokens whose keys are cached."""
+        cm, P, n = self.cache_manager, self.page_size, req.cached_len
+        if not cm.enabled:
+            raise ValueError("fork: pages are shared through the prefix cache, which is off")
+        if not 0 <= copies <= 1024 or n <= 0 or len(req.input_ids) < n or req.is_chunked_prefill:
+            raise ValueError("fork: a request whose prompt has been read and whose tokens are known")
+        part, full = n % P, n // P * P
+        if copies > self.table_manager.available_size() or (part and copies * P > cm.available_size()):
+            raise ValueError("fork: not enough table rows or pages")
+        cm.cache_req(req, finished=False)
+        handle = req.cache_handle
+        if full:   # (the same tokens may be cached in other pages than the request's own, which are free then)
+            self.tables.write_pages(np.full(full, req.table_idx, np.int32), np.arange(full, dtype=np.int32), handle.matched_indices()[:full])
+        new = cm.allocate_pages(copies if part else 0)
+        rows, out = [], []
+        for _ in range(copies):
+            cm.lock(handle)
+            rows.append(self.table_manager.allocate())
+            self._next_uid += 1
+            self._held[rows[-1]] = -(-n // P)
+            out.append(Req(req.input_ids.copy(), rows[-1], n, req.device_len, req.max_device_len, self._next_uid, False, handle))
+        pages, tokens = self.tables.page_table, self.tables.token_pool
+        pages[rows, :full] = pages[req.table_idx, :full]
+        for row, slot in zip(rows, new):
+            end = min(full + P, pages.shape[1])
+            pages[row, full:end] = np.arange(slot, slot + end - full)
+        tokens[rows, :n + 1] = tokens[req.table_idx, :n + 1]
+        if self.engine is not None and copies:
+            self.engine.fork_rows([req.table_idx] * copies, rows, n, [slot // P for slot in new] if part else [0] * copies)
+        return out
+
     def slots_of(self, req: Req) -> np.ndarray:
         """The request's page-table row (one slot per position; unallocated positions read 0)."""
         return self.tables.page_table[req.table_idx]

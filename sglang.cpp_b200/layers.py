@@ -273,6 +273,18 @@ class MHAKVCache:
         self.k_buffer_ = self.kv_buffer_[0]
         self.v_buffer_ = self.kv_buffer_[1]
 
+    @classmethod
+    def over(cls, kv_buffer: torch.Tensor, page_size: int) -> "MHAKVCache":
+        """On memory that is there already (an engine's pool): contiguous bf16 [2, layers, slots, kv_heads, head_dim]."""
+        _cuda_bf16(kv_buffer, "kv_buffer")
+        _check(kv_buffer.dim() == 5 and kv_buffer.size(0) == 2 and kv_buffer.is_contiguous() and page_size > 0
+               and kv_buffer.size(2) % page_size == 0, "kv_buffer must be [2, layers, pages * page_size, kv_heads, head_dim]")
+        c = cls.__new__(cls)
+        _, c.num_layers_, c.total_slots, c.kv_heads_, c.head_dim_ = kv_buffer.shape
+        c.num_pages_, c.page_size_ = c.total_slots // page_size, page_size
+        c.kv_buffer_, c.k_buffer_, c.v_buffer_ = kv_buffer, kv_buffer[0], kv_buffer[1]
+        return c
+
     def k_cache(self, layer_id: int) -> torch.Tensor:
         return self.k_buffer_[layer_id]
 

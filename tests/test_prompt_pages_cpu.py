@@ -137,3 +137,80 @@ def test_oracles_on_known_answers():
     got, t2, where, used = compact_oracle(got, t, [0, 1, 3], [4, 3, 1], 2, 6, held=[5, 0])
     assert used == 4 and where.tolist() == [0, -1, 2, -1, 1, 3]
     assert t2[1].tolist() == [4, 5, 2, 3, -1, -1] and got[0, 0, 2:4, 0, 0].tolist() == [0, 9] and got[0, 0, 6:8, 0, 0].tolist() == [10, 11]
+
+
+def _batcher(pkg, page, pages=40, rows=8):
+    from sglang_cpp_b200.host_batch import HostBatcher
+    return HostBatcher(None, pages, page, rows, max_seq_len=64)
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+@pytest.mark.parametrize("length", [21, 32])
+def test_forked_requests_share_whole_pages(pkg, page, length):
+    hb = _batcher(pkg, page, pages=128 // page)
+    r = hb.add_request(np.arange(length), 20)
+    hb.allocate([r])
+    r.complete_one()
+    hb.tables.token_pool[r.table_idx, length] = 77
+    free = len(hb.cache_manager.free_pages)
+    kids = hb.fork(r, 3)
+    full, part = length // page * page, length % page
+    assert free - len(hb.cache_manager.free_pages) == (3 if part else 0)
+    mine = hb.slots_of(r)
+    own = set()
+    for k in kids:
+        row = hb.slots_of(k)
+        assert np.array_equal(row[:full], mine[:full]) and k.cached_len == length and k.device_len == length + 1
+        assert np.array_equal(hb.tables.token_pool[k.table_idx, :length + 1], list(range(length)) + [77])
+        if part:
+            assert row[full] % page == 0 and np.array_equal(row[full:full + page], np.arange(row[full], row[full] + page))
+            own.add(int(row[full]))
+    assert len(own) == (3 if part else 0) and not own & set(mine[:length].tolist())
+    # each goes on with tokens of its own, two of them with the same ones
+    reqs = [r] + kids
+    for step in range(9):
+        hb.allocate(reqs)
+        for i, q in enumerate(reqs):
+            q.append_host_token(100 * min(i, 2) + step)
+            q.complete_one()
+    used = [set(hb.slots_of(q)[full:q.cached_len].tolist()) for q in reqs]
+    assert all(not a & b for i, a in enumerate(used) for b in used[:i])
+    for q in reqs:
+        hb.release(q)
+    hb.cache_manager.check_integrity()
+    assert hb.cache_manager.prefix_cache.protected_size == 0 and len(hb.table_manager.free_rows) == 8
+
+
+def test_fork_of_a_prompt_that_is_cached_elsewhere(pkg):
+    """Two requests with one prompt in pages of their own: the second one, forked behind the first, goes over to the first one's pages."""
+    hb = _batcher(pkg, 4)
+    a, b = hb.add_request(np.arange(14), 9), hb.add_request(np.arange(14), 9)
+    hb.allocate([a, b])
+    for r in (a, b):
+        r.complete_one()
+    assert not set(hb.slots_of(a)[:14].tolist()) & set(hb.slots_of(b)[:14].tolist())
+    x = hb.fork(a, 1) + hb.fork(b, 2)
+    assert all(np.array_equal(hb.slots_of(k)[:12], hb.slots_of(a)[:12]) for k in x + [b])
+    for r in [a, b] + x:
+        hb.release(r)
+    hb.cache_manager.check_integrity()
+
+
+def test_fork_refusals(pkg):
+    hb = _batcher(pkg, 16, pages=4, rows=4)
+    r = hb.add_request(np.arange(20), 9)
+    with pytest.raises(ValueError):
+        hb.fork(r, 1)                 # nothing read yet
+    hb.allocate([r])
+    r.complete_one()
+    for copies in (-1, 4, 3, 1025):   # (four rows, one of them taken; two free pages)
+        with pytest.raises(ValueError):
+            hb.fork(r, copies)
+    r.complete_one()
+    with pytest.raises(ValueError):
+        hb.fork(r, 1)                 # a token that the host has not been told
+    r.append_host_token(5)
+    assert hb.fork(r, 0) == [] and len(hb.fork(r, 2)) == 2
+    hb.cache_manager.enabled = False
+    with pytest.raises(ValueError):
+        hb.fork(r, 1)

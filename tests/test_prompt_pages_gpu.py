@@ -700,3 +700,111 @@ def test_a_prompt_answered_several_times(L, page):
     assert_prompt((got, want[2][stay].float()), [x[stay] for x in want])
     assert torch.equal(paged.decode(nq[stay.tolist()], 0, t, *keep), got)
     assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("page,length", [(1, 37), (16, 37), (16, 48)])
+def test_an_engine_request_forked(pkg, page, length):
+    """Forked requests go on as requests with the same tokens in pages of their own do, whatever the others write."""
+    from oracle import token_loop_oracle as O
+    from sglang_cpp_b200.engine import Engine, EngineConfig
+    from sglang_cpp_b200.host_batch import HostBatcher
+
+    cfg = O.ModelConfig(3, 256, 4, 2, 128, 512, 2048, 1e-6, 1e6, 512, True, True, True)
+    weights = O.init_weights(cfg, seed=0, std=0.02)
+    ids = np.random.default_rng(5).integers(0, 2048, size=length).astype(np.int32)
+
+    def start(prefix_cache):
+        e = Engine(cfg, EngineConfig(page, 512 // page, 8, 512, 1024))
+        e.load_weights(weights)
+        return e, HostBatcher(e, 512 // page, page, 8, enable_prefix_cache=prefix_cache)
+
+    def decode(hb, reqs, steps):
+        out = []
+        for _ in range(steps):
+            next_token = hb.decode(reqs)
+            next_token.synchronize()
+            out.append(hb.engine.logits(len(reqs)).float())
+            for r, t in zip(reqs, next_token.next_tokens_cpu[:len(reqs)].tolist()):
+                r.append_host_token(t)
+        return torch.stack(out)
+
+    engine, hb = start(True)
+    first = hb.add_request(ids, 30)
+    tokens = hb.prefill([first])
+    tokens.synchronize()
+    answer = int(tokens.next_tokens_cpu[0])
+    first.append_host_token(answer)
+    kids = hb.fork(first, 3)
+    reqs = [first] + kids
+    said = [answer, 11, 1500, answer]              # two go on as they would have, two with another token
+    for r, t in zip(reqs, said):
+        r.input_ids = np.append(r.input_ids[:length], np.int32(t))
+    hb.tables.write_tokens([r.table_idx for r in reqs], [length] * 4, said)
+    got = decode(hb, reqs, 6)
+    assert torch.equal(got[:, 0], got[:, 3])
+    table = hb.tables.page_table
+    assert np.array_equal(engine.read_table("page_table")[:-1, :length], table[:-1, :length])   # (the last row is the dummy request's)
+    # a fork of a fork, in mid-answer
+    more = hb.fork(kids[0], 2)
+    again = decode(hb, kids[:1] + more, 3)
+    assert torch.equal(again[:, 0], again[:, 1]) and torch.equal(again[:, 0], again[:, 2])
+
+    plain, hb2 = start(False)
+    alone = [hb2.add_request(np.append(ids, np.int32(t)), 29) for t in said[:3]]
+    first_logits = []
+    for r in alone:                                # (prompts of one more token: their last row is the forked ones' first step)
+        tokens = hb2.prefill([r])
+        tokens.synchronize()
+        first_logits.append(plain.logits(1).float()[0])
+        r.append_host_token(int(tokens.next_tokens_cpu[0]))
+    assert float((got[0, :3] - torch.stack(first_logits)).abs().max()) <= 2e-2
+    tail = decode(hb2, alone, 5)
+    same = [i for i in range(3) if np.array_equal(reqs[i].input_ids[:length + 6], alone[i].input_ids[:length + 6])]
+    assert len(same) >= 2                          # (near ties of the logits may part them)
+    for i in same:
+        assert float((got[1:, i] - tail[:, i]).abs().max()) <= 2e-2
+    for r in reqs + more:
+        hb.release(r)
+    hb.cache_manager.check_integrity()
+    engine.synchronize()
+
+
+def test_an_engine_pool_counted_and_compacted(pkg, L):
+    """CachePages over an engine's pool, on its stream: the dummy request's page takes no part."""
+    from oracle import token_loop_oracle as O
+    from sglang_cpp_b200.engine import Engine, EngineConfig
+    from sglang_cpp_b200.host_batch import HostBatcher
+
+    cfg = O.ModelConfig(2, 256, 4, 2, 128, 512, 1024, 1e-6, 1e6, 512, True, True, True)
+    engine = Engine(cfg, EngineConfig(16, 32, 4, 512, 1024))
+    engine.load_weights(O.init_weights(cfg, seed=1, std=0.02))
+    hb = HostBatcher(engine, 32, 16, 4, enable_prefix_cache=False)
+    reqs = [hb.add_request(np.arange(n, dtype=np.int32) + 7, 20) for n in (50, 33, 70)]
+    hb.prefill(reqs).synchronize()
+    for r in reqs:
+        r.append_host_token(3)
+        hb.tables.write_tokens([r.table_idx], [r.cached_len], [3])
+    hb.release(reqs.pop(0))
+    hb.decode(reqs).synchronize()
+    before = engine.logits(2).clone()
+    pages = engine.cache_pages()
+    assert pages.pages_ == 32
+    stream = engine.cuda_stream()
+    rows, lens = [r.table_idx for r in reqs], [r.cached_len for r in reqs]
+    with torch.cuda.stream(stream):
+        refs, free, number = pages.count(engine.page_table(), *ints(rows, lens))
+        where, used = pages.compact(engine.page_table(), *ints(rows, lens))
+        stream.synchronize()
+    held = sum(-(-n // 16) for n in lens)
+    assert int(used) == held and int(number) == 32 - held and int(refs.sum()) == held
+    table = engine.read_table("page_table")
+    for r, n in zip(rows, lens):
+        assert np.array_equal(table[r, :n], where.cpu().numpy()[hb.tables.page_table[r, :n] // 16] * 16 + np.arange(n) % 16)
+    # the same step once more, from the moved pages
+    for r in reqs:
+        r.cached_len -= 1
+        r.device_len -= 1
+    engine.forward_batch(1, rows, [r.cached_len for r in reqs], [1] * 2, write_pos=[-1] * 2).synchronize()
+    assert torch.equal(engine.logits(2), before)
+    with pytest.raises(L.B200Error):
+        L.MHAKVCache.over(torch.zeros(2, 1, 30, 2, 64, dtype=bf16, device="cuda"), 16)
