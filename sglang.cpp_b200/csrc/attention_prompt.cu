@@ -620,7 +620,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                     for (int c = 0; c < 4; ++c) {
                         uint32_t packed[16];
                         if (c == 2 && half_only) {
-                            if (keys16 > 64) {
+                            if (kt + 1 < mine || keys16 > kTile / 2) {
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) packed[i] = 0;
                                 tmem_st_32x32b_x16(p_addr + 32, packed);

@@ -35,6 +35,12 @@ PROMPTS = {   # lengths, heads, KV heads, head dimension
     "heads of 8": ([150, 33], 8, 2, 8),
     "heads of 40": ([150, 33], 6, 2, 40),
     "long": ([2500, 700], 16, 2, 128),
+    "three heads per KV head, long": ([1700, 800], 6, 2, 64),
+    "five heads per KV head, long": ([1500], 10, 2, 128),
+    "six heads per KV head, long": ([1300, 900], 12, 2, 96),
+    "eleven heads per KV head, long": ([1100], 22, 2, 64),
+    "forty heads per KV head, long": ([700], 40, 1, 128),
+    "sixty-five heads per KV head": ([400], 65, 1, 64),
     "many of all lengths": ([1 + 37 * i % 211 for i in range(90)], 8, 4, 64),
     "a long one among short ones": ([5] * 20 + [1700] + [9] * 30, 8, 8, 128),
 }
