@@ -9,17 +9,34 @@
 //     softmax              one thread per row takes its 128 scores to registers, keeps a reference maximum and the sum, and writes
 //                          the probabilities to TMEM as bf16
 //     O += P V             P the A operand from TMEM, V MN-major from the layout that TMA delivers, O in TMEM for the whole row
-// The reference is moved only where a row's maximum has outgrown it by 2^8 (sum and division use the same reference: exact), so that a
-// tile behind the first is exponentiated with the reference as it stands while its maximum is found beside, and once more in the rare
-// case that the reference has to move.
+// The reference is the maximum of a row's first tile, and moves only where a later tile's probabilities add up to more than 2^24 (sum and
+// division use the same reference: exact; weights and sums are floating-point numbers, as right for 2^24 as for 1).  Tiles behind the first
+// therefore need no maximum: they are exponentiated at once, and once more in the rare case that the sum says so.
 //
 // A CTA per SM walks over items, the longest of all sequences and heads first, in turns that change direction.  Roles: warp 0 finds the
-// items and fetches Q and K, warp 2 V, one thread of warp 1 issues S, one of warp 3 P V, warps 4-7 and 8-11 are the softmax of the two tiles.
-// Each goes on to its next item by itself, so that an item's output is written while the next one's first products run.
+// items and fetches Q and K, warp 2 V, one thread of warp 1 issues S, one of warp 3 P V, warps 4-7 and 8-11 are the softmax of the two tiles,
+// warps 12-15 write results.  Each goes on to its next item by itself, so that an item's results are written while the next one's first products
+// run.
 //
 // Keys behind a row are masked as scores; as values they meet weights of 0, which is right for numbers only.  Rows behind a sequence
-// become zeros in shared memory; where a row's result is no number, values that it does not see are looked through, and if one is to
-// blame the row is summed up once more without them.
+// become zeros in shared memory; where a row's result is no number, values that it does not see are looked through at the end, and if one
+// is to blame the row is summed up once more without them.
+//
+// What bounds it: for long prompts products and exponentials, 2048 cycles each per K/V tile and pair of query tiles (68 % of the tensor pipe, 68 % of
+// the units for exponentials), and power: 2 x 8000 tokens of 32 / 8 heads run at 1.2 to 1.3 PFLOP/s, the library's products at 1.43 sustained.
+// For short ones the chain of an item's steps (first copies, S, softmax, P V, results) with half of either pipe idle.  What cost most on the
+// way there was code: roles that run side by side share small instruction caches, and cold code ran at 5 cycles per instruction and more.
+// The steps (us, replays; 64 texts of 1 to 700 tokens, 32 / 8 heads / 7 of 333 to 2100, 24 / 8 heads of 64 / 2 of 7900 to 8192, 32 / 8):
+//     a warp per row and head, without tensor cores                                       13348 / 7672 / 154089
+//     tensor cores; the softmax warps write results, the tiles take turns at exponentials   315 / 107 / 1171
+//     without turns                                                                         228 / 89 / 983
+//     masks 32 keys at a time, results in a loop, V looked through only if need be          166 / 70 / 930
+//     results by warps of their own; no maximum behind the first tile                       187 / 78 / 938
+//     ... waits of a few instructions, loops over the two tiles (132 -> 80 KB of code)      143 / 58 / 856
+//     halves of a tile that no row of a warp sees left out                                  139 / 56 / 850
+// Tried and left: an item's rows on their way to L2 ahead of it (no faster, 8 % slower with all of them); masked tiles 32 keys at a time in loops of
+// their own (single tokens 88 -> 76, but 2 x 8000 tokens 846 -> 943); quarters instead of halves left out (2 x 8000 856 -> 910); results 32
+// columns at a time (registers spill: 143 -> 211).
 #include "common.cuh"
 #include "kernels.h"
 #include "tcgen05.cuh"
@@ -37,7 +54,7 @@ static_assert(128 * (2 * kFewRegs + 2 * kSoftmaxRegs) <= kThreads * 128, "");
 constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16 under the 128-byte swizzle
 constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns
 constexpr int kAgain = 2048;                // query tiles of a CTA that are noted one by one
-constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more
+constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more (products with values up to 2^100 fit)
 
 // Sizes by the padded head dimension.
 template <int DP>

@@ -1,4 +1,16 @@
 // Pages of a cache: copied, shared by rows that go on from other rows, counted, moved to the front of the pool.
+//
+//   copy     the first tokens[i] slots of page src[i] -> page dst[i], in every plane
+//   fork     table[child, j] = table[parent, j] for whole pages of the first len positions; the len mod page tokens behind them are copied to a
+//            new page, whose slots the row names from there on
+//   count    refs[g] = how many (row, page of the row's length) pairs name page g; free = the pages with refs 0, ascending
+//   compact  U = the number of pages with refs > 0; the i-th of them at U or behind moves to the i-th free page below U; the rows' slots
+//            follow: a page's new number is itself below U, otherwise dst[rank among the late ones]
+//
+// Copies are bound by memory: 2 bytes of traffic per byte at 0.97 to 0.98 of the measured copy bandwidth where hundreds of pages move.  Everything
+// else is a few thousand integers: launches, trips to memory in a chain and barriers.  So a copy of few pages is one launch, counting a
+// small pool one CTA, and the kernels of a longer chain start ahead of the end of the one before.
+// Nothing depends on the order of atomics: counts are sums, and lists are made by ranks.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -8,9 +20,8 @@ namespace {
 constexpr int kMaxFork = 1024;        // entries of a fork call
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnit = 512;            // bytes that a warp moves with one vector per lane; four of them at a time
-constexpr int kFewPairs = 128;        // pairs of a copy call that every CTA looks through by itself
-constexpr int kSmallPool = 40960;     // pages that one CTA counts in its shared memory ...
-constexpr int64_t kSmallHeld = 65536; // ... where no more than that many are held
+constexpr int kFewPairs = 32;         // pairs of a copy call that every CTA looks through by itself
+constexpr int kSmallPool = 12000;     // pages, and five quarters of those held, that one CTA counts in its shared memory
 constexpr int kWords = 8;             // of 32 pages that a warp ranks where many CTAs do (32: 7 us to mark a million pages, 8: 3)
 constexpr int kChunk = kWarps * kWords * 32;
 
@@ -596,9 +607,12 @@ int check_held(const char* name, const HeldParams& p) {
     return B200_OK;
 }
 
-// Do the pages and their holders fit one CTA?  (Lengths are on the device: rows may be as long as the table's.)
+// Does one CTA count them sooner than many, in four launches?  (Lengths are on the device: rows may be as long as the table's.)  us by one, by many:
+// 1000 pages of which 800 are held 3.7, 8.5, 9600 times held 6.6, 10.2, 64000 times 18, 14; 9000 pages 5.8, 6.8 and 8.7, 7.1 and 20, 8.2; 20000
+// pages 8.0, 6.9.
 bool small(const HeldParams& p) {
-    return p.num_pages <= kSmallPool && div_ceil64(p.table.cols, p.page_size) * p.count + p.held_count <= kSmallHeld;
+    const int64_t held = div_ceil64(p.table.cols, p.page_size) * p.count + p.held_count;
+    return p.num_pages + held * 5 / 4 <= kSmallPool;
 }
 // The pages held, counted and as bits, by many CTAs.
 int launch_held(const HeldParams& p, int32_t* refs, uint32_t* bits, int32_t* counts, int chunks, cudaStream_t stream) {
@@ -648,15 +662,17 @@ int b200_copy_pages(const b200_page_pool* pool, const int32_t* src, const int32_
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const Units units = units_of(p);
     const int grid = move_grid(p, units, count, true);
-    // Few pairs: each CTA compares its own with all (700 of 1.8 MB: 5 us less than with a kernel for that).  Many: one CTA, with a bit per page.
+    // Few pairs that all SMs move at once: every CTA compares all of them.  Others: one CTA does, with a bit per page, ahead of the copies.  (us
+    // with that kernel, without: 1 page of 1.8 MB 5.6, 3.7; 16 12.4, 13.5; 128 78, 228; 16 pages of 115 KB 5.7, 4.1; 64 7.1, 7.8; 64 of 1 KB 5.3, 5.5.)
     int32_t* slots = nullptr;
-    if (count > kFewPairs) {
+    const bool ahead = count > kFewPairs || grid > sm_count() * 8;
+    if (ahead) {
         const Scratch w = scratch_in(workspace, x);
         slots = w.ints[0];
         B200_CHECK_CUDA(launch_kernel(copy_check_kernel, dim3(1), dim3(1024), 0, s, dim3(1, 1, 1), src, dst, tokens, count, p.page_size, p.num_pages,
                                       div_ceil(p.num_pages, 32), w.bits, w.bits2, slots, status));
     }
-    FollowOn follow(count > kFewPairs);
+    FollowOn follow(ahead);
     B200_CHECK_CUDA(launch_kernel(copy_pages_kernel, dim3(grid), dim3(kThreads), 0, s, dim3(1, 1, 1), p, units, src, dst, tokens, slots, count, status));
     return B200_OK;
 }
@@ -684,7 +700,9 @@ int b200_fork_rows(const b200_page_pool* pool, int32_t* page_table, int64_t tabl
     p.lens = lens;
     p.new_pages = new_pages;
     p.count = count;
-    const int parts = max(1, min(div_ceil(sm_count() * 8, count), 64));
+    // (96 rows with half a page of 8.4 MB each: 32.5 us with CTAs for eight per SM, 31.1 with sixteen, 32.2, 34.5, 37.6 with 24, 32, 48: each compares
+    // the entries.)
+    const int parts = max(1, min(div_ceil(sm_count() * 16, count), 64));
     B200_CHECK_CUDA(launch_kernel(fork_rows_kernel, dim3(parts, count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), dim3(1, 1, 1), p));
     return B200_OK;
 }
