@@ -21,7 +21,7 @@ constexpr int kMaxFork = 1024;        // entries of a fork call
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnit = 512;            // bytes that a warp moves with one vector per lane; four of them at a time
 constexpr int kFewPairs = 32;         // pairs of a copy call that every CTA looks through by itself
-constexpr int kSmallPool = 12000;     // pages, and five quarters of those held, that one CTA counts in its shared memory
+constexpr int kSmallPool = 24000;     // pages, and five quarters of those held, that one CTA counts in its shared memory
 constexpr int kWords = 8;             // of 32 pages that a warp ranks where many CTAs do (32: 7 us to mark a million pages, 8: 3)
 constexpr int kChunk = kWarps * kWords * 32;
 
@@ -608,8 +608,9 @@ int check_held(const char* name, const HeldParams& p) {
 }
 
 // Does one CTA count them sooner than many, in four launches?  (Lengths are on the device: rows may be as long as the table's.)  us by one, by many:
-// 1000 pages of which 800 are held 3.7, 8.5, 9600 times held 6.6, 10.2, 64000 times 18, 14; 9000 pages 5.8, 6.8 and 8.7, 7.1 and 20, 8.2; 20000
-// pages 8.0, 6.9.
+// 1000 pages of which 800 are held 3.3, 8.5, 9600 times held 6.6, 8.4, 64000 times 18, 13; 9000 pages 5.2, 6.8 and 8.7, 6.7 and 20, 8.0; 20000
+// pages 8.0, 6.7.  Three launches less are 5 us of the caller's time besides (64 rows of up to 2000 tokens, 9000 pages of 16: a call that nothing
+// captures 13.8 by one, 19.2 by many), so that one CTA may take 2 us longer.
 bool small(const HeldParams& p) {
     const int64_t held = div_ceil64(p.table.cols, p.page_size) * p.count + p.held_count;
     return p.num_pages + held * 5 / 4 <= kSmallPool;
