@@ -23,7 +23,7 @@
 // is to blame the row is summed up once more without them.
 //
 // What bounds it: for long prompts products and exponentials, 2048 cycles each per K/V tile and pair of query tiles (68 % of the tensor pipe, 68 % of
-// the units for exponentials), and power: 2 x 8000 tokens of 32 / 8 heads run at 1.2 to 1.3 PFLOP/s, the library's products at 1.43 sustained.
+// the units for exponentials), and power: 2 x 8000 tokens of 32 / 8 heads run at 1.16 to 1.17 PFLOP/s one behind another, up to 1.34 with idle time between; the library's products at 1.43 sustained.
 // For short ones the chain of an item's steps (first copies, S, softmax, P V, results) with half of either pipe idle.  What cost most on the
 // way there was code: roles that run side by side share small instruction caches, and cold code ran at 5 cycles per instruction and more.
 // The steps (us, replays; 64 texts of 1 to 700 tokens, 32 / 8 heads / 7 of 333 to 2100, 24 / 8 heads of 64 / 2 of 7900 to 8192, 32 / 8):
@@ -33,7 +33,7 @@
 //     masks 32 keys at a time, results in a loop, V looked through only if need be          166 / 70 / 930
 //     results by warps of their own; no maximum behind the first tile                       187 / 78 / 938
 //     ... waits of a few instructions, loops over the two tiles (132 -> 80 KB of code)      143 / 58 / 856
-//     halves of a tile that no row of a warp sees left out                                  139 / 56 / 850
+//     halves of a tile that no row of a warp sees left out                                  141 / 54 / 874
 // Tried and left: an item's rows on their way to L2 ahead of it (no faster, 8 % slower with all of them); masked tiles 32 keys at a time in loops of
 // their own (single tokens 88 -> 76, but 2 x 8000 tokens 846 -> 943); quarters instead of halves left out (2 x 8000 856 -> 910); results 32
 // columns at a time (registers spill: 143 -> 211).
