@@ -334,7 +334,7 @@ B200_API int b200_attention_shared_prefix(const b200_shared_prefix_args* args, b
  * they were.  An indptr that decreases or leaves [0, tokens] is reported as tokens + 1 in the status words, and nothing is written.
  * An infinity or NaN among keys and values reaches the rows that see it and no others.
  * bf16; head_dim a multiple of 8 up to 128; q_heads a multiple of kv_heads with up to 128 heads per KV head; up to 1024 sequences.  q, k, v 16-byte
- * aligned, their strides positive multiples of 8. */
+ * aligned, their strides positive multiples of 8.  out and lse overlap none of the inputs. */
 typedef struct b200_prompt_attention_args {
     void* out;
     float* lse;
@@ -351,7 +351,8 @@ B200_API int b200_attention_prompt(const b200_prompt_attention_args* args, b200_
 
 /* A pool of num_planes arrays (keys and values of every layer: 2 * layers planes of one allocation) of num_pages pages of page_size
  * slots of slot_bytes each, plane_stride bytes apart: slot s of plane l begins at planes + l * plane_stride + s * slot_bytes; page g is
- * slots [g * page_size, (g + 1) * page_size).  Any type; slot_bytes, plane_stride and planes multiples of 16; num_pages * page_size below 2^31.
+ * slots [g * page_size, (g + 1) * page_size).  Any type; slot_bytes, plane_stride and planes multiples of 16; num_pages * page_size below 2^31,
+ * num_pages at most 2^30.
  * num_pages may leave out the last pages of the allocation (a dummy request's): they are then no pages for these calls. */
 typedef struct b200_page_pool {
     void* planes;
@@ -372,7 +373,7 @@ B200_API int b200_copy_pages(const b200_page_pool* pool, const int32_t* src, con
 /* Rows of a page table (int32 [table_rows, table_cols], a slot per position, rows page_table_stride apart) that go on from other rows:
  * row children[i] gets positions [0, lens[i]) of row parents[i].  Whole pages are shared; where lens[i] ends inside a page, the tokens of
  * that part are copied to page new_pages[i] in every plane, whose slots the child's row names up to the page's end (new_pages[i] is not looked
- * at elsewhere).  Other positions of the row stay.  All arrays [count] on the device, count <= 1024.  Left out and
+ * at elsewhere): pages that no row nor anybody else holds, which is the caller's to see to.  Other positions of the row stay.  All arrays [count] on the device, count <= 1024.  Left out and
  * reported in the status words: an entry whose rows, length, part page or new page there are not (that value + 1), one that has a row as both child and
  * parent, or a child that another entry has as child or parent (row + 1), and one whose new page another entry also takes or
  * copies from (page + 1). */
@@ -383,7 +384,7 @@ B200_API int b200_fork_rows(const b200_page_pool* pool, int32_t* page_table, int
 /* Which pages are held, and which are free, once rows of a page table share pages: refs[g] = how many of the rows rows[i] of lens[i]
  * positions (i < count) hold page g, plus how often `held` names it (pages that somebody holds outside the table, a prefix cache
  * for instance; NULL with held_count 0); free_pages = the pages with refs 0 in ascending order, then -1; free_count their number.
- * refs, free_pages int32 [num_pages], free_count int32 [1].  A row named twice counts twice.  Lengths are cut to [0, table_cols].
+ * refs, free_pages int32 [num_pages], free_count int32 [1]; count up to 2^20, held_count up to 2^30.  A row named twice counts twice.  Lengths are cut to [0, table_cols].
  * Rows, slots and pages that there are not count for nothing and are reported in the status words (that value + 1). */
 B200_API int b200_count_pages(int32_t* refs, int32_t* free_pages, int32_t* free_count, const int32_t* page_table,
                               int64_t table_rows, int64_t page_table_stride, int64_t table_cols, const int32_t* rows,
@@ -392,7 +393,7 @@ B200_API int b200_count_pages(int32_t* refs, int32_t* free_pages, int32_t* free_
 
 /* Pages in use moved to the front: with U pages held (as b200_count_pages counts), the i-th held page from U on moves to the i-th free
  * page below U, in every plane; map[g] = where page g is now (g itself for most), -1 for a page that nobody held; used[0] = U.
- * table_out (rows table_out_stride apart; may be the page table itself) gets the new slots of positions [0, lens[i]) of the rows,
+ * table_out (rows table_out_stride apart; the page table itself, or memory that overlaps none of it) gets the new slots of positions [0, lens[i]) of the rows,
  * to the end of each last page as far as table_cols reach; nothing else of it is written.  The moved pages' old places keep their contents.
  * Reports as b200_count_pages does.  Pools of other shapes behind the same table follow with b200_copy_pages from
  * page g to map[g]. */

@@ -22,6 +22,8 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnit = 512;            // bytes that a warp moves with one vector per lane; four of them at a time
 constexpr int kFewPairs = 32;         // pairs of a copy call that every CTA looks through by itself
 constexpr int kSmallPool = 24000;     // pages, and five quarters of those held, that one CTA counts in its shared memory
+// Counters of int go on by up to a grid's threads behind the last page or number; the rows' pages are multiplied in 64 bits.
+constexpr int kMaxPages = 1 << 30, kMaxRows = 1 << 20;
 constexpr int kWords = 8;             // of 32 pages that a warp ranks where many CTAs do (32: 7 us to mark a million pages, 8: 3)
 constexpr int kChunk = kWarps * kWords * 32;
 
@@ -577,6 +579,7 @@ int check_pool(const b200_page_pool* pool, const char* name, Pool* out) {
     B200_CHECK_ARG(pool != nullptr, "%s: NULL pool", name);
     B200_CHECK_ARG(pool->page_size >= 1 && pool->num_pages >= 1 && static_cast<int64_t>(pool->page_size) * pool->num_pages <= 0x7fffffff,
                    "%s: page_size and num_pages must be positive, of fewer than 2^31 slots", name);
+    B200_CHECK_ARG(pool->num_pages <= kMaxPages, "%s: num_pages must be at most 2^30", name);
     B200_CHECK_ARG(pool->num_planes >= 1 && static_cast<int64_t>(pool->num_planes) * pool->num_pages <= 0x7fffffff,
                    "%s: num_planes must be positive, with fewer than 2^31 pages in all planes", name);
     B200_CHECK_ARG(pool->slot_bytes >= 16 && pool->slot_bytes % 16 == 0, "%s: slot_bytes must be a positive multiple of 16", name);
@@ -601,7 +604,8 @@ int check_workspace(const char* name, const void* workspace, int64_t bytes, cons
 int check_held(const char* name, const HeldParams& p) {
     int err = check_table(name, p.table.rows, p.table.stride, p.table.cols);
     if (err != B200_OK) return err;
-    B200_CHECK_ARG(p.count >= 0 && p.held_count >= 0, "%s: count and held_count must not be negative", name);
+    B200_CHECK_ARG(p.count >= 0 && p.count <= kMaxRows && p.held_count >= 0 && p.held_count <= kMaxPages,
+                   "%s: count must be in [0, 2^20] and held_count in [0, 2^30]", name);
     B200_CHECK_ARG(p.count == 0 || (p.rows && p.lens && (p.table.slots || p.table.rows * p.table.cols == 0)), "%s: NULL tensor", name);
     B200_CHECK_ARG(p.held_count == 0 || p.held, "%s: NULL tensor", name);
     return B200_OK;
@@ -715,6 +719,7 @@ int b200_count_pages(int32_t* refs, int32_t* free_pages, int32_t* free_count, co
     using namespace b200;
     B200_CHECK_ARG(page_size >= 1 && num_pages >= 1 && static_cast<int64_t>(page_size) * num_pages <= 0x7fffffff,
                    "count_pages: page_size and num_pages must be positive, of fewer than 2^31 slots");
+    B200_CHECK_ARG(num_pages <= kMaxPages, "count_pages: num_pages must be at most 2^30");
     B200_CHECK_ARG(refs && free_pages && free_count, "count_pages: NULL tensor");
     HeldParams p{Table{page_table, table_rows, page_table_stride, table_cols}, rows, lens, held, count, held_count, page_size, num_pages, nullptr};
     int err = check_held("count_pages", p);

@@ -214,3 +214,17 @@ def test_fork_refusals(pkg):
     hb.cache_manager.enabled = False
     with pytest.raises(ValueError):
         hb.fork(r, 1)
+
+
+@pytest.mark.parametrize("call,pool,change,text", [
+    ("count", {}, dict(count=(1 << 20) + 1), "count"), ("count", {}, dict(count=0x7fffffff), "count"),
+    ("count", {}, dict(held=P, held_count=(1 << 30) + 1), "count"), ("count", {}, dict(held=P, held_count=0x7fffffff), "count"),
+    ("compact", {}, dict(count=0x7fffffff), "count"), ("compact", {}, dict(held=P, held_count=0x7fffffff), "count"),
+    ("count", {}, dict(page_size=1, num_pages=(1 << 30) + 1, ws_bytes=1 << 40), "num_pages"),
+    ("copy", dict(page_size=1, num_planes=1, num_pages=0x7fffffff), dict(copies=0x7fffffff, ws_bytes=1 << 40), "num_pages"),
+    ("compact", dict(page_size=1, num_planes=1, num_pages=0x7fffffff), dict(ws_bytes=1 << 40), "num_pages"),
+])
+def test_numbers_that_loop_counters_would_pass(pkg, call, pool, change, text):
+    """Counters of int go on by up to 2^22 behind the last number: 2^30 leaves room."""
+    lib = pkg.load_library()
+    assert _calls(lib, _pool(**pool), **change)[call]() == 1 and text in lib.b200_last_error().decode(), lib.b200_last_error()
