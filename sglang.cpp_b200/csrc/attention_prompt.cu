@@ -20,7 +20,8 @@
 //
 // Keys behind a row are masked as scores; as values they meet weights of 0, which is right for numbers only.  Rows behind a sequence
 // become zeros in shared memory; where a row's result is no number, values that it does not see are looked through at the end, and if one
-// is to blame the row is summed up once more without them.
+// is to blame the row is summed up once more without them, a thread per row (16 / 8 heads, one block behind 8000 keys: 78 ms; 115 with one load at a time).
+// It is rare, and code that ran it faster would stand in the way of the rest.
 //
 // What bounds it: for long prompts products and exponentials, 2048 cycles each per K/V tile and pair of query tiles (68 % of the tensor pipe, 68 % of
 // the units for exponentials), and power: 2 x 8000 tokens of 32 / 8 heads run at 1.16 to 1.17 PFLOP/s one behind another, up to 1.34 with idle time between; the library's products at 1.43 sustained.
@@ -33,7 +34,7 @@
 //     masks 32 keys at a time, results in a loop, V looked through only if need be          166 / 70 / 930
 //     results by warps of their own; no maximum behind the first tile                       187 / 78 / 938
 //     ... waits of a few instructions, loops over the two tiles (132 -> 80 KB of code)      143 / 58 / 856
-//     halves of a tile that no row of a warp sees left out                                  141 / 54 / 874
+//     halves of a tile that no row of a warp sees left out                                  139 to 141 / 54 to 62 / 874 to 891
 // Tried and left: an item's rows on their way to L2 ahead of it (no faster, 8 % slower with all of them); masked tiles 32 keys at a time in loops of
 // their own (single tokens 88 -> 76, but 2 x 8000 tokens 846 -> 943); quarters instead of halves left out (2 x 8000 856 -> 910); results 32
 // columns at a time (registers spill: 143 -> 211).
@@ -212,7 +213,7 @@ __device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, 
 #pragma unroll 1
         for (int key = 0; key <= tok; ++key) {
             float s = 0.f;
-#pragma unroll 1
+#pragma unroll 4
             for (int d = 0; d < p.dim; d += 8) {
                 const Vec8 a = load8(q + d), b = load8(k + key * p.k_st + d);
 #pragma unroll
