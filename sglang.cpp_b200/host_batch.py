@@ -585,10 +585,13 @@ class HostBatcher:
     def fork(self, req: Req, copies: int) -> list:
         """``copies`` requests that go on where ``req`` stands, for several answers to one prompt (no counterpart in the reference): they
         share the whole pages of its sequence through the prefix cache and get copies of the last part page and of its tokens, the next
-        one's included.  Between steps; ``req.input_ids`` has to hold the tokens whose keys are cached."""
+        one's included.  Between steps; ``req.input_ids`` has to hold the tokens whose keys are cached.  Engines whose layers are listed one by
+        one do not fork (a pool per layer).  A fork that is refused, or that the engine cannot do, takes no rows, pages or locks."""
         cm, P, n = self.cache_manager, self.page_size, req.cached_len
         if not cm.enabled:
             raise ValueError("fork: pages are shared through the prefix cache, which is off")
+        if getattr(self.engine, "stack", False):
+            raise ValueError("fork: the engine has a pool per layer, whose pages are not copied")
         if not 0 <= copies <= 1024 or n <= 0 or len(req.input_ids) < n or req.is_chunked_prefill:
             raise ValueError("fork: a request whose prompt has been read and whose tokens are known")
         part, full = n % P, n // P * P
@@ -599,21 +602,27 @@ class HostBatcher:
         if full:   # (the same tokens may be cached in other pages than the request's own, which are free then)
             self.tables.write_pages(np.full(full, req.table_idx, np.int32), np.arange(full, dtype=np.int32), handle.matched_indices()[:full])
         new = cm.allocate_pages(copies if part else 0)
-        rows, out = [], []
-        for _ in range(copies):
+        rows = [self.table_manager.allocate() for _ in range(copies)]
+        if self.engine is not None and copies:
+            try:
+                self.engine.fork_rows([req.table_idx] * copies, rows, n, [slot // P for slot in new] if part else [0] * copies)
+            except BaseException:   # (nobody is told of these rows and pages)
+                for row in reversed(rows):
+                    self.table_manager.free(row)
+                cm.free_pages = new + cm.free_pages
+                raise
+        out = []
+        for row in rows:
             cm.lock(handle)
-            rows.append(self.table_manager.allocate())
             self._next_uid += 1
-            self._held[rows[-1]] = -(-n // P)
-            out.append(Req(req.input_ids.copy(), rows[-1], n, req.device_len, req.max_device_len, self._next_uid, False, handle))
+            self._held[row] = -(-n // P)
+            out.append(Req(req.input_ids.copy(), row, n, req.device_len, req.max_device_len, self._next_uid, False, handle))
         pages, tokens = self.tables.page_table, self.tables.token_pool
         pages[rows, :full] = pages[req.table_idx, :full]
         for row, slot in zip(rows, new):
             end = min(full + P, pages.shape[1])
             pages[row, full:end] = np.arange(slot, slot + end - full)
         tokens[rows, :n + 1] = tokens[req.table_idx, :n + 1]
-        if self.engine is not None and copies:
-            self.engine.fork_rows([req.table_idx] * copies, rows, n, [slot // P for slot in new] if part else [0] * copies)
         return out
 
     def slots_of(self, req: Req) -> np.ndarray:

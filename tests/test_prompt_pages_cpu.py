@@ -228,3 +228,42 @@ def test_numbers_that_loop_counters_would_pass(pkg, call, pool, change, text):
     """Counters of int go on by up to 2^22 behind the last number: 2^30 leaves room."""
     lib = pkg.load_library()
     assert _calls(lib, _pool(**pool), **change)[call]() == 1 and text in lib.b200_last_error().decode(), lib.b200_last_error()
+
+
+class _Refuses:
+    """An engine whose fork fails; ``stack``: one that has a pool per layer."""
+
+    def __init__(self, cols, stack):
+        self.pt_cols, self.stack, self.forks = cols, stack, 0
+
+    def write_page_table(self, *a):
+        pass
+
+    write_token_pool = write_page_table
+
+    def fork_rows(self, *a):
+        self.forks += 1
+        raise RuntimeError("no")
+
+
+@pytest.mark.parametrize("stack", [False, True])
+@pytest.mark.parametrize("length", [21, 32])
+def test_a_fork_that_the_engine_refuses_takes_nothing(pkg, stack, length):
+    from sglang_cpp_b200.host_batch import HostBatcher
+    engine = _Refuses(64, stack)
+    hb = HostBatcher(engine, 8, 16, 4)
+    cm = hb.cache_manager
+    r = hb.add_request(np.arange(length), 9)
+    hb.allocate([r])
+    r.complete_one()
+    hb.cache_prefix(r)
+    rows, pages, table, uid = list(hb.table_manager.free_rows), list(cm.free_pages), hb.tables.page_table.copy(), hb._next_uid
+    protected = cm.prefix_cache.protected_size
+    with pytest.raises(ValueError if stack else RuntimeError):
+        hb.fork(r, 3)
+    assert engine.forks == (0 if stack else 1)
+    assert hb.table_manager.free_rows == rows and cm.free_pages == pages and hb._next_uid == uid
+    assert cm.prefix_cache.protected_size == protected and np.array_equal(hb.tables.page_table, table)
+    hb.release(r)
+    cm.check_integrity()
+    assert cm.prefix_cache.protected_size == 0 and len(hb.table_manager.free_rows) == 4 and not hb._held
