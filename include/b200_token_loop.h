@@ -361,7 +361,7 @@ typedef struct b200_page_pool {
     int32_t num_planes, slot_bytes, page_size, num_pages;
 } b200_page_pool;
 
-/* Bytes of scratch of the calls below for a pool of so many pages.  Not initialised; calls that share it run one after another
+/* Bytes of scratch of the calls below for a pool of so many pages (-1: there are no pools of so many).  Not initialised; calls that share it run one after another
  * (so does the replay of graphs that captured them). */
 B200_API int64_t b200_pages_workspace_bytes(int num_pages);
 

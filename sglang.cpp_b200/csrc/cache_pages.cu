@@ -646,7 +646,7 @@ int launch_small(Kernel kernel, const HeldParams& p, cudaStream_t stream, Args..
 extern "C" {
 
 int64_t b200_pages_workspace_bytes(int num_pages) {
-    if (num_pages < 1) return -1;
+    if (num_pages < 1 || num_pages > b200::kMaxPages) return -1;
     return b200::layout_of(num_pages).bytes;
 }
 

@@ -267,3 +267,9 @@ def test_a_fork_that_the_engine_refuses_takes_nothing(pkg, stack, length):
     hb.release(r)
     cm.check_integrity()
     assert cm.prefix_cache.protected_size == 0 and len(hb.table_manager.free_rows) == 4 and not hb._held
+
+
+def test_pages_workspace_of_more_pages_than_there_may_be(pkg):
+    size = pkg.load_library().b200_pages_workspace_bytes
+    assert size(1 << 30) > size((1 << 30) - 100_000) > 3 * 4 * ((1 << 30) - 100_000)
+    assert [size(n) for n in ((1 << 30) + 1, 2 ** 31 - 2048, 2 ** 31 - 1)] == [-1] * 3
