@@ -220,7 +220,8 @@ __device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, 
                 for (int e = 0; e < 8; ++e) s = fmaf(a.v[e], b.v[e], s);
             }
             s *= p.scale_log2;
-            const float now = fmaxf(m, s), old = now == -INFINITY ? 1.f : exp2f(m - now), w = now == -INFINITY ? 0.f : exp2f(s - now);
+            const float now = fmaxf(m, s), old = now == -INFINITY ? 1.f : exp2f(m - now);
+            const float w = now > -INFINITY ? exp2f(s - now) : s == -INFINITY ? 0.f : s;   // (a score that is no number is a weight that is none)
             m = now;
             sum = fmaf(sum, old, w);
 #pragma unroll

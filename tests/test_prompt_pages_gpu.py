@@ -814,3 +814,51 @@ def test_an_engine_pool_counted_and_compacted(pkg, L):
     assert torch.equal(engine.logits(2), before)
     with pytest.raises(L.B200Error):
         L.MHAKVCache.over(torch.zeros(2, 1, 30, 2, 64, dtype=bf16, device="cuda"), 16)
+
+
+@pytest.mark.parametrize("name", ["more pages than a CTA's", "a large pool of few"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_pages_captured_where_many_ctas_count(L, name, in_place):
+    """Pools that more than one CTA looks through, and pairs that are compared ahead of the copies: count, compact and copy behind one another
+    on one workspace, in a graph."""
+    s, table, rows, lens = _holders(name, 1, 8, 1)
+    n_pairs, longest = 300, int(lens.max())
+    assert s.pages > 24000 and n_pairs > 32
+    cache = s.cache(L)
+    pages = L.CachePages(cache)
+    pages.workspace.fill_(255)
+    t, r, n = ints(table, rows, lens)
+    out = t.clone() if in_place else torch.full_like(t, -3)
+    target = t if in_place else out
+    src, dst, held, tokens = ints(np.zeros(n_pairs), np.zeros(n_pairs), np.zeros(7), np.zeros(n_pairs))
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        pages.count(t, r, n)
+    stream.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        refs, free, number = pages.count(t, r, n, held)
+        where, used = pages.compact(t, r, n, held, out=None if in_place else out)
+        pages.copy(src, dst, tokens)
+        refs2, free2, number2 = pages.count(target, r, n)
+    for seed in range(3):
+        rng = np.random.default_rng(seed)
+        lens2 = np.minimum(lens, rng.integers(0, longest + 1, size=len(lens))).astype(np.int32)
+        pair = rng.permutation(s.pages)[:2 * n_pairs]
+        few, more = rng.integers(-1, s.page + 1, size=n_pairs), rng.integers(0, s.pages, size=7)
+        t.copy_(torch.from_numpy(table))
+        if not in_place:
+            out.fill_(-3)
+        for a, b in zip((n, src, dst, tokens, held), (lens2, pair[:n_pairs], pair[n_pairs:], few, more)):
+            a.copy_(torch.from_numpy(b.astype(np.int32)))
+        cache.kv_buffer_.copy_(s.kv.view(bf16))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = count_oracle(table, rows, lens2, s.page, s.pages, more)
+        assert np.array_equal(refs.cpu().numpy(), want[0]) and np.array_equal(free.cpu().numpy(), want[1]) and int(number) == want[2]
+        kv, t2, where2, used2 = compact_oracle(s.kv, table, rows, lens2, s.page, s.pages, more, None if in_place else np.full_like(table, -3))
+        assert np.array_equal(target.cpu().numpy(), t2) and np.array_equal(where.cpu().numpy(), where2) and int(used) == used2
+        assert torch.equal(s.contents(cache), copy_oracle(kv, s.page, s.pages, pair[:n_pairs].tolist(), pair[n_pairs:].tolist(), few.tolist())[0])
+        want = count_oracle(t2, rows, lens2, s.page, s.pages)
+        assert np.array_equal(refs2.cpu().numpy(), want[0]) and np.array_equal(free2.cpu().numpy(), want[1]) and int(number2) == want[2]
+    assert L.read_device_status() == (0, 0)
