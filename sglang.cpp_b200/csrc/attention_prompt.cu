@@ -19,9 +19,11 @@
 // run.
 //
 // Keys behind a row are masked as scores; as values they meet weights of 0, which is right for numbers only.  Rows behind a sequence
-// become zeros in shared memory; where a row's result is no number, values that it does not see are looked through at the end, and if one
-// is to blame the row is summed up once more without them, a thread per row (16 / 8 heads, one block behind 8000 keys: 78 ms; 115 with one load at a time).
-// It is rare, and code that ran it faster would stand in the way of the rest.
+// become zeros in shared memory.  Sums of weights of 2^24 a tile and more also leave the range of numbers with values from 2^79 on, whose mean
+// does not.  So where a row's result is no number, values are looked through at the end, and if one that the row does not see or a large one may be to
+// blame, the row is summed up once more from what it sees, by weights that add up to 1, a thread per row (16 / 8 heads, one block behind 8000 keys: 58 ms,
+// behind 1024 7.1; values of all keys looked through and nothing found: 1.1 ms a call of 8000).  It is rare, and code that ran it faster would stand
+// in the way of the rest.
 //
 // What bounds it: for long prompts products and exponentials, 2048 cycles each per K/V tile and pair of query tiles (68 % of the tensor pipe, 68 % of
 // the units for exponentials), and power: 2 x 8000 tokens of 32 / 8 heads run at 1.16 to 1.17 PFLOP/s one behind another, up to 1.34 with idle time between; the library's products at 1.43 sustained.
@@ -55,7 +57,8 @@ static_assert(128 * (2 * kFewRegs + 2 * kSoftmaxRegs) <= kThreads * 128, "");
 constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16 under the 128-byte swizzle
 constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns
 constexpr int kAgain = 2048;                // query tiles of a CTA that are noted one by one
-constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more (products with values up to 2^100 fit)
+constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more
+constexpr uint32_t kLargeBits = (127 + 80) << 7;   // of bf16 2^80: kMostSum of at most 2^21 tiles times smaller values stay below 2^125
 
 // Sizes by the padded head dimension.
 template <int DP>
@@ -187,58 +190,73 @@ struct Walk {
     }
 };
 
-// A warp's rows of a query tile once more, from the keys that each row sees and no others, where a value that is no number has met the
-// weight 0 of a row before it: the values of tokens [first, end) are looked through, and if all are numbers nothing is done (the rows are what
-// their own keys make them).  tok, h: the row's token and head of the group.
+// A warp's rows of a query tile once more, from the keys that each row sees and no others and with weights that add up to 1, where a row is no number
+// and its keys need not be to blame: a value that is no number among those of tokens [first, end) may have met the weight 0 of a row before it,
+// and values from 2^79 on the sum of all weights, which only then are divided by it.  If there are neither, nothing is done (the rows are
+// what their own values make them).  tok, h: the row's token and head of the group.
 __device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, int kv_head, int first, int end, int tok, int h, bool store) {
-    const int lane = threadIdx.x & 31, vectors = p.dim >> 3;
+    const int lane = threadIdx.x & 31, vectors = p.dim >> 3, keys = 32 / vectors, sub = lane / vectors, column = (lane - sub * vectors) * 8;
     const __nv_bfloat16* v = p.v + static_cast<int64_t>(seq_first) * p.v_st + kv_head * p.v_sh;
     const __nv_bfloat16* k = p.k + static_cast<int64_t>(seq_first) * p.k_st + kv_head * p.k_sh;
+    // two numbers at a time: exponents and fractions as integers, 0x7f80 and more for no numbers, which 0x80 more make negative before `first`
     bool found = false;
 #pragma unroll 1
-    for (int i = first * vectors + lane; i < end * vectors; i += 32) {
-        const int key = i / vectors;
-        const Vec8 x = load8(v + key * p.v_st + (i - key * vectors) * 8);
+    for (int last = end - 1; last >= 0 && !__any_sync(0xffffffffu, found); last -= 8 * keys) {
+        uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) found = found || !isfinite(x.v[e]);
+        for (int u = 0; u < 8; ++u) {
+            const int key = last - u * keys - sub;
+            if (sub >= keys || key < 0) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(v + key * p.v_st + column);
+            const uint32_t seen = key < first ? 0x00800080u : 0u;
+            most = __vmaxs2(__vmaxs2(most, (x.x & 0x7fff7fffu) + seen), (x.y & 0x7fff7fffu) + seen);
+            most = __vmaxs2(__vmaxs2(most, (x.z & 0x7fff7fffu) + seen), (x.w & 0x7fff7fffu) + seen);
+        }
+        found = (most & 0xffffu) >= kLargeBits || most >> 16 >= kLargeBits;
     }
     if (!__any_sync(0xffffffffu, found)) return;
     const int64_t row = seq_first + tok, head = kv_head * p.group + h;
     const __nv_bfloat16* q = p.q + row * p.q_st + head * p.q_sh;
-#pragma unroll 1
-    for (int c = 0; c < p.dim; c += 32) {
-        float o[32], m = -INFINITY, sum = 0.f;
+    auto score = [&](int key) {
+        float s = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < p.dim; d += 8) {
+            const Vec8 a = load8(q + d), b = load8(k + key * p.k_st + d);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            for (int e = 0; e < 8; ++e) s = fmaf(a.v[e], b.v[e], s);
+        }
+        return __fmul_rn(s, p.scale_log2);   // (the same number in both passes, whatever is made of it)
+    };
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int key = 0; key <= tok; ++key) {
+        const float s = score(key), now = fmaxf(m, s);
+        sum = now > -INFINITY ? fmaf(sum, exp2f(m - now), exp2f(s - now)) : s == -INFINITY ? sum : s;   // (a score that is no number makes the sum none)
+        m = now;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum;
+#pragma unroll 1
+    for (int c = 0; c < p.dim; c += 64) {
+        float o[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) o[i] = 0.f;
 #pragma unroll 1
         for (int key = 0; key <= tok; ++key) {
-            float s = 0.f;
-#pragma unroll 4
-            for (int d = 0; d < p.dim; d += 8) {
-                const Vec8 a = load8(q + d), b = load8(k + key * p.k_st + d);
+            const float w = m == -INFINITY ? inv : exp2f(score(key) - m) * inv;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s = fmaf(a.v[e], b.v[e], s);
-            }
-            s *= p.scale_log2;
-            const float now = fmaxf(m, s), old = now == -INFINITY ? 1.f : exp2f(m - now);
-            const float w = now > -INFINITY ? exp2f(s - now) : s == -INFINITY ? 0.f : s;   // (a score that is no number is a weight that is none)
-            m = now;
-            sum = fmaf(sum, old, w);
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
+            for (int e = 0; e < 64; e += 8) {
                 if (c + e >= p.dim) break;
                 const Vec8 x = load8(v + key * p.v_st + c + e);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[e + i] = fmaf(w, x.v[i], o[e + i] * old);
+                for (int i = 0; i < 8; ++i) o[e + i] = fmaf(w, x.v[i], o[e + i]);
             }
         }
-        const float inv = sum > 0.f ? 1.f / sum : sum;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
+        for (int e = 0; e < 64; e += 8) {
             if (!store || c + e >= p.dim) break;
             Vec8 x;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x.v[i] = o[e + i] * inv;
+            for (int i = 0; i < 8; ++i) x.v[i] = o[e + i];
             store8(p.out + (row * p.q_heads + head) * p.dim + c + e, x);
         }
     }

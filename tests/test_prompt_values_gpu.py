@@ -50,3 +50,42 @@ def test_rows_of_scores_that_are_no_numbers(L, form):
     hit[a:a + n, 2:4] = True
     assert_prompt((torch.where(hit, want[0].to(bf16), got), torch.where(hit.any(-1), want[2].float(), lse)), want)
     assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [128, 64, 72])
+@pytest.mark.parametrize("size", [2.0 ** 90, 2.0 ** 101, 2.0 ** 120, 2.0 ** 127])
+def test_large_values(L, form, dim, size):
+    """Numbers up to the type's largest, where a score per tile of keys behind the first one is larger by 16 (its weight e^16 < 2^24 of the first
+    ones'): the weighted sums of up to 16 tiles pass 2^128 where the means do not."""
+    s = of_form(form, [2100, 140, 1] if form == "two tiles" else [2100, 7], 8, 4, dim, seed=2)
+    q, k, v = s.parts(s.rows)
+    q[:], k[:] = 0.0, 0.0
+    q[:, :, 0] = 16.0
+    for a, n in zip(s.indptr[:-1], s.lens):
+        k[a + 130:a + n:131, :, 0] = math.sqrt(dim)
+        k[a + 100:a + n:57, :, 0] = -math.sqrt(dim)
+    x = v.float().clamp(-1.99, 1.99)
+    v[:] = torch.where(x.abs() < 1.0, torch.sign(x) + x * 0.5, x).to(bf16) * size
+    v[:, 0] = v[:, 0].abs()
+    assert bool(torch.isfinite(v).all())
+    assert_prompt(s.run(L), s.want("cuda"))
+    assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_mean_of_the_largest_value(L, form):
+    """Equal weights of the type's largest numbers; one column has a NaN besides, from its row on."""
+    s = of_form(form, [200, 90], 8, 4, 128, seed=3, q_scale=0.0)
+    _, _, v = s.parts(s.rows)
+    most = torch.finfo(bf16).max
+    v[:] = torch.where(v.float() < 0, -most, most).to(bf16)
+    v[:, 1] = most
+    want = s.want("cuda")
+    v[150, 1, 9] = float("nan")
+    out, lse = s.run(L)
+    got = out.reshape(-1, 8, 128)
+    assert bool(torch.isnan(got[150:200, 2:4, 9]).all()) and bool((got[:150, 2:4] == most).all()) and bool((got[200:, 2:4] == most).all())
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[150:200, 2:4, 9] = True
+    assert_prompt((torch.where(hit, want[0].to(bf16), got), lse), want)
