@@ -333,7 +333,8 @@ B200_API int b200_attention_shared_prefix(const b200_shared_prefix_args* args, b
  * on the device: a captured call follows what it holds at its replay, up to its tokens and batch.  Rows of no sequence are left as
  * they were.  An indptr that decreases or leaves [0, tokens] is reported as tokens + 1 in the status words, and nothing is written.
  * An infinity or NaN among keys and values reaches the rows that see it and no others; among values it costs time where a block of rows
- * sees it in part, and so do values from 2^79 on whose sums leave the range of fp32 (7 ms per block behind 1000 keys, 58 behind 8000).
+ * sees it in part, unless the block's first row has a NaN in the same column, and so do values from 2^79 on whose sums leave the range of
+ * fp32 (7 ms per block behind 1000 keys, 58 behind 8000).
  * bf16; head_dim a multiple of 8 up to 128; q_heads a multiple of kv_heads with up to 128 heads per KV head; up to 1024 sequences.  q, k, v 16-byte
  * aligned, their strides positive multiples of 8.  out and lse overlap none of the inputs. */
 typedef struct b200_prompt_attention_args {

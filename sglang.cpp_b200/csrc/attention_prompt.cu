@@ -22,7 +22,8 @@
 // become zeros in shared memory.  Sums of weights of 2^24 a tile and more also leave the range of numbers with values from 2^79 on, whose mean
 // does not.  So where a row's result is no number, values are looked through at the end, and if one that the row does not see or a large one may be to
 // blame, the row is summed up once more from what it sees, by weights that add up to 1, a thread per row (16 / 8 heads, one block behind 8000 keys: 58 ms,
-// behind 1024 7.1; values of all keys looked through and nothing found: 1.1 ms a call of 8000).  It is rare, and code that ran it faster would stand
+// behind 1024 7.1; values of all keys looked through and nothing found: 1.1 ms a call of 8000).  Rows that no value can make numbers are left: a NaN among
+// their scores, columns whose first value that all see is one (2 x 8000 tokens of NaN throughout 528 -> 0.8 ms).  It is rare, and code that ran it faster would stand
 // in the way of the rest.
 //
 // What bounds it: for long prompts products and exponentials, 2048 cycles each per K/V tile and pair of query tiles (68 % of the tensor pipe, 68 % of
@@ -198,7 +199,13 @@ __device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, 
     const int lane = threadIdx.x & 31, vectors = p.dim >> 3, keys = 32 / vectors, sub = lane / vectors, column = (lane - sub * vectors) * 8;
     const __nv_bfloat16* v = p.v + static_cast<int64_t>(seq_first) * p.v_st + kv_head * p.v_sh;
     const __nv_bfloat16* k = p.k + static_cast<int64_t>(seq_first) * p.k_st + kv_head * p.k_sh;
-    // two numbers at a time: exponents and fractions as integers, 0x7f80 and more for no numbers, which 0x80 more make negative before `first`
+    // Two numbers at a time: exponents and fractions as integers, 0x7f80 and more for no numbers, which 0x80 more make negative before `first`.
+    // Columns in which `first`, which all rows see, is NaN: they are NaN whatever else there is.
+    const bool looks = sub < keys;
+    const uint4 x0 = looks ? *reinterpret_cast<const uint4*>(v + first * p.v_st + column) : make_uint4(0, 0, 0, 0);
+    auto mask_of = [&](uint32_t w) { return looks ? __vcmpleu2(w & 0x7fff7fffu, 0x7f807f80u) & 0x7fff7fffu : 0u; };
+    const uint4 mask = make_uint4(mask_of(x0.x), mask_of(x0.y), mask_of(x0.z), mask_of(x0.w));
+    if (!__any_sync(0xffffffffu, (mask.x | mask.y | mask.z | mask.w) != 0)) return;
     bool found = false;
 #pragma unroll 1
     for (int last = end - 1; last >= 0 && !__any_sync(0xffffffffu, found); last -= 8 * keys) {
@@ -206,11 +213,11 @@ __device__ __noinline__ void sum_up_again(const PromptParams& p, int seq_first, 
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int key = last - u * keys - sub;
-            if (sub >= keys || key < 0) continue;
+            if (!looks || key < 0) continue;
             const uint4 x = *reinterpret_cast<const uint4*>(v + key * p.v_st + column);
             const uint32_t seen = key < first ? 0x00800080u : 0u;
-            most = __vmaxs2(__vmaxs2(most, (x.x & 0x7fff7fffu) + seen), (x.y & 0x7fff7fffu) + seen);
-            most = __vmaxs2(__vmaxs2(most, (x.z & 0x7fff7fffu) + seen), (x.w & 0x7fff7fffu) + seen);
+            most = __vmaxs2(__vmaxs2(most, (x.x & mask.x) + seen), (x.y & mask.y) + seen);
+            most = __vmaxs2(__vmaxs2(most, (x.z & mask.z) + seen), (x.w & mask.w) + seen);
         }
         found = (most & 0xffffu) >= kLargeBits || most >> 16 >= kLargeBits;
     }
@@ -755,6 +762,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                 tc_fence_after();
                 const uint32_t o_addr = tmem_base + (static_cast<uint32_t>(qtr * 32) << 16) + X::kColO + static_cast<uint32_t>(tile) * DP;
                 float2 odd = make_float2(0.f, 0.f);   // 0 as long as all are numbers
+                const bool may_be = r_tok < rows && ml.y - ml.y == 0.f;   // (a sum that is no number: the row's own keys)
 #pragma unroll 1
                 for (int c = 0; c * 32 < p.dim; ++c) {
 #pragma unroll
@@ -793,7 +801,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                     }
                     __syncwarp();
                 }
-                if (__any_sync(0xffffffffu, !(odd.x == 0.f && odd.y == 0.f)) && lane == 0) {
+                if (__any_sync(0xffffffffu, may_be && !(odd.x == 0.f && odd.y == 0.f)) && lane == 0) {
                     const int at = min(2 * n + tile, kAgain);
                     atomicOr(&s_again[at >> 5], 1u << (at & 31));
                 }

@@ -89,3 +89,27 @@ def test_mean_of_the_largest_value(L, form):
     hit = torch.zeros_like(got, dtype=torch.bool)
     hit[150:200, 2:4, 9] = True
     assert_prompt((torch.where(hit, want[0].to(bf16), got), lse), want)
+
+
+@pytest.mark.parametrize("bad", [float("nan")])
+def test_values_that_are_all_no_numbers_cost_little(L, bad):
+    """Where every row is no number by its own keys, nothing is summed up again."""
+    s = PromptSetup([3000, 2900], 8, 4, 128, seed=4)
+    indptr = torch.from_numpy(s.indptr).cuda()
+
+    def time(rows):
+        s.run(L, rows, indptr)
+        a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+        a.record()
+        for _ in range(3):
+            out, _ = s.run(L, rows, indptr)
+        b.record()
+        b.synchronize()
+        return a.elapsed_time(b) / 3, out
+
+    plain, _ = time(s.rows.cuda())
+    for part in (2, 1):   # the values, the keys as well
+        s.parts(s.rows)[part][:] = bad
+        took, out = time(s.rows.cuda())
+        assert bool(torch.isnan(out).all())
+        assert took < 10 * plain + 1.0, (took, plain)
