@@ -59,6 +59,7 @@ constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows x 64 bf16 under the 128-
 constexpr uint32_t kStageBytes = 32 * 64;   // a warp's output rows, 32 columns
 constexpr int kAgain = 2048;                // query tiles of a CTA that are noted one by one
 constexpr float kMostSum = 1 << 24;         // the reference moves where a row's probabilities of a tile add up to more
+constexpr float kFar = 1 << 14;              // the scaled reference is rounded before it is subtracted: by 2^-11 here, beyond 2^31 weights overflow or vanish
 constexpr uint32_t kLargeBits = (127 + 80) << 7;   // of bf16 2^80: kMostSum of at most 2^21 tiles times smaller values stay below 2^125
 
 // Sizes by the padded head dimension.
@@ -657,7 +658,23 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                             }
                         }
                     }
-                    const float mb = m_ref == -INFINITY ? INFINITY : m_ref * sc;   // (no key seen yet: probabilities 0)
+                    float mb = m_ref == -INFINITY ? INFINITY : m_ref * sc;   // (no key seen yet: probabilities 0)
+                    if (move) {
+                        const bool far = fabsf(mb) > kFar && fabsf(m_ref) < INFINITY;
+                        if (__any_sync(0xffffffffu, far)) {   // (rare) differences of the raw scores instead, which are exact where they matter
+                            const float2 to = make_float2(far ? -m_ref : 0.f, far ? -m_ref : 0.f);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    const float2 d = add2(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), to);
+                                    s[c][i] = __float_as_uint(d.x);
+                                    s[c][i + 1] = __float_as_uint(d.y);
+                                }
+                            }
+                            if (far) mb = 0.f;
+                        }
+                    }
                     const float2 sc2 = make_float2(sc, sc), mb2 = make_float2(-mb, -mb);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -682,7 +699,7 @@ prompt_attention_kernel(const __grid_constant__ PromptMaps maps, const __grid_co
                         tmem_st_32x32b_x16(p_addr + c * 16, packed);
                     }
                     tile_sum = sum.x + sum.y;
-                    if (move || !__any_sync(0xffffffffu, tile_sum > kMostSum || m_ref == -INFINITY)) break;
+                    if (move || !__any_sync(0xffffffffu, tile_sum > kMostSum || fabsf(mb) > kFar)) break;
                     move = true;
                 }
                 tmem_st_wait();

@@ -113,3 +113,27 @@ def test_values_that_are_all_no_numbers_cost_little(L, bad):
         took, out = time(s.rows.cuda())
         assert bool(torch.isnan(out).all())
         assert took < 10 * plain + 1.0, (took, plain)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 4, 128), (6, 2, 64)])
+@pytest.mark.parametrize("where", ["throughout", "behind the first tile", "by their scale"])
+def test_scores_beyond_2_to_the_31(L, form, heads, kv_heads, dim, where):
+    """Scores are exact products here, far apart or equal: a row is the mean of the values of its largest ones.  Weights are 1 or nothing: what
+    is off is their sum's quotient (two roundings of 2^-24) and the output's rounding."""
+    s = of_form(form, [300, 140, 60], heads, kv_heads, dim, seed=5)
+    q, k, _ = s.parts(s.rows)
+    gen = torch.Generator().manual_seed(6)
+    size = 1.0 if where == "by their scale" else 2.0 ** 20
+    q[:], k[:] = 0.0, 0.0
+    q[:, :, 1] = torch.where(torch.rand(q.shape[:2], generator=gen) < 0.5, -size, size).to(bf16)
+    k[:, :, 1] = (torch.randint(-3, 4, k.shape[:2], generator=gen) * size).to(bf16)
+    if where == "behind the first tile":
+        for a in s.indptr[:-1]:
+            k[a:a + 140] = 0.0
+    s.scale = 1e30 if where == "by their scale" else s.scale
+    out, lse = s.run(L, sm_scale=s.scale)
+    want, size, want_lse, terms = s.want("cuda")
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    assert_prompt((out, want_lse), (want, size, want_lse, torch.zeros_like(terms)))
+    assert_prompt((want.to(bf16), lse), (want, size, want_lse, terms))
