@@ -137,3 +137,134 @@ def test_scores_beyond_2_to_the_31(L, form, heads, kv_heads, dim, where):
     assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
     assert_prompt((out, want_lse), (want, size, want_lse, torch.zeros_like(terms)))
     assert_prompt((want.to(bf16), lse), (want, size, want_lse, terms))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 8, 128), (8, 8, 128), (6, 2, 128), (8, 2, 64), (8, 4, 96), (8, 4, 72), (14, 2, 80)])
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+def test_odd_values_reach_only_what_sees_them(L, form, heads, kv_heads, dim, bad):
+    """An infinity or NaN among keys and values at many places, both query tiles' among them."""
+    s = of_form(form, [200, 131, 60, 300], heads, kv_heads, dim, seed=7)
+    want = list(s.want("cuda"))
+    _, k, v = s.parts(s.rows)
+    rng, group = np.random.default_rng(8), heads // kv_heads
+    hit = torch.zeros(sum(s.lens), heads, dim, dtype=torch.bool, device="cuda")
+    keys = torch.zeros_like(hit)
+    for i, (a, n) in enumerate(zip(s.indptr[:-1], s.lens)):
+        if i % 4 == 2:
+            continue
+        for at in sorted(rng.integers(0, n, size=3).tolist() + [n - 1, min(n - 1, 100)]):
+            g, c = int(rng.integers(kv_heads)), int(rng.integers(dim))
+            v[a + at, g, c] = bad
+            hit[a + at:a + n, g * group:(g + 1) * group, c] = True
+        if i % 3 == 0:
+            at, g = int(rng.integers(n)), int(rng.integers(kv_heads))
+            k[a + at, g] = bad
+            keys[a + at:a + n, g * group:(g + 1) * group] = True
+    out, lse = s.run(L)
+    got = out.reshape(hit.shape)
+    any_hit = hit | keys
+    assert_prompt((torch.where(any_hit, want[0].to(bf16), got), torch.where(keys.any(-1), want[2].float(), lse)), want)
+    assert not bool(torch.isfinite(got[keys]).reshape(-1, dim).all(-1).any())
+    only = got[hit & ~keys]
+    assert bool((torch.isnan(only) if bad != bad else only == bad).all())
+    assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 4, 128), (12, 2, 128), (8, 4, 64), (10, 2, 80), (8, 8, 72), (6, 2, 96), (4, 4, 8)])
+def test_neighbours_of_no_numbers(L, form, heads, kv_heads, dim):
+    """Every other sequence, and the rows around all of them, are NaN throughout: the rest is as if they were not there."""
+    lens = [130, 3, 77, 64, 257, 19, 128, 1, 200, 40]
+    s = of_form(form, lens, heads, kv_heads, dim, seed=9, before=5, behind=9, pad=24)
+    want = s.want("cuda")
+    odd = torch.zeros(sum(s.lens), dtype=torch.bool)
+    for i, (a, n) in enumerate(zip(s.indptr[:-1], s.lens)):
+        if i % 2:
+            s.rows[a:a + n] = float("nan")
+            odd[a - 5:a - 5 + n] = True
+    out = torch.full((s.rows.shape[0], heads * dim), 7.0, dtype=bf16, device="cuda")
+    _, lse = s.run(L, out=out)
+    n = sum(s.lens)
+    assert bool((out[:5] == 7).all()) and bool((out[5 + n:] == 7).all())
+    got, got_lse, odd = out[5:5 + n], lse[5:5 + n], odd.cuda()
+    assert bool(torch.isnan(got[odd]).all()) and bool(torch.isnan(got_lse[odd]).all())
+    assert_prompt((torch.where(odd[:, None], want[0].to(bf16).reshape(got.shape), got), torch.where(odd[:, None], want[2].float(), got_lse)), want)
+    assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 4, 128), (6, 2, 64), (10, 2, 96)])
+def test_large_small_and_growing_scores_of_two_tiles(L, heads, kv_heads, dim):
+    lens = [300, 140, 700]
+    for q_scale in (60.0, 0.0):
+        s = of_form("two tiles", lens, heads, kv_heads, dim, seed=10, q_scale=q_scale)
+        assert_prompt(s.run(L), s.want("cuda"))
+    s = of_form("two tiles", lens, heads, kv_heads, dim, seed=11)
+    q, k, _ = s.parts(s.rows)
+    q[:] = 1.0
+    rise = torch.cat([torch.arange(n) for n in s.lens])[:, None, None] / 64.0
+    for sign in (1.0, -1.0):
+        k[:] = (sign * rise).to(bf16)
+        assert_prompt(s.run(L), s.want("cuda"))
+    jumps = torch.cat([torch.arange(n) // 40 % 3 for n in s.lens])[:, None, None] * 4.0   # (the reference moves in the middle of rows)
+    k[:] = jumps.to(bf16)
+    assert_prompt(s.run(L), s.want("cuda"))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 8, 128), (24, 8, 64), (8, 4, 96)])
+def test_captured_calls_of_two_tiles(L, heads, kv_heads, dim):
+    """One graph, replayed for other lengths: as many rows, from one sequence to all of them short."""
+    total, batch = 1500, 12
+    first = of_form("two tiles", [total // batch] * batch, heads, kv_heads, dim, seed=12)
+    rows, indptr = first.rows.cuda(), torch.from_numpy(first.indptr).cuda()
+    total, batch = rows.shape[0], len(first.lens)
+    out = torch.zeros(total, heads * dim, dtype=bf16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        first.run(L, rows, indptr, out=out)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        _, lse = first.run(L, rows, indptr, out=out)
+    rng = np.random.default_rng(13)
+    for k in range(5):
+        cuts = np.sort(rng.integers(0, total + 1, size=batch - 1)) if k else np.full(batch - 1, total)
+        lens = np.diff(np.concatenate([[0], cuts, [total]])).tolist()
+        s = PromptSetup(lens, heads, kv_heads, dim, seed=14 + k)
+        rows.copy_(s.rows)
+        indptr.copy_(torch.from_numpy(s.indptr))
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_prompt((out, lse), s.want("cuda"))
+    assert L.read_device_status() == (0, 0)
+
+
+def test_more_items_of_a_cta_than_are_noted_one_by_one(L):
+    """1024 sequences of two tokens and 192 heads: some 1300 items per CTA, of which 1024 are noted; the last value of each
+    sequence from the 700th on is NaN."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    s = PromptSetup([2] * 1024, 192, 192, 8, seed=15)
+    assert in_pairs(s) and 1024 * 192 > 1024 * sms
+    want = s.want("cuda")
+    _, _, v = s.parts(s.rows)
+    hit = torch.zeros(2048, 192, 8, dtype=torch.bool, device="cuda")
+    v[1401::2, :, 5] = float("nan")
+    hit[1401::2, :, 5] = True
+    out, lse = s.run(L)
+    got = out.reshape(hit.shape)
+    assert bool(torch.isnan(got[hit]).all())
+    assert_prompt((torch.where(hit, want[0].to(bf16), got), lse), want)
+    assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_a_call_repeats_itself(L, form):
+    s = of_form(form, [300, 131, 60], 16, 4, 128, seed=16)
+    rows, indptr = s.rows.cuda(), torch.from_numpy(s.indptr).cuda()
+    out, lse = s.run(L, rows, indptr)
+    for _ in range(20):
+        again, lse2 = s.run(L, rows, indptr)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
