@@ -310,7 +310,8 @@ class Engine:
 
     def cache_pages(self):
         """``layers.CachePages`` over the K/V pool of all layers, without the dummy request's page: to copy, share, count or move
-        pages between steps, on ``cuda_stream``.  (Models whose layers are listed one by one have a pool per layer.)"""
+        pages between steps, on ``cuda_stream``.  (Models whose layers are listed one by one have a pool per layer.)  Whoever keeps books of
+        pages has to follow a compaction by its map: ``HostBatcher.compact`` does both."""
         from .layers import CachePages, MHAKVCache
         if self.stack:
             raise _lib.B200Error(4, "a pool per layer: CachePages needs the K/V of all layers in one")
@@ -331,6 +332,17 @@ class Engine:
             tokens = self.device_view("token_pool").view(torch.int32).view(self.config.max_running_req + 1, self.pt_cols)
             tokens[new.long(), :length + 1] = tokens[old.long(), :length + 1]
             stream.synchronize()   # (the index tensors may go)
+
+    def compact_pages(self, rows, lens, held) -> np.ndarray:
+        """Moves the pages of the first ``lens`` positions of the table's ``rows``, and ``held`` ones, to the front of the pool and renames them in the
+        table.  Returns where each page is now, -1 for free ones: the caller's own books of pages follow by it."""
+        stream = self.cuda_stream()
+        if self._pages is None:
+            self._pages = self.cache_pages()
+        with torch.cuda.stream(stream):
+            which, n, held = (torch.from_numpy(_i32(a)).to(self._pages.workspace.device) for a in (rows, lens, held))
+            where, _ = self._pages.compact(self.page_table(), which, n, held)
+            return where.cpu().numpy()
 
     def cuda_stream(self) -> torch.cuda.Stream:
         """The stream that steps are enqueued on."""

@@ -167,6 +167,15 @@ class RadixPrefixCache:
             node.timestamp = tic
         return node, prefix
 
+    def nodes(self) -> list:
+        """All nodes but the root."""
+        out, stack = [], list(self.root.children.values())
+        while stack:
+            n = stack.pop()
+            out.append(n)
+            stack.extend(n.children.values())
+        return out
+
     def match_prefix(self, ids) -> CacheHandle:
         node, n = self._walk(np.asarray(ids, dtype=np.int32))
         return CacheHandle(n, node)
@@ -391,6 +400,27 @@ class CacheManager:
         else:
             req.cache_handle = handle
             self.lock(handle)
+
+    def cached_pages(self) -> np.ndarray:
+        """The pages that the prefix cache holds."""
+        slots = [n.value for n in self.prefix_cache.nodes()]
+        return np.concatenate(slots)[::self.page_size] // self.page_size if slots else np.zeros(0, np.int32)
+
+    def pages_moved(self, where: np.ndarray, rows, lens) -> None:
+        """Page g is now page where[g] (-1: nobody held it): names them anew in positions [0, lens[i]) of the mirror's rows[i] and in the prefix
+        cache; all others are free, in ascending order."""
+        P, table = self.page_size, self.tables.page_table
+        where = np.asarray(where)
+        held = [table[r, :n:P] // P for r, n in zip(rows, lens)] + [self.cached_pages()]
+        if self._lazy is not None or len(where) != self.num_pages or any((where[pages] < 0).any() for pages in held):
+            raise ValueError("pages_moved: pages that are held have no place, or are being freed")
+        name = lambda slots: (where[slots // P] * P + slots % P).astype(np.int32)
+        for r, n in zip(rows, lens):
+            table[r, :n] = name(table[r, :n])
+        for n in self.prefix_cache.nodes():
+            n.value = name(n.value)
+        taken = set(where[where >= 0].tolist())
+        self.free_pages = [g * P for g in range(self.num_pages) if g not in taken]
 
     def check_integrity(self) -> None:
         cached = (self.prefix_cache.evictable_size + self.prefix_cache.protected_size) // self.page_size
@@ -624,6 +654,24 @@ class HostBatcher:
             pages[row, full:end] = np.arange(slot, slot + end - full)
         tokens[rows, :n + 1] = tokens[req.table_idx, :n + 1]
         return out
+
+    def compact(self) -> int:
+        """Moves the pages that requests and the prefix cache hold to the front of the pool (no counterpart in the reference) and names them anew
+        in the host's books: the table's mirror, cached prefixes, free pages.  Between steps.  Returns how many are in use."""
+        cm, cols = self.cache_manager, self.tables.page_table.shape[1]
+        rows = sorted(self._held)
+        lens = [min(self._held[r] * self.page_size, cols) for r in rows]
+        cached = cm.cached_pages()
+        if self.engine is not None:
+            where = self.engine.compact_pages(rows, lens, cached)
+        else:   # the same on the host: late pages to the holes, in order
+            table, P = self.tables.page_table, self.page_size
+            used = np.unique(np.concatenate([cached] + [table[r, :n:P] // P for r, n in zip(rows, lens)]))
+            where = np.full(cm.num_pages, -1, np.int32)
+            where[used] = used
+            where[used[used >= len(used)]] = np.setdiff1d(np.arange(len(used)), used)
+        cm.pages_moved(where, rows, lens)
+        return int((where >= 0).sum())
 
     def slots_of(self, req: Req) -> np.ndarray:
         """The request's page-table row (one slot per position; unallocated positions read 0)."""

@@ -273,3 +273,82 @@ def test_pages_workspace_of_more_pages_than_there_may_be(pkg):
     size = pkg.load_library().b200_pages_workspace_bytes
     assert size(1 << 30) > size((1 << 30) - 100_000) > 3 * 4 * ((1 << 30) - 100_000)
     assert [size(n) for n in ((1 << 30) + 1, 2 ** 31 - 2048, 2 ** 31 - 1)] == [-1] * 3
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+def test_compacted_books(pkg, page):
+    """Requests, forks and cached prefixes read the same contents behind a compaction, and nothing that is allocated later is theirs."""
+    rng = np.random.default_rng(page)
+    hb = _batcher(pkg, page, pages=320 // page, rows=10)
+    cm, memory = hb.cache_manager, np.full(320, -1)
+
+    def check(reqs):               # (a position's contents: the tokens up to it)
+        for r in reqs:
+            for i in range(r.cached_len):
+                assert memory[hb.slots_of(r)[i]] == hash(tuple(r.input_ids[:i + 1].tolist()))
+
+    def start(ids):
+        r = hb.add_request(ids, 20)
+        hb.allocate([r])
+        for i in range(r.cached_len, len(ids)):
+            memory[hb.slots_of(r)[i]] = hash(tuple(ids[:i + 1].tolist()))
+        r.complete_one()
+        hb.cache_prefix(r)
+        return r
+
+    first = [start(rng.integers(0, 99, size=n)) for n in (21, 32, 7, 18)]
+    kids = hb.fork(first[1], 2) + hb.fork(first[0], 2)
+    for k, parent in zip(kids, [first[1]] * 2 + [first[0]] * 2):    # the copied part page
+        full = k.cached_len // page * page
+        memory[hb.slots_of(k)[full:k.cached_len]] = memory[hb.slots_of(parent)[full:k.cached_len]]
+    live = first + kids
+    for step in range(3):
+        for r in live:
+            r.append_host_token(int(rng.integers(99)))
+        hb.allocate(live)
+        for r in live:
+            memory[hb.slots_of(r)[r.cached_len]] = hash(tuple(r.input_ids.tolist()))
+            r.complete_one()
+        check(live)
+        for r in (live.pop(0), live.pop()):
+            hb.release(r)
+        before = {g: memory[g * page:(g + 1) * page].copy() for g in range(cm.num_pages)}
+        moved = {}
+        real = cm.pages_moved
+        cm.pages_moved = lambda where, *a: (moved.update(enumerate(where.tolist())), real(where, *a))
+        used = hb.compact()
+        del cm.pages_moved
+        memory[:] = -1
+        for g, to in moved.items():
+            if to >= 0:
+                memory[to * page:(to + 1) * page] = before[g]
+        assert sorted(to for to in moved.values() if to >= 0) == list(range(used))
+        assert cm.free_pages == [g * page for g in range(used, cm.num_pages)]
+        check(live)
+        assert hb.compact() == used                      # (nothing moves again)
+        check(live)
+    again = start(first[0].input_ids[:21].copy())        # from the prefix cache, in its new place
+    assert again.cache_handle.cached_len >= 20 // page * page
+    check(live + [again])
+    for r in live + [again]:
+        hb.release(r)
+    cm.check_integrity()
+    assert cm.prefix_cache.protected_size == 0 and hb.compact() == len(cm.cached_pages())
+    with pytest.raises(ValueError):
+        cm.pages_moved(np.full(cm.num_pages, -1), [], [])
+
+
+def test_compaction_that_the_engine_refuses_changes_no_books(pkg):
+    from sglang_cpp_b200.host_batch import HostBatcher
+    engine = _Refuses(64, True)
+    engine.compact_pages = lambda *a: (_ for _ in ()).throw(RuntimeError("no"))
+    hb = HostBatcher(engine, 8, 16, 4)
+    a, b = hb.add_request(np.arange(20), 9), hb.add_request(np.arange(50) + 3, 9)
+    hb.allocate([a, b])
+    for r in (a, b):
+        r.complete_one()
+    hb.release(a)
+    table, free = hb.tables.page_table.copy(), list(hb.cache_manager.free_pages)
+    with pytest.raises(RuntimeError):
+        hb.compact()
+    assert np.array_equal(hb.tables.page_table, table) and hb.cache_manager.free_pages == free

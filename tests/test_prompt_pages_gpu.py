@@ -862,3 +862,58 @@ def test_pages_captured_where_many_ctas_count(L, name, in_place):
         want = count_oracle(t2, rows, lens2, s.page, s.pages)
         assert np.array_equal(refs2.cpu().numpy(), want[0]) and np.array_equal(free2.cpu().numpy(), want[1]) and int(number2) == want[2]
     assert L.read_device_status() == (0, 0)
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_an_engine_compacted_with_the_hosts_books(pkg, L, page):
+    """Two engines take the same steps, one of them with its pages compacted in between: the logits are the same, requests that begin
+    later among them."""
+    from oracle import token_loop_oracle as O
+    from sglang_cpp_b200.engine import Engine, EngineConfig
+    from sglang_cpp_b200.host_batch import HostBatcher
+
+    cfg = O.ModelConfig(2, 256, 4, 2, 128, 512, 1024, 1e-6, 1e6, 512, True, True, True)
+    weights = O.init_weights(cfg, seed=2, std=0.02)
+
+    def steps(compacts):
+        engine = Engine(cfg, EngineConfig(page, 640 // page, 6, 512, 1024))
+        engine.load_weights(weights)
+        hb, logits, rng = HostBatcher(engine, 640 // page, page, 6), [], np.random.default_rng(3)
+
+        def run(call, reqs):
+            tokens = call(reqs)
+            tokens.synchronize()
+            logits.append(engine.logits(len(reqs)).clone())
+            for r, t in zip(reqs, tokens.next_tokens_cpu[:len(reqs)].tolist()):
+                r.append_host_token(t)
+
+        def begin(n):
+            r = hb.add_request(rng.integers(0, 1024, size=n), 30)
+            run(hb.prefill, [r])
+            hb.cache_prefix(r)
+            return r
+
+        reqs = [begin(n) for n in (50, 33, 70)]
+        reqs += hb.fork(reqs[1], 2)
+        for _ in range(3):
+            for _ in range(4):
+                run(hb.decode, reqs)
+            hb.release(reqs.pop(0))
+            tree = hb.cache_manager.prefix_cache
+            hb.cache_manager.free_indices(tree.evict(min(page, tree.evictable_size)))    # (holes in the pool)
+            if compacts:
+                used = hb.compact()
+                assert sorted(hb.cache_manager.free_pages) == [g * page for g in range(used, 640 // page)]
+                table = engine.read_table("page_table")
+                for r in reqs:
+                    assert np.array_equal(table[r.table_idx, :r.cached_len], hb.slots_of(r)[:r.cached_len])
+            reqs.append(begin(int(rng.integers(20, 60))))
+        for r in reqs:
+            hb.release(r)
+        hb.cache_manager.check_integrity()
+        engine.synchronize()
+        return logits
+
+    for a, b in zip(steps(False), steps(True)):
+        assert torch.equal(a, b)
+    assert L.read_device_status() == (0, 0)
