@@ -386,7 +386,8 @@ B200_API int b200_fork_rows(const b200_page_pool* pool, int32_t* page_table, int
 /* Which pages are held, and which are free, once rows of a page table share pages: refs[g] = how many of the rows rows[i] of lens[i]
  * positions (i < count) hold page g, plus how often `held` names it (pages that somebody holds outside the table, a prefix cache
  * for instance; NULL with held_count 0); free_pages = the pages with refs 0 in ascending order, then -1; free_count their number.
- * refs, free_pages int32 [num_pages], free_count int32 [1]; count up to 2^20, held_count up to 2^30.  A row named twice counts twice.  Lengths are cut to [0, table_cols].
+ * refs, free_pages int32 [num_pages], free_count int32 [1]; count up to 2^20, held_count up to 2^30.  A row named twice counts twice (a page
+ * at most 2^31 - 1 times in all).  Lengths are cut to [0, table_cols].
  * Rows, slots and pages that there are not count for nothing and are reported in the status words (that value + 1). */
 B200_API int b200_count_pages(int32_t* refs, int32_t* free_pages, int32_t* free_count, const int32_t* page_table,
                               int64_t table_rows, int64_t page_table_stride, int64_t table_cols, const int32_t* rows,

@@ -293,7 +293,7 @@ __device__ __forceinline__ void each_page(const HeldParams& p, int i, int first,
         int slot[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) slot[k] = at + k * stride < len ? row[at + k * stride] : 0;
-        const bool alike = at + 3 * stride < len && slot[0] == slot[1] && slot[0] == slot[2] && slot[0] == slot[3];   // (a dummy's page throughout)
+        const bool alike = at + 3 * stride < len && slot[0] == slot[1] && slot[0] == slot[2] && slot[0] == slot[3];   // (zeros behind a row's pages)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (at + k * stride >= len || (alike && k > 0)) break;
@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(kThreads)
 count_held_kernel(const HeldParams p, int32_t* refs) {
     pdl_launch_dependents();
     pdl_wait_prior();
-    // A row whose table names one page throughout, a dummy's for instance: one addition per warp and four places of it.  (Half a million
-    // additions to one page one by one: 300 us; by warps 17.)
+    // Rows whose lengths reach past their pages name page 0 from there on, where tables begin as zeros: one addition per warp and four places
+    // of it.  (Half a million additions to one page one by one: 300 us; by warps 17.  The framework's own requests have no such lengths.)
     each_page(p, blockIdx.x, blockIdx.y * kThreads + threadIdx.x, gridDim.y * kThreads, [&](int g, int n) {
         const uint32_t with = __activemask();
         int same;
@@ -565,10 +565,10 @@ Units units_of(const Pool& pool) {
     u.planes_div = divisor(static_cast<uint32_t>(pool.num_planes));
     return u;
 }
-// CTAs for `pairs` pages: one for every 16 KB.  As long as they are known to be there, up to 128 waves of them: those that run at a time then work
-// on neighbouring pages (700 pages of 1.8 MB: 421 us with one wave, 407 with four, 398 with sixteen, 396 with all).  Where `pairs` is what there may
-// be at most, four waves, or half a one if even that is little (800 of 1600 such pages in use 170 us with one wave, 164 with four; 6 short
-// requests in a pool of 64 pages 11.7, 13, 17 us with half a wave, one, four).
+// CTAs for `pairs` pages: one for every 16 KB.  As long as they are known to be there, up to sixteen waves of them (a wave: eight CTAs per SM): those
+// that run at a time then work on neighbouring pages (700 pages of 1.8 MB: 421 us with one wave, 407 with four, 398 with sixteen, 396 with all).  Where
+// `pairs` is what there may be at most, four waves, or half a one if even that is little (800 of 1600 such pages in use 170 us with one wave, 164
+// with four; 6 short requests in a pool of 64 pages 11.7, 13, 17 us with half a wave, one, four).
 int move_grid(const Pool& pool, const Units& u, int64_t pairs, bool known) {
     const int64_t runs = pairs * pool.num_planes, units = u.group_log < 5 ? (runs >> (5 - u.group_log)) + 1 : runs * u.per_run;
     const int64_t wave = static_cast<int64_t>(sm_count()) * 8;
